@@ -22,8 +22,10 @@ HEADERS = sorted(glob.glob(os.path.join(CSRC, "*.h"))) + [os.path.join(os.path.d
 # -ffp-contract=off: the sufficient-statistics updates must round product and sum
 # separately (bit-identical m / S to the reference); hot loops call fma() explicitly.
 # -fvisibility=hidden: the shared object exports the BGMM_API entry points of include/bgmm.h and nothing else.
+# -packed-fp32-ops: no packed single-precision arithmetic (some of its forms have given wrong results on this hardware);
+# hipcc's host pass does not know the feature and says so, which is harmless.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fvisibility=hidden",
-         "-Wall", "-Wno-unused-result"]
+         "-Wall", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def hipcc():

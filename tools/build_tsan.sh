@@ -8,7 +8,7 @@ RT=/opt/rocm/lib/llvm/lib/clang/22/lib/linux/libclang_rt.tsan-x86_64.so
 if [ "$1" = "--rt" ]; then echo $RT; exit 0; fi
 set -e
 cd "$(dirname "$0")/../pybgmm_amd/csrc"
-FLAGS="--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC -ffp-contract=off -fvisibility=hidden -fsanitize=thread -Wno-option-ignored"
+FLAGS="--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC -ffp-contract=off -fvisibility=hidden -fsanitize=thread -Wno-option-ignored -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p _obj
 for f in api_context api_inputs api_perm api_sweep api_group api_comm; do
   hipcc $FLAGS -c $f.hip -o _obj/${f}_tsan.o &

@@ -7,7 +7,7 @@ NAME=$1; shift
 FILE=${FILE:-kernels_home.hip}
 BASE=${FILE%.hip}
 cd "$(dirname "$0")/../pybgmm_amd/csrc"
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fvisibility=hidden"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fvisibility=hidden -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p _obj
 hipcc $FLAGS "$@" -c $FILE -o _obj/${BASE}_$NAME.o
 OBJS=$(ls _obj/*.hip.o | grep -v $FILE.o)
