@@ -1,7 +1,7 @@
 """
-Build libbgmm_hip.so (hipcc, gfx950 only) in-tree next to its sources.
+Build libbgmm_hip.so and libbgmm_ops.so (hipcc, gfx950 only) in-tree next to their sources.
 
-The shared object is git-ignored but travels to the GPU box with the gpurun
+The shared objects are git-ignored but travel to the GPU box with the gpurun
 snapshot.  ``build()`` is idempotent: it recompiles only sources newer than
 their objects.
 """
@@ -17,8 +17,15 @@ LIB = os.path.join(HERE, "libbgmm_hip.so")
 SOURCES = ["api_context.hip", "api_inputs.hip", "api_perm.hip", "api_sweep.hip", "api_group.hip", "api_comm.hip", "kernels_state.hip", "kernels_score.hip", "kernels_prune.hip", "kernels_choice.hip",
            "kernels_resolve.hip", "kernels_rng.hip", "kernels_seq.hip", "kernels_gram.hip", "kernels_home.hip", "kernels_safe.hip",
            "kernels_perm.hip", "kernels_resid.hip"]
+INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 # every header next to the sources + the public one: editing any of them rebuilds every object
-HEADERS = sorted(glob.glob(os.path.join(CSRC, "*.h"))) + [os.path.join(os.path.dirname(HERE), "include", "bgmm.h")]
+HEADERS = sorted(h for h in glob.glob(os.path.join(CSRC, "*.h")) if not os.path.basename(h).startswith("ops_")) + [os.path.join(INCLUDE, "bgmm.h")]
+# the operators on torch tensors (pybgmm_amd.ops): a library of its own, because it has to bind to the HIP runtime that
+# torch brings, while libbgmm_hip.so links the system's (a process may hold both)
+OPS_LIB = os.path.join(HERE, "libbgmm_ops.so")
+OPS_SOURCES = ["ops_common.hip", "ops_groups.hip", "ops_products.hip", "ops_products_f64.hip", "ops_products_f32.hip",
+               "ops_products_f16.hip", "ops_products_bf16.hip", "ops_route.hip", "ops_verify.hip"]
+OPS_HEADERS = sorted(glob.glob(os.path.join(CSRC, "ops_*.h"))) + [os.path.join(INCLUDE, "bgmm_ops.h")]
 # -ffp-contract=off: the sufficient-statistics updates must round product and sum
 # separately (bit-identical m / S to the reference); hot loops call fma() explicitly.
 # -fvisibility=hidden: the shared object exports the BGMM_API entry points of include/bgmm.h and nothing else.
@@ -43,14 +50,21 @@ def _stale(target, deps):
 
 
 def build(force=False, verbose=False, extra_flags=()):
+    """Both libraries; returns the path of libbgmm_hip.so."""
+    # -no-hip-rt: libbgmm_ops.so does not link a HIP runtime (include/bgmm_ops.h says which one it binds to)
+    _build_one(OPS_LIB, OPS_SOURCES, OPS_HEADERS, ["-no-hip-rt"], force, verbose, extra_flags)
+    return _build_one(LIB, SOURCES, HEADERS, [], force, verbose, extra_flags)
+
+
+def _build_one(lib, sources, headers, link_flags, force, verbose, extra_flags):
     objdir = os.path.join(CSRC, "_obj")
     os.makedirs(objdir, exist_ok=True)
     cc = hipcc()
     jobs = []
-    for src in SOURCES:
+    for src in sources:
         s = os.path.join(CSRC, src)
         o = os.path.join(objdir, src + ".o")
-        if force or _stale(o, [s] + HEADERS):
+        if force or _stale(o, [s] + headers):
             jobs.append([cc] + FLAGS + list(extra_flags) + ["-c", s, "-o", o])
 
     def run(cmd):
@@ -68,10 +82,10 @@ def build(force=False, verbose=False, extra_flags=()):
             for o in outs:
                 if o.strip():
                     print(o)
-    objs = [os.path.join(objdir, s + ".o") for s in SOURCES]
-    if force or jobs or _stale(LIB, objs):
-        run([cc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs)
-    return LIB
+    objs = [os.path.join(objdir, s + ".o") for s in sources]
+    if force or jobs or _stale(lib, objs):
+        run([cc, "--offload-arch=gfx950", "-shared", "-fPIC"] + link_flags + ["-o", lib] + objs)
+    return lib
 
 
 if __name__ == "__main__":

@@ -1,0 +1,59 @@
+// Shared by the operators of libbgmm_ops.so (include/bgmm_ops.h): element types, wave helpers, error reporting.
+#pragma once
+#include "../../include/bgmm_ops.h"
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+typedef long long i64;
+typedef _Float16 f16_t;
+typedef __bf16 bf16_t;
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef double v4d __attribute__((ext_vector_type(4)));
+
+// What an element type accumulates in.
+template <class T> struct Acc { typedef float type; typedef v4f v4; };
+template <> struct Acc<double> { typedef double type; typedef v4d v4; };
+
+// f(a null pointer of the element type's own): the dispatch of the C entry points, whose checks know the four types
+template <class F> int by_type(int dtype, F f) {
+    switch (dtype) {
+    case BGMM_F64: return f((double *)nullptr);
+    case BGMM_F32: return f((float *)nullptr);
+    case BGMM_F16: return f((f16_t *)nullptr);
+    default: return f((bf16_t *)nullptr);
+    }
+}
+
+int ops_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+int ops_launched(const char *what);         // the status of the launch just made
+
+__device__ __forceinline__ int wave_lane() { return threadIdx.x & 63; }
+
+// Lanes of the wave whose `key` (bits 0 .. nbits-1) equals this lane's; inactive lanes are in no group.
+__device__ __forceinline__ unsigned long long wave_match(int key, int nbits, bool active) {
+    unsigned long long m = __ballot(active);
+    for (int b = 0; b < nbits; ++b) {
+        const unsigned long long set = __ballot((key >> b) & 1);
+        m &= ((key >> b) & 1) ? set : ~set;
+    }
+    return m;
+}
+
+// Which bucket tile t belongs to: the last b in 0 .. n-1 with first[b] <= t (first is non-decreasing, first[0] = 0; t is
+// below first[n]).  64 candidates per probe: two probes up to 4096 buckets, three beyond.  Every wave of a workgroup
+// finds the same answer by itself.
+__device__ __forceinline__ int find_bucket(const int *first, int n, int t) {
+    int lo = 0, span = n;
+    while (span > 1) {
+        const int step = (span + 63) >> 6;
+        const int at = lo + wave_lane() * step;
+        const int v = (at < n && wave_lane() * step < span) ? first[at] : 0x7fffffff;
+        const int below = __popcll(__ballot(v <= t));
+        lo += (below - 1) * step;
+        span = step < n - lo ? step : n - lo;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}

@@ -1,0 +1,212 @@
+// Rows grouped by component: a stable counting sort of P labels into K + 1 buckets (bucket K: unassigned rows).
+//
+//   order = argsort(bucket, stable), offsets = exclusive sum of the bucket sizes,
+//   first[l][b] = sum over b' < b of ceil(size(b') / (16 << l))
+//
+// Stable and without atomics across workgroups, so that a grouping is the same every time: the gradients that sum over a
+// group's rows in this order are too.  A wave owns a segment of consecutive rows and a histogram of its own in LDS; the 64
+// rows it looks at together find their equals with one ballot per label bit.
+//
+// Up to kSmall rows one workgroup does everything in one launch (a single served row pays one launch, not three).  Beyond:
+// histograms per segment, an exclusive sum over the segments per bucket, the scatter -- bound by the latency of the
+// segments' dependent LDS steps, not by the 12 P bytes that move.
+#include "ops_common.h"
+
+namespace {
+
+constexpr int kSmall = 8192;            // rows of the one-workgroup form
+constexpr int kWaves = 16;              // its waves
+constexpr int kSmallBuckets = 960;      // its buckets (K + 1): 16 histograms, the sizes and the sums fit 64 KB of LDS
+constexpr int kSegWaves = 4;            // segments (waves) per workgroup of the three-launch form while 4 histograms fit 64 KB
+
+__device__ __forceinline__ int bucket_of(const int64_t *labels, i64 i, int K) {
+    const int64_t z = labels[i];
+    return z >= 0 && z < K ? (int)z : K;
+}
+
+__device__ __forceinline__ int wave_incl_scan(int v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(v, o);
+        if (wave_lane() >= o) v += t;
+    }
+    return v;
+}
+
+// Exclusive sum of f(0 .. n-1) over the whole workgroup, handed to g(b, sum before b); returns the total.  `part` holds one
+// int per wave plus one; ends behind a barrier.
+template <class F, class G>
+__device__ __forceinline__ int block_scan(int n, int *part, F f, G g) {
+    const int nw = blockDim.x >> 6, w = threadIdx.x >> 6;
+    int carry = 0;
+    for (int base = 0; base < n; base += blockDim.x) {
+        const int b = base + threadIdx.x;
+        const int v = b < n ? f(b) : 0;
+        const int incl = wave_incl_scan(v);
+        if (wave_lane() == 63) part[w] = incl;
+        __syncthreads();
+        int before = carry, total = 0;
+        for (int j = 0; j < nw; ++j) {
+            if (j < w) before += part[j];
+            total += part[j];
+        }
+        if (b < n) g(b, before + incl - v);
+        carry += total;
+        __syncthreads();
+    }
+    return carry;
+}
+
+__device__ __forceinline__ void write_level(int level, int K, const int *size_of, int *first, int *part) {
+    int *out = first + (i64)level * (K + 2);
+    const int lg = 4 + level;
+    const int total = block_scan(K + 1, part, [&](int b) { return (int)(((i64)size_of[b] + (1 << lg) - 1) >> lg); },
+                                 [&](int b, int s) { out[b] = s; });
+    if (threadIdx.x == 0) out[K + 1] = total;
+}
+
+// A wave walks rows [lo, hi): cursor[b] moves by the rows of bucket b, write(i, b, place) sees every row's place.
+template <class W>
+__device__ __forceinline__ void walk(const int64_t *labels, i64 lo, i64 hi, int K, int nbits, int *cursor, W write) {
+    const int lane = wave_lane();
+    for (i64 i0 = lo; i0 < hi; i0 += 64) {
+        const i64 i = i0 + lane;
+        const bool on = i < hi;
+        const int b = on ? bucket_of(labels, i, K) : 0;
+        const unsigned long long same = wave_match(b, nbits, on);
+        const int leader = on ? __ffsll((unsigned long long)same) - 1 : lane;
+        int at = 0;
+        if (on && leader == lane) at = atomicAdd(&cursor[b], __popcll(same));       // (LDS, this wave's own counters)
+        at = __shfl(at, leader);
+        if (on) write(i, b, at + __popcll(same & ((1ull << lane) - 1)));
+    }
+}
+
+__global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels, int P, int K, int nbits, int *bucket, int *order,
+                                                           int *offsets, int *first) {
+    extern __shared__ int lds[];
+    int *hist = lds;                          // [kWaves][K + 1]
+    int *sizes = hist + kWaves * (K + 1);     // [K + 1]
+    int *part = sizes + K + 1;                // [kWaves]
+    const int B = K + 1, w = threadIdx.x >> 6;
+    for (int j = threadIdx.x; j < kWaves * B; j += blockDim.x) hist[j] = 0;
+    __syncthreads();
+    const int per = ((P + kWaves - 1) / kWaves + 63) & ~63;
+    const int lo = w * per < P ? w * per : P, hi = lo + per < P ? lo + per : P;
+    walk(labels, lo, hi, K, nbits, hist + w * B, [&](i64 i, int b, int) { bucket[i] = b; });
+    __syncthreads();
+    for (int b = threadIdx.x; b < B; b += blockDim.x) {
+        int s = 0;
+        for (int j = 0; j < kWaves; ++j) {
+            const int n = hist[j * B + b];
+            hist[j * B + b] = s;
+            s += n;
+        }
+        sizes[b] = s;
+    }
+    __syncthreads();
+    block_scan(B, part, [&](int b) { return sizes[b]; },
+               [&](int b, int s) {
+                   offsets[b] = s;
+                   for (int j = 0; j < kWaves; ++j) hist[j * B + b] += s;
+               });
+    if (threadIdx.x == 0) offsets[B] = P;
+    walk(labels, lo, hi, K, nbits, hist + w * B, [&](i64 i, int, int at) { order[at] = (int)i; });
+    for (int l = 0; l < BGMM_OPS_LEVELS; ++l) write_level(l, K, sizes, first, part);
+}
+
+__global__ void group_count(const int64_t *labels, i64 P, int K, int nbits, int seg, int nseg, int *bucket, int *counts) {
+    extern __shared__ int lds[];
+    const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * (blockDim.x >> 6) + w;
+    int *hist = lds + w * B;
+    for (int b = wave_lane(); b < B; b += 64) hist[b] = 0;
+    __syncthreads();
+    const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
+    walk(labels, lo, hi, K, nbits, hist, [&](i64 i, int b, int) { bucket[i] = b; });
+    __syncthreads();
+    if (s < nseg)
+        for (int b = wave_lane(); b < B; b += 64) counts[(i64)s * B + b] = hist[b];
+}
+
+// One wave per bucket: counts[.][b] becomes the exclusive sum over the segments, sizes[b] the total.
+__global__ void group_columns(int *counts, int nseg, int B, int *sizes) {
+    const int b = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    if (b >= B) return;
+    int carry = 0;
+    for (int s0 = 0; s0 < nseg; s0 += 64) {
+        const int s = s0 + wave_lane();
+        const int v = s < nseg ? counts[(i64)s * B + b] : 0;
+        const int incl = wave_incl_scan(v);
+        if (s < nseg) counts[(i64)s * B + b] = carry + incl - v;
+        carry += __shfl(incl, 63);
+    }
+    if (wave_lane() == 0) sizes[b] = carry;
+}
+
+__global__ void group_scatter(const int64_t *labels, i64 P, int K, int nbits, int seg, int nseg, const int *counts, const int *sizes,
+                              int *order, int *offsets, int *first) {
+    extern __shared__ int lds[];
+    const int nw = blockDim.x >> 6;
+    const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * nw + w;
+    int *start = lds + nw * B, *part = start + B;
+    block_scan(B, part, [&](int b) { return sizes[b]; }, [&](int b, int v) { start[b] = v; });
+    int *cursor = lds + w * B;
+    if (s < nseg)
+        for (int b = wave_lane(); b < B; b += 64) cursor[b] = start[b] + counts[(i64)s * B + b];
+    __syncthreads();
+    const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
+    walk(labels, lo, hi, K, nbits, cursor, [&](i64 i, int, int at) { order[at] = (int)i; });
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= B; b += blockDim.x) offsets[b] = b < B ? start[b] : (int)P;
+    for (int l = blockIdx.x; l < BGMM_OPS_LEVELS; l += gridDim.x) write_level(l, K, sizes, first, part);
+}
+
+struct Split { int seg, nseg, waves; };
+
+// Rows per segment: at least 512, and enough that the segments' histograms hold no more counters than there are rows.
+Split split_of(i64 P, int K) {
+    Split s;
+    i64 seg = K + 1 > 512 ? K + 1 : 512;
+    seg = (seg + 63) & ~(i64)63;
+    s.seg = (int)seg;
+    s.nseg = (int)((P + seg - 1) / seg);
+    s.waves = (K + 1) * kSegWaves <= 12 * 1024 ? kSegWaves : 1;      // (LDS: one histogram per wave and the buckets' starts, 64 KB)
+    return s;
+}
+
+bool small_form(i64 P, int K) { return P <= kSmall && K + 1 <= kSmallBuckets; }
+
+}  // namespace
+
+extern "C" int64_t bgmm_group_rows_ws(int64_t P, int32_t K) {
+    if (P < 0 || K < 1 || small_form(P, K)) return 0;
+    const Split s = split_of(P, K);
+    return 4 * ((int64_t)s.nseg + 1) * (K + 1);
+}
+
+extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int32_t *bucket, int32_t *order, int32_t *offsets,
+                               int32_t *first, void *ws, int64_t ws_bytes, void *stream) {
+    if (P < 0 || P > 0x7fffffff - 65536) return ops_fail(BGMM_OPS_EINVAL, "group_rows: P = %lld rows (0 .. 2^31 - 65537)", (long long)P);
+    if (K < 1) return ops_fail(BGMM_OPS_EINVAL, "group_rows: K = %d components", K);
+    if (K > BGMM_OPS_MAX_COMPONENTS) return ops_fail(BGMM_OPS_EUNSUPPORTED, "group_rows: K = %d components (at most %d)", K, BGMM_OPS_MAX_COMPONENTS);
+    if (!offsets || !first || (P > 0 && (!labels || !bucket || !order))) return ops_fail(BGMM_OPS_EINVAL, "group_rows: a null pointer");
+    if (ws_bytes < bgmm_group_rows_ws(P, K) || (bgmm_group_rows_ws(P, K) > 0 && !ws)) return ops_fail(BGMM_OPS_EINVAL, "group_rows: workspace too small");
+    hipStream_t st = (hipStream_t)stream;
+    const int B = K + 1;
+    int nbits = 1;
+    while ((1 << nbits) < B) ++nbits;
+    if (small_form(P, K)) {
+        const size_t lds = sizeof(int) * ((size_t)(kWaves + 1) * B + kWaves);
+        group_small<<<1, 64 * kWaves, lds, st>>>(labels, (int)P, K, nbits, bucket, order, offsets, first);
+        return ops_launched("group_rows");
+    }
+    const Split s = split_of(P, K);
+    int *counts = (int *)ws, *sizes = counts + (size_t)s.nseg * B;
+    // (P = 0 with many components: no segment, but the sums over nothing and the empty offsets are still written)
+    const int blocks = s.nseg > 0 ? (s.nseg + s.waves - 1) / s.waves : 1;
+    group_count<<<blocks, 64 * s.waves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, nbits, s.seg, s.nseg, bucket, counts);
+    group_columns<<<(B + 3) / 4, 256, 0, st>>>(counts, s.nseg, B, sizes);
+    group_scatter<<<blocks, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + 16), st>>>(labels, P, K, nbits, s.seg, s.nseg, counts, sizes,
+                                                                                                order, offsets, first);
+    return ops_launched("group_rows");
+}

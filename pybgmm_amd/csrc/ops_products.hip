@@ -1,0 +1,168 @@
+// C entry points of the products with a component's own matrix: checks, tile sizes, splits, the dispatch on the element type.
+#include "ops_products.h"
+
+namespace {
+
+int size_of(int dtype) { return dtype == BGMM_F64 ? 8 : dtype == BGMM_F32 ? 4 : 2; }
+int acc_size(int dtype) { return dtype == BGMM_F64 ? 8 : 4; }
+bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+i64 at_most(i64 a, i64 b) { return a < b ? a : b; }
+
+// Rows that share a component on average: up to 16 a tile of 16 rows, whose workgroup streams the weights with little else.
+bool small_tiles(i64 P, int K) { return P <= 16 * (i64)K; }
+int rows_tile(i64 P, int K) { return small_tiles(P, K) ? 16 : 128; }
+i64 rows_tiles(i64 P, int K, int tile) { return P / tile + at_most(K, P) + 1; }      // at most, the rows of no component included
+int cols_tile(bool small, int ndim) { return small ? 128 : ndim <= 16 ? 16 : ndim <= 64 ? 64 : 128; }
+
+// Chunk of rows of the weights' gradient (a level of the grouping): as long as about a thousand workgroups remain, 1024 ..
+// 32768 rows; a chunk leaves a tile of partial sums, which 1024 rows outweigh.
+int weight_level(i64 P, int K, int idim, int odim) {
+    const int t = idim <= 16 && odim <= 16 ? 16 : idim <= 64 && odim <= 64 ? 64 : 128;
+    const i64 tiles = (i64)((idim + t - 1) / t) * ((odim + t - 1) / t);
+    int level = 6;
+    while (level < BGMM_OPS_LEVELS - 1 && P / (16 << (level + 1)) * tiles >= 1024) ++level;
+    return level;
+}
+
+int check(const char *what, int dtype, i64 P, int K, int a, int b) {
+    if (dtype < BGMM_F64 || dtype > BGMM_BF16) return ops_fail(BGMM_OPS_EINVAL, "%s: element type %d", what, dtype);
+    if (P < 0 || P > 0x7fffffff - 65536 || K < 1 || a < 1 || b < 1)
+        return ops_fail(BGMM_OPS_EINVAL, "%s: P = %lld, K = %d, dimensions %d and %d", what, (long long)P, K, a, b);
+    if (K > BGMM_OPS_MAX_COMPONENTS) return ops_fail(BGMM_OPS_EUNSUPPORTED, "%s: K = %d components (at most %d)", what, K, BGMM_OPS_MAX_COMPONENTS);
+    return BGMM_OPS_OK;
+}
+
+}  // namespace
+
+extern "C" int bgmm_rows_product_splits(int32_t dtype, int64_t P, int32_t K, int32_t kdim, int32_t ndim) {
+    if (check("rows_product_splits", dtype, P, K, kdim, ndim) != BGMM_OPS_OK || P == 0) return 1;
+    const bool small = small_tiles(P, K);
+    const int bn = cols_tile(small, ndim);
+    const i64 groups = rows_tiles(P, K, rows_tile(P, K)) * ((ndim + bn - 1) / bn);
+    const int steps = (kdim * size_of(dtype) + kStepBytes - 1) / kStepBytes;
+    // (256 compute units: fill them twice over, but leave a part four steps to do)
+    i64 s = at_most(512 / (groups > 0 ? groups : 1), steps / 4);
+    return (int)(s < 1 ? 1 : at_most(s, 16));
+}
+
+extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_stride, int32_t in_div, const void *w, int64_t w_component,
+                                 int64_t w_row, int32_t kcontig, const void *bias, int64_t bias_row, const void *gates, void *out,
+                                 int64_t out_stride, void *ws, int32_t splits, int64_t P, int32_t K, int32_t kdim, int32_t ndim,
+                                 const int32_t *order, const int32_t *offsets, const int32_t *first, void *stream) {
+    const int rc = check("rows_product", dtype, P, K, kdim, ndim);
+    if (rc) return rc;
+    if (P == 0) return BGMM_OPS_OK;
+    if (!in || !w || !order || !offsets || !first || !out == !ws) return ops_fail(BGMM_OPS_EINVAL, "rows_product: a null pointer (and exactly one of out, ws)");
+    if (in_div < 1 || splits < 1 || (out && splits != 1) || in_stride < 0 || out_stride < 0)
+        return ops_fail(BGMM_OPS_EINVAL, "rows_product: in_div %d, splits %d, strides %lld %lld", in_div, splits, (long long)in_stride, (long long)out_stride);
+    const int S = size_of(dtype), E = 16 / S;
+    const bool small = small_tiles(P, K);
+    const int bm = rows_tile(P, K), bn = cols_tile(small, ndim), level = small ? 0 : 3;
+    RowsArgs a;
+    a.bucket_first = first + (size_t)level * (K + 2);
+    a.offsets = offsets;
+    a.order = order;
+    a.K = K;
+    a.in = in;
+    a.in_stride = in_stride;
+    a.in_div = in_div;
+    a.w = w;
+    a.w_component = w_component;
+    a.w_row = w_row;
+    a.bias = bias;
+    a.bias_row = bias_row;
+    a.gates = gates;
+    a.out = out;
+    a.out_stride = out_stride;
+    a.ws = ws;
+    a.P = P;
+    a.kdim = kdim;
+    a.ndim = ndim;
+    a.splits = splits;
+    a.n_tiles = (ndim + bn - 1) / bn;
+    a.out_vec = ndim % 4 == 0 && (ws ? aligned(ws, 16) : out_stride % 4 == 0 && aligned(out, S == 2 ? 8 : 16));
+    const bool vec = aligned(in, 16) && aligned(w, 16) && in_stride % E == 0 && w_component % E == 0 && w_row % E == 0 && kdim % E == 0 &&
+                     (kcontig || ndim % E == 0);
+    const i64 blocks = (rows_tiles(P, K, bm) * a.n_tiles * splits + 7) & ~(i64)7;
+    if (blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "rows_product: %lld tiles", (long long)blocks);
+    return by_type(dtype, [&](auto *t) { return launch_rows<std::remove_pointer_t<decltype(t)>>(a, kcontig != 0, vec, small, blocks, (hipStream_t)stream); });
+}
+
+extern "C" int64_t bgmm_weight_product_ws(int32_t dtype, int64_t P, int32_t K, int32_t idim, int32_t odim) {
+    if (check("weight_product_ws", dtype, P, K, idim, odim) != BGMM_OPS_OK) return 0;
+    const i64 rows = (i64)16 << weight_level(P, K, idim, odim);
+    if (P <= rows) return 0;
+    return (2 * P / rows + 2) * ((i64)idim * odim + odim) * acc_size(dtype);
+}
+
+extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_stride, int32_t in_div, const void *d, int64_t d_stride,
+                                   int32_t d_div, const void *gates, void *dw, void *db, void *ws, int64_t ws_bytes, int64_t P, int32_t K,
+                                   int32_t idim, int32_t odim, const int32_t *order, const int32_t *offsets, const int32_t *first, void *stream) {
+    const int rc = check("weight_product", dtype, P, K, idim, odim);
+    if (rc) return rc;
+    if (!dw && !db) return BGMM_OPS_OK;
+    if (!offsets || !first || (P > 0 && (!in || !d || !order))) return ops_fail(BGMM_OPS_EINVAL, "weight_product: a null pointer");
+    if (in_div < 1 || d_div < 1 || in_stride < 0 || d_stride < 0) return ops_fail(BGMM_OPS_EINVAL, "weight_product: divisors %d %d, strides %lld %lld", in_div, d_div, (long long)in_stride, (long long)d_stride);
+    if (ws_bytes < bgmm_weight_product_ws(dtype, P, K, idim, odim) || (ws_bytes > 0 && (!ws || !aligned(ws, 16))))
+        return ops_fail(BGMM_OPS_EINVAL, "weight_product: workspace of %lld bytes", (long long)ws_bytes);
+    if (K > 65535) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: K = %d", K);
+    const int S = size_of(dtype), E = 16 / S;
+    const int t = idim <= 16 && odim <= 16 ? 16 : idim <= 64 && odim <= 64 ? 64 : 128;
+    WeightArgs a;
+    a.level = weight_level(P, K, idim, odim);
+    a.bucket_first = first + (size_t)a.level * (K + 2);
+    a.offsets = offsets;
+    a.order = order;
+    a.K = K;
+    a.in = in;
+    a.in_stride = in_stride;
+    a.in_div = in_div;
+    a.d = d;
+    a.d_stride = d_stride;
+    a.d_div = d_div;
+    a.gates = gates;
+    a.dw = dw;
+    a.db = db;
+    a.ws = ws;
+    a.idim = idim;
+    a.odim = odim;
+    a.i_tiles = (idim + t - 1) / t;
+    a.o_tiles = (odim + t - 1) / t;
+    const bool vec = aligned(in, 16) && aligned(d, 16) && in_stride % E == 0 && d_stride % E == 0 && idim % E == 0 && odim % E == 0;
+    const i64 blocks = P == 0 ? 0 : ((P / ((i64)16 << a.level) + at_most(K, P)) * a.i_tiles * a.o_tiles + 7) & ~(i64)7;
+    if (blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: %lld tiles", (long long)blocks);
+    return by_type(dtype, [&](auto *t_) { return launch_weight<std::remove_pointer_t<decltype(t_)>>(a, vec, blocks, (hipStream_t)stream); });
+}
+
+extern "C" int bgmm_combine(int32_t dtype, const void *ws, int32_t splits, int64_t rows, int32_t k, int32_t K, const int32_t *bucket,
+                            const void *gates, void *out, int64_t out_stride, int32_t dim, void *dgates, const void *in, int64_t in_stride,
+                            const void *bias, int64_t bias_row, const void *d, int64_t d_stride, int32_t d_div, int32_t ddim, void *stream) {
+    const int rc = check("combine", dtype, rows, K, dim, 1);
+    if (rc) return rc;
+    if (k < 1 || k > BGMM_OPS_MAX_CHOSEN || splits < 1) return ops_fail(BGMM_OPS_EINVAL, "combine: k = %d (1 .. %d), splits %d", k, BGMM_OPS_MAX_CHOSEN, splits);
+    if (rows == 0) return BGMM_OPS_OK;
+    if (!ws || !bucket || (!out && !dgates) || (dgates && (!gates || !in)) || (dgates && bias && (!d || d_div < 1 || ddim < 1)))
+        return ops_fail(BGMM_OPS_EINVAL, "combine: a null pointer");
+    CombineArgs a;
+    a.bucket = bucket;
+    a.K = K;
+    a.k = k;
+    a.splits = splits;
+    a.rows = rows;
+    a.P = rows * k;
+    a.ws = ws;
+    a.gates = gates;
+    a.out = out;
+    a.out_stride = out_stride;
+    a.dim = dim;
+    a.dgates = dgates;
+    a.in = in;
+    a.in_stride = in_stride;
+    a.bias = bias;
+    a.bias_row = bias_row;
+    a.d = d;
+    a.d_stride = d_stride;
+    a.d_div = d_div < 1 ? 1 : d_div;
+    a.ddim = ddim;
+    return by_type(dtype, [&](auto *t) { return launch_combine<std::remove_pointer_t<decltype(t)>>(a, (hipStream_t)stream); });
+}

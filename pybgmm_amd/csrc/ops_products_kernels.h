@@ -1,0 +1,454 @@
+// The kernels behind ops_products.h, instantiated once per element type (ops_products_{f64,f32,f16,bf16}.hip).
+#pragma once
+#include "ops_products.h"
+
+template <class T> __device__ __forceinline__ float as_f32(T v) { return (float)v; }
+
+// Four consecutive elements of an output row from an accumulator; `avail` of them exist.
+template <class T, class V> __device__ __forceinline__ void store4(T *p, const V &v, int avail, bool vec) {
+    if (vec) {
+        struct alignas(sizeof(T) * 4 < 16 ? sizeof(T) * 4 : 16) Four { T e[4]; } o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.e[i] = (T)v[i];
+        if (avail > 0) *(Four *)p = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < avail) p[i] = (T)v[i];
+    }
+}
+
+template <class T, bool KCONTIG, bool VEC, int BM, int BN, int WN, int WM>
+__global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
+    typedef typename Acc<T>::type A;
+    typedef typename Acc<T>::v4 A4;
+    constexpr int FA = BN / WN / 16, FB = BM / WM / 16;
+    constexpr int XP = (BM + 31) / 32, WP = (BN + 31) / 32;        // granules a thread moves per step
+    __shared__ __attribute__((aligned(128))) char lds[2][(BM + BN) * kStepBytes];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave % WN, wm = wave / WN;
+
+    // ---- which tile: component by component, blocks of eight row tiles, within a block every column tile in turn
+    const int tiles = a.bucket_first[a.ws ? a.K : a.K + 1];
+    i64 id = die_order((i64)tiles * a.n_tiles * a.splits);
+    if (id < 0) return;
+    const int split = (int)(id % a.splits);
+    id /= a.splits;
+    const int e = find_bucket(a.bucket_first, a.K + 1, (int)(id / a.n_tiles));
+    const int tile0 = a.bucket_first[e], my_tiles = a.bucket_first[e + 1] - tile0;
+    int local = (int)(id - (i64)tile0 * a.n_tiles);
+    constexpr int kBlock = 8;
+    const int blk = local / (kBlock * a.n_tiles);
+    local -= blk * kBlock * a.n_tiles;
+    const int in_block = my_tiles - blk * kBlock < kBlock ? my_tiles - blk * kBlock : kBlock;
+    const int nt = local / in_block, rt = blk * kBlock + local % in_block;
+    const int row0 = a.offsets[e] + rt * BM, left = a.offsets[e + 1] - row0, n_rows = left < BM ? left : BM;
+    const int *list = a.order + row0;
+    const int n0 = nt * BN;
+
+    if (e == a.K) {                 // rows of no component: zeros
+        T *out = (T *)a.out;
+        const int n = a.ndim - n0 < BN ? a.ndim - n0 : BN;
+        for (int j = tid; j < n_rows * n; j += 256) out[(i64)list[j / n] * a.out_stride + n0 + j % n] = (T)0.0f;
+        return;
+    }
+
+    // ---- contraction range of this split, in whole steps
+    const int steps_all = (a.kdim + kStep<T> - 1) / kStep<T>;
+    const int s_lo = (int)((i64)steps_all * split / a.splits), s_hi = (int)((i64)steps_all * (split + 1) / a.splits);
+    const int k_end = s_hi * kStep<T> < a.kdim ? s_hi * kStep<T> : a.kdim;
+
+    const T *xrow[XP];
+#pragma unroll
+    for (int p = 0; p < XP; ++p) {
+        int r = (tid >> 3) + p * 32;
+        r = r < n_rows ? r : n_rows - 1;                    // (a row twice rather than a branch: its results are not stored)
+        xrow[p] = (const T *)a.in + (i64)((unsigned)list[r] / (unsigned)a.in_div) * a.in_stride;
+    }
+    const T *w = (const T *)a.w + (i64)e * a.w_component;
+    typedef MTile<T, BN> WTile;
+    Granule gx[XP], gw[WP];
+    const auto fetch = [&](int k0) {
+        const int kk = k0 + (tid & 7) * kGran<T>;
+#pragma unroll
+        for (int p = 0; p < XP; ++p)
+            if (BM >= 32 || tid < BM * 8) gx[p] = load_granule<T, VEC>(xrow[p] + kk, k_end - kk);
+#pragma unroll
+        for (int p = 0; p < WP; ++p) {
+            if (BN < 32 && tid >= BN * 8) continue;
+            if (KCONTIG) {
+                const int n = n0 + (tid >> 3) + p * 32;
+                gw[p] = load_granule<T, VEC>(w + (i64)n * a.w_row + kk, n < a.ndim ? k_end - kk : 0);
+            } else {
+                const int g = tid + p * 256, k = k0 + g / WTile::kPerRow, n = n0 + (g % WTile::kPerRow) * kGran<T>;
+                gw[p] = load_granule<T, VEC>(w + (i64)k * a.w_row + n, k < k_end ? a.ndim - n : 0);
+            }
+        }
+    };
+    const auto put = [&](char *buf) {
+#pragma unroll
+        for (int p = 0; p < XP; ++p)
+            if (BM >= 32 || tid < BM * 8) *(v4i *)(buf + KTile<T>::at((tid >> 3) + p * 32, tid & 7)) = gx[p].raw;
+        char *wb = buf + BM * kStepBytes;
+#pragma unroll
+        for (int p = 0; p < WP; ++p) {
+            if (BN < 32 && tid >= BN * 8) continue;
+            if (KCONTIG) {
+                *(v4i *)(wb + KTile<T>::at((tid >> 3) + p * 32, tid & 7)) = gw[p].raw;
+            } else {
+                const int g = tid + p * 256;
+                *(v4i *)(wb + WTile::at(g / WTile::kPerRow, g % WTile::kPerRow)) = gw[p].raw;
+            }
+        }
+    };
+
+    A4 acc[FA][FB];
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+        for (int j = 0; j < FB; ++j) acc[i][j] = (A4){0, 0, 0, 0};
+
+    if (s_lo < s_hi) {
+        fetch(s_lo * kStep<T>);
+        put(lds[0]);
+    }
+    __syncthreads();
+    for (int s = s_lo; s < s_hi; ++s) {
+        const char *buf = lds[(s - s_lo) & 1], *wb = buf + BM * kStepBytes;
+        if (s + 1 < s_hi) fetch((s + 1) * kStep<T>);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks && s * kStep<T> + kStep<T> / 2 >= k_end) break;
+            Granule fa[FA], fb[FB];
+#pragma unroll
+            for (int i = 0; i < FA; ++i) {
+                const int block = wn * FA * 16 + i * 16;
+                fa[i] = KCONTIG ? KTile<T>::template read<true>(wb, block, ks) : WTile::template read<true>(wb, block, ks);
+            }
+#pragma unroll
+            for (int j = 0; j < FB; ++j) fb[j] = KTile<T>::template read<false>(buf, wm * FB * 16 + j * 16, ks);
+#pragma unroll
+            for (int i = 0; i < FA; ++i)
+#pragma unroll
+                for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j]);
+        }
+        if (s + 1 < s_hi) put(lds[(s + 1 - s_lo) & 1]);
+        __syncthreads();
+    }
+
+    // ---- results: lane l has elements 4 (l / 16) .. + 3 of the block's columns for row l % 16 of the block's rows
+    const T *bias = a.bias && split == 0 ? (const T *)a.bias + (i64)e * a.bias_row : nullptr;
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+        const int n = n0 + (wn * FA + i) * 16 + (lane >> 4) * 4, avail = a.ndim - n;
+        A4 b = {0, 0, 0, 0};
+        if (bias) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (c < avail) b[c] = (A)bias[n + c];
+        }
+#pragma unroll
+        for (int j = 0; j < FB; ++j) {
+            const int m = (wm * FB + j) * 16 + (lane & 15);
+            if (m >= n_rows) continue;
+            const i64 p = list[m];
+            A4 v = acc[i][j] + b;
+            if (a.ws) {
+                store4((A *)a.ws + ((i64)split * a.P + p) * a.ndim + n, v, avail, a.out_vec);
+            } else {
+                if (a.gates) v *= ((const A *)a.gates)[p];
+                store4((T *)a.out + p * a.out_stride + n, v, avail, a.out_vec);
+            }
+        }
+    }
+}
+
+// dW: the rows of a chunk are the contraction, both operands have it outermost (MTile).  Half precision: g d is rounded to
+// the operand type before the product (like the operands themselves), its column sums for db are not.
+template <class T, bool VEC, int BI, int BO, int WO, int WI>
+__global__ __launch_bounds__(256) void weight_kernel(WeightArgs a) {
+    typedef typename Acc<T>::type A;
+    typedef typename Acc<T>::v4 A4;
+    constexpr int FA = BO / WO / 16, FB = BI / WI / 16;
+    constexpr int IP = (BI + 31) / 32, OP = (BO + 31) / 32;
+    typedef MTile<T, BI> ITile;
+    typedef MTile<T, BO> OTile;
+    __shared__ __attribute__((aligned(128))) char lds[2][(BI + BO) * kStepBytes];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wo = wave % WO, wi = wave / WO;
+    const i64 out_tiles = (i64)a.i_tiles * a.o_tiles;
+    const i64 id = die_order((i64)a.bucket_first[a.K] * out_tiles);
+    if (id < 0) return;
+    const int chunk = (int)(id / out_tiles), tile = (int)(id % out_tiles);
+    const int e = find_bucket(a.bucket_first, a.K, chunk);
+    const int c = chunk - a.bucket_first[e], chunks = a.bucket_first[e + 1] - a.bucket_first[e];
+    const int rows_per = 16 << a.level;
+    const int row0 = a.offsets[e] + c * rows_per, left = a.offsets[e + 1] - row0, n_rows = left < rows_per ? left : rows_per;
+    const int *list = a.order + row0;
+    const int i0 = (tile % a.i_tiles) * BI, o0 = (tile / a.i_tiles) * BO;
+    const A *gates = (const A *)a.gates;
+    const bool want_db = a.db && i0 == 0;
+
+    Granule gi[IP], go[OP];
+    A dsum[OP][kGran<T>];
+#pragma unroll
+    for (int p = 0; p < OP; ++p)
+#pragma unroll
+        for (int j = 0; j < kGran<T>; ++j) dsum[p][j] = 0;
+    const auto fetch = [&](int r0) {
+#pragma unroll
+        for (int p = 0; p < IP; ++p) {
+            if (BI < 32 && tid >= BI * 8) continue;
+            const int g = tid + p * 256, r = r0 + g / ITile::kPerRow, n = i0 + (g % ITile::kPerRow) * kGran<T>;
+            const int rr = r < n_rows ? r : n_rows - 1;
+            gi[p] = load_granule<T, VEC>((const T *)a.in + (i64)((unsigned)list[rr] / (unsigned)a.in_div) * a.in_stride + n,
+                                         r < n_rows ? a.idim - n : 0);
+        }
+#pragma unroll
+        for (int p = 0; p < OP; ++p) {
+            if (BO < 32 && tid >= BO * 8) continue;
+            const int g = tid + p * 256, r = r0 + g / OTile::kPerRow, n = o0 + (g % OTile::kPerRow) * kGran<T>;
+            const int rr = r < n_rows ? r : n_rows - 1;
+            const int pair = list[rr];
+            go[p] = load_granule<T, VEC>((const T *)a.d + (i64)((unsigned)pair / (unsigned)a.d_div) * a.d_stride + n,
+                                         r < n_rows ? a.odim - n : 0);
+            if (gates) {
+                const A gate = gates[pair];
+                T *el = Elems<T>::of(go[p]);
+#pragma unroll
+                for (int j = 0; j < kGran<T>; ++j) {
+                    const A v = r < n_rows ? (A)el[j] * gate : (A)0;
+                    dsum[p][j] += v;
+                    el[j] = (T)v;
+                }
+            } else if (want_db) {
+                T *el = Elems<T>::of(go[p]);
+#pragma unroll
+                for (int j = 0; j < kGran<T>; ++j) dsum[p][j] += (A)el[j];
+            }
+        }
+    };
+    const auto put = [&](char *buf) {
+#pragma unroll
+        for (int p = 0; p < IP; ++p) {
+            if (BI < 32 && tid >= BI * 8) continue;
+            const int g = tid + p * 256;
+            *(v4i *)(buf + ITile::at(g / ITile::kPerRow, g % ITile::kPerRow)) = gi[p].raw;
+        }
+#pragma unroll
+        for (int p = 0; p < OP; ++p) {
+            if (BO < 32 && tid >= BO * 8) continue;
+            const int g = tid + p * 256;
+            *(v4i *)(buf + BI * kStepBytes + OTile::at(g / OTile::kPerRow, g % OTile::kPerRow)) = go[p].raw;
+        }
+    };
+
+    A4 acc[FA][FB];
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+        for (int j = 0; j < FB; ++j) acc[i][j] = (A4){0, 0, 0, 0};
+    fetch(0);
+    put(lds[0]);
+    __syncthreads();
+    const int steps = (n_rows + kStep<T> - 1) / kStep<T>;
+    for (int s = 0; s < steps; ++s) {
+        const char *buf = lds[s & 1];
+        if (s + 1 < steps) fetch((s + 1) * kStep<T>);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if (WO * WI < 4 && wave >= WO * WI) break;          // (a tile too small for four waves: the others only move data)
+            Granule fa[FA], fb[FB];
+#pragma unroll
+            for (int i = 0; i < FA; ++i) fa[i] = OTile::template read<true>(buf + BI * kStepBytes, (wo * FA + i) * 16, ks);
+#pragma unroll
+            for (int j = 0; j < FB; ++j) fb[j] = ITile::template read<false>(buf, (wi * FB + j) * 16, ks);
+#pragma unroll
+            for (int i = 0; i < FA; ++i)
+#pragma unroll
+                for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j]);
+        }
+        if (s + 1 < steps) put(lds[(s + 1) & 1]);
+        __syncthreads();
+    }
+
+    // a component with one chunk is finished here; several leave partial sums, added in the chunks' order by weight_reduce
+    A *slot = nullptr;
+    if (chunks > 1) slot = (A *)a.ws + ((((i64)a.offsets[e] * 2) >> (4 + a.level)) + c) * ((i64)a.idim * a.odim + a.odim);
+    const bool o_vec = (a.odim & 3) == 0;
+    if (a.dw && wave < WO * WI) {
+#pragma unroll
+        for (int i = 0; i < FA; ++i) {
+            const int o = o0 + (wo * FA + i) * 16 + (lane >> 4) * 4;
+#pragma unroll
+            for (int j = 0; j < FB; ++j) {
+                const int r = i0 + (wi * FB + j) * 16 + (lane & 15);
+                if (r >= a.idim) continue;
+                if (slot) store4(slot + (i64)r * a.odim + o, acc[i][j], a.odim - o, o_vec);
+                else store4((T *)a.dw + ((i64)e * a.idim + r) * a.odim + o, acc[i][j], a.odim - o, o_vec);
+            }
+        }
+    }
+    if (!want_db) return;
+    // column sums: a thread has those of its granule's columns over its own rows; the threads of a column add up in order
+    A *sums = (A *)lds;                       // [rows of a pass][BO]
+    constexpr int kRowsPass = BO < 32 ? BO * 8 / OTile::kPerRow : 256 / OTile::kPerRow;
+    __syncthreads();
+    if (BO >= 32 || tid < BO * 8) {
+#pragma unroll
+        for (int j = 0; j < kGran<T>; ++j) {
+            A v = 0;
+#pragma unroll
+            for (int p = 0; p < OP; ++p) v += dsum[p][j];
+            sums[(tid / OTile::kPerRow) * BO + (tid % OTile::kPerRow) * kGran<T> + j] = v;
+        }
+    }
+    __syncthreads();
+    for (int n = tid; n < BO && o0 + n < a.odim; n += 256) {
+        A v = 0;
+        for (int r = 0; r < kRowsPass; ++r) v += sums[r * BO + n];
+        if (slot) slot[(i64)a.idim * a.odim + o0 + n] = v;
+        else ((T *)a.db)[(i64)e * a.odim + o0 + n] = (T)v;
+    }
+}
+
+// Components with several chunks: their partial sums in order.  Components without rows: zeros.
+template <class T> __global__ __launch_bounds__(256) void weight_reduce(WeightArgs a) {
+    typedef typename Acc<T>::type A;
+    const int e = blockIdx.y;
+    const int chunks = a.bucket_first[e + 1] - a.bucket_first[e];
+    if (chunks == 1) return;
+    const i64 n_w = (i64)a.idim * a.odim, size = n_w + a.odim;
+    const A *slot = (const A *)a.ws + (((i64)a.offsets[e] * 2) >> (4 + a.level)) * size;
+    for (i64 j = (i64)blockIdx.x * 256 + threadIdx.x; j < size; j += (i64)gridDim.x * 256) {
+        const bool is_w = j < n_w;
+        if (is_w ? !a.dw : !a.db) continue;
+        A v = 0;
+        for (int c = 0; c < chunks; ++c) v += slot[c * size + j];
+        if (is_w) ((T *)a.dw)[(i64)e * n_w + j] = (T)v;
+        else ((T *)a.db)[(i64)e * a.odim + (j - n_w)] = (T)v;
+    }
+}
+
+// out[i] = sum over j of g_ij u_ij, u_ij the sum of its splits: one thread per four elements.
+template <class T> __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
+    typedef typename Acc<T>::type A;
+    const int quads = (a.dim + 3) >> 2;
+    for (i64 t = (i64)blockIdx.x * 256 + threadIdx.x; t < a.rows * quads; t += (i64)gridDim.x * 256) {
+        const i64 i = t / quads;
+        const int c = (int)(t - i * quads) * 4, avail = a.dim - c < 4 ? a.dim - c : 4;
+        A v[4] = {0, 0, 0, 0};
+        for (int j = 0; j < a.k; ++j) {
+            const i64 p = i * a.k + j;
+            if (a.bucket[p] >= a.K) continue;
+            A u[4] = {0, 0, 0, 0};
+            for (int s = 0; s < a.splits; ++s) {
+                const A *src = (const A *)a.ws + ((i64)s * a.P + p) * a.dim + c;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (x < avail) u[x] += src[x];
+            }
+            const A g = a.gates ? ((const A *)a.gates)[p] : (A)1;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] += g * u[x];
+        }
+        T *out = (T *)a.out + i * a.out_stride + c;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (x < avail) out[x] = (T)v[x];
+    }
+}
+
+// The same with the gates' gradient in . u_ij + b . d_i: one wave per row.  KJ >= k.
+template <class T, int KJ> __global__ __launch_bounds__(256) void combine_gates_kernel(CombineArgs a) {
+    typedef typename Acc<T>::type A;
+    const int lane = wave_lane();
+    const i64 i = (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= a.rows) return;
+    A dot[KJ], g[KJ];
+    int e[KJ];
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) {
+        dot[j] = 0;
+        e[j] = j < a.k ? a.bucket[i * a.k + j] : a.K;
+        g[j] = e[j] < a.K ? ((const A *)a.gates)[i * a.k + j] : (A)0;
+    }
+    const T *in = (const T *)a.in + i * a.in_stride;
+    for (int c = lane; c < a.dim; c += 64) {
+        A v = 0;
+        const A x = (A)in[c];
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+            if (e[j] >= a.K) continue;
+            A u = 0;
+            for (int s = 0; s < a.splits; ++s) u += ((const A *)a.ws)[((i64)s * a.P + i * a.k + j) * a.dim + c];
+            dot[j] += x * u;
+            v += g[j] * u;
+        }
+        if (a.out) ((T *)a.out)[i * a.out_stride + c] = (T)v;
+    }
+    if (a.bias) {
+        for (int c = lane; c < a.ddim; c += 64) {
+#pragma unroll
+            for (int j = 0; j < KJ; ++j)
+                if (e[j] < a.K) {
+                    const i64 p = i * a.k + j;
+                    dot[j] += (A)((const T *)a.bias)[(i64)e[j] * a.bias_row + c] * (A)((const T *)a.d)[(p / a.d_div) * a.d_stride + c];
+                }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) {
+        if (j >= a.k) break;
+        A v = dot[j];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        if (lane == 0) ((A *)a.dgates)[i * a.k + j] = v;
+    }
+}
+
+template <class T, bool KCONTIG, bool VEC> static void rows_by_tile(const RowsArgs &a, bool small, i64 blocks, hipStream_t st) {
+    const dim3 g((unsigned)blocks);
+    if (small) rows_kernel<T, KCONTIG, VEC, 16, 128, 4, 1><<<g, 256, 0, st>>>(a);
+    else if (a.ndim <= 16) rows_kernel<T, KCONTIG, VEC, 128, 16, 1, 4><<<g, 256, 0, st>>>(a);
+    else if (a.ndim <= 64) rows_kernel<T, KCONTIG, VEC, 128, 64, 2, 2><<<g, 256, 0, st>>>(a);
+    else rows_kernel<T, KCONTIG, VEC, 128, 128, 2, 2><<<g, 256, 0, st>>>(a);
+}
+
+template <class T> int launch_rows(const RowsArgs &a, bool kcontig, bool vec, bool small, i64 blocks, hipStream_t st) {
+    if (kcontig) vec ? rows_by_tile<T, true, true>(a, small, blocks, st) : rows_by_tile<T, true, false>(a, small, blocks, st);
+    else vec ? rows_by_tile<T, false, true>(a, small, blocks, st) : rows_by_tile<T, false, false>(a, small, blocks, st);
+    return ops_launched("rows_product");
+}
+
+template <class T, bool VEC> static void weight_by_tile(const WeightArgs &a, i64 blocks, hipStream_t st) {
+    const dim3 g((unsigned)blocks);
+    if (a.idim <= 16 && a.odim <= 16) weight_kernel<T, VEC, 16, 16, 1, 1><<<g, 256, 0, st>>>(a);
+    else if (a.idim <= 64 && a.odim <= 64) weight_kernel<T, VEC, 64, 64, 2, 2><<<g, 256, 0, st>>>(a);
+    else weight_kernel<T, VEC, 128, 128, 2, 2><<<g, 256, 0, st>>>(a);
+}
+
+template <class T> int launch_weight(const WeightArgs &a, bool vec, i64 blocks, hipStream_t st) {
+    if (blocks > 0) vec ? weight_by_tile<T, true>(a, blocks, st) : weight_by_tile<T, false>(a, blocks, st);
+    const i64 size = (i64)a.idim * a.odim + a.odim;
+    const i64 bx = (size + 1023) / 1024 < 256 ? (size + 1023) / 1024 : 256;
+    weight_reduce<T><<<dim3((unsigned)bx, (unsigned)a.K), 256, 0, st>>>(a);
+    return ops_launched("weight_product");
+}
+
+template <class T> int launch_combine(const CombineArgs &a, hipStream_t st) {
+    if (a.rows == 0) return BGMM_OPS_OK;
+    if (a.dgates) {
+        const dim3 g((unsigned)((a.rows + 3) / 4));
+        if (a.k == 1) combine_gates_kernel<T, 1><<<g, 256, 0, st>>>(a);
+        else if (a.k == 2) combine_gates_kernel<T, 2><<<g, 256, 0, st>>>(a);
+        else if (a.k <= 4) combine_gates_kernel<T, 4><<<g, 256, 0, st>>>(a);
+        else if (a.k <= 8) combine_gates_kernel<T, 8><<<g, 256, 0, st>>>(a);
+        else combine_gates_kernel<T, 32><<<g, 256, 0, st>>>(a);
+    } else {
+        const i64 threads = a.rows * ((a.dim + 3) / 4);
+        const i64 b = (threads + 255) / 256 < 65536 ? (threads + 255) / 256 : 65536;
+        combine_kernel<T><<<dim3((unsigned)b), 256, 0, st>>>(a);
+    }
+    return ops_launched("combine");
+}

@@ -213,6 +213,78 @@ class GaussianComponents(object):
     def log_post_pred_k(self, i, k):
         return float(self._ctx.log_post_pred(i)[k])
 
+    # --- points that need not be the training data (extension; torch tensors and the operators of pybgmm_amd.ops) ----
+    def _predictive_factors(self):
+        """The Student-t predictives of the K components and, last, of the prior (gaussian_components.py:207-251, 319-344):
+        ``(A, c, dof, log_const)`` with ``|x A_k + c_k|^2`` the squared Mahalanobis distance under component k and
+        ``log_const_k - (dof_k + D) / 2 log1p(|.|^2 / dof_k)`` its log density."""
+        if self._cov_type != "full":
+            raise NotImplementedError("defined for full-covariance components")
+        D, prior = self.D, self.prior
+        counts = self._ctx.counts()
+        m, S, _, _ = self._ctx.stats(False)
+        K = len(counts)
+        A, c, dof, const = np.empty((K + 1, D, D)), np.empty((K + 1, D)), np.empty(K + 1), np.empty(K + 1)
+        for k in range(K + 1):
+            n = int(counts[k]) if k < K else 0
+            k_N, v_N = prior.k_0 + n, prior.v_0 + n
+            mean = m[k] / k_N if k < K else np.asarray(prior.m_0, dtype=np.float64)
+            S_N = S[k] - k_N * np.outer(mean, mean) if k < K else np.asarray(prior.S_0, dtype=np.float64)
+            dof[k] = v_N - D + 1
+            chol = np.linalg.cholesky((k_N + 1.0) / (k_N * dof[k]) * S_N)
+            A[k] = np.linalg.inv(chol).T
+            c[k] = -mean.dot(A[k])
+            const[k] = (gammaln((dof[k] + D) / 2.0) - gammaln(dof[k] / 2.0) - D / 2.0 * (np.log(dof[k]) + self._cached_log_pi)
+                        - np.log(np.diag(chol)).sum())
+        return A, c, dof, const
+
+    def _on_device(self, X):
+        """(X as a float64 tensor on this model's GPU, function that gives a result the caller's kind of array)."""
+        import torch
+        dev = torch.device("cuda", self._device)
+        if isinstance(X, torch.Tensor):
+            x, back = X.to(dev, torch.float64), (lambda t: t)
+        else:
+            x, back = torch.from_numpy(np.ascontiguousarray(X, dtype=np.float64)).to(dev), (lambda t: t.cpu().numpy())
+        if x.dim() != 2 or x.shape[1] != self.D:
+            raise ValueError("X has to be n x %d" % self.D)
+        return x, back
+
+    def standardise(self, X=None, labels=None):
+        """Every point in the coordinates of its own component's predictive, ``L_k^{-1} (x - mean_k)`` with the predictive's
+        scale ``L_k L_k'``: residuals for checks of the fit.  Default: the training data under the current assignments; a
+        label that is no component (-1) gives zeros.  One grouped product (``pybgmm_amd.ops``)."""
+        import torch
+        from .. import ops
+        A, c, _, _ = self._predictive_factors()
+        if labels is None:
+            if X is not None:
+                raise ValueError("points that are not the training data need labels")
+            labels = self.assignments
+        x, back = self._on_device(self.X if X is None else X)
+        z = torch.as_tensor(labels).to(x.device, torch.int64)
+        if tuple(z.shape) != (x.shape[0],):
+            raise ValueError("one label per point")
+        if len(c) == 1:                                              # (no component yet)
+            return back(torch.zeros_like(x))
+        A, c = torch.from_numpy(A[:-1]).to(x.device), torch.from_numpy(c[:-1]).to(x.device)
+        return back(ops.grouped_matmul(x, A, ops.group_rows(z, len(c)), bias=c))
+
+    def log_predictive(self, X):
+        """n x (K + 1): log predictive density of every point under every component and, last, under the prior."""
+        import torch
+        x, back = self._on_device(X)
+        A, c, dof, const = (torch.from_numpy(a).to(x.device) for a in self._predictive_factors())
+        K1, D = c.shape
+        wide = A.permute(1, 0, 2).reshape(D, K1 * D)
+        out = torch.empty((x.shape[0], K1), dtype=torch.float64, device=x.device)
+        step = max(1, (1 << 27) // (K1 * D))                         # (every pair at once is a plain product: a GB at a time)
+        for i in range(0, x.shape[0], step):
+            r = torch.addmm(c.reshape(-1), x[i:i + step], wide)
+            q = r.square_().view(-1, K1, D).sum(2)
+            out[i:i + step] = const - 0.5 * (dof + D) * torch.log1p(q / dof)
+        return back(out)
+
     def log_marg_k(self, k):
         return self._ctx.log_marg_k(k)
 

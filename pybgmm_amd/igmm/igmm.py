@@ -119,6 +119,24 @@ class IGMM(GMM):
         """log p(X, z) (igmm.py:199-215), evaluated on the device."""
         return self.components._ctx.log_marg()
 
+    def posterior_labels(self, X, k=1):
+        """
+        The ``k`` most probable labels of new points and their posterior probabilities, given the current components: the
+        weights of one visit of the sampler (igmm/crpmm.py:68-75), ``log n_k + log predictive`` for every component and
+        ``log alpha + log prior predictive`` for label K, "a component of its own".  Full covariance.  (extension)
+
+        X : n x D array, or a float64 tensor on this model's GPU.  Returns ``(labels, weights)``, n x k, of X's kind,
+        ordered by probability; the weights are shares of the whole posterior.  (``pybgmm_amd.ops.route``)
+        """
+        import torch
+        from .. import ops
+        x, back = self.components._on_device(X)
+        K = self.components.K
+        prior = np.log(np.concatenate([self.components.counts[:K].astype(np.float64), [self.alpha]]))
+        log_weights = self.components.log_predictive(x) + torch.from_numpy(prior).to(x.device)
+        labels, weights = ops.route(log_weights, k, renormalise=False)
+        return back(labels), back(weights)
+
     def log_marg_host(self):
         """The same quantity assembled on the host from downloaded counts and the
         per-component device marginals (cross-check for tests)."""

@@ -1,0 +1,847 @@
+"""
+The operators of pybgmm_amd.ops against plain implementations in 64 bits (include/bgmm_ops.h).
+
+Tolerances.  A result rounded to a type of precision eps is off by eps / 2 of its value; a sum of m products held in a type
+of precision acc is off by at most m acc / 2 (and a few more roundings) of the sum of the products' magnitudes, whatever
+its order: `close` takes both, the second from the same sum over magnitudes.
+"""
+import ctypes
+import math
+import os
+import re
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+gpu = pytest.mark.gpu
+TYPES = [torch.float64, torch.float32, torch.float16, torch.bfloat16]
+
+
+def acc_of(dt):
+    return torch.float64 if dt == torch.float64 else torch.float32
+
+
+def half_step(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def close(got, want, magnitude, terms, operand=0.0):
+    """got (its type's rounding) against want (64 bits); magnitude: the sum of the terms' magnitudes; operand: relative error
+    of a single term (operands rounded before the product)."""
+    want, magnitude = want.to(got.device), magnitude.to(got.device)
+    acc = half_step(acc_of(got.dtype))
+    tol = half_step(got.dtype) * want.abs() * (1 + 1e-3) + (acc * (terms + 8) + operand) * magnitude + torch.finfo(got.dtype).tiny
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), "%d of %d off, worst %g over its tolerance" % (
+        int(bad.sum()), bad.numel(), float(((got.double() - want).abs() / tol)[bad].max()))
+
+
+# ------------------------------------------------------------------------------------------ the C-ABI and refusals (CPU)
+def test_header_symbols_are_exported_and_bound():
+    from pybgmm_amd.ops import _native as nat
+    hdr = open(os.path.join(ROOT, "include", "bgmm_ops.h")).read()
+    declared = set(re.findall(r"\b(bgmm_[a-z_0-9]+)\s*\(", hdr)) - {"bgmm_create"}
+    calls = set(n for n in declared if re.search(r"BGMM_OPS_API [^;]*\b%s\s*\(" % n, hdr))
+    assert calls == set(nat.SIGNATURES), calls.symmetric_difference(nat.SIGNATURES)
+    L = nat.load()
+    for name in calls:
+        assert hasattr(L, name)
+    for name, value in (("MAX_COMPONENTS", nat.MAX_COMPONENTS), ("MAX_CHOSEN", nat.MAX_CHOSEN), ("LEVELS", nat.LEVELS)):
+        assert int(re.search(r"BGMM_OPS_%s\s*=\s*(\d+)" % name, hdr).group(1)) == value
+
+
+def test_the_operators_bind_to_the_runtime_of_torch():
+    from pybgmm_amd import _lib
+    from pybgmm_amd.ops import _native as nat
+    _lib.load()                                     # (may bring another HIP runtime into the process)
+    path = nat.load().bgmm_ops_runtime_path().decode()
+    assert os.path.samefile(path, os.path.join(os.path.dirname(torch.__file__), "lib", "libamdhip64.so"))
+
+
+def cpu_groups(shape, K):
+    from pybgmm_amd import ops
+    t = torch.zeros(4, dtype=torch.int32)
+    return ops.RowGroups(shape, K, t, t, t, t)
+
+
+def refused(code, call, *args, **kw):
+    from pybgmm_amd._lib import BGMMError
+    with pytest.raises(BGMMError) as ei:
+        call(*args, **kw)
+    assert ei.value.code == code, ei.value
+    return str(ei.value)
+
+
+def test_refusals_of_route_and_group_rows():
+    from pybgmm_amd import ops
+    lw = torch.zeros(3, 5)
+    refused(-1, ops.route, [1.0], 1)
+    refused(-1, ops.route, lw[0], 1)
+    refused(-1, ops.route, lw.long(), 1)
+    refused(-1, ops.route, lw, 0)
+    refused(-1, ops.route, lw, 6)
+    refused(-1, ops.route, lw, 1.5)
+    refused(-5, ops.route, torch.zeros(2, 64), 33)
+    assert "HIP" in refused(-2, ops.route, lw, 2)
+    z = torch.zeros(4, dtype=torch.int64)
+    refused(-1, ops.group_rows, z.int(), 3)
+    refused(-1, ops.group_rows, z.view(1, 2, 2), 3)
+    refused(-1, ops.group_rows, torch.zeros(2, 33, dtype=torch.int64), 3)
+    refused(-1, ops.group_rows, torch.zeros(2, 0, dtype=torch.int64), 3)
+    refused(-1, ops.group_rows, z, 0)
+    refused(-5, ops.group_rows, z, 8001)
+    refused(-2, ops.group_rows, z, 3)
+
+
+def test_refusals_of_grouped_matmul():
+    from pybgmm_amd import ops
+    g1, g2 = cpu_groups((4,), 3), cpu_groups((4, 2), 3)
+    x, w, b = torch.zeros(4, 6), torch.zeros(3, 6, 5), torch.zeros(3, 5)
+    mm = ops.grouped_matmul
+    refused(-1, mm, x, w, None)
+    refused(-1, mm, x.long(), w.long(), g1)
+    refused(-1, mm, x, w.double(), g1)
+    refused(-1, mm, x, w, g1, bias=b.double())
+    refused(-1, mm, x, w[:2], g1)
+    refused(-1, mm, x, w[0], g1)
+    refused(-1, mm, x[:3], w, g1)
+    refused(-1, mm, x[:, :5], w, g1)
+    refused(-1, mm, torch.zeros(4, 2, 6), w, g1)                # a row per label needs a grouping of (n, k) labels
+    refused(-1, mm, torch.zeros(4, 3, 6), w, g2)
+    refused(-1, mm, x, w, g1, bias=b[:, :4])
+    refused(-1, mm, x, w, g1, gates=torch.zeros(4, 1))
+    refused(-1, mm, x, w, g2, gates=torch.zeros(4))
+    refused(-1, mm, x, w, g1, gates=torch.zeros(4).double())
+    refused(-1, mm, x.bfloat16(), w.bfloat16(), g1, gates=torch.zeros(4).bfloat16())
+    refused(-1, mm, x, torch.zeros(3, 6, 0), g1)
+    refused(-2, mm, x, w, g1, bias=b, gates=torch.zeros(4))
+
+
+def test_refusals_of_verify_drafts():
+    from pybgmm_amd import ops
+    v = ops.verify_drafts
+    p, q, z = torch.zeros(2, 4, 5), torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.int64)
+    ua, ud = torch.zeros(2, 3, dtype=torch.float64), torch.zeros(2, dtype=torch.float64)
+    refused(-1, v, p[0], q, z, ua, ud)
+    refused(-1, v, p[:, :3], q, z, ua, ud)
+    refused(-1, v, p[..., :4], q, z, ua, ud)
+    refused(-1, v, p.double(), q, z, ua, ud)
+    refused(-1, v, p.long(), q.long(), z, ua, ud)
+    refused(-1, v, p, q, z.int(), ua, ud)
+    refused(-1, v, p, q, z[:, :2], ua, ud)
+    refused(-1, v, p, q, z, ua.float(), ud)
+    refused(-1, v, p, q, z, ua, ud[:1])
+    refused(-1, v, p, q, z, ua, ud, lengths=torch.zeros(2, dtype=torch.int32))
+    refused(-1, v, p[..., :0], q[..., :0], z, ua, ud)
+    refused(-2, v, p, q, z, ua, ud)
+
+
+def test_c_entry_points_refuse_before_they_launch():
+    """Sizes, types, null pointers: negative codes with a message, no launch (this runs without a device)."""
+    from pybgmm_amd.ops import _native as nat
+    L = nat.load()
+    buf = ctypes.create_string_buffer(4096)
+    p = ctypes.addressof(buf)
+    calls = [
+        (-1, L.bgmm_group_rows(p, -1, 3, p, p, p, p, p, 0, None)),
+        (-1, L.bgmm_group_rows(p, 1 << 31, 3, p, p, p, p, p, 0, None)),
+        (-1, L.bgmm_group_rows(p, 5, 0, p, p, p, p, p, 0, None)),
+        (-5, L.bgmm_group_rows(p, 5, 8001, p, p, p, p, p, 0, None)),
+        (-1, L.bgmm_group_rows(None, 5, 3, p, p, p, p, p, 0, None)),
+        (-1, L.bgmm_group_rows(p, 100000, 3, p, p, p, p, p, 8, None)),
+        (-1, L.bgmm_route(9, p, 4, 2, 4, 1, 1, p, p, None, None)),
+        (-1, L.bgmm_route(1, p, 4, 2, 4, 5, 1, p, p, None, None)),
+        (-5, L.bgmm_route(1, p, 64, 2, 64, 33, 1, p, p, None, None)),
+        (-1, L.bgmm_route(1, None, 4, 2, 4, 1, 1, p, p, None, None)),
+        (-1, L.bgmm_route_backward(1, p, 4, 2, 4, 1, 0, p, p, None, p, p, None)),
+        (-1, L.bgmm_verify_drafts(1, p, 4, 4, p, 4, 4, p, p, p, None, 1, -1, 4, p, p, None)),
+        (-1, L.bgmm_verify_drafts(1, p, 4, 4, None, 4, 4, p, p, p, None, 1, 1, 4, p, p, None)),
+        (-1, L.bgmm_verify_drafts(1, p, 4, 4, p, 4, 4, p, p, p, None, 1, 1, 0, p, p, None)),
+        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, p, 1, 8, 2, 4, 4, p, p, p, None)),     # out and ws
+        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 2, 8, 2, 4, 4, p, p, p, None)),  # splits without ws
+        (-1, L.bgmm_rows_product(1, p, 4, 0, p, 4, 4, 0, None, 0, None, p, 4, None, 1, 8, 2, 4, 4, p, p, p, None)),
+        (-1, L.bgmm_rows_product(4, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 1, 8, 2, 4, 4, p, p, p, None)),
+        (-1, L.bgmm_weight_product(1, p, 4, 1, p, 4, 1, None, p, None, None, 0, 1 << 20, 2, 4, 4, p, p, p, None)),   # workspace
+        (-1, L.bgmm_weight_product(1, None, 4, 1, p, 4, 1, None, p, None, None, 0, 8, 2, 4, 4, p, p, p, None)),
+        (-1, L.bgmm_combine(1, p, 1, 4, 33, 2, p, None, p, 4, 4, None, None, 0, None, 0, None, 0, 1, 1, None)),
+        (-1, L.bgmm_combine(1, p, 1, 4, 1, 2, p, None, p, 4, 4, p, p, 4, None, 0, None, 0, 1, 1, None)),             # dgates without gates
+    ]
+    for i, (want, got) in enumerate(calls):
+        assert got == want, (i, got)
+    assert L.bgmm_ops_last_error()
+
+
+# ------------------------------------------------------------------------------------------ route
+def route_ref(lw, k, renormalise):
+    """Labels and weights in 64 bits, one row at a time."""
+    n, K = lw.shape
+    labels, weights = torch.full((n, k), -1, dtype=torch.int64), torch.zeros(n, k, dtype=torch.float64)
+    for i in range(n):
+        row = lw[i].double().tolist()
+        at = sorted((j for j in range(K) if row[j] > -math.inf), key=lambda j: (-row[j], j))
+        if not at:
+            continue
+        top = row[at[0]]
+
+        def ratio(v):
+            return 1.0 if v == top else math.exp(v - top)
+        total = math.fsum(ratio(row[j]) for j in (at[:k] if renormalise else at))
+        for c, j in enumerate(at[:k]):
+            labels[i, c], weights[i, c] = j, ratio(row[j]) / total
+    return labels, weights
+
+
+def route_grad_ref(lw, labels, weights, dw, renormalise):
+    n, K = lw.shape
+    d = torch.zeros(n, K, dtype=torch.float64)
+    for i in range(n):
+        on = [(c, int(j)) for c, j in enumerate(labels[i]) if j >= 0]
+        s = math.fsum(float(weights[i, c] * dw[i, c]) for c, _ in on)
+        if not renormalise and on:
+            row = lw[i].double()
+            row = torch.where(torch.isnan(row), torch.tensor(-math.inf, dtype=torch.float64), row)
+            p = torch.where(row == row.max(), torch.ones(K, dtype=torch.float64), torch.exp(row - row.max()))
+            d[i] = -s * p / p.sum()
+        for c, j in on:
+            d[i, j] += float(weights[i, c]) * (float(dw[i, c]) - (s if renormalise else 0.0))
+    return d
+
+
+def route_rows(n, K, dt, seed):
+    g = torch.Generator().manual_seed(seed)
+    lw = torch.randn(n, K, generator=g, dtype=torch.float64) * 4
+    lw[torch.rand(n, K, generator=g) < 0.1] = -math.inf
+    lw[torch.rand(n, K, generator=g) < 0.02] = math.nan
+    lw[torch.rand(n, K, generator=g) < 0.2] = 0.5                     # ties
+    if n > 4:
+        lw[0] = -math.inf                                             # nothing to choose
+        lw[1] = torch.finfo(dt).min                                   # a mask of the type's lowest value is a value like others
+        lw[2, : max(1, K // 2)] = -math.inf
+        lw[3] = math.nan
+        lw[4, K - 1] = math.inf
+    return lw.to(dt)
+
+
+@gpu
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n,K,k", [(1, 1, 1), (1, 200, 4), (7, 2, 2), (33, 64, 6), (65, 100, 1), (20, 129, 8), (9, 1000, 32), (5, 5000, 3), (300, 17, 17)])
+@pytest.mark.parametrize("renormalise", [True, False])
+def test_route_forward_and_backward(dt, n, K, k, renormalise):
+    from pybgmm_amd import ops
+    lw = route_rows(n, K, dt, 1000 * n + K)
+    x = lw.cuda().requires_grad_()
+    labels, w = ops.route(x, k, renormalise=renormalise)
+    want_l, want_w = route_ref(lw, k, renormalise)
+    assert torch.equal(labels.cpu(), want_l)
+    # exp is off by about an ulp of its value, the difference in its argument by half a step of |l_j - m| <= 40 at most
+    acc = half_step(acc_of(dt))
+    tol = acc * (K + 100) * want_w + 1e-30
+    assert w.dtype == acc_of(dt) and bool(((w.cpu().double() - want_w).abs() <= tol).all())
+    with torch.no_grad():
+        l2, w2 = ops.route(x, k, renormalise=renormalise)
+    assert torch.equal(l2, labels) and torch.equal(w2, w)
+    dw = torch.randn(n, k, generator=torch.Generator().manual_seed(n), dtype=acc_of(dt))
+    got, = torch.autograd.grad(w, x, dw.cuda())
+    want = route_grad_ref(lw, want_l, want_w, dw, renormalise)
+    assert got.dtype == dt
+    scale = (want_w * dw.double()).abs().sum(1, keepdim=True)
+    tol = half_step(dt) * want.abs() * 1.001 + acc * (K + 200) * scale + torch.finfo(dt).tiny
+    assert bool(((got.cpu().double() - want).abs() <= tol).all())
+
+
+@gpu
+def test_route_rows_with_strides_and_no_rows():
+    from pybgmm_amd import ops
+    lw = route_rows(40, 96, torch.float32, 3).cuda()
+    for view in (lw[::2], lw[:, :50], lw.t().contiguous().t(), lw[5:6], lw[:, 3:80][::3]):
+        got, want = ops.route(view, 3), ops.route(view.contiguous(), 3)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        x, y = view.detach().requires_grad_(), view.contiguous().requires_grad_()
+        ga = torch.autograd.grad(ops.route(x, 3, renormalise=False)[1].sum(1).square().sum(), x)[0]
+        gb = torch.autograd.grad(ops.route(y, 3, renormalise=False)[1].sum(1).square().sum(), y)[0]
+        assert torch.equal(ga, gb)
+    labels, w = ops.route(lw[:0], 2)
+    assert labels.shape == (0, 2) and w.shape == (0, 2)
+
+
+@gpu
+def test_route_gradient_against_differences():
+    from pybgmm_amd import ops
+    x = torch.randn(6, 11, dtype=torch.float64, device="cuda", generator=torch.Generator("cuda").manual_seed(4)).requires_grad_()
+    for renormalise in (True, False):
+        assert torch.autograd.gradcheck(lambda t: ops.route(t, 3, renormalise=renormalise)[1], (x,), eps=1e-6, atol=1e-8, rtol=1e-5)
+
+
+# ------------------------------------------------------------------------------------------ group_rows
+@gpu
+@pytest.mark.parametrize("shape,K", [((0,), 3), ((0,), 2000), ((1,), 1), ((5,), 8000), ((64,), 7), ((1000, 4), 64), ((8192,), 959), ((8192,), 960),
+                                     ((8193,), 3), ((40000,), 200), ((30011, 3), 3071), ((30011,), 3072), ((100003,), 8000), ((1000000,), 100)])
+def test_group_rows(shape, K):
+    from pybgmm_amd import ops
+    g = torch.Generator().manual_seed(K + len(shape))
+    z = torch.randint(-1, K, shape, generator=g)
+    if z.numel() > 3:
+        z.view(-1)[1], z.view(-1)[2] = K, -(1 << 40)              # outside: no component
+        z.view(-1)[3] = 1 << 33
+    grp = ops.group_rows(z.cuda(), K)
+    flat = z.view(-1)
+    bucket = torch.where((flat >= 0) & (flat < K), flat, torch.tensor(K))
+    assert torch.equal(grp.bucket.cpu().long(), bucket)
+    assert torch.equal(grp.order.cpu().long(), torch.argsort(bucket, stable=True))
+    size = torch.bincount(bucket, minlength=K + 1)
+    off = torch.cat([torch.zeros(1, dtype=torch.int64), size.cumsum(0)])
+    assert torch.equal(grp.offsets.cpu().long(), off)
+    assert torch.equal(grp.counts.cpu().long(), size[:K])
+    first = grp.first.view(12, K + 2).cpu().long()
+    for level in range(12):
+        tiles = (size + (16 << level) - 1) // (16 << level)
+        assert torch.equal(first[level], torch.cat([torch.zeros(1, dtype=torch.int64), tiles.cumsum(0)])), level
+
+
+@gpu
+def test_group_rows_one_component_has_all_and_non_contiguous_labels():
+    from pybgmm_amd import ops
+    z = torch.full((50000,), 5, device="cuda")
+    grp = ops.group_rows(z, 9)
+    assert torch.equal(grp.order.long(), torch.arange(50000, device="cuda")) and grp.counts.tolist() == [0] * 5 + [50000] + [0] * 3
+    z = torch.randint(0, 9, (100, 6), device="cuda")[:, ::2]
+    assert torch.equal(ops.group_rows(z, 9).order, ops.group_rows(z.contiguous(), 9).order)
+
+
+# ------------------------------------------------------------------------------------------ grouped_matmul
+def products_ref(x, w, z, bias, gates, dy=None):
+    """Everything in 64 bits on x's device, with the sums over magnitudes next to every result."""
+    K, din, dout = w.shape
+    n, k = z.shape
+    per = x.dim() == 3
+    X, W = x.double(), w.double()
+    pair, mag = [torch.zeros(n, k, dout, dtype=torch.float64, device=x.device) for _ in range(2)]
+    out = {}
+    if dy is not None:
+        dpair, dmag = [torch.zeros(n, k, din, dtype=torch.float64, device=x.device) for _ in range(2)]
+        dw, dwm = torch.zeros_like(W), torch.zeros_like(W)
+        db, dbm = [torch.zeros(K, dout, dtype=torch.float64, device=x.device) for _ in range(2)]
+        dg, dgm = [torch.zeros(n, k, dtype=torch.float64, device=x.device) for _ in range(2)]
+    for e in range(K):
+        i, j = torch.nonzero(z == e, as_tuple=True)
+        if i.numel() == 0:
+            continue
+        xe = X[i, j] if per else X[i]
+        be = bias[e].double() if bias is not None else torch.zeros(dout, dtype=torch.float64, device=x.device)
+        u, um = xe @ W[e] + be, xe.abs() @ W[e].abs() + be.abs()
+        ge = gates.double().view(n, k)[i, j][:, None] if gates is not None else torch.ones(i.numel(), 1, dtype=torch.float64, device=x.device)
+        pair[i, j], mag[i, j] = ge * u, ge.abs() * um
+        if dy is not None:
+            d = dy.double().view(n, k, dout)[i, j] if gates is None else dy.double()[i]
+            wt = W[e].t().contiguous()
+            v, vm = d @ wt, d.abs() @ wt.abs()
+            dpair[i, j], dmag[i, j] = ge * v, ge.abs() * vm
+            dw[e], dwm[e] = xe.t().contiguous() @ (ge * d), xe.abs().t().contiguous() @ (ge * d).abs()
+            db[e], dbm[e] = (ge * d).sum(0), (ge * d).abs().sum(0)
+            dg[i, j] = (xe * v).sum(1) + (d * be).sum(1)
+            dgm[i, j] = (xe.abs() * vm).sum(1) + (d * be).abs().sum(1)
+    summed = gates is not None
+    out["y"] = (pair.sum(1), mag.sum(1)) if summed else (pair, mag)
+    if dy is not None:
+        out["x"] = (dpair, dmag) if per else (dpair.sum(1), dmag.sum(1))
+        out["w"], out["b"], out["g"] = (dw, dwm), (db, dbm), (dg, dgm)
+    return out
+
+
+def product_case(n, k, K, din, dout, dt, seed, flat=False, per_label=False, bias=True, gates=True):
+    g = torch.Generator("cuda").manual_seed(seed)
+
+    def randn(*s):
+        return torch.randn(*s, generator=g, device="cuda", dtype=torch.float64).to(dt)
+    share = torch.rand(K, generator=g, device="cuda") ** 3 + 1e-3
+    z = torch.multinomial(share, max(n, 1) * k, replacement=True, generator=g).view(-1, k)[:n]
+    z[torch.rand(n, k, generator=g, device="cuda") < 0.05] = -1
+    if n > 2:
+        z[1] = -1                                                    # a row of no component at all
+    x = randn(n, k, din) if per_label else randn(n, din)
+    if n > 2:
+        x[1] = math.nan                                              # ... whose contents nobody reads
+    w = randn(K, din, dout)
+    b = randn(K, dout) if bias else None
+    gt = None
+    if gates:
+        gt = torch.rand(n, k, generator=g, device="cuda", dtype=acc_of(dt)) + 0.1
+        if n > 2:
+            gt[1] = math.nan
+        if flat:
+            gt = gt[:, 0]
+    return (z[:, 0] if flat else z).contiguous(), x, w, b, gt, g
+
+
+CASES = [
+    # n, k, K, din, dout
+    (1, 1, 1, 1, 1), (1, 4, 64, 256, 128), (3, 2, 5, 64, 64), (1, 2, 3, 2048, 40), (17, 1, 40, 96, 200), (130, 1, 3, 64, 64),
+    (257, 2, 4, 130, 66), (1000, 1, 7, 16, 16), (999, 3, 6, 33, 5), (700, 1, 2, 128, 300), (2050, 1, 20, 192, 77), (5000, 2, 9, 72, 136),
+    (4000, 1, 1, 20, 16), (64, 8, 16, 513, 129),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("form", ["plain", "gated", "per_label", "per_label_gated"])
+def test_grouped_matmul_forward_and_backward(dt, case, form):
+    from pybgmm_amd import ops
+    n, k, K, din, dout = case
+    gated, per_label = "gated" in form, "per_label" in form
+    flat = k == 1 and not per_label
+    z, x, w, b, gt, g = product_case(n, k, K, din, dout, dt, sum(case), flat=flat, per_label=per_label, bias=form != "per_label", gates=gated)
+    groups = ops.group_rows(z, K)
+    leaves = [t.requires_grad_() for t in (x, w, b, gt) if t is not None]
+    y = ops.grouped_matmul(x, w, groups, bias=b, gates=gt)
+    assert y.dtype == dt and tuple(y.shape) == ((n, dout) if gated or flat else (n, k, dout))
+    with torch.no_grad():
+        assert torch.equal(ops.grouped_matmul(x, w, groups, bias=b, gates=gt), y)
+    dy = torch.randn(y.shape, generator=g, device="cuda", dtype=torch.float64).to(dt)
+    grads = torch.autograd.grad(y, leaves, dy)
+    again = torch.autograd.grad(ops.grouped_matmul(x, w, groups, bias=b, gates=gt), leaves, dy)
+    assert all(torch.equal(a, c) for a, c in zip(grads, again))
+    names = ["x", "w"] + (["b"] if b is not None else []) + (["g"] if gated else [])
+    ref = products_ref(x.detach(), w.detach(), z.view(n, k), None if b is None else b.detach(), None if gt is None else gt.detach(), dy)
+    close(y.detach(), ref["y"][0].view(y.shape), ref["y"][1].view(y.shape), din + k + 16)
+    rows = int((z.view(-1) >= 0).sum())
+    for name, got in zip(names, grads):
+        want, mag = (t.view(got.shape) for t in ref[name])
+        terms = {"x": dout + k, "w": rows, "b": rows, "g": din + 2 * dout}[name] + 16
+        # (16-bit types: a gated row of dy is rounded to the operands' type before the weights' gradient sums its products)
+        close(got, want, mag, terms, operand=half_step(dt) * 1.001 if name == "w" and gated and dt.itemsize == 2 else 0.0)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float64, torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,K,din,dout", [(40000, 2, 64, 64), (70000, 3, 16, 16), (35000, 1, 136, 40)])
+def test_long_groups_are_split_and_joined(dt, rows, K, din, dout):
+    from pybgmm_amd import ops
+    z, x, w, b, _, g = product_case(rows, 1, K, din, dout, dt, rows, flat=True, gates=False)
+    groups = ops.group_rows(z, K)
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = ops.grouped_matmul(x, w, groups, bias=b)
+    dy = torch.randn(y.shape, generator=g, device="cuda", dtype=torch.float64).to(dt)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    ref = products_ref(x.detach(), w.detach(), z.view(-1, 1), b.detach(), None, dy)
+    close(y.detach(), ref["y"][0][:, 0], ref["y"][1][:, 0], din + 16)
+    close(dx, ref["x"][0], ref["x"][1], dout + 16)
+    close(dw, *ref["w"], rows)
+    close(db, *ref["b"], rows)
+
+
+@gpu
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+def test_strides_alignment_and_transposed_weights(dt):
+    from pybgmm_amd import ops
+    n, K, din, dout = 300, 4, 72, 56
+    z, x, w, b, _, g = product_case(n, 1, K, din, dout, dt, 11, flat=True, gates=False)
+    groups = ops.group_rows(z, K)
+    want = ops.grouped_matmul(x, w, groups, bias=b)
+    wide = torch.zeros(n, din + 5, device="cuda", dtype=dt)
+    wide[:, 3:3 + din] = x
+    odd = torch.zeros(K * din * dout + 1, device="cuda", dtype=dt)
+    odd[1:] = w.reshape(-1)
+    views = {
+        "x inside wider rows": (wide[:, 3:3 + din], w, b),
+        "x by columns": (x.t().contiguous().t(), w, b),
+        "weights by output": (x, w.transpose(1, 2).contiguous().transpose(1, 2), b),
+        "weights off alignment": (x, odd[1:].view(K, din, dout), b),
+        "weights by component last": (x, w.permute(1, 2, 0).contiguous().permute(2, 0, 1), b),
+        "bias broadcast from one row": (x, w, b[:1].expand(K, dout)),
+    }
+    for name, (xv, wv, bv) in views.items():
+        ref = want if "bias" not in name else ops.grouped_matmul(x, w, groups, bias=bv.contiguous())
+        got = ops.grouped_matmul(xv, wv, groups, bias=bv)
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(ref)), name
+    # gradients of the views arrive in the leaves' own shape
+    leaf = w.transpose(1, 2).contiguous().requires_grad_()
+    wl = w.clone().requires_grad_()
+    xs = x.clone().requires_grad_()
+    dy = torch.randn(n, dout, generator=g, device="cuda", dtype=torch.float64).to(dt)
+    ga = torch.autograd.grad(ops.grouped_matmul(xs, leaf.transpose(1, 2), groups), (xs, leaf), dy)
+    gb = torch.autograd.grad(ops.grouped_matmul(xs, wl, groups), (xs, wl), dy)
+    assert torch.equal(ga[0], gb[0]) and torch.equal(ga[1].transpose(1, 2), gb[1])
+    one = torch.ones(1, device="cuda", dtype=dt).expand(n, dout)                 # a gradient broadcast from one number
+    gc = torch.autograd.grad(ops.grouped_matmul(xs, wl, groups), (xs, wl), one)
+    gd = torch.autograd.grad(ops.grouped_matmul(xs, wl, groups), (xs, wl), one.contiguous())
+    assert all(torch.equal(a, c) for a, c in zip(gc, gd))
+
+
+@gpu
+def test_grouped_matmul_without_rows_and_components_without_rows():
+    from pybgmm_amd import ops
+    w, b = torch.randn(5, 8, 6, device="cuda", requires_grad=True), torch.randn(5, 6, device="cuda", requires_grad=True)
+    x = torch.randn(0, 8, device="cuda", requires_grad=True)
+    y = ops.grouped_matmul(x, w, ops.group_rows(torch.zeros(0, dtype=torch.int64, device="cuda"), 5), bias=b)
+    assert y.shape == (0, 6)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
+    assert dx.shape == (0, 8) and not dw.any() and not db.any()
+    x = torch.randn(7, 8, device="cuda", requires_grad=True)
+    y = ops.grouped_matmul(x, w, ops.group_rows(torch.full((7,), -1, device="cuda"), 5), bias=b)
+    assert not y.any()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.full_like(y, math.nan))
+    assert not dx.any() and not dw.any() and not db.any()
+    y = ops.grouped_matmul(x, w, ops.group_rows(torch.tensor([3] * 7, device="cuda"), 5), bias=b)
+    dw, = torch.autograd.grad(y, (w,), torch.ones_like(y))
+    assert dw[3].any() and not dw[[0, 1, 2, 4]].any()
+
+
+@gpu
+def test_grouped_matmul_gradients_against_differences():
+    from pybgmm_amd import ops
+    z, x, w, b, gt, _ = product_case(5, 2, 3, 4, 3, torch.float64, 2)
+    x = torch.nan_to_num(x).requires_grad_()
+    gt = torch.nan_to_num(gt).requires_grad_()
+    w.requires_grad_()
+    b.requires_grad_()
+    groups = ops.group_rows(z, 3)
+    assert torch.autograd.gradcheck(lambda x, w, b, g: ops.grouped_matmul(x, w, groups, bias=b, gates=g), (x, w, b, gt), eps=1e-6, atol=1e-7)
+    assert torch.autograd.gradcheck(lambda x, w, b: ops.grouped_matmul(x, w, groups, bias=b), (x, w, b), eps=1e-6, atol=1e-7)
+
+
+@gpu
+def test_some_gradients_only():
+    from pybgmm_amd import ops
+    z, x, w, b, gt, g = product_case(200, 2, 5, 40, 24, torch.float32, 8)
+    groups = ops.group_rows(z, 5)
+    full = [t.clone().requires_grad_() for t in (x, w, b, gt)]
+    dy = torch.randn(200, 24, device="cuda", generator=g)
+    want = torch.autograd.grad(ops.grouped_matmul(full[0], full[1], groups, bias=full[2], gates=full[3]), full, dy)
+    for i in range(4):
+        leaf = (x, w, b, gt)[i].clone().requires_grad_()
+        args = [leaf if j == i else (x, w, b, gt)[j] for j in range(4)]
+        got, = torch.autograd.grad(ops.grouped_matmul(args[0], args[1], groups, bias=args[2], gates=args[3]), leaf, dy)
+        assert torch.equal(got, want[i]), i
+
+
+# ------------------------------------------------------------------------------------------ verify_drafts
+def verify_ref(p, q, z, ua, ud, lengths):
+    """One sequence at a time in exact rational arithmetic (the inputs are floats: every sum below is exact)."""
+    from fractions import Fraction
+
+    def clean(v):
+        return Fraction(v) if v > 0 and v < math.inf else Fraction(0)
+    B, T, V = q.shape
+    out, acc = torch.full((B, T + 1), -1, dtype=torch.int64), torch.zeros(B, dtype=torch.int64)
+    for b in range(B):
+        length, a = min(max(int(lengths[b]), 0), T), 0
+        while a < length:
+            j = int(z[b, a])
+            # (the product of the comparison is rounded to 64 bits, as stated)
+            if not (0 <= j < V and float(ua[b, a]) * float(clean(float(q[b, a, j]))) < float(clean(float(p[b, a, j])))):
+                break
+            out[b, a] = j
+            a += 1
+        acc[b] = a
+        row = [clean(float(v)) for v in p[b, a].double()]
+        w = row
+        if a < length:
+            w = [max(x - clean(float(y)), Fraction(0)) for x, y in zip(row, q[b, a].double())]
+            if not any(w):
+                w = row
+        total, at = sum(w), Fraction(0)
+        goal = Fraction(float(ud[b])) * total
+        for j in range(V):
+            at += w[j]
+            if w[j] > 0 and at > goal:
+                out[b, a] = j
+                break
+    return out, acc
+
+
+def verify_case(B, T, V, dt, seed, spread=0.6):
+    g = torch.Generator().manual_seed(seed)
+    lp = torch.randn(B, T + 1, V, generator=g, dtype=torch.float64) * 2
+    lq = lp[:, :T] + torch.randn(B, T, V, generator=g, dtype=torch.float64) * spread
+    p, q = torch.softmax(lp, -1).to(dt), torch.softmax(lq, -1).to(dt)
+    z = torch.multinomial(torch.softmax(lq, -1).view(B * T, V), 1, generator=g).view(B, T) if B * T else torch.zeros(B, T, dtype=torch.int64)
+    ua, ud = torch.rand(B, T, generator=g, dtype=torch.float64), torch.rand(B, generator=g, dtype=torch.float64)
+    lengths = torch.randint(-1, T + 2, (B,), generator=g)
+    return p, q, z, ua, ud, lengths
+
+
+def verify_on_gpu(*args):
+    from pybgmm_amd import ops
+    out, acc = ops.verify_drafts(*(t.cuda() for t in args[:5]), lengths=args[5].cuda())
+    return out.cpu(), acc.cpu()
+
+
+@gpu
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("B,T,V", [(1, 1, 1), (1, 0, 7), (3, 4, 2), (50, 8, 20), (40, 3, 200), (5, 70, 33), (6, 2, 1025), (4, 5, 5003), (2, 3, 20000)])
+def test_verify_drafts(dt, B, T, V):
+    args = verify_case(B, T, V, dt, B * V + T)
+    want = verify_ref(*args)
+    got = verify_on_gpu(*args)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[0], want[0])
+
+
+@gpu
+def test_verify_drafts_without_lengths_strides_and_no_sequences():
+    from pybgmm_amd import ops
+    p, q, z, ua, ud, _ = verify_case(12, 4, 50, torch.float32, 5)
+    want = verify_ref(p, q, z, ua, ud, torch.full((12,), 4))
+    dev = [t.cuda() for t in (p, q, z, ua, ud)]
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(ops.verify_drafts(*dev), want))
+    pv = torch.zeros(5, 12, 64, device="cuda")
+    pv[..., 7:57] = dev[0].transpose(0, 1)
+    qv = dev[1].permute(2, 0, 1).contiguous().permute(1, 2, 0)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(ops.verify_drafts(pv.transpose(0, 1)[..., 7:57], qv, *dev[2:]), want))
+    out, acc = ops.verify_drafts(*(t[:0] for t in dev))
+    assert out.shape == (0, 5) and acc.shape == (0,)
+
+
+@gpu
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+def test_verify_drafts_at_the_edges(dt):
+    """Values next to a border, rows without weight, labels outside: everything here is exact in every type."""
+    V = 8
+    one = torch.zeros(V, dtype=dt)
+    one[3] = 1
+    half = torch.zeros(V, dtype=dt)
+    half[2], half[5] = 0.5, 0.5
+    none = torch.zeros(V, dtype=dt)
+    bad = torch.tensor([math.nan, -1, math.inf, 0, 0.25, math.nan, 0.25, -math.inf], dtype=dt)
+    rows = [
+        # p at the draft, p behind, q, label, u_accept, u_draw
+        (half, one, half, 2, 0.999, 0.0),        # p = q: always accepted; the draw from p behind
+        (half, one, one, 3, 0.0, 0.0),           # p = 0 at the label, q > 0, u = 0: 0 < 0 is false
+        (half, one, none, 2, 0.9, 0.3),          # q = 0 at the label: accepted
+        (none, one, none, 2, 0.0, 0.5),          # p = q = 0: rejected, nothing to draw from
+        (half, one, half, 9, 0.0, 0.49999),      # a label outside: rejected, p - q = 0 everywhere: the draw from p
+        (half, one, half, -1, 0.0, 0.5),         # ... on the border: the cumulative sum has to EXCEED u * total
+        (half, one, one, 3, 0.5, 0.0),           # u = 0: the first label with any weight
+        (half, one, one, 3, 0.5, 1 - 2.0 ** -53),
+        (bad, one, half, 4, 0.999, 0.0),         # q = 0 there
+        (bad, one, half, 2, 0.1, 0.75),          # p infinite there: counts as zero; the draw from what is finite and positive
+        (half, bad, half, 5, 0.2, 0.5),
+        (half, none, half, 5, 0.2, 0.5),
+    ]
+    p = torch.stack([torch.stack([r[0], r[1]]) for r in rows])
+    q = torch.stack([r[2][None] for r in rows])
+    z = torch.tensor([[r[3]] for r in rows])
+    ua, ud = torch.tensor([[r[4]] for r in rows], dtype=torch.float64), torch.tensor([r[5] for r in rows], dtype=torch.float64)
+    args = (p, q, z, ua, ud, torch.ones(len(rows), dtype=torch.int64))
+    want, got = verify_ref(*args), verify_on_gpu(*args)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[0], want[0]), (got, want)
+    assert want[1].tolist() == [1, 0, 1, 0, 0, 0, 0, 0, 1, 0, 1, 1]
+    assert want[0][3].tolist() == [-1, -1] and want[0][5].tolist() == [5, -1] and want[0][4].tolist() == [2, -1]
+
+
+@gpu
+def test_verified_labels_follow_the_target():
+    """The property the operator exists for: whatever the draft, the first label is distributed as the target says."""
+    g = torch.Generator("cuda").manual_seed(9)
+    from pybgmm_amd import ops
+    B, V = 400000, 6
+    p = torch.softmax(torch.randn(V, generator=g, device="cuda", dtype=torch.float64), 0)
+    q = torch.softmax(torch.randn(V, generator=g, device="cuda", dtype=torch.float64) * 2, 0)
+    z = torch.multinomial(q.float(), B, replacement=True, generator=g)[:, None]
+    ua, ud = torch.rand(B, 1, generator=g, device="cuda", dtype=torch.float64), torch.rand(B, generator=g, device="cuda", dtype=torch.float64)
+    out, acc = ops.verify_drafts(p.expand(B, 2, V), q.expand(B, 1, V), z, ua, ud)
+    share = torch.bincount(out[:, 0], minlength=V).double() / B
+    # (six standard deviations of a share of B draws; the draft's own float32 sampling is off by about 1e-7)
+    assert bool(((share - p).abs() <= 6 * torch.sqrt(p * (1 - p) / B) + 1e-6).all())
+    want = torch.minimum(p, q).sum()
+    assert abs(float(acc.double().mean() - want)) <= 6 * math.sqrt(0.25 / B) + 1e-6
+
+
+# ------------------------------------------------------------------------------------------ together
+def layer(lw, x, w1, b1, w2, k, K):
+    from pybgmm_amd import ops
+    labels, weights = ops.route(lw, k)
+    groups = ops.group_rows(labels, K)
+    h = torch.tanh(ops.grouped_matmul(x, w1, groups, bias=b1))
+    return ops.grouped_matmul(h, w2, groups, gates=weights)
+
+
+def layer_inputs(n=150, K=6, k=2, din=24, hid=40, dout=12):
+    g = torch.Generator("cuda").manual_seed(21)
+    t = [torch.randn(*s, generator=g, device="cuda", dtype=torch.float64) * 0.5 for s in
+         ((n, K), (n, din), (K, din, hid), (K, hid), (K, hid, dout))]
+    return t, k, K
+
+
+@gpu
+def test_a_layer_of_experts_routed_and_trained():
+    """route -> group_rows -> grouped_matmul twice, forward and backward, against the same layer written densely."""
+    t, k, K = layer_inputs()
+    leaves = [a.clone().requires_grad_() for a in t]
+    y = layer(*leaves, k, K)
+    dense = [a.clone().requires_grad_() for a in t]
+    lw, x, w1, b1, w2 = dense
+    top = torch.topk(lw, k, dim=1)
+    wts = torch.softmax(top.values, 1)
+    h = torch.tanh((x[:, None, None, :] @ w1[top.indices])[:, :, 0] + b1[top.indices])
+    want = ((h[:, :, None, :] @ w2[top.indices])[:, :, 0] * wts[..., None]).sum(1)
+    assert torch.allclose(y, want, rtol=0, atol=1e-12)
+    dy = torch.randn_like(y)
+    for a, b in zip(torch.autograd.grad(y, leaves, dy), torch.autograd.grad(want, dense, dy)):
+        assert torch.allclose(a, b, rtol=0, atol=1e-11)
+
+
+@gpu
+def test_another_stream_and_two_calls_at_once():
+    t, k, K = layer_inputs()
+    with torch.no_grad():
+        want = layer(*t, k, K)
+        half = layer(*[a * 0.5 for a in t], k, K)
+        torch.cuda.synchronize()
+        s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+        other = [a * 0.5 for a in t]
+        s1.wait_stream(torch.cuda.current_stream())
+        s2.wait_stream(torch.cuda.current_stream())
+        got = []
+        for _ in range(5):
+            with torch.cuda.stream(s1):
+                a = layer(*t, k, K)
+            with torch.cuda.stream(s2):
+                b = layer(*other, k, K)
+            got.append((a, b))
+        s1.synchronize()
+        s2.synchronize()
+    for a, b in got:
+        assert torch.equal(a, want) and torch.equal(b, half)
+
+
+@gpu
+def test_captured_and_replayed():
+    """The layer and a verification in one graph: every replay on new inputs equals the eager result."""
+    from pybgmm_amd import ops
+    t, k, K = layer_inputs(n=700)
+    draft = [a.cuda() for a in verify_case(9, 4, 300, torch.float32, 77)]
+    static = [a.clone() for a in t]
+    sdraft = [a.clone() for a in draft]
+
+    def both(a, d):
+        return (layer(*a, k, K),) + tuple(ops.verify_drafts(*d[:5], lengths=d[5]))
+    with torch.no_grad():
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            both(static, sdraft)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = both(static, sdraft)
+        for r in range(4):
+            new = [a + 0.3 * r * torch.randn_like(a) for a in t]
+            nd = [a.cuda() for a in verify_case(9, 4, 300, torch.float32, 100 + r)]
+            for dst, src in zip(static + sdraft, new + nd):
+                dst.copy_(src)
+            graph.replay()
+            torch.cuda.synchronize()
+            want = both(new, nd)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b), r
+
+
+@gpu
+def test_a_training_step_captured_and_replayed():
+    t, k, K = layer_inputs(n=300)
+    static = [a.clone().requires_grad_() for a in t]
+    dy = torch.randn(300, 12, device="cuda", dtype=torch.float64)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(layer(*static, k, K), static, dy)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(layer(*static, k, K), static, dy)
+    for r in range(3):
+        new = [a + 0.2 * r * torch.randn_like(a) for a in t]
+        with torch.no_grad():
+            for dst, src in zip(static, new):
+                dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        leaves = [a.clone().requires_grad_() for a in new]
+        want = torch.autograd.grad(layer(*leaves, k, K), leaves, dy)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), r
+
+
+@gpu
+def test_rows_beyond_32_bits_of_elements():
+    """A target whose rows start beyond 2^31 elements, and rows of x beyond 2^32 bytes."""
+    from pybgmm_amd import ops
+    V = 1 << 20
+    p = torch.zeros(1100, 2, V, device="cuda", dtype=torch.float16)              # 2.3e9 elements
+    q = torch.zeros(1, 1, V, device="cuda", dtype=torch.float16).expand(1100, 1, V)
+    p[1099, 0, 12345] = 0.5
+    p[1099, 1, V - 1] = 1
+    z = torch.full((1100, 1), 12345, device="cuda")
+    u = torch.full((1100, 1), 0.5, device="cuda", dtype=torch.float64)
+    out, acc = ops.verify_drafts(p, q, z, u, u[:, 0].contiguous())
+    assert out[1099].tolist() == [12345, V - 1] and int(acc.sum()) == 1 and bool((out[:1099] == -1).all())
+    del p, q
+    n, d = 2200000, 1024
+    x = torch.zeros(n, d, device="cuda", dtype=torch.float16)                    # 2.25e9 elements
+    x[n - 1] = 1
+    w = torch.ones(2, d, 16, device="cuda", dtype=torch.float16)
+    z = torch.zeros(n, dtype=torch.int64, device="cuda")
+    z[n - 1] = 1
+    y = ops.grouped_matmul(x, w, ops.group_rows(z, 2))
+    assert bool((y[n - 1] == d).all()) and not bool(y[:n - 1].any())
+
+
+# ------------------------------------------------------------------------------------------ the model classes' own calls
+@gpu
+def test_posterior_labels_and_standardised_points():
+    import numpy as np
+    from pybgmm_amd.igmm import CRPMM
+    from pybgmm_amd.prior import NIW
+    from pybgmm_amd.utils import gendata
+    import random
+    random.seed(3)
+    np.random.seed(3)
+    X, _ = gendata.synth_mixture(600, 5, 4, seed=2)
+    mm = CRPMM(X, NIW(np.zeros(5), 0.05, 8, np.eye(5)), 1.0, None, assignments="rand", K=6)
+    mm.collapsed_gibbs_sampler(5, np.zeros(600, dtype=int))
+    comp, K = mm.components, mm.components.K
+    # the densities are the sampler's own: log_post_pred of a training point, the prior's log predictive
+    dens = comp.log_predictive(X[:40])
+    for i in range(40):
+        np.testing.assert_allclose(dens[i, :K], comp.log_post_pred(i), rtol=1e-9, atol=1e-9)
+        np.testing.assert_allclose(dens[i, K], comp.log_prior(i), rtol=1e-9, atol=1e-9)
+    # labels and weights: the visit's normalised weights
+    lw = dens + np.log(np.append(comp.counts[:K].astype(float), mm.alpha))
+    p = np.exp(lw - lw.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    labels, w = mm.posterior_labels(X[:40], k=min(3, K + 1))
+    order = np.argsort(-lw, axis=1, kind="stable")[:, :labels.shape[1]]
+    np.testing.assert_array_equal(labels, order)
+    np.testing.assert_allclose(w, np.take_along_axis(p, order, 1), rtol=1e-9, atol=1e-13)
+    t_labels, t_w = mm.posterior_labels(torch.from_numpy(X[:40]).cuda(), k=labels.shape[1])
+    assert np.array_equal(t_labels.cpu().numpy(), labels) and np.array_equal(t_w.cpu().numpy(), w)
+    # standardised points: mean and scale of the predictive taken out
+    r = comp.standardise()
+    z, counts = comp.assignments, comp.counts
+    m, S = comp.m_N_numerators, comp.S_N_partials
+    for i in range(0, 600, 37):
+        k = z[i]
+        kN, vN = 0.05 + counts[k], 8 + counts[k]
+        mean = m[k] / kN
+        cov = (kN + 1) / (kN * (vN - 5 + 1)) * (S[k] - kN * np.outer(mean, mean))
+        want = np.linalg.solve(np.linalg.cholesky(cov), X[i] - mean)
+        np.testing.assert_allclose(r[i], want, rtol=1e-9, atol=1e-9)
+    assert not comp.standardise(X[:3], np.array([-1, 0, -1]))[[0, 2]].any()
+    with pytest.raises(ValueError):
+        comp.standardise(X[:3])
+    with pytest.raises(ValueError):
+        mm.posterior_labels(X[:, :4])
+
+
+@gpu
+def test_diagonal_components_have_no_factors():
+    import numpy as np
+    from pybgmm_amd.igmm import CRPMM
+    from pybgmm_amd.prior import NIW
+    X = np.random.RandomState(0).randn(30, 3)
+    mm = CRPMM(X, NIW(np.zeros(3), 0.1, 5, np.ones(3)), 1.0, None, assignments="rand", K=2, covariance_type="diag")
+    with pytest.raises(NotImplementedError):
+        mm.posterior_labels(X)
