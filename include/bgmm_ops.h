@@ -117,10 +117,13 @@ BGMM_OPS_API int bgmm_route_backward(int32_t dtype, const void *log_weights, int
  *   target [B][T + 1][V], draft [B][T][V]  strides _b, _t;  labels [B][T];  u_accept [B][T], u_draw [B] in [0, 1)
  *   lengths [B]: drafts of each sequence (0 .. T, clamped), or NULL: T
  *   out [B][T + 1]: the accepted labels, the drawn one, -1 behind;  accepted [B]
+ *   ws: bgmm_verify_drafts_ws(B, V) bytes
  */
+BGMM_OPS_API int64_t bgmm_verify_drafts_ws(int64_t B, int64_t V);
 BGMM_OPS_API int bgmm_verify_drafts(int32_t dtype, const void *target, int64_t target_b, int64_t target_t, const void *draft, int64_t draft_b,
                                     int64_t draft_t, const int64_t *labels, const double *u_accept, const double *u_draw,
-                                    const int64_t *lengths, int64_t B, int32_t T, int64_t V, int64_t *out, int64_t *accepted, void *stream);
+                                    const int64_t *lengths, int64_t B, int32_t T, int64_t V, int64_t *out, int64_t *accepted, void *ws,
+                                    int64_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

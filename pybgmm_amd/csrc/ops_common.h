@@ -42,6 +42,39 @@ __device__ __forceinline__ unsigned long long wave_match(int key, int nbits, boo
     return m;
 }
 
+// Exchange within a row of 16 lanes without the LDS crossbar; all-reduce of groups of G lanes (8, 16, 32, 64).
+template <int CTRL> __device__ __forceinline__ int lane_move(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false); }
+template <int CTRL> __device__ __forceinline__ float lane_move(float v) { return __int_as_float(lane_move<CTRL>(__float_as_int(v))); }
+template <int CTRL> __device__ __forceinline__ double lane_move(double v) {
+    return __hiloint2double(lane_move<CTRL>(__double2hiint(v)), lane_move<CTRL>(__double2loint(v)));
+}
+template <int G, class V, class F> __device__ __forceinline__ V group_reduce(V v, F f) {
+    v = f(v, lane_move<0xB1>(v));                   // quad_perm [1,0,3,2]
+    v = f(v, lane_move<0x4E>(v));                   // quad_perm [2,3,0,1]
+    v = f(v, lane_move<0x141>(v));                  // row_half_mirror
+    if (G >= 16) v = f(v, lane_move<0x140>(v));     // row_mirror
+    if (G >= 32) v = f(v, __shfl_xor(v, 16));
+    if (G >= 64) v = f(v, __shfl_xor(v, 32));
+    return v;
+}
+template <int G, class V> __device__ __forceinline__ V group_sum(V v) {
+    return group_reduce<G>(v, [](V a, V b) { return a + b; });
+}
+
+// Inclusive sum over the wave's lanes: inside a row of 16 by row shifts, the rows' totals through readlane.
+__device__ __forceinline__ double lane_read(double v, int l) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
+}
+__device__ __forceinline__ double wave_scan_sum(double v) {
+    v += lane_move<0x111>(v);
+    v += lane_move<0x112>(v);
+    v += lane_move<0x114>(v);
+    v += lane_move<0x118>(v);
+    const double t0 = lane_read(v, 15), t1 = t0 + lane_read(v, 31), t2 = t1 + lane_read(v, 47);
+    const int row = wave_lane() >> 4;
+    return v + (row == 0 ? 0.0 : row == 1 ? t0 : row == 2 ? t1 : t2);
+}
+
 // Which bucket tile t belongs to: the last b in 0 .. n-1 with first[b] <= t (first is non-decreasing, first[0] = 0; t is
 // below first[n]).  64 candidates per probe: two probes up to 4096 buckets, three beyond.  Every wave of a workgroup
 // finds the same answer by itself.

@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kSmall = 8192;            // rows of the one-workgroup form
 constexpr int kWaves = 16;              // its waves
-constexpr int kSmallBuckets = 960;      // its buckets (K + 1): 16 histograms, the sizes and the sums fit 64 KB of LDS
+constexpr int kSmallBuckets = 940;      // its buckets (K + 1): 16 histograms, the sizes and the sums fit 64 KB of LDS
 constexpr int kSegWaves = 4;            // segments (waves) per workgroup of the three-launch form while 4 histograms fit 64 KB
 
 __device__ __forceinline__ int bucket_of(const int64_t *labels, i64 i, int K) {
@@ -57,12 +57,49 @@ __device__ __forceinline__ int block_scan(int n, int *part, F f, G g) {
     return carry;
 }
 
-__device__ __forceinline__ void write_level(int level, int K, const int *size_of, int *first, int *part) {
-    int *out = first + (i64)level * (K + 2);
-    const int lg = 4 + level;
-    const int total = block_scan(K + 1, part, [&](int b) { return (int)(((i64)size_of[b] + (1 << lg) - 1) >> lg); },
-                                 [&](int b, int s) { out[b] = s; });
-    if (threadIdx.x == 0) out[K + 1] = total;
+// All the prefix sums over buckets at once: offsets (handed to place(b, start)) and every level of tiles.  `part`:
+// kSums * waves ints.
+constexpr int kSums = BGMM_OPS_LEVELS + 1;
+template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows, const int *size_of, int *offsets, int *first, int *part, P place) {
+    const int nw = blockDim.x >> 6, w = threadIdx.x >> 6, B = K + 1;
+    int carry[kSums];
+#pragma unroll
+    for (int l = 0; l < kSums; ++l) carry[l] = 0;
+    for (int base = 0; base < B; base += blockDim.x) {
+        const int b = base + threadIdx.x, size = b < B ? size_of[b] : 0;
+        int incl[kSums];
+#pragma unroll
+        for (int l = 0; l < kSums; ++l) {
+            const int v = l == 0 ? size : (int)(((i64)size + (8 << l) - 1) >> (3 + l));
+            const int t = wave_incl_scan(v);
+            if (wave_lane() == 63) part[l * nw + w] = t;
+            incl[l] = t - v;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int l = 0; l < kSums; ++l) {
+            int before = carry[l] + incl[l];
+            for (int j = 0; j < nw; ++j) {
+                const int t = part[l * nw + j];
+                if (j < w) before += t;
+                carry[l] += t;
+            }
+            if (b < B) {
+                if (l == 0) {
+                    offsets[b] = before;
+                    place(b, before);
+                } else {
+                    first[(i64)(l - 1) * (K + 2) + b] = before;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        offsets[B] = P_rows;
+#pragma unroll
+        for (int l = 1; l < kSums; ++l) first[(i64)(l - 1) * (K + 2) + B] = carry[l];
+    }
 }
 
 // A wave walks rows [lo, hi): cursor[b] moves by the rows of bucket b, write(i, b, place) sees every row's place.
@@ -85,19 +122,19 @@ __device__ __forceinline__ void walk(const int64_t *labels, i64 lo, i64 hi, int 
 __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels, int P, int K, int nbits, int *bucket, int *order,
                                                            int *offsets, int *first) {
     extern __shared__ int lds[];
-    int *hist = lds;                          // [kWaves][K + 1]
-    int *sizes = hist + kWaves * (K + 1);     // [K + 1]
-    int *part = sizes + K + 1;                // [kWaves]
-    const int B = K + 1, w = threadIdx.x >> 6;
-    for (int j = threadIdx.x; j < kWaves * B; j += blockDim.x) hist[j] = 0;
+    const int B = K + 1, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    int *hist = lds;                          // [waves][K + 1]
+    int *sizes = hist + nw * B;               // [K + 1]
+    int *part = sizes + B;                    // [kSums * waves]
+    for (int j = threadIdx.x; j < nw * B; j += blockDim.x) hist[j] = 0;
     __syncthreads();
-    const int per = ((P + kWaves - 1) / kWaves + 63) & ~63;
+    const int per = ((P + nw - 1) / nw + 63) & ~63;
     const int lo = w * per < P ? w * per : P, hi = lo + per < P ? lo + per : P;
     walk(labels, lo, hi, K, nbits, hist + w * B, [&](i64 i, int b, int) { bucket[i] = b; });
     __syncthreads();
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
         int s = 0;
-        for (int j = 0; j < kWaves; ++j) {
+        for (int j = 0; j < nw; ++j) {
             const int n = hist[j * B + b];
             hist[j * B + b] = s;
             s += n;
@@ -105,14 +142,10 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
         sizes[b] = s;
     }
     __syncthreads();
-    block_scan(B, part, [&](int b) { return sizes[b]; },
-               [&](int b, int s) {
-                   offsets[b] = s;
-                   for (int j = 0; j < kWaves; ++j) hist[j * B + b] += s;
-               });
-    if (threadIdx.x == 0) offsets[B] = P;
+    write_sums(K, P, sizes, offsets, first, part, [&](int b, int start) {
+        for (int j = 0; j < nw; ++j) hist[j * B + b] += start;
+    });
     walk(labels, lo, hi, K, nbits, hist + w * B, [&](i64 i, int, int at) { order[at] = (int)i; });
-    for (int l = 0; l < BGMM_OPS_LEVELS; ++l) write_level(l, K, sizes, first, part);
 }
 
 __global__ void group_count(const int64_t *labels, i64 P, int K, int nbits, int seg, int nseg, int *bucket, int *counts) {
@@ -128,16 +161,27 @@ __global__ void group_count(const int64_t *labels, i64 P, int K, int nbits, int 
         for (int b = wave_lane(); b < B; b += 64) counts[(i64)s * B + b] = hist[b];
 }
 
-// One wave per bucket: counts[.][b] becomes the exclusive sum over the segments, sizes[b] the total.
+// One wave per bucket: counts[.][b] becomes the exclusive sum over the segments, sizes[b] the total.  A lane has kRun
+// consecutive segments, so that a round has kRun loads in flight instead of one.
+constexpr int kRun = 8;
 __global__ void group_columns(int *counts, int nseg, int B, int *sizes) {
     const int b = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
     if (b >= B) return;
     int carry = 0;
-    for (int s0 = 0; s0 < nseg; s0 += 64) {
-        const int s = s0 + wave_lane();
-        const int v = s < nseg ? counts[(i64)s * B + b] : 0;
-        const int incl = wave_incl_scan(v);
-        if (s < nseg) counts[(i64)s * B + b] = carry + incl - v;
+    for (int s0 = 0; s0 < nseg; s0 += 64 * kRun) {
+        const int s = s0 + wave_lane() * kRun;
+        int v[kRun], sum = 0;
+#pragma unroll
+        for (int r = 0; r < kRun; ++r) v[r] = s + r < nseg ? counts[(i64)(s + r) * B + b] : 0;
+#pragma unroll
+        for (int r = 0; r < kRun; ++r) sum += v[r];
+        const int incl = wave_incl_scan(sum);
+        int before = carry + incl - sum;
+#pragma unroll
+        for (int r = 0; r < kRun; ++r) {
+            if (s + r < nseg) counts[(i64)(s + r) * B + b] = before;
+            before += v[r];
+        }
         carry += __shfl(incl, 63);
     }
     if (wave_lane() == 0) sizes[b] = carry;
@@ -149,16 +193,14 @@ __global__ void group_scatter(const int64_t *labels, i64 P, int K, int nbits, in
     const int nw = blockDim.x >> 6;
     const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * nw + w;
     int *start = lds + nw * B, *part = start + B;
-    block_scan(B, part, [&](int b) { return sizes[b]; }, [&](int b, int v) { start[b] = v; });
+    if (blockIdx.x == 0) write_sums(K, (int)P, sizes, offsets, first, part, [&](int b, int v) { start[b] = v; });
+    else block_scan(B, part, [&](int b) { return sizes[b]; }, [&](int b, int v) { start[b] = v; });
     int *cursor = lds + w * B;
     if (s < nseg)
         for (int b = wave_lane(); b < B; b += 64) cursor[b] = start[b] + counts[(i64)s * B + b];
     __syncthreads();
     const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
     walk(labels, lo, hi, K, nbits, cursor, [&](i64 i, int, int at) { order[at] = (int)i; });
-    if (blockIdx.x == 0)
-        for (int b = threadIdx.x; b <= B; b += blockDim.x) offsets[b] = b < B ? start[b] : (int)P;
-    for (int l = blockIdx.x; l < BGMM_OPS_LEVELS; l += gridDim.x) write_level(l, K, sizes, first, part);
 }
 
 struct Split { int seg, nseg, waves; };
@@ -196,8 +238,9 @@ extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int3
     int nbits = 1;
     while ((1 << nbits) < B) ++nbits;
     if (small_form(P, K)) {
-        const size_t lds = sizeof(int) * ((size_t)(kWaves + 1) * B + kWaves);
-        group_small<<<1, 64 * kWaves, lds, st>>>(labels, (int)P, K, nbits, bucket, order, offsets, first);
+        const int waves = P <= 1024 ? 4 : kWaves;
+        const size_t lds = sizeof(int) * ((size_t)(waves + 1) * B + kSums * waves);
+        group_small<<<1, 64 * waves, lds, st>>>(labels, (int)P, K, nbits, bucket, order, offsets, first);
         return ops_launched("group_rows");
     }
     const Split s = split_of(P, K);
@@ -206,7 +249,7 @@ extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int3
     const int blocks = s.nseg > 0 ? (s.nseg + s.waves - 1) / s.waves : 1;
     group_count<<<blocks, 64 * s.waves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, nbits, s.seg, s.nseg, bucket, counts);
     group_columns<<<(B + 3) / 4, 256, 0, st>>>(counts, s.nseg, B, sizes);
-    group_scatter<<<blocks, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + 16), st>>>(labels, P, K, nbits, s.seg, s.nseg, counts, sizes,
+    group_scatter<<<blocks, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + kSums * s.waves), st>>>(labels, P, K, nbits, s.seg, s.nseg, counts, sizes,
                                                                                                 order, offsets, first);
     return ops_launched("group_rows");
 }

@@ -192,4 +192,4 @@ struct CombineArgs {
 // One product with rows; `small`: tiles of 16 rows, else 128.  `kcontig`: the weights' contiguous axis is the contraction.
 template <class T> int launch_rows(const RowsArgs &a, bool kcontig, bool vec, bool small, i64 blocks, hipStream_t st);
 template <class T> int launch_weight(const WeightArgs &a, bool vec, i64 blocks, hipStream_t st);
-template <class T> int launch_combine(const CombineArgs &a, hipStream_t st);
+template <class T> int launch_combine(const CombineArgs &a, bool vec, hipStream_t st);

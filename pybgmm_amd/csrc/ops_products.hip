@@ -164,5 +164,9 @@ extern "C" int bgmm_combine(int32_t dtype, const void *ws, int32_t splits, int64
     a.d_stride = d_stride;
     a.d_div = d_div < 1 ? 1 : d_div;
     a.ddim = ddim;
-    return by_type(dtype, [&](auto *t) { return launch_combine<std::remove_pointer_t<decltype(t)>>(a, (hipStream_t)stream); });
+    const int S = size_of(dtype);
+    const auto fours = [&](const void *p, i64 stride) { return !p || (stride % 4 == 0 && aligned(p, S == 2 ? 8 : 16)); };
+    const bool vec = dim % 4 == 0 && aligned(ws, 16) && fours(out, out_stride) &&
+                     (!dgates || (fours(in, in_stride) && (!bias || (ddim % 4 == 0 && fours(bias, bias_row) && fours(d, d_stride)))));
+    return by_type(dtype, [&](auto *t) { return launch_combine<std::remove_pointer_t<decltype(t)>>(a, vec, (hipStream_t)stream); });
 }

@@ -2,4 +2,4 @@
 
 template int launch_rows<bf16_t>(const RowsArgs &, bool, bool, bool, i64, hipStream_t);
 template int launch_weight<bf16_t>(const WeightArgs &, bool, i64, hipStream_t);
-template int launch_combine<bf16_t>(const CombineArgs &, hipStream_t);
+template int launch_combine<bf16_t>(const CombineArgs &, bool, hipStream_t);

@@ -18,8 +18,12 @@ template <class T, class V> __device__ __forceinline__ void store4(T *p, const V
     }
 }
 
+// Steps of operands in flight in registers.  A 128 x 128 step of half precision is 1024 cycles of matrix instructions, less than
+// a load from memory takes under load: two.  Single and double precision spend 4096 on theirs: one.
+template <class T> constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;
+
 template <class T, bool KCONTIG, bool VEC, int BM, int BN, int WN, int WM>
-__global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
+__global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
     typedef typename Acc<T>::type A;
     typedef typename Acc<T>::v4 A4;
     constexpr int FA = BN / WN / 16, FB = BM / WM / 16;
@@ -67,37 +71,37 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     }
     const T *w = (const T *)a.w + (i64)e * a.w_component;
     typedef MTile<T, BN> WTile;
-    Granule gx[XP], gw[WP];
-    const auto fetch = [&](int k0) {
-        const int kk = k0 + (tid & 7) * kGran<T>;
+    struct Held { Granule x[XP], w[WP]; } held[kAhead<T>];
+    const auto fetch = [&](Held &h, int s) {
+        const int k0 = s * kStep<T>, kk = k0 + (tid & 7) * kGran<T>;
 #pragma unroll
         for (int p = 0; p < XP; ++p)
-            if (BM >= 32 || tid < BM * 8) gx[p] = load_granule<T, VEC>(xrow[p] + kk, k_end - kk);
+            if (BM >= 32 || tid < BM * 8) h.x[p] = load_granule<T, VEC>(xrow[p] + kk, k_end - kk);
 #pragma unroll
         for (int p = 0; p < WP; ++p) {
             if (BN < 32 && tid >= BN * 8) continue;
             if (KCONTIG) {
                 const int n = n0 + (tid >> 3) + p * 32;
-                gw[p] = load_granule<T, VEC>(w + (i64)n * a.w_row + kk, n < a.ndim ? k_end - kk : 0);
+                h.w[p] = load_granule<T, VEC>(w + (i64)n * a.w_row + kk, n < a.ndim ? k_end - kk : 0);
             } else {
                 const int g = tid + p * 256, k = k0 + g / WTile::kPerRow, n = n0 + (g % WTile::kPerRow) * kGran<T>;
-                gw[p] = load_granule<T, VEC>(w + (i64)k * a.w_row + n, k < k_end ? a.ndim - n : 0);
+                h.w[p] = load_granule<T, VEC>(w + (i64)k * a.w_row + n, k < k_end ? a.ndim - n : 0);
             }
         }
     };
-    const auto put = [&](char *buf) {
+    const auto put = [&](const Held &h, char *buf) {
 #pragma unroll
         for (int p = 0; p < XP; ++p)
-            if (BM >= 32 || tid < BM * 8) *(v4i *)(buf + KTile<T>::at((tid >> 3) + p * 32, tid & 7)) = gx[p].raw;
+            if (BM >= 32 || tid < BM * 8) *(v4i *)(buf + KTile<T>::at((tid >> 3) + p * 32, tid & 7)) = h.x[p].raw;
         char *wb = buf + BM * kStepBytes;
 #pragma unroll
         for (int p = 0; p < WP; ++p) {
             if (BN < 32 && tid >= BN * 8) continue;
             if (KCONTIG) {
-                *(v4i *)(wb + KTile<T>::at((tid >> 3) + p * 32, tid & 7)) = gw[p].raw;
+                *(v4i *)(wb + KTile<T>::at((tid >> 3) + p * 32, tid & 7)) = h.w[p].raw;
             } else {
                 const int g = tid + p * 256;
-                *(v4i *)(wb + WTile::at(g / WTile::kPerRow, g % WTile::kPerRow)) = gw[p].raw;
+                *(v4i *)(wb + WTile::at(g / WTile::kPerRow, g % WTile::kPerRow)) = h.w[p].raw;
             }
         }
     };
@@ -107,18 +111,10 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     for (int i = 0; i < FA; ++i)
 #pragma unroll
         for (int j = 0; j < FB; ++j) acc[i][j] = (A4){0, 0, 0, 0};
-
-    if (s_lo < s_hi) {
-        fetch(s_lo * kStep<T>);
-        put(lds[0]);
-    }
-    __syncthreads();
-    for (int s = s_lo; s < s_hi; ++s) {
-        const char *buf = lds[(s - s_lo) & 1], *wb = buf + BM * kStepBytes;
-        if (s + 1 < s_hi) fetch((s + 1) * kStep<T>);
+    const auto compute = [&](const char *buf) {
+        const char *wb = buf + BM * kStepBytes;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            if (ks && s * kStep<T> + kStep<T> / 2 >= k_end) break;
             Granule fa[FA], fb[FB];
 #pragma unroll
             for (int i = 0; i < FA; ++i) {
@@ -132,9 +128,33 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 #pragma unroll
                 for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j]);
         }
-        if (s + 1 < s_hi) put(lds[(s + 1 - s_lo) & 1]);
-        __syncthreads();
+    };
+
+    // step s: its operands are in lds[s & 1], those of s + 1 (and s + 2) on their way
+    const int n_steps = s_hi - s_lo;
+    if (n_steps > 0) {
+        fetch(held[0], s_lo);
+        if (kAhead<T> == 2 && n_steps > 1) fetch(held[kAhead<T> - 1], s_lo + 1);
+        put(held[0], lds[0]);
     }
+    __syncthreads();
+    int s = 0;
+    const auto step = [&](int slot) {               // slot = s & 1, known at compile time
+        if (kAhead<T> == 2) {
+            if (s + 2 < n_steps) fetch(held[slot], s_lo + s + 2);
+        } else {
+            if (s + 1 < n_steps) fetch(held[0], s_lo + s + 1);
+        }
+        compute(lds[slot]);
+        if (s + 1 < n_steps) put(held[kAhead<T> == 2 ? 1 - slot : 0], lds[1 - slot]);
+        __syncthreads();
+        ++s;
+    };
+    while (s + 1 < n_steps) {
+        step(0);
+        step(1);
+    }
+    if (s < n_steps) step(0);
 
     // ---- results: lane l has elements 4 (l / 16) .. + 3 of the block's columns for row l % 16 of the block's rows
     const T *bias = a.bias && split == 0 ? (const T *)a.bias + (i64)e * a.bias_row : nullptr;
@@ -165,15 +185,15 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 
 // dW: the rows of a chunk are the contraction, both operands have it outermost (MTile).  Half precision: g d is rounded to
 // the operand type before the product (like the operands themselves), its column sums for db are not.
-template <class T, bool VEC, int BI, int BO, int WO, int WI>
-__global__ __launch_bounds__(256) void weight_kernel(WeightArgs a) {
+template <class T, bool VEC, int BT, int WO, int WI>
+__global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
     typedef typename Acc<T>::type A;
     typedef typename Acc<T>::v4 A4;
-    constexpr int FA = BO / WO / 16, FB = BI / WI / 16;
-    constexpr int IP = (BI + 31) / 32, OP = (BO + 31) / 32;
-    typedef MTile<T, BI> ITile;
-    typedef MTile<T, BO> OTile;
-    __shared__ __attribute__((aligned(128))) char lds[2][(BI + BO) * kStepBytes];
+    constexpr int FA = BT / WO / 16, FB = BT / WI / 16;
+    constexpr int NP = (BT + 31) / 32;                          // granules of either operand a thread moves per step
+    constexpr bool kAll = BT >= 32;                             // every thread moves some
+    typedef MTile<T, BT> Tile;
+    __shared__ __attribute__((aligned(128))) char lds[2][2 * BT * kStepBytes];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wo = wave % WO, wi = wave / WO;
     const i64 out_tiles = (i64)a.i_tiles * a.o_tiles;
@@ -185,61 +205,59 @@ __global__ __launch_bounds__(256) void weight_kernel(WeightArgs a) {
     const int rows_per = 16 << a.level;
     const int row0 = a.offsets[e] + c * rows_per, left = a.offsets[e + 1] - row0, n_rows = left < rows_per ? left : rows_per;
     const int *list = a.order + row0;
-    const int i0 = (tile % a.i_tiles) * BI, o0 = (tile / a.i_tiles) * BO;
+    const int i0 = (tile % a.i_tiles) * BT, o0 = (tile / a.i_tiles) * BT;
     const A *gates = (const A *)a.gates;
     const bool want_db = a.db && i0 == 0;
 
-    Granule gi[IP], go[OP];
-    A dsum[OP][kGran<T>];
+    // a thread moves the same granule column of rows r, r + kRows, ...; both operands' rows go by the same index, read one
+    // step before its rows are asked for
+    constexpr int kRows = 256 / Tile::kPerRow < kStep<T> ? 256 / Tile::kPerRow : kStep<T>;
+    const int my_row = tid / Tile::kPerRow, my_col = (tid % Tile::kPerRow) * kGran<T>;
+    struct Held { Granule i[NP], o[NP]; A gate[NP]; } held[kAhead<T>];
+    int at[NP];
+    const auto look = [&](int s) {
 #pragma unroll
-    for (int p = 0; p < OP; ++p)
-#pragma unroll
-        for (int j = 0; j < kGran<T>; ++j) dsum[p][j] = 0;
-    const auto fetch = [&](int r0) {
-#pragma unroll
-        for (int p = 0; p < IP; ++p) {
-            if (BI < 32 && tid >= BI * 8) continue;
-            const int g = tid + p * 256, r = r0 + g / ITile::kPerRow, n = i0 + (g % ITile::kPerRow) * kGran<T>;
-            const int rr = r < n_rows ? r : n_rows - 1;
-            gi[p] = load_granule<T, VEC>((const T *)a.in + (i64)((unsigned)list[rr] / (unsigned)a.in_div) * a.in_stride + n,
-                                         r < n_rows ? a.idim - n : 0);
+        for (int p = 0; p < NP; ++p) {
+            const int r = s * kStep<T> + my_row + p * kRows;
+            at[p] = list[r < n_rows ? r : n_rows - 1];
         }
+    };
+    const auto fetch = [&](Held &h, int s) {        // (at: the indices of step s; leaves those of s + 1)
+        if (kAll || tid < BT * 8) {
 #pragma unroll
-        for (int p = 0; p < OP; ++p) {
-            if (BO < 32 && tid >= BO * 8) continue;
-            const int g = tid + p * 256, r = r0 + g / OTile::kPerRow, n = o0 + (g % OTile::kPerRow) * kGran<T>;
-            const int rr = r < n_rows ? r : n_rows - 1;
-            const int pair = list[rr];
-            go[p] = load_granule<T, VEC>((const T *)a.d + (i64)((unsigned)pair / (unsigned)a.d_div) * a.d_stride + n,
-                                         r < n_rows ? a.odim - n : 0);
+            for (int p = 0; p < NP; ++p) {
+                const bool on = s * kStep<T> + my_row + p * kRows < n_rows;
+                h.i[p] = load_granule<T, VEC>((const T *)a.in + (i64)((unsigned)at[p] / (unsigned)a.in_div) * a.in_stride + i0 + my_col,
+                                              on ? a.idim - i0 - my_col : 0);
+                h.o[p] = load_granule<T, VEC>((const T *)a.d + (i64)((unsigned)at[p] / (unsigned)a.d_div) * a.d_stride + o0 + my_col,
+                                              on ? a.odim - o0 - my_col : 0);
+                if (gates) h.gate[p] = on ? gates[at[p]] : (A)0;
+            }
+        }
+        look(s + 1);
+    };
+    A dsum[kGran<T>];
+#pragma unroll
+    for (int j = 0; j < kGran<T>; ++j) dsum[j] = 0;
+    const auto put = [&](Held &h, char *buf) {
+        if (!kAll && tid >= BT * 8) return;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
             if (gates) {
-                const A gate = gates[pair];
-                T *el = Elems<T>::of(go[p]);
+                T *el = Elems<T>::of(h.o[p]);
 #pragma unroll
                 for (int j = 0; j < kGran<T>; ++j) {
-                    const A v = r < n_rows ? (A)el[j] * gate : (A)0;
-                    dsum[p][j] += v;
+                    const A v = (A)el[j] * h.gate[p];
+                    dsum[j] += v;
                     el[j] = (T)v;
                 }
             } else if (want_db) {
-                T *el = Elems<T>::of(go[p]);
+                T *el = Elems<T>::of(h.o[p]);
 #pragma unroll
-                for (int j = 0; j < kGran<T>; ++j) dsum[p][j] += (A)el[j];
+                for (int j = 0; j < kGran<T>; ++j) dsum[j] += (A)el[j];
             }
-        }
-    };
-    const auto put = [&](char *buf) {
-#pragma unroll
-        for (int p = 0; p < IP; ++p) {
-            if (BI < 32 && tid >= BI * 8) continue;
-            const int g = tid + p * 256;
-            *(v4i *)(buf + ITile::at(g / ITile::kPerRow, g % ITile::kPerRow)) = gi[p].raw;
-        }
-#pragma unroll
-        for (int p = 0; p < OP; ++p) {
-            if (BO < 32 && tid >= BO * 8) continue;
-            const int g = tid + p * 256;
-            *(v4i *)(buf + BI * kStepBytes + OTile::at(g / OTile::kPerRow, g % OTile::kPerRow)) = go[p].raw;
+            *(v4i *)(buf + Tile::at(my_row + p * kRows, tid % Tile::kPerRow)) = h.i[p].raw;
+            *(v4i *)(buf + BT * kStepBytes + Tile::at(my_row + p * kRows, tid % Tile::kPerRow)) = h.o[p].raw;
         }
     };
 
@@ -248,29 +266,44 @@ __global__ __launch_bounds__(256) void weight_kernel(WeightArgs a) {
     for (int i = 0; i < FA; ++i)
 #pragma unroll
         for (int j = 0; j < FB; ++j) acc[i][j] = (A4){0, 0, 0, 0};
-    fetch(0);
-    put(lds[0]);
-    __syncthreads();
-    const int steps = (n_rows + kStep<T> - 1) / kStep<T>;
-    for (int s = 0; s < steps; ++s) {
-        const char *buf = lds[s & 1];
-        if (s + 1 < steps) fetch((s + 1) * kStep<T>);
+    const auto compute = [&](const char *buf) {
+        if (WO * WI < 4 && wave >= WO * WI) return;             // (a tile too small for four waves: the others only move data)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            if (WO * WI < 4 && wave >= WO * WI) break;          // (a tile too small for four waves: the others only move data)
             Granule fa[FA], fb[FB];
 #pragma unroll
-            for (int i = 0; i < FA; ++i) fa[i] = OTile::template read<true>(buf + BI * kStepBytes, (wo * FA + i) * 16, ks);
+            for (int i = 0; i < FA; ++i) fa[i] = Tile::template read<true>(buf + BT * kStepBytes, (wo * FA + i) * 16, ks);
 #pragma unroll
-            for (int j = 0; j < FB; ++j) fb[j] = ITile::template read<false>(buf, (wi * FB + j) * 16, ks);
+            for (int j = 0; j < FB; ++j) fb[j] = Tile::template read<false>(buf, (wi * FB + j) * 16, ks);
 #pragma unroll
             for (int i = 0; i < FA; ++i)
 #pragma unroll
                 for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j]);
         }
-        if (s + 1 < steps) put(lds[(s + 1) & 1]);
+    };
+    const int n_steps = (n_rows + kStep<T> - 1) / kStep<T>;     // (at least one: a chunk has rows)
+    look(0);
+    fetch(held[0], 0);
+    if (kAhead<T> == 2 && n_steps > 1) fetch(held[kAhead<T> - 1], 1);
+    put(held[0], lds[0]);
+    __syncthreads();
+    int s = 0;
+    const auto step = [&](int slot) {
+        if (kAhead<T> == 2) {
+            if (s + 2 < n_steps) fetch(held[slot], s + 2);
+        } else {
+            if (s + 1 < n_steps) fetch(held[0], s + 1);
+        }
+        compute(lds[slot]);
+        if (s + 1 < n_steps) put(held[kAhead<T> == 2 ? 1 - slot : 0], lds[1 - slot]);
         __syncthreads();
+        ++s;
+    };
+    while (s + 1 < n_steps) {
+        step(0);
+        step(1);
     }
+    if (s < n_steps) step(0);
 
     // a component with one chunk is finished here; several leave partial sums, added in the chunks' order by weight_reduce
     A *slot = nullptr;
@@ -291,22 +324,16 @@ __global__ __launch_bounds__(256) void weight_kernel(WeightArgs a) {
     }
     if (!want_db) return;
     // column sums: a thread has those of its granule's columns over its own rows; the threads of a column add up in order
-    A *sums = (A *)lds;                       // [rows of a pass][BO]
-    constexpr int kRowsPass = BO < 32 ? BO * 8 / OTile::kPerRow : 256 / OTile::kPerRow;
+    A *sums = (A *)lds;                       // [kRows][BT]
     __syncthreads();
-    if (BO >= 32 || tid < BO * 8) {
+    if (kAll || tid < BT * 8) {
 #pragma unroll
-        for (int j = 0; j < kGran<T>; ++j) {
-            A v = 0;
-#pragma unroll
-            for (int p = 0; p < OP; ++p) v += dsum[p][j];
-            sums[(tid / OTile::kPerRow) * BO + (tid % OTile::kPerRow) * kGran<T> + j] = v;
-        }
+        for (int j = 0; j < kGran<T>; ++j) sums[my_row * BT + my_col + j] = dsum[j];
     }
     __syncthreads();
-    for (int n = tid; n < BO && o0 + n < a.odim; n += 256) {
+    for (int n = tid; n < BT && o0 + n < a.odim; n += 256) {
         A v = 0;
-        for (int r = 0; r < kRowsPass; ++r) v += sums[r * BO + n];
+        for (int r = 0; r < kRows; ++r) v += sums[r * BT + n];
         if (slot) slot[(i64)a.idim * a.odim + o0 + n] = v;
         else ((T *)a.db)[(i64)e * a.odim + o0 + n] = (T)v;
     }
@@ -330,37 +357,63 @@ template <class T> __global__ __launch_bounds__(256) void weight_reduce(WeightAr
     }
 }
 
+// Four elements of a row as accumulators; VEC: all there and aligned.
+template <class S, class A, bool VEC> __device__ __forceinline__ void load4(const S *p, int avail, A (&v)[4]) {
+    struct alignas(sizeof(S) * 4 < 16 ? sizeof(S) * 4 : 16) Four { S e[4]; };
+    if (VEC) {
+        const Four f = *(const Four *)p;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = (A)f.e[x];
+    } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = x < avail ? (A)p[x] : (A)0;
+    }
+}
+
+// u_p, the sum of its parts
+template <class A, bool VEC> __device__ __forceinline__ void parts4(const A *src, i64 part, int splits, int avail, A (&u)[4]) {
+    load4<A, A, VEC>(src, avail, u);
+    int s = 1;
+    for (; s + 3 <= splits; s += 3) {               // (three more in flight at a time)
+        A t[3][4];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) load4<A, A, VEC>(src + (s + q) * part, avail, t[q]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) u[x] += t[q][x];
+    }
+    for (; s < splits; ++s) {
+        A t[4];
+        load4<A, A, VEC>(src + s * part, avail, t);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) u[x] += t[x];
+    }
+}
+
 // out[i] = sum over j of g_ij u_ij, u_ij the sum of its splits: one thread per four elements.
-template <class T> __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
+template <class T, bool VEC> __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
     typedef typename Acc<T>::type A;
     const int quads = (a.dim + 3) >> 2;
     for (i64 t = (i64)blockIdx.x * 256 + threadIdx.x; t < a.rows * quads; t += (i64)gridDim.x * 256) {
         const i64 i = t / quads;
-        const int c = (int)(t - i * quads) * 4, avail = a.dim - c < 4 ? a.dim - c : 4;
-        A v[4] = {0, 0, 0, 0};
+        const int c = (int)(t - i * quads) * 4, avail = a.dim - c;
+        typename Acc<T>::v4 v = {0, 0, 0, 0};
         for (int j = 0; j < a.k; ++j) {
             const i64 p = i * a.k + j;
             if (a.bucket[p] >= a.K) continue;
-            A u[4] = {0, 0, 0, 0};
-            for (int s = 0; s < a.splits; ++s) {
-                const A *src = (const A *)a.ws + ((i64)s * a.P + p) * a.dim + c;
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    if (x < avail) u[x] += src[x];
-            }
+            A u[4];
+            parts4<A, VEC>((const A *)a.ws + p * a.dim + c, a.P * a.dim, a.splits, avail, u);
             const A g = a.gates ? ((const A *)a.gates)[p] : (A)1;
 #pragma unroll
             for (int x = 0; x < 4; ++x) v[x] += g * u[x];
         }
-        T *out = (T *)a.out + i * a.out_stride + c;
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-            if (x < avail) out[x] = (T)v[x];
+        store4((T *)a.out + i * a.out_stride + c, v, avail, VEC);
     }
 }
 
 // The same with the gates' gradient in . u_ij + b . d_i: one wave per row.  KJ >= k.
-template <class T, int KJ> __global__ __launch_bounds__(256) void combine_gates_kernel(CombineArgs a) {
+template <class T, int KJ, bool VEC> __global__ __launch_bounds__(256) void combine_gates_kernel(CombineArgs a) {
     typedef typename Acc<T>::type A;
     const int lane = wave_lane();
     const i64 i = (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -374,26 +427,34 @@ template <class T, int KJ> __global__ __launch_bounds__(256) void combine_gates_
         g[j] = e[j] < a.K ? ((const A *)a.gates)[i * a.k + j] : (A)0;
     }
     const T *in = (const T *)a.in + i * a.in_stride;
-    for (int c = lane; c < a.dim; c += 64) {
-        A v = 0;
-        const A x = (A)in[c];
+    for (int c = lane * 4; c < a.dim; c += 256) {
+        const int avail = a.dim - c;
+        typename Acc<T>::v4 v = {0, 0, 0, 0};
+        A x[4];
+        load4<T, A, VEC>(in + c, avail, x);
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
             if (e[j] >= a.K) continue;
-            A u = 0;
-            for (int s = 0; s < a.splits; ++s) u += ((const A *)a.ws)[((i64)s * a.P + i * a.k + j) * a.dim + c];
-            dot[j] += x * u;
-            v += g[j] * u;
+            A u[4];
+            parts4<A, VEC>((const A *)a.ws + (i * a.k + j) * a.dim + c, a.P * a.dim, a.splits, avail, u);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                dot[j] += x[q] * u[q];
+                v[q] += g[j] * u[q];
+            }
         }
-        if (a.out) ((T *)a.out)[i * a.out_stride + c] = (T)v;
+        if (a.out) store4((T *)a.out + i * a.out_stride + c, v, avail, VEC);
     }
     if (a.bias) {
-        for (int c = lane; c < a.ddim; c += 64) {
+        for (int c = lane * 4; c < a.ddim; c += 256) {
 #pragma unroll
             for (int j = 0; j < KJ; ++j)
                 if (e[j] < a.K) {
-                    const i64 p = i * a.k + j;
-                    dot[j] += (A)((const T *)a.bias)[(i64)e[j] * a.bias_row + c] * (A)((const T *)a.d)[(p / a.d_div) * a.d_stride + c];
+                    A b[4], d[4];
+                    load4<T, A, VEC>((const T *)a.bias + (i64)e[j] * a.bias_row + c, a.ddim - c, b);
+                    load4<T, A, VEC>((const T *)a.d + ((i * a.k + j) / a.d_div) * a.d_stride + c, a.ddim - c, d);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) dot[j] += b[q] * d[q];
                 }
         }
     }
@@ -423,9 +484,9 @@ template <class T> int launch_rows(const RowsArgs &a, bool kcontig, bool vec, bo
 
 template <class T, bool VEC> static void weight_by_tile(const WeightArgs &a, i64 blocks, hipStream_t st) {
     const dim3 g((unsigned)blocks);
-    if (a.idim <= 16 && a.odim <= 16) weight_kernel<T, VEC, 16, 16, 1, 1><<<g, 256, 0, st>>>(a);
-    else if (a.idim <= 64 && a.odim <= 64) weight_kernel<T, VEC, 64, 64, 2, 2><<<g, 256, 0, st>>>(a);
-    else weight_kernel<T, VEC, 128, 128, 2, 2><<<g, 256, 0, st>>>(a);
+    if (a.idim <= 16 && a.odim <= 16) weight_kernel<T, VEC, 16, 1, 1><<<g, 256, 0, st>>>(a);
+    else if (a.idim <= 64 && a.odim <= 64) weight_kernel<T, VEC, 64, 2, 2><<<g, 256, 0, st>>>(a);
+    else weight_kernel<T, VEC, 128, 2, 2><<<g, 256, 0, st>>>(a);
 }
 
 template <class T> int launch_weight(const WeightArgs &a, bool vec, i64 blocks, hipStream_t st) {
@@ -436,19 +497,24 @@ template <class T> int launch_weight(const WeightArgs &a, bool vec, i64 blocks, 
     return ops_launched("weight_product");
 }
 
-template <class T> int launch_combine(const CombineArgs &a, hipStream_t st) {
+template <class T, bool VEC> static void combine_gates(const CombineArgs &a, hipStream_t st) {
+    const dim3 g((unsigned)((a.rows + 3) / 4));
+    if (a.k == 1) combine_gates_kernel<T, 1, VEC><<<g, 256, 0, st>>>(a);
+    else if (a.k == 2) combine_gates_kernel<T, 2, VEC><<<g, 256, 0, st>>>(a);
+    else if (a.k <= 4) combine_gates_kernel<T, 4, VEC><<<g, 256, 0, st>>>(a);
+    else if (a.k <= 8) combine_gates_kernel<T, 8, VEC><<<g, 256, 0, st>>>(a);
+    else combine_gates_kernel<T, 32, VEC><<<g, 256, 0, st>>>(a);
+}
+
+template <class T> int launch_combine(const CombineArgs &a, bool vec, hipStream_t st) {
     if (a.rows == 0) return BGMM_OPS_OK;
     if (a.dgates) {
-        const dim3 g((unsigned)((a.rows + 3) / 4));
-        if (a.k == 1) combine_gates_kernel<T, 1><<<g, 256, 0, st>>>(a);
-        else if (a.k == 2) combine_gates_kernel<T, 2><<<g, 256, 0, st>>>(a);
-        else if (a.k <= 4) combine_gates_kernel<T, 4><<<g, 256, 0, st>>>(a);
-        else if (a.k <= 8) combine_gates_kernel<T, 8><<<g, 256, 0, st>>>(a);
-        else combine_gates_kernel<T, 32><<<g, 256, 0, st>>>(a);
+        vec ? combine_gates<T, true>(a, st) : combine_gates<T, false>(a, st);
     } else {
         const i64 threads = a.rows * ((a.dim + 3) / 4);
         const i64 b = (threads + 255) / 256 < 65536 ? (threads + 255) / 256 : 65536;
-        combine_kernel<T><<<dim3((unsigned)b), 256, 0, st>>>(a);
+        if (vec) combine_kernel<T, true><<<dim3((unsigned)b), 256, 0, st>>>(a);
+        else combine_kernel<T, false><<<dim3((unsigned)b), 256, 0, st>>>(a);
     }
     return ops_launched("combine");
 }

@@ -28,13 +28,116 @@ template <class A> __device__ __forceinline__ A neg_inf();
 template <> __device__ __forceinline__ float neg_inf<float>() { return -__builtin_inff(); }
 template <> __device__ __forceinline__ double neg_inf<double>() { return -__builtin_inf(); }
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
+// exp(x) for x <= 0: 2^k exp(r), |r| <= ln 2 / 2, k ln 2 taken off in two parts; the Taylor series to r^13 / 13! leaves
+// 4e-18.  Twenty instructions where the library's takes twice as many; below 1e-308 the result is zero.
+__device__ __forceinline__ double exp_of(double x) {
+    const double k = __builtin_rint(x * 1.4426950408889634074);
+    double r = __builtin_fma(k, -0x1.62e42fefa39efp-1, x);      // ln 2 rounded to 53 bits ...
+    r = __builtin_fma(k, -0x1.abc9e3b39803fp-56, r);            // ... and what it is short by
+    double y = 1.0 / 6227020800.0;
+    y = __builtin_fma(y, r, 1.0 / 479001600.0);
+    y = __builtin_fma(y, r, 1.0 / 39916800.0);
+    y = __builtin_fma(y, r, 1.0 / 3628800.0);
+    y = __builtin_fma(y, r, 1.0 / 362880.0);
+    y = __builtin_fma(y, r, 1.0 / 40320.0);
+    y = __builtin_fma(y, r, 1.0 / 5040.0);
+    y = __builtin_fma(y, r, 1.0 / 720.0);
+    y = __builtin_fma(y, r, 1.0 / 120.0);
+    y = __builtin_fma(y, r, 1.0 / 24.0);
+    y = __builtin_fma(y, r, 1.0 / 6.0);
+    y = __builtin_fma(y, r, 0.5);
+    y = __builtin_fma(y, r, 1.0);
+    y = __builtin_fma(y, r, 1.0);
+    return x > -708.0 ? __builtin_ldexp(y, (int)k) : 0.0;
+}
+// 2^(x log2 e) on the hardware's exponential, the rounding of the product made good to first order (its error alone is |x|
+// half steps); below 1e-38 the result is zero.
+__device__ __forceinline__ float exp_of(float x) {
+    const float t = x * 1.44269504f;
+    const float low = __builtin_fmaf(x, 1.44269504f, -t) + x * 1.92596303e-8f;
+    const float y = __builtin_amdgcn_exp2f(t);
+    return x > -87.0f ? __builtin_fmaf(y, low * 0.693147181f, y) : 0.0f;
+}
 
 // exp(v - m) with v == m exactly 1, infinities included
 template <class A> __device__ __forceinline__ A ratio(A v, A m) { return v == m ? (A)1 : exp_of(v - m); }
 
-// One wave per row; the row is read again for every chosen component (from the caches).
+// What a thread gets of a row: granule `g` (E elements, E = 1 or 16 bytes' worth) of its row, -inf behind the end and for NaN.
+template <class T, int E, class A> __device__ __forceinline__ void load_logs(const T *row, int c, int K, A *v) {
+    if (E == 1) {
+        const A x = c < K ? (A)row[c] : neg_inf<A>();
+        v[0] = x > neg_inf<A>() ? x : neg_inf<A>();
+    } else {
+        struct alignas(16) Pack { T e[E]; };
+        if (c < K) {                                            // (K is whole granules)
+            const Pack p = *(const Pack *)(row + c);
+#pragma unroll
+            for (int q = 0; q < E; ++q) {
+                const A x = (A)p.e[q];
+                v[q] = x > neg_inf<A>() ? x : neg_inf<A>();
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < E; ++q) v[q] = neg_inf<A>();
+        }
+    }
+}
+
+// G lanes per row hold it in registers, NG granules of E elements each: read once.  A round takes the maximum, then the lowest
+// index that has it, then takes that element out: six instructions per element and round.  Lane r of the group keeps
+// round r's result (k <= G).
+template <class T, int G, int NG, int E> __global__ __launch_bounds__(256) void route_rows_kernel(RouteArgs a) {
+    typedef typename Acc<T>::type A;
+    const int lane = threadIdx.x & (G - 1);
+    const i64 i = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const bool on = i < a.n;                                    // (rows behind the last: their lanes reduce along)
+    const T *row = (const T *)a.l + (on ? i : 0) * a.stride;
+    A v[NG * E];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) load_logs<T, E>(row, (g * G + lane) * E, a.K, v + g * E);
+    A top = neg_inf<A>(), mine = neg_inf<A>(), total = 0;
+    int mine_at = -1;
+    for (int r = 0; r < a.k; ++r) {
+        A m = v[0];
+#pragma unroll
+        for (int q = 1; q < NG * E; ++q) m = v[q] > m ? v[q] : m;
+        m = group_reduce<G>(m, [](A x, A y) { return x > y ? x : y; });
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int q = NG * E - 1; q >= 0; --q) at = v[q] == m ? (q / E) * G * E + q % E : at;
+        at = at == 0x7fffffff ? at : at + lane * E;
+        at = group_reduce<G>(at, [](int x, int y) { return x < y ? x : y; });
+        if (r == 0) {
+            top = m;
+            if (!a.renormalise) {
+#pragma unroll
+                for (int q = 0; q < NG * E; ++q) total += v[q] > neg_inf<A>() ? ratio(v[q], top) : (A)0;
+                total = group_sum<G>(total);
+            }
+        }
+        const bool some = m > neg_inf<A>();
+        if (lane == r) {
+            mine = m;
+            mine_at = some ? at : -1;
+        }
+        const int g = at / E, slot = g % G == lane ? (g / G) * E + at % E : -1;
+#pragma unroll
+        for (int q = 0; q < NG * E; ++q) v[q] = q == slot ? neg_inf<A>() : v[q];
+    }
+    const A e = mine_at >= 0 ? ratio(mine, top) : (A)0;
+    if (a.renormalise) total = group_sum<G>(e);
+    if (!on) return;
+    if (lane < a.k) {
+        a.labels[i * a.k + lane] = mine_at;
+        ((A *)a.weights)[i * a.k + lane] = mine_at >= 0 ? e / total : (A)0;
+    }
+    if (a.stats && lane == 0) {
+        ((A *)a.stats)[2 * i] = top;
+        ((A *)a.stats)[2 * i + 1] = total;
+    }
+}
+
+// Any K and k: one wave per row, which is read again for every chosen component (from the caches).
 template <class T> __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     typedef typename Acc<T>::type A;
     const int lane = wave_lane();
@@ -84,46 +187,73 @@ template <class T> __global__ __launch_bounds__(256) void route_kernel(RouteArgs
     }
 }
 
-template <class T> __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a) {
+// A workgroup owns `rows` whole rows of the gradient, a contiguous stretch: it writes them once, coalesced (zeros, or what the
+// softmax over all gives), and behind a barrier the chosen elements again with their full value.
+constexpr int kBackRows = 64;
+template <class T> __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a, int rows) {
     typedef typename Acc<T>::type A;
-    const int lane = wave_lane();
-    const i64 i = (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= a.n) return;
-    A w = 0, g = 0;
-    int at = -1;
-    if (lane < a.k) {
-        at = (int)a.labels[i * a.k + lane];
-        if (at >= 0) {
-            w = ((const A *)a.weights)[i * a.k + lane];
-            g = ((const A *)a.dweights)[i * a.k + lane];
-        }
-    }
-    const A wg = w * g;
-    A s = wg;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    const A d = a.renormalise ? w * (g - s) : wg;
-    A top = 0, scale = 0;
-    if (!a.renormalise) {
-        top = ((const A *)a.stats)[2 * i];
-        const A total = ((const A *)a.stats)[2 * i + 1];
-        scale = top > neg_inf<A>() ? s / total : (A)0;
-    }
-    const T *row = (const T *)a.l + i * a.stride;
-    T *out = (T *)a.dl + i * a.K;
-    for (int c0 = 0; c0 < a.K; c0 += 64) {
-        const int c = c0 + lane;
-        A v = 0;
-        if (!a.renormalise && c < a.K) {
-            const A l = (A)row[c];
-            if (l > neg_inf<A>() && top > neg_inf<A>()) v = -scale * ratio(l, top);
-        }
+    __shared__ A sums[kBackRows], tops[kBackRows], scales[kBackRows];
+    const i64 i0 = (i64)blockIdx.x * rows;
+    const int n = a.n - i0 < rows ? (int)(a.n - i0) : rows;
+    for (int r = threadIdx.x; r < n; r += 256) {
+        A s = 0;
         for (int j = 0; j < a.k; ++j) {
-            const A dj = __shfl(d, j);
-            if (__shfl(at, j) == c) v += dj;
+            const i64 at = (i0 + r) * a.k + j;
+            if (a.labels[at] >= 0) s += ((const A *)a.weights)[at] * ((const A *)a.dweights)[at];
         }
-        if (c < a.K) out[c] = (T)v;
+        sums[r] = s;
+        if (!a.renormalise) {
+            tops[r] = ((const A *)a.stats)[2 * (i0 + r)];
+            scales[r] = tops[r] > neg_inf<A>() ? s / ((const A *)a.stats)[2 * (i0 + r) + 1] : (A)0;
+        }
     }
+    __syncthreads();
+    const auto spread = [&](int r, i64 c) {                     // the softmax over all
+        const A l = (A)((const T *)a.l)[(i0 + r) * a.stride + c];
+        return l > neg_inf<A>() && tops[r] > neg_inf<A>() ? -scales[r] * ratio(l, tops[r]) : (A)0;
+    };
+    T *out = (T *)a.dl + i0 * a.K;
+    const i64 size = (i64)n * a.K;
+    if (a.renormalise) {
+        constexpr int E = 16 / (int)sizeof(T);
+        struct alignas(16) Zeros { T e[E]; };
+        Zeros z;
+#pragma unroll
+        for (int q = 0; q < E; ++q) z.e[q] = (T)0.0f;
+        const i64 whole = ((uintptr_t)out & 15) == 0 ? size / E : 0;
+        for (i64 g = threadIdx.x; g < whole; g += 256) ((Zeros *)out)[g] = z;
+        for (i64 x = whole * E + threadIdx.x; x < size; x += 256) out[x] = (T)0.0f;
+    } else {
+        for (i64 x = threadIdx.x; x < size; x += 256) out[x] = (T)spread((int)(x / a.K), x % a.K);
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < n * a.k; x += 256) {
+        const int r = x / a.k;
+        const i64 at = i0 * a.k + x;
+        const i64 c = a.labels[at];
+        if (c < 0) continue;
+        const A w = ((const A *)a.weights)[at], g = ((const A *)a.dweights)[at];
+        out[(i64)r * a.K + c] = (T)(a.renormalise ? w * (g - sums[r]) : spread(r, c) + w * g);
+    }
+}
+
+// The register form for this K and k, or false.  G: 8 lanes up to 16 elements each, then 16, 32, 64; at least k.
+template <class T, int G, int E> bool route_by_size(const RouteArgs &a, hipStream_t st) {
+    const int need = (a.K + G * E - 1) / (G * E);
+    constexpr int kMost = 16 / E;
+    const dim3 g((unsigned)((a.n + 256 / G - 1) / (256 / G)));
+    if (need <= (kMost + 3) / 4) route_rows_kernel<T, G, (kMost + 3) / 4, E><<<g, 256, 0, st>>>(a);
+    else if (need <= kMost / 2) route_rows_kernel<T, G, (kMost + 1) / 2, E><<<g, 256, 0, st>>>(a);
+    else if (need <= (kMost * 7 + 7) / 8 && kMost > 4) route_rows_kernel<T, G, (kMost * 7 + 7) / 8, E><<<g, 256, 0, st>>>(a);
+    else route_rows_kernel<T, G, kMost, E><<<g, 256, 0, st>>>(a);
+    return true;
+}
+template <class T, int E> bool route_in_registers(const RouteArgs &a, hipStream_t st) {
+    if (a.K <= 8 * 16 && a.k <= 8) return route_by_size<T, 8, E>(a, st);
+    if (a.K <= 16 * 16 && a.k <= 16) return route_by_size<T, 16, E>(a, st);
+    if (a.K <= 32 * 16) return route_by_size<T, 32, E>(a, st);
+    if (a.K <= 64 * 16) return route_by_size<T, 64, E>(a, st);
+    return false;
 }
 
 int check(const char *what, int dtype, i64 n, int K, int k, i64 stride) {
@@ -144,8 +274,12 @@ extern "C" int bgmm_route(int32_t dtype, const void *log_weights, int64_t stride
     if (!log_weights || !labels || !weights) return ops_fail(BGMM_OPS_EINVAL, "route: a null pointer");
     RouteArgs a = {log_weights, stride, n, K, k, renormalise != 0, labels, weights, stats, nullptr, nullptr};
     const dim3 g((unsigned)((n + 3) / 4));
+    const hipStream_t st = (hipStream_t)stream;
     return by_type(dtype, [&](auto *t) {
-        route_kernel<std::remove_pointer_t<decltype(t)>><<<g, 256, 0, (hipStream_t)stream>>>(a);
+        typedef std::remove_pointer_t<decltype(t)> T;
+        constexpr int E = 16 / (int)sizeof(T);
+        const bool vec = ((uintptr_t)log_weights & 15) == 0 && stride % E == 0 && K % E == 0;
+        if (!(vec ? route_in_registers<T, E>(a, st) : route_in_registers<T, 1>(a, st))) route_kernel<T><<<g, 256, 0, st>>>(a);
         return ops_launched("route");
     });
 }
@@ -158,9 +292,12 @@ extern "C" int bgmm_route_backward(int32_t dtype, const void *log_weights, int64
     if (!labels || !weights || !dweights || !dlog_weights || (!renormalise && (!log_weights || !stats)))
         return ops_fail(BGMM_OPS_EINVAL, "route_backward: a null pointer");
     RouteArgs a = {log_weights, stride, n, K, k, renormalise != 0, (int64_t *)labels, (void *)weights, (void *)stats, dweights, dlog_weights};
-    const dim3 g((unsigned)((n + 3) / 4));
+    // rows of a workgroup: about 8192 elements, a multiple of eight (so that stretches of any K start on 16 bytes)
+    int rows = 8;
+    while (rows < kBackRows && (i64)rows * K < 8192) rows *= 2;
+    const dim3 g((unsigned)((n + rows - 1) / rows));
     return by_type(dtype, [&](auto *t) {
-        route_backward_kernel<std::remove_pointer_t<decltype(t)>><<<g, 256, 0, (hipStream_t)stream>>>(a);
+        route_backward_kernel<std::remove_pointer_t<decltype(t)>><<<g, 256, 0, (hipStream_t)stream>>>(a, rows);
         return ops_launched("route_backward");
     });
 }

@@ -10,9 +10,10 @@
 // probability is kept and the remainder is what max(0, p - q) holds.  All comparisons and sums are in 64 bits: probabilities of
 // fewer bits are exact there, so that a draw depends on the order of the sum in the last bits of the total only.
 //
-// Bound by reading one row of the target (and of the draft) per sequence.  The sum over V labels is hierarchical: sixteen regions,
-// one wave each, then sixteen parts of the region that holds the draw, then a scan of 64 labels at a time: V (1 + 1/16 + 1/256)
-// reads and no table whose size would bound V.
+// Bound by reading one row of the target (and of the draft) per sequence, and for a few sequences by the latency of the chain
+// label -> its probabilities -> the row.  Up to 1024 labels a wave has a sequence and its row in registers, one launch.  Beyond,
+// a workgroup sums a chunk of a row (16-byte loads, however the row is aligned), so that one sequence already fills many
+// compute units, and a second launch finds the chunk that holds the draw and reads only that again.
 #include "ops_common.h"
 
 namespace {
@@ -41,52 +42,9 @@ template <class T> __device__ __forceinline__ double weight(const T *p, const T 
     return r > 0 ? r : 0.0;
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-constexpr int kParts = 16;
-
-// Sums of the sixteen parts of [lo, hi), one wave each; every thread returns with the same part that holds `target` (relative
-// to the sum before lo; target < 0: none wanted) and *before = the sum in front of it.  -1: nothing positive.
-template <class T>
-__device__ __forceinline__ int find_part(const T *p, const T *q, i64 lo, i64 hi, double *sums, double *total, double u, double *target, double *before) {
-    const int w = threadIdx.x >> 6;
-    const i64 len = (hi - lo + kParts - 1) / kParts;
-    const i64 a = lo + w * len < hi ? lo + w * len : hi, b = a + len < hi ? a + len : hi;
-    double s = 0;
-    for (i64 j = a + wave_lane(); j < b; j += 64) s += weight(p, q, j);
-    s = wave_sum64(s);
-    __syncthreads();
-    if (wave_lane() == 0) sums[w] = s;
-    __syncthreads();
-    double at = *before;
-    if (total) {                // the whole row: its sum gives the target
-        double t = 0;
-        for (int j = 0; j < kParts; ++j) t += sums[j];
-        *total = t;
-        *target = u * t;
-    }
-    int last = -1;
-    double last_before = at;
-    for (int j = 0; j < kParts; ++j) {
-        if (sums[j] > 0) {
-            last = j;
-            last_before = at;
-            if (at + sums[j] > *target) break;
-        }
-        at += sums[j];
-    }
-    *before = last_before;
-    return last;
-}
-
-template <class T> __global__ __launch_bounds__(64 * kParts) void verify_kernel(VerifyArgs a) {
-    __shared__ double sums[kParts];
-    const int b = blockIdx.x, lane = wave_lane();
-    // ---- acceptance: every wave finds the same
+// The drafts accepted: the same for every lane of every wave that asks.
+template <class T> __device__ __forceinline__ int accepted_drafts(const VerifyArgs &a, i64 b, int *length) {
+    const int lane = wave_lane();
     i64 len = a.lengths ? a.lengths[b] : a.T;
     len = len < 0 ? 0 : len > a.T ? a.T : len;
     const T *tgt = (const T *)a.target + b * a.target_b, *dft = (const T *)a.draft + b * a.draft_b;
@@ -95,74 +53,262 @@ template <class T> __global__ __launch_bounds__(64 * kParts) void verify_kernel(
         const int t = t0 + lane;
         bool ok = false;
         if (t < len) {
-            const i64 z = a.labels[(i64)b * a.T + t];
-            if (z >= 0 && z < a.V) ok = a.u_accept[(i64)b * a.T + t] * clean(dft[t * a.draft_t + z]) < clean(tgt[t * a.target_t + z]);
+            const i64 z = a.labels[b * a.T + t];
+            if (z >= 0 && z < a.V) ok = a.u_accept[b * a.T + t] * clean(dft[t * a.draft_t + z]) < clean(tgt[t * a.target_t + z]);
         }
         const unsigned long long bad = __ballot(!ok);       // (lanes behind the length end the run)
         const int run = bad ? __ffsll(bad) - 1 : 64;
         acc += run;
         if (run < 64) break;
     }
-    const bool rejected = acc < len;
-    const T *p = tgt + acc * a.target_t, *q = rejected ? dft + acc * a.draft_t : nullptr;
-    // ---- the draw
-    const double u = a.u_draw[b];
-    double total = 0, target = 0, before = 0;
-    int part = find_part(p, q, 0, a.V, sums, &total, u, &target, &before);
-    if (part < 0 && q) {
-        q = nullptr;
-        before = 0;
-        part = find_part(p, q, 0, a.V, sums, &total, u, &target, &before);
-    }
-    i64 drawn = -1;
-    if (part >= 0) {
-        i64 len1 = (a.V + kParts - 1) / kParts, lo = part * len1, hi = lo + len1 < a.V ? lo + len1 : a.V;
-        part = find_part(p, q, lo, hi, sums, (double *)nullptr, u, &target, &before);
-        const i64 len2 = (hi - lo + kParts - 1) / kParts;
-        lo += part * len2;
-        hi = lo + len2 < hi ? lo + len2 : hi;
-        if (threadIdx.x < 64) {
-            for (i64 j0 = lo; j0 < hi; j0 += 64) {
-                const i64 j = j0 + lane;
-                const double w = j < hi ? weight(p, q, j) : 0.0;
-                double s = w;
+    *length = (int)len;
+    return acc;
+}
+
+// One wave writes a sequence's results.
+__device__ __forceinline__ void write_labels(const VerifyArgs &a, i64 b, int acc, i64 drawn) {
+    for (int t = wave_lane(); t <= a.T; t += 64) a.out[b * (a.T + 1) + t] = t < acc ? a.labels[b * a.T + t] : t == acc ? drawn : -1;
+    if (wave_lane() == 0) a.accepted[b] = acc;
+}
+
+// ---- few labels: a wave per sequence, NV x 64 >= V
+template <class T, int NV> __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
+    const i64 b = (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (b >= a.B) return;
+    const int lane = wave_lane();
+    int len;
+    const int acc = accepted_drafts<T>(a, b, &len);
+    const T *p = (const T *)a.target + b * a.target_b + acc * a.target_t;
+    const T *q = acc < len ? (const T *)a.draft + b * a.draft_b + acc * a.draft_t : nullptr;
+    double w[NV], res[NV], total = 0;
 #pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const double t = __shfl_up(s, o);
-                    if (lane >= o) s += t;
-                }
-                const unsigned long long pos = __ballot(w > 0), hit = __ballot(w > 0 && before + s > target);
-                if (hit) {
-                    drawn = j0 + __ffsll(hit) - 1;
-                    break;
-                }
-                if (pos) drawn = j0 + 63 - __clzll(pos);    // (rounding: the last one with any weight)
-                before += __shfl(s, 63);
+    for (int j = 0; j < NV; ++j) {
+        const int c = j * 64 + lane;
+        w[j] = c < a.V ? clean(p[c]) : 0.0;
+        res[j] = w[j];
+        if (q) {
+            const double r = w[j] - (c < a.V ? clean(q[c]) : 0.0);
+            res[j] = r > 0 ? r : 0.0;
+        }
+        total += res[j];
+    }
+    total = group_sum<64>(total);
+    const bool use_p = !(total > 0);
+    if (use_p && q) {
+        total = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) total += w[j];
+        total = group_sum<64>(total);
+    }
+    const double goal = a.u_draw[b] * total;
+    double before = 0;
+    i64 drawn = -1;
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        if (found || j * 64 >= a.V) continue;
+        const double x = use_p ? w[j] : res[j];
+        const double s = wave_scan_sum(x);
+        const unsigned long long pos = __ballot(x > 0), hit = __ballot(x > 0 && before + s > goal);
+        if (hit) {
+            drawn = j * 64 + __ffsll(hit) - 1;
+            found = true;
+        } else {
+            if (pos) drawn = j * 64 + 63 - __clzll(pos);        // (rounding: the last one with any weight)
+            before += lane_read(s, 63);
+        }
+    }
+    write_labels(a, b, acc, drawn);
+}
+
+// ---- many labels: chunks of a row
+template <class T> constexpr int kPack = 16 / (int)sizeof(T);
+
+// 16 bytes of a row at any alignment its elements have
+template <class T> __device__ __forceinline__ void load_pack(const T *p, T *v) {
+    struct alignas(16) Pack { T e[kPack<T>]; } k;
+    __builtin_memcpy(&k, p, 16);
+#pragma unroll
+    for (int j = 0; j < kPack<T>; ++j) v[j] = k.e[j];
+}
+
+// Sums of max(0, p - q) (p where q is null) and of p over [lo, hi) by `n` threads, this one the `me`-th.
+template <class T> __device__ __forceinline__ void sum_span(const T *p, const T *q, i64 lo, i64 hi, int me, int n, double *res, double *all) {
+    constexpr int E = kPack<T>;
+    double r = 0, s = 0;
+    i64 j = lo + (i64)me * E;
+    for (; j + E <= hi; j += (i64)n * E) {
+        T x[E], y[E];
+        load_pack(p + j, x);
+        if (q) load_pack(q + j, y);
+#pragma unroll
+        for (int c = 0; c < E; ++c) {
+            const double w = clean(x[c]);
+            s += w;
+            if (q) {
+                const double d = w - clean(y[c]);
+                r += d > 0 ? d : 0.0;
             }
         }
     }
-    if (threadIdx.x < 64) {
-        for (int t = lane; t <= a.T; t += 64)
-            a.out[(i64)b * (a.T + 1) + t] = t < acc ? a.labels[(i64)b * a.T + t] : t == acc ? drawn : -1;
-        if (lane == 0) a.accepted[b] = acc;
+    for (; j < hi && j < lo + (hi - lo + E - 1) / E * E; ++j) {          // (the last, shorter pack: one thread's)
+        const double w = clean(p[j]);
+        s += w;
+        if (q) {
+            const double d = w - clean(q[j]);
+            r += d > 0 ? d : 0.0;
+        }
+    }
+    *all = s;
+    *res = q ? r : s;
+}
+
+// ws: [B][chunks][2] sums, [B] accepted, [B] lengths
+struct VerifyWs {
+    double *sums;
+    int *acc, *len;
+    int chunks;
+    i64 chunk;
+};
+
+template <class T> __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a, VerifyWs w) {
+    __shared__ double part[4][2];
+    const i64 b = blockIdx.x / w.chunks;
+    const int c = (int)(blockIdx.x % w.chunks);
+    int len;
+    const int acc = accepted_drafts<T>(a, b, &len);
+    const T *p = (const T *)a.target + b * a.target_b + acc * a.target_t;
+    const T *q = acc < len ? (const T *)a.draft + b * a.draft_b + acc * a.draft_t : nullptr;
+    const i64 lo = c * w.chunk, hi = lo + w.chunk < a.V ? lo + w.chunk : a.V;
+    double res, all;
+    sum_span(p, q, lo, hi, threadIdx.x, 256, &res, &all);
+    res = group_sum<64>(res);
+    all = group_sum<64>(all);
+    if (wave_lane() == 0) {
+        part[threadIdx.x >> 6][0] = res;
+        part[threadIdx.x >> 6][1] = all;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) w.sums[((i64)b * w.chunks + c) * 2 + threadIdx.x] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+    if (c == 0 && threadIdx.x == 0) {
+        w.acc[b] = acc;
+        w.len[b] = len;
     }
 }
 
+// The part that holds the goal, from n sums in memory: the first whose running sum exceeds it (else, by rounding, the last with
+// any weight; -1: none has).  *before becomes the sum in front of it.  One wave.
+template <class F> __device__ __forceinline__ int pick(int n, F sum_of, double goal, double *before) {
+    int last = -1;
+    double at = *before;
+    for (int c0 = 0; c0 < n; c0 += 64) {
+        const int c = c0 + wave_lane();
+        const double x = c < n ? sum_of(c) : 0.0;
+        const double s = wave_scan_sum(x);
+        const unsigned long long pos = __ballot(x > 0), hit = __ballot(x > 0 && at + s > goal);
+        const int l = hit ? __ffsll(hit) - 1 : pos ? 63 - __clzll(pos) : -1;
+        if (l >= 0) {
+            last = c0 + l;
+            *before = at + lane_read(s - x, l);
+        }
+        if (hit) break;
+        at += lane_read(s, 63);
+    }
+    return last;
+}
+
+constexpr int kDrawWaves = 16;
+template <class T> __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyArgs a, VerifyWs w) {
+    __shared__ double part[kDrawWaves];
+    const i64 b = blockIdx.x;
+    const int acc = w.acc[b], len = w.len[b], wave = threadIdx.x >> 6;
+    const T *p = (const T *)a.target + b * a.target_b + acc * a.target_t;
+    const T *q = acc < len ? (const T *)a.draft + b * a.draft_b + acc * a.draft_t : nullptr;
+    const double *sums = w.sums + b * w.chunks * 2;
+    // every wave picks the chunk for itself
+    double total[2] = {0, 0};
+    for (int c = wave_lane(); c < w.chunks; c += 64) {
+        total[0] += sums[2 * c];
+        total[1] += sums[2 * c + 1];
+    }
+    const double res = group_sum<64>(total[0]), all = group_sum<64>(total[1]);
+    const int which = res > 0 ? 0 : 1;
+    if (which) q = nullptr;
+    const double goal = a.u_draw[b] * (which ? all : res);
+    double before = 0;
+    const int c = pick(w.chunks, [&](int j) { return sums[2 * j + which]; }, goal, &before);
+    i64 drawn = -1;
+    if (c >= 0) {
+        // sixteen parts of the chunk, one per wave; then 64 labels at a time
+        const i64 lo = c * w.chunk, hi = lo + w.chunk < a.V ? lo + w.chunk : a.V;
+        const i64 len1 = ((hi - lo + kDrawWaves - 1) / kDrawWaves + 63) & ~(i64)63;
+        const i64 lo1 = lo + wave * len1 < hi ? lo + wave * len1 : hi, hi1 = lo1 + len1 < hi ? lo1 + len1 : hi;
+        double r, s;
+        sum_span(p, q, lo1, hi1, wave_lane(), 64, &r, &s);
+        r = group_sum<64>(r);
+        if (wave_lane() == 0) part[wave] = r;
+        __syncthreads();
+        if (wave == 0) {
+            const int k = pick(kDrawWaves, [&](int j) { return part[j]; }, goal, &before);
+            if (k >= 0) {
+                const i64 lo2 = lo + k * len1, hi2 = lo2 + len1 < hi ? lo2 + len1 : hi;
+                const int j = pick((int)(hi2 - lo2), [&](int x) { return weight(p, q, lo2 + x); }, goal, &before);
+                if (j >= 0) drawn = lo2 + j;
+            }
+        }
+    }
+    if (wave == 0) write_labels(a, b, acc, drawn);
+}
+
+// Labels per chunk: enough workgroups for the chip (two thousand), at least 4096.
+i64 chunk_of(i64 B, i64 V) {
+    i64 chunk = 4096;
+    while (chunk < 32768 && B * ((V + chunk - 1) / chunk) > 4096) chunk *= 2;
+    return chunk;
+}
+bool few_labels(i64 V) { return V <= 1024; }
+
 }  // namespace
+
+extern "C" int64_t bgmm_verify_drafts_ws(int64_t B, int64_t V) {
+    if (B < 1 || V < 1 || few_labels(V)) return 0;
+    const i64 chunk = chunk_of(B, V);
+    return B * ((V + chunk - 1) / chunk) * 16 + B * 8;
+}
 
 extern "C" int bgmm_verify_drafts(int32_t dtype, const void *target, int64_t target_b, int64_t target_t, const void *draft, int64_t draft_b,
                                   int64_t draft_t, const int64_t *labels, const double *u_accept, const double *u_draw, const int64_t *lengths,
-                                  int64_t B, int32_t T, int64_t V, int64_t *out, int64_t *accepted, void *stream) {
+                                  int64_t B, int32_t T, int64_t V, int64_t *out, int64_t *accepted, void *ws, int64_t ws_bytes, void *stream) {
     if (dtype < BGMM_F64 || dtype > BGMM_BF16) return ops_fail(BGMM_OPS_EINVAL, "verify_drafts: element type %d", dtype);
     if (B < 0 || T < 0 || T > (1 << 20) || V < 1 || target_b < 0 || target_t < 0 || draft_b < 0 || draft_t < 0)
         return ops_fail(BGMM_OPS_EINVAL, "verify_drafts: B = %lld, T = %d, V = %lld", (long long)B, T, (long long)V);
-    if (B > 0x7fffffff || V > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "verify_drafts: B = %lld, V = %lld", (long long)B, (long long)V);
+    if (B > (1 << 24) || V > 0x7fffffff - 65536) return ops_fail(BGMM_OPS_EUNSUPPORTED, "verify_drafts: B = %lld (at most 2^24), V = %lld (at most 2^31 - 65537)", (long long)B, (long long)V);
     if (B == 0) return BGMM_OPS_OK;
     if (!target || !u_draw || !out || !accepted || (T > 0 && (!draft || !labels || !u_accept)))
         return ops_fail(BGMM_OPS_EINVAL, "verify_drafts: a null pointer");
-    VerifyArgs a = {target, draft, target_b, target_t, draft_b, draft_t, labels, u_accept, u_draw, lengths, (int)B, T, V, out, accepted};
+    const i64 need = bgmm_verify_drafts_ws(B, V);
+    if (ws_bytes < need || (need > 0 && (!ws || ((uintptr_t)ws & 7)))) return ops_fail(BGMM_OPS_EINVAL, "verify_drafts: workspace of %lld bytes", (long long)ws_bytes);
+    const VerifyArgs a = {target, draft, target_b, target_t, draft_b, draft_t, labels, u_accept, u_draw, lengths, (int)B, T, V, out, accepted};
+    const hipStream_t st = (hipStream_t)stream;
+    VerifyWs w = {};
+    if (need > 0) {
+        w.chunk = chunk_of(B, V);
+        w.chunks = (int)((V + w.chunk - 1) / w.chunk);
+        w.sums = (double *)ws;
+        w.acc = (int *)(w.sums + B * w.chunks * 2);
+        w.len = w.acc + B;
+        if (B * w.chunks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "verify_drafts: %lld chunks", (long long)(B * w.chunks));
+    }
     return by_type(dtype, [&](auto *t) {
-        verify_kernel<std::remove_pointer_t<decltype(t)>><<<dim3((unsigned)B), 64 * kParts, 0, (hipStream_t)stream>>>(a);
+        typedef std::remove_pointer_t<decltype(t)> E;
+        const dim3 g((unsigned)((B + 3) / 4));
+        if (V <= 64) verify_rows_kernel<E, 1><<<g, 256, 0, st>>>(a);
+        else if (V <= 256) verify_rows_kernel<E, 4><<<g, 256, 0, st>>>(a);
+        else if (few_labels(V)) verify_rows_kernel<E, 16><<<g, 256, 0, st>>>(a);
+        else {
+            verify_sums_kernel<E><<<dim3((unsigned)(B * w.chunks)), 256, 0, st>>>(a, w);
+            verify_draw_kernel<E><<<dim3((unsigned)B), 64 * kDrawWaves, 0, st>>>(a, w);
+        }
         return ops_launched("verify_drafts");
     });
 }

@@ -33,7 +33,8 @@ SIGNATURES = {
     "bgmm_combine": (_i32, [_i32, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp]),
     "bgmm_route": (_i32, [_i32, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "bgmm_route_backward": (_i32, [_i32, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "bgmm_verify_drafts": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i64, _vp, _vp, _vp]),
+    "bgmm_verify_drafts": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "bgmm_verify_drafts_ws": (_i64, [_i64, _i64]),
 }
 
 _lib = None
@@ -67,15 +68,15 @@ def check(rc):
         raise BGMMError(rc, (_lib.bgmm_ops_last_error() or b"").decode())
 
 
-def require(ok, message):
-    """Argument checks of the operators: BGMM_EINVAL, as the library's own."""
-    if not ok:
-        raise BGMMError(-1, message)
+def refuse(message, *args, code=-1):
+    """An argument that an operator does not take: BGMM_EINVAL (or the code given), as the library's own."""
+    raise BGMMError(code, message % args)
 
 
 def require_tensors(what, **tensors):
     for name, t in tensors.items():
-        require(t is None or isinstance(t, torch.Tensor), "%s: %s is no torch tensor" % (what, name))
+        if t is not None and not isinstance(t, torch.Tensor):
+            refuse("%s: %s is no torch tensor", what, name)
 
 
 def require_device(what, **tensors):
@@ -84,12 +85,30 @@ def require_device(what, **tensors):
     for name, t in tensors.items():
         if t is None:
             continue
-        if t.device.type != "cuda":
-            raise BGMMError(-2, "%s: %s is on %s; the operators run on HIP devices only" % (what, name, t.device))
+        d = t.device
+        if d.type != "cuda":
+            refuse("%s: %s is on %s; the operators run on HIP devices only", what, name, d, code=-2)
         if device is None:
-            device = t.device
-        require(t.device == device, "%s: %s is on %s, the others on %s" % (what, name, t.device, device))
+            device = d
+        elif d != device:
+            refuse("%s: %s is on %s, the others on %s", what, name, d, device)
     return device
+
+
+class _Here(object):
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def on(device):
+    """Context with `device` current (nothing to do, and nothing paid, where it is already)."""
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def acc_dtype(dtype):
@@ -102,4 +121,4 @@ def ptr(t):
 
 
 def stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)

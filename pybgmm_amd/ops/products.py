@@ -21,22 +21,30 @@ def grouped_matmul(x, weight, groups, bias=None, gates=None):
     with respect to x, weight, bias and gates (once); the sums run in a fixed order.  float64 / 32 / 16, bfloat16.
     """
     what = "grouped_matmul"
-    nat.require(isinstance(groups, RowGroups), "%s: groups is no RowGroups" % what)
+    if not (isinstance(groups, RowGroups)):
+        nat.refuse("%s: groups is no RowGroups", what)
     nat.require_tensors(what, x=x, weight=weight, bias=bias, gates=gates)
     n, k, K = groups.n, groups.k, groups.n_components
-    nat.require(x.dtype in nat.DTYPES, "%s: x is %s" % (what, x.dtype))
-    nat.require(weight.dtype == x.dtype and (bias is None or bias.dtype == x.dtype), "%s: x, weight and bias have to be of one type" % what)
-    nat.require(weight.dim() == 3 and weight.shape[0] == K and min(weight.shape) >= 1, "%s: weight is %s, not (%d, d_in, d_out)" % (what, tuple(weight.shape), K))
+    if not (x.dtype in nat.DTYPES):
+        nat.refuse("%s: x is %s", what, x.dtype)
+    if not (weight.dtype == x.dtype and (bias is None or bias.dtype == x.dtype)):
+        nat.refuse("%s: x, weight and bias have to be of one type", what)
+    if not (weight.dim() == 3 and weight.shape[0] == K and min(weight.shape) >= 1):
+        nat.refuse("%s: weight is %s, not (%d, d_in, d_out)", what, tuple(weight.shape), K)
     d_in, d_out = weight.shape[1:]
     per_label = x.dim() == 3
-    nat.require(tuple(x.shape) == ((n, k, d_in) if per_label and len(groups.labels_shape) == 2 else (n, d_in)),
-                "%s: x is %s with a grouping of %s labels and %d inputs" % (what, tuple(x.shape), groups.labels_shape, d_in))
-    nat.require(bias is None or tuple(bias.shape) == (K, d_out), "%s: bias is %s, not (%d, %d)" % (what, None if bias is None else tuple(bias.shape), K, d_out))
+    if not (tuple(x.shape) == ((n, k, d_in) if per_label and len(groups.labels_shape) == 2 else (n, d_in))):
+        nat.refuse("%s: x is %s with a grouping of %s labels and %d inputs", what, tuple(x.shape), groups.labels_shape, d_in)
+    if not (bias is None or tuple(bias.shape) == (K, d_out)):
+        nat.refuse("%s: bias is %s, not (%d, %d)", what, None if bias is None else tuple(bias.shape), K, d_out)
     if gates is not None:
-        nat.require(tuple(gates.shape) == groups.labels_shape, "%s: gates are %s, the labels %s" % (what, tuple(gates.shape), groups.labels_shape))
-        nat.require(gates.dtype == nat.acc_dtype(x.dtype), "%s: gates are %s, not %s" % (what, gates.dtype, nat.acc_dtype(x.dtype)))
+        if not (tuple(gates.shape) == groups.labels_shape):
+            nat.refuse("%s: gates are %s, the labels %s", what, tuple(gates.shape), groups.labels_shape)
+        if not (gates.dtype == nat.acc_dtype(x.dtype)):
+            nat.refuse("%s: gates are %s, not %s", what, gates.dtype, nat.acc_dtype(x.dtype))
     dev = nat.require_device(what, x=x, weight=weight, bias=bias, gates=gates)
-    nat.require(dev == groups.device, "%s: the grouping is on %s, x on %s" % (what, groups.device, dev))
+    if not (dev == groups.device):
+        nat.refuse("%s: the grouping is on %s, x on %s", what, groups.device, dev)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, gates)):
         return _GroupedMatmul.apply(x, weight, bias, gates, groups)
     return _forward(x, weight, bias, gates, groups)
@@ -82,7 +90,7 @@ def _forward(x, weight, bias, gates, groups):
     gates = None if gates is None else gates.contiguous()
     summed = gates is not None and k > 1
     y = torch.empty((n, d_out) if gates is not None else groups.labels_shape + (d_out,), dtype=dt, device=dev)
-    with torch.cuda.device(dev):
+    with nat.on(dev):
         splits = L.bgmm_rows_product_splits(nat.DTYPES[dt], P, K, d_in, d_out)
         if splits == 1 and not summed:
             _product(x, x_stride, x_div, weight, False, bias, gates, y, None, 1, groups, P)
@@ -119,7 +127,7 @@ class _GroupedMatmul(torch.autograd.Function):
         d, d_stride = _rows(dy)
         d_div = k if gates is not None else 1
         dx = dw = db = dg = None
-        with torch.cuda.device(dev):
+        with nat.on(dev):
             st = nat.stream(dev)
             if need_x or need_g:
                 splits = L.bgmm_rows_product_splits(code, P, K, d_out, d_in)

@@ -16,12 +16,15 @@ def route(log_weights, k, renormalise=True):
     """
     what = "route"
     nat.require_tensors(what, log_weights=log_weights)
-    nat.require(log_weights.dim() == 2, "%s: log_weights has %d axes, not 2" % (what, log_weights.dim()))
-    nat.require(log_weights.dtype in nat.DTYPES, "%s: log_weights are %s" % (what, log_weights.dtype))
+    if not (log_weights.dim() == 2):
+        nat.refuse("%s: log_weights has %d axes, not 2", what, log_weights.dim())
+    if not (log_weights.dtype in nat.DTYPES):
+        nat.refuse("%s: log_weights are %s", what, log_weights.dtype)
     K = log_weights.shape[1]
-    nat.require(int(k) == k and 1 <= k <= K, "%s: k = %s of %d components" % (what, k, K))
+    if not (int(k) == k and 1 <= k <= K):
+        nat.refuse("%s: k = %s of %d components", what, k, K)
     if k > nat.MAX_CHOSEN:
-        raise nat.BGMMError(-5, "%s: k = %d (at most %d)" % (what, k, nat.MAX_CHOSEN))
+        nat.refuse("%s: k = %d (at most %d)", what, k, nat.MAX_CHOSEN, code=-5)
     nat.require_device(what, log_weights=log_weights)
     if torch.is_grad_enabled() and log_weights.requires_grad:
         return _Route.apply(log_weights, int(k), bool(renormalise))
@@ -43,7 +46,7 @@ def _route(lw, k, renormalise, want_stats):
     labels = torch.empty((n, k), dtype=torch.int64, device=lw.device)
     weights = torch.empty((n, k), dtype=acc, device=lw.device)
     stats = torch.empty((n, 2), dtype=acc, device=lw.device) if want_stats else None
-    with torch.cuda.device(lw.device):
+    with nat.on(lw.device):
         nat.check(L.bgmm_route(nat.DTYPES[lw.dtype], nat.ptr(lw), stride, n, K, k, int(renormalise), nat.ptr(labels), nat.ptr(weights),
                                nat.ptr(stats), nat.stream(lw.device)))
     return labels, weights, stats
@@ -70,7 +73,7 @@ class _Route(torch.autograd.Function):
         n = labels.shape[0]
         dweights = dweights.contiguous()
         out = torch.empty((n, ctx.K), dtype=ctx.dtype, device=labels.device)
-        with torch.cuda.device(out.device):
+        with nat.on(out.device):
             nat.check(L.bgmm_route_backward(nat.DTYPES[ctx.dtype], nat.ptr(lw), stride, n, ctx.K, ctx.k, int(ctx.renormalise), nat.ptr(labels),
                                             nat.ptr(weights), nat.ptr(stats), nat.ptr(dweights), nat.ptr(out), nat.stream(out.device)))
         return out, None, None
@@ -106,13 +109,16 @@ def group_rows(labels, n_components):
     """
     what = "group_rows"
     nat.require_tensors(what, labels=labels)
-    nat.require(labels.dtype == torch.int64, "%s: labels are %s, not int64" % (what, labels.dtype))
-    nat.require(labels.dim() in (1, 2), "%s: labels have %d axes, not 1 or 2" % (what, labels.dim()))
-    nat.require(labels.dim() == 1 or 1 <= labels.shape[1] <= nat.MAX_CHOSEN,
-                "%s: %d labels per row (1 .. %d)" % (what, labels.shape[-1] if labels.dim() == 2 else 1, nat.MAX_CHOSEN))
-    nat.require(int(n_components) == n_components and n_components >= 1, "%s: %s components" % (what, n_components))
+    if not (labels.dtype == torch.int64):
+        nat.refuse("%s: labels are %s, not int64", what, labels.dtype)
+    if not (labels.dim() in (1, 2)):
+        nat.refuse("%s: labels have %d axes, not 1 or 2", what, labels.dim())
+    if not (labels.dim() == 1 or 1 <= labels.shape[1] <= nat.MAX_CHOSEN):
+        nat.refuse("%s: %d labels per row (1 .. %d)", what, labels.shape[-1] if labels.dim() == 2 else 1, nat.MAX_CHOSEN)
+    if not (int(n_components) == n_components and n_components >= 1):
+        nat.refuse("%s: %s components", what, n_components)
     if n_components > nat.MAX_COMPONENTS:
-        raise nat.BGMMError(-5, "%s: %d components (at most %d)" % (what, n_components, nat.MAX_COMPONENTS))
+        nat.refuse("%s: %d components (at most %d)", what, n_components, nat.MAX_COMPONENTS, code=-5)
     nat.require_device(what, labels=labels)
     L = nat.load()
     K, P = int(n_components), labels.numel()
@@ -124,7 +130,7 @@ def group_rows(labels, n_components):
     store = torch.empty(2 * P + (K + 2) + n_first + ws_bytes // 4, dtype=torch.int32, device=dev)
     bucket, order, offsets, first = store[:P], store[P:2 * P], store[2 * P:2 * P + K + 2], store[2 * P + K + 2:2 * P + K + 2 + n_first]
     ws = store[2 * P + K + 2 + n_first:]
-    with torch.cuda.device(dev):
+    with nat.on(dev):
         nat.check(L.bgmm_group_rows(nat.ptr(flat), P, K, nat.ptr(bucket), nat.ptr(order), nat.ptr(offsets), nat.ptr(first), nat.ptr(ws),
                                     ws_bytes, nat.stream(dev)))
     return RowGroups(labels.shape, K, bucket, order, offsets, first)
