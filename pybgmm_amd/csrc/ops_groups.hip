@@ -8,8 +8,8 @@
 // rows it looks at together find their equals with one ballot per label bit.
 //
 // Up to kSmall rows one workgroup does everything in one launch (a single served row pays one launch, not three).  Beyond:
-// histograms per segment, an exclusive sum over the segments per bucket, the scatter -- bound by the latency of the
-// segments' dependent LDS steps, not by the 12 P bytes that move.
+// histograms per segment and workgroup, an exclusive sum over the workgroups per bucket, the scatter -- bound by the
+// latency of the segments' dependent LDS steps, not by the 20 P bytes that move.
 #include "ops_common.h"
 
 namespace {
@@ -17,7 +17,7 @@ namespace {
 constexpr int kSmall = 8192;            // rows of the one-workgroup form
 constexpr int kWaves = 16;              // its waves
 constexpr int kSmallBuckets = 940;      // its buckets (K + 1): 16 histograms, the sizes and the sums fit 64 KB of LDS
-constexpr int kSegWaves = 4;            // segments (waves) per workgroup of the three-launch form while 4 histograms fit 64 KB
+constexpr int kSegRows = 1024;          // rows of a segment (a wave's) of the three-launch form
 
 __device__ __forceinline__ int bucket_of(const int64_t *labels, i64 i, int K) {
     const int64_t z = labels[i];
@@ -102,20 +102,30 @@ template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows,
     }
 }
 
-// A wave walks rows [lo, hi): cursor[b] moves by the rows of bucket b, write(i, b, place) sees every row's place.
-template <class W>
-__device__ __forceinline__ void walk(const int64_t *labels, i64 lo, i64 hi, int K, int nbits, int *cursor, W write) {
+// A wave walks rows [lo, hi): cursor[b] moves by the rows of bucket b = bucket_at(i), write(i, b, place) sees every row's place.
+template <class L, class W>
+__device__ __forceinline__ void walk(i64 lo, i64 hi, int nbits, int *cursor, L bucket_at, W write) {
+    constexpr int kAhead = 4;
     const int lane = wave_lane();
-    for (i64 i0 = lo; i0 < hi; i0 += 64) {
-        const i64 i = i0 + lane;
-        const bool on = i < hi;
-        const int b = on ? bucket_of(labels, i, K) : 0;
-        const unsigned long long same = wave_match(b, nbits, on);
-        const int leader = on ? __ffsll((unsigned long long)same) - 1 : lane;
-        int at = 0;
-        if (on && leader == lane) at = atomicAdd(&cursor[b], __popcll(same));       // (LDS, this wave's own counters)
-        at = __shfl(at, leader);
-        if (on) write(i, b, at + __popcll(same & ((1ull << lane) - 1)));
+    for (i64 i0 = lo; i0 < hi; i0 += 64 * kAhead) {
+        int bs[kAhead];
+#pragma unroll
+        for (int r = 0; r < kAhead; ++r) {
+            const i64 i = i0 + r * 64 + lane;
+            bs[r] = i < hi ? bucket_at(i) : 0;
+        }
+#pragma unroll
+        for (int r = 0; r < kAhead; ++r) {
+            const i64 i = i0 + r * 64 + lane;
+            const bool on = i < hi;
+            const int b = bs[r];
+            const unsigned long long same = wave_match(b, nbits, on);
+            const int leader = on ? __ffsll((unsigned long long)same) - 1 : lane;
+            int at = 0;
+            if (on && leader == lane) at = atomicAdd(&cursor[b], __popcll(same));   // (LDS, this wave's own counters)
+            at = __shfl(at, leader);
+            if (on) write(i, b, at + __popcll(same & ((1ull << lane) - 1)));
+        }
     }
 }
 
@@ -130,7 +140,7 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
     __syncthreads();
     const int per = ((P + nw - 1) / nw + 63) & ~63;
     const int lo = w * per < P ? w * per : P, hi = lo + per < P ? lo + per : P;
-    walk(labels, lo, hi, K, nbits, hist + w * B, [&](i64 i, int b, int) { bucket[i] = b; });
+    walk(lo, hi, nbits, hist + w * B, [&](i64 i) { return bucket_of(labels, i, K); }, [&](i64 i, int b, int) { bucket[i] = b; });
     __syncthreads();
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
         int s = 0;
@@ -145,25 +155,32 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
     write_sums(K, P, sizes, offsets, first, part, [&](int b, int start) {
         for (int j = 0; j < nw; ++j) hist[j * B + b] += start;
     });
-    walk(labels, lo, hi, K, nbits, hist + w * B, [&](i64 i, int, int at) { order[at] = (int)i; });
+    walk(lo, hi, nbits, hist + w * B, [&](i64 i) { return bucket_of(labels, i, K); }, [&](i64 i, int, int at) { order[at] = (int)i; });
 }
 
-__global__ void group_count(const int64_t *labels, i64 P, int K, int nbits, int seg, int nseg, int *bucket, int *counts) {
+// within[segment][b]: the workgroup's earlier segments' rows of bucket b;  counts[workgroup][b]: all of its.
+__global__ void group_count(const int64_t *labels, i64 P, int K, int nbits, int nseg, int *bucket, int *within, int *counts) {
     extern __shared__ int lds[];
-    const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * (blockDim.x >> 6) + w;
+    const int B = K + 1, w = threadIdx.x >> 6, nw = blockDim.x >> 6, s = blockIdx.x * nw + w;
     int *hist = lds + w * B;
     for (int b = wave_lane(); b < B; b += 64) hist[b] = 0;
     __syncthreads();
-    const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
-    walk(labels, lo, hi, K, nbits, hist, [&](i64 i, int b, int) { bucket[i] = b; });
+    const i64 lo = (i64)s * kSegRows < P ? (i64)s * kSegRows : P, hi = lo + kSegRows < P ? lo + kSegRows : P;
+    walk(lo, hi, nbits, hist, [&](i64 i) { return bucket_of(labels, i, K); }, [&](i64 i, int b, int) { bucket[i] = b; });
     __syncthreads();
-    if (s < nseg)
-        for (int b = wave_lane(); b < B; b += 64) counts[(i64)s * B + b] = hist[b];
+    for (int b = threadIdx.x; b < B; b += blockDim.x) {
+        int sum = 0;
+        for (int j = 0; j < nw; ++j) {
+            if (blockIdx.x * nw + j < nseg) within[(i64)(blockIdx.x * nw + j) * B + b] = sum;
+            sum += lds[j * B + b];
+        }
+        counts[(i64)blockIdx.x * B + b] = sum;
+    }
 }
 
-// One wave per bucket: counts[.][b] becomes the exclusive sum over the segments, sizes[b] the total.  A lane has kRun
-// consecutive segments, so that a round has kRun loads in flight instead of one.
-constexpr int kRun = 8;
+// One wave per bucket: counts[.][b] becomes the exclusive sum over the workgroups, sizes[b] the total.  A lane has kRun
+// consecutive ones, so that a round has kRun loads in flight instead of one.
+constexpr int kRun = 4;
 __global__ void group_columns(int *counts, int nseg, int B, int *sizes) {
     const int b = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
     if (b >= B) return;
@@ -187,32 +204,34 @@ __global__ void group_columns(int *counts, int nseg, int B, int *sizes) {
     if (wave_lane() == 0) sizes[b] = carry;
 }
 
-__global__ void group_scatter(const int64_t *labels, i64 P, int K, int nbits, int seg, int nseg, const int *counts, const int *sizes,
+// The last workgroup writes the prefix sums instead.
+__global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int nseg, const int *within, const int *counts, const int *sizes,
                               int *order, int *offsets, int *first) {
     extern __shared__ int lds[];
     const int nw = blockDim.x >> 6;
     const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * nw + w;
     int *start = lds + nw * B, *part = start + B;
-    if (blockIdx.x == 0) write_sums(K, (int)P, sizes, offsets, first, part, [&](int b, int v) { start[b] = v; });
-    else block_scan(B, part, [&](int b) { return sizes[b]; }, [&](int b, int v) { start[b] = v; });
+    if (blockIdx.x == gridDim.x - 1) {
+        write_sums(K, (int)P, sizes, offsets, first, part, [](int, int) {});
+        return;
+    }
+    block_scan(B, part, [&](int b) { return sizes[b]; }, [&](int b, int v) { start[b] = v + counts[(i64)blockIdx.x * B + b]; });
     int *cursor = lds + w * B;
     if (s < nseg)
-        for (int b = wave_lane(); b < B; b += 64) cursor[b] = start[b] + counts[(i64)s * B + b];
+        for (int b = wave_lane(); b < B; b += 64) cursor[b] = start[b] + within[(i64)s * B + b];
     __syncthreads();
-    const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
-    walk(labels, lo, hi, K, nbits, cursor, [&](i64 i, int, int at) { order[at] = (int)i; });
+    const i64 lo = (i64)s * kSegRows < P ? (i64)s * kSegRows : P, hi = lo + kSegRows < P ? lo + kSegRows : P;
+    walk(lo, hi, nbits, cursor, [&](i64 i) { return bucket[i]; }, [&](i64 i, int, int at) { order[at] = (int)i; });
 }
 
-struct Split { int seg, nseg, waves; };
+struct Split { int nseg, waves, groups; };
 
-// Rows per segment: at least 512, and enough that the segments' histograms hold no more counters than there are rows.
+// Segments per workgroup: eight while their histograms, the buckets' starts and the sums fit 64 KB of LDS.
 Split split_of(i64 P, int K) {
     Split s;
-    i64 seg = K + 1 > 512 ? K + 1 : 512;
-    seg = (seg + 63) & ~(i64)63;
-    s.seg = (int)seg;
-    s.nseg = (int)((P + seg - 1) / seg);
-    s.waves = (K + 1) * kSegWaves <= 12 * 1024 ? kSegWaves : 1;      // (LDS: one histogram per wave and the buckets' starts, 64 KB)
+    s.nseg = (int)((P + kSegRows - 1) / kSegRows);
+    s.waves = K + 1 <= 1780 ? 8 : K + 1 <= 3200 ? 4 : 1;
+    s.groups = (s.nseg + s.waves - 1) / s.waves;
     return s;
 }
 
@@ -223,7 +242,7 @@ bool small_form(i64 P, int K) { return P <= kSmall && K + 1 <= kSmallBuckets; }
 extern "C" int64_t bgmm_group_rows_ws(int64_t P, int32_t K) {
     if (P < 0 || K < 1 || small_form(P, K)) return 0;
     const Split s = split_of(P, K);
-    return 4 * ((int64_t)s.nseg + 1) * (K + 1);
+    return 4 * ((int64_t)s.nseg + s.groups + 1) * (K + 1);
 }
 
 extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int32_t *bucket, int32_t *order, int32_t *offsets,
@@ -244,12 +263,11 @@ extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int3
         return ops_launched("group_rows");
     }
     const Split s = split_of(P, K);
-    int *counts = (int *)ws, *sizes = counts + (size_t)s.nseg * B;
+    int *within = (int *)ws, *counts = within + (size_t)s.nseg * B, *sizes = counts + (size_t)s.groups * B;
     // (P = 0 with many components: no segment, but the sums over nothing and the empty offsets are still written)
-    const int blocks = s.nseg > 0 ? (s.nseg + s.waves - 1) / s.waves : 1;
-    group_count<<<blocks, 64 * s.waves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, nbits, s.seg, s.nseg, bucket, counts);
-    group_columns<<<(B + 3) / 4, 256, 0, st>>>(counts, s.nseg, B, sizes);
-    group_scatter<<<blocks, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + kSums * s.waves), st>>>(labels, P, K, nbits, s.seg, s.nseg, counts, sizes,
-                                                                                                order, offsets, first);
+    if (s.groups > 0) group_count<<<s.groups, 64 * s.waves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, nbits, s.nseg, bucket, within, counts);
+    group_columns<<<(B + 3) / 4, 256, 0, st>>>(counts, s.groups, B, sizes);
+    group_scatter<<<s.groups + 1, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + kSums * s.waves), st>>>(bucket, P, K, nbits, s.nseg, within, counts,
+                                                                                                                  sizes, order, offsets, first);
     return ops_launched("group_rows");
 }

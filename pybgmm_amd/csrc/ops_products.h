@@ -61,10 +61,13 @@ constexpr int kStepBytes = 128;                                  // of the contr
 template <class T> constexpr int kStep = kStepBytes / (int)sizeof(T);
 template <class T> constexpr int kGran = 16 / (int)sizeof(T);    // elements per granule
 
-// Column (or row) of a 16-wide block that the matrix instruction's index r stands for, so that a lane's four results are
-// consecutive: the double-precision instruction gives lane l rows l / 16 + 4 i, the others rows 4 (l / 16) + i.
+// Column (or row) of a 16-wide block that the matrix instruction's index r stands for, so that what a lane stores at once is
+// 16 consecutive bytes and the four lanes of a row 64: the double-precision instruction gives lane l rows l / 16 + 4 i, the
+// others rows 4 (l / 16) + i.  result_col: the block's column of a lane's result i.
 template <class T> __device__ __forceinline__ int result_row(int r) { return r; }
-template <> __device__ __forceinline__ int result_row<double>(int r) { return (r & 3) * 4 + (r >> 2); }
+template <> __device__ __forceinline__ int result_row<double>(int r) { return (r >> 3) * 8 + (r & 3) * 2 + ((r >> 2) & 1); }
+template <class T> __device__ __forceinline__ int result_col(int q, int i) { return q * 4 + i; }
+template <> __device__ __forceinline__ int result_col<double>(int q, int i) { return (i >> 1) * 8 + q * 2 + (i & 1); }
 
 template <class T> struct KTile {
     static __device__ __forceinline__ int at(int row, int granule) { return row * kStepBytes + ((granule ^ (row & 7)) << 4); }
@@ -109,13 +112,18 @@ template <class T, int WIDTH> struct MTile {
     }
 };
 
-// 16 bytes at p of which the first `avail` elements exist (the rest become zero).  VEC: p is 16-byte aligned and avail a
-// whole granule or nothing.
-template <class T, bool VEC> __device__ __forceinline__ Granule load_granule(const T *p, int avail) {
+// 16 bytes at p, at whatever alignment its elements have
+template <class T> __device__ __forceinline__ Granule load_whole(const T *p) {
+    Granule g;
+    __builtin_memcpy(&g.raw, p, 16);
+    return g;
+}
+// 16 bytes at p of which the first `avail` elements exist; the rest become zero
+template <class T> __device__ __forceinline__ Granule load_part(const T *p, int avail) {
     Granule g;
     g.raw = (v4i){0, 0, 0, 0};
-    if (VEC) {
-        if (avail > 0) g.raw = *(const v4i *)p;
+    if (avail >= kGran<T>) {
+        g = load_whole(p);
     } else {
         T *e = Elems<T>::of(g);
 #pragma unroll
@@ -125,11 +133,19 @@ template <class T, bool VEC> __device__ __forceinline__ Granule load_granule(con
     return g;
 }
 
+// n / d for n < 2^31 by one multiplication: (n m) >> s with m = floor(2^s / d) + 1, s = 31 + ceil(log2 d).  The error
+// n (m - 2^s / d) / 2^s is below n / 2^s <= 1 / d, so the quotient is exact.
+struct Divisor {
+    unsigned m;
+    int s;
+};
+__device__ __forceinline__ int divide(int n, Divisor d) { return (int)(((unsigned long long)(unsigned)n * d.m) >> d.s); }
+
 // Workgroups go round the eight dies in turn: number them so that a die gets a contiguous stretch, whose operands its own L2
 // then holds.  -1: no work.
-__device__ __forceinline__ i64 die_order(i64 useful) {
-    const i64 per = (useful + 7) >> 3, b = blockIdx.x;
-    const i64 i = (b & 7) * per + (b >> 3);
+__device__ __forceinline__ int die_order(int useful) {
+    const int per = (useful + 7) >> 3, b = blockIdx.x;
+    const int i = (b & 7) * per + (b >> 3);
     return (b >> 3) < per && i < useful ? i : -1;
 }
 
@@ -139,7 +155,7 @@ struct RowsArgs {
     int K;
     const void *in;                 // row src = p / in_div of `in`
     i64 in_stride;
-    int in_div;
+    Divisor in_div;
     const void *w;                  // W_e[k][n] at e * w_component + k * w_row + n, or [n][k] at ... + n * w_row + k
     i64 w_component, w_row;
     const void *bias;               // [K][n], row stride bias_row, or null
@@ -159,10 +175,10 @@ struct WeightArgs {
     int K, level;
     const void *in;                 // row p / in_div
     i64 in_stride;
-    int in_div;
+    Divisor in_div;
     const void *d;                  // row p / d_div
     i64 d_stride;
-    int d_div;
+    Divisor d_div;
     const void *gates;
     void *dw, *db;                  // element type, [K][idim][odim] and [K][odim] (db may be null; dw too)
     void *ws;                       // accumulator type: a slot of idim * odim + odim per chunk of a component with several

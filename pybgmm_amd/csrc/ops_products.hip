@@ -6,6 +6,11 @@ namespace {
 int size_of(int dtype) { return dtype == BGMM_F64 ? 8 : dtype == BGMM_F32 ? 4 : 2; }
 int acc_size(int dtype) { return dtype == BGMM_F64 ? 8 : 4; }
 bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+Divisor divisor(int d) {
+    int lg = 0;
+    while ((1ll << lg) < d) ++lg;
+    return {(unsigned)((1ull << (31 + lg)) / (unsigned)d + 1), 31 + lg};
+}
 i64 at_most(i64 a, i64 b) { return a < b ? a : b; }
 
 // Rows that share a component on average: up to 16 a tile of 16 rows, whose workgroup streams the weights with little else.
@@ -14,12 +19,12 @@ int rows_tile(i64 P, int K) { return small_tiles(P, K) ? 16 : 128; }
 i64 rows_tiles(i64 P, int K, int tile) { return P / tile + at_most(K, P) + 1; }      // at most, the rows of no component included
 int cols_tile(bool small, int ndim) { return small ? 128 : ndim <= 16 ? 16 : ndim <= 64 ? 64 : 128; }
 
-// Chunk of rows of the weights' gradient (a level of the grouping): as long as about a thousand workgroups remain, 1024 ..
-// 32768 rows; a chunk leaves a tile of partial sums, which 1024 rows outweigh.
+// Chunk of rows of the weights' gradient (a level of the grouping): as long as about a thousand workgroups remain, 256 ..
+// 32768 rows; a chunk leaves a tile of partial sums, which 256 rows of both operands outweigh.
 int weight_level(i64 P, int K, int idim, int odim) {
     const int t = idim <= 16 && odim <= 16 ? 16 : idim <= 64 && odim <= 64 ? 64 : 128;
     const i64 tiles = (i64)((idim + t - 1) / t) * ((odim + t - 1) / t);
-    int level = 6;
+    int level = 4;
     while (level < BGMM_OPS_LEVELS - 1 && P / (16 << (level + 1)) * tiles >= 1024) ++level;
     return level;
 }
@@ -65,7 +70,7 @@ extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_strid
     a.K = K;
     a.in = in;
     a.in_stride = in_stride;
-    a.in_div = in_div;
+    a.in_div = divisor(in_div);
     a.w = w;
     a.w_component = w_component;
     a.w_row = w_row;
@@ -116,10 +121,10 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
     a.K = K;
     a.in = in;
     a.in_stride = in_stride;
-    a.in_div = in_div;
+    a.in_div = divisor(in_div);
     a.d = d;
     a.d_stride = d_stride;
-    a.d_div = d_div;
+    a.d_div = divisor(d_div);
     a.gates = gates;
     a.dw = dw;
     a.db = db;

@@ -22,6 +22,27 @@ template <class T, class V> __device__ __forceinline__ void store4(T *p, const V
 // a load from memory takes under load: two.  Single and double precision spend 4096 on theirs: one.
 template <class T> constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;
 
+// A lane's four results of a block of 16 columns of an output row (result_col); `avail` columns of the block exist.  S: what is
+// stored, T: the product's element type.
+template <class T, class S, class V> __device__ __forceinline__ void store_block(S *p, const V &v, int avail, bool vec) {
+    const int q = wave_lane() >> 4;
+    if constexpr (sizeof(T) == 8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = result_col<T>(q, 2 * h);
+            if (vec) {
+                struct alignas(16) Two { S e[2]; } o = {{(S)v[2 * h], (S)v[2 * h + 1]}};
+                if (c < avail) *(Two *)(p + c) = o;
+            } else {
+                if (c < avail) p[c] = (S)v[2 * h];
+                if (c + 1 < avail) p[c + 1] = (S)v[2 * h + 1];
+            }
+        }
+    } else {
+        store4(p + q * 4, v, avail - q * 4, vec);
+    }
+}
+
 template <class T, bool KCONTIG, bool VEC, int BM, int BN, int WN, int WM>
 __global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
     typedef typename Acc<T>::type A;
@@ -34,13 +55,13 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
 
     // ---- which tile: component by component, blocks of eight row tiles, within a block every column tile in turn
     const int tiles = a.bucket_first[a.ws ? a.K : a.K + 1];
-    i64 id = die_order((i64)tiles * a.n_tiles * a.splits);
+    int id = die_order(tiles * a.n_tiles * a.splits);
     if (id < 0) return;
-    const int split = (int)(id % a.splits);
+    const int split = id % a.splits;
     id /= a.splits;
-    const int e = find_bucket(a.bucket_first, a.K + 1, (int)(id / a.n_tiles));
+    const int e = find_bucket(a.bucket_first, a.K + 1, id / a.n_tiles);
     const int tile0 = a.bucket_first[e], my_tiles = a.bucket_first[e + 1] - tile0;
-    int local = (int)(id - (i64)tile0 * a.n_tiles);
+    int local = id - tile0 * a.n_tiles;
     constexpr int kBlock = 8;
     const int blk = local / (kBlock * a.n_tiles);
     local -= blk * kBlock * a.n_tiles;
@@ -59,35 +80,64 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
 
     // ---- contraction range of this split, in whole steps
     const int steps_all = (a.kdim + kStep<T> - 1) / kStep<T>;
-    const int s_lo = (int)((i64)steps_all * split / a.splits), s_hi = (int)((i64)steps_all * (split + 1) / a.splits);
+    const int s_lo = steps_all * split / a.splits, s_hi = steps_all * (split + 1) / a.splits;
     const int k_end = s_hi * kStep<T> < a.kdim ? s_hi * kStep<T> : a.kdim;
 
-    const T *xrow[XP];
+    // What a thread moves: granule column tid % 8 of the rows tid / 8 + 32 p of a KTile, granules tid + 256 p of an MTile.  VEC:
+    // every granule is whole and aligned; places outside (rows behind the last, columns behind ndim) read a neighbour that
+    // exists, whose results are not stored, so that the loop has loads and additions only; behind k_end, in the last step of a
+    // contraction that is not whole steps, both operands become zero on their way to LDS.
+    typedef MTile<T, BN> WTile;
+    const int kcol = (tid & 7) * kGran<T>;
+    const T *xp[XP], *wp[WP];
 #pragma unroll
     for (int p = 0; p < XP; ++p) {
-        int r = (tid >> 3) + p * 32;
-        r = r < n_rows ? r : n_rows - 1;                    // (a row twice rather than a branch: its results are not stored)
-        xrow[p] = (const T *)a.in + (i64)((unsigned)list[r] / (unsigned)a.in_div) * a.in_stride;
+        const int r = (tid >> 3) + p * 32;
+        xp[p] = (const T *)a.in + (i64)divide(list[r < n_rows ? r : n_rows - 1], a.in_div) * a.in_stride + s_lo * kStep<T> + kcol;
     }
     const T *w = (const T *)a.w + (i64)e * a.w_component;
-    typedef MTile<T, BN> WTile;
+    const i64 w_step = KCONTIG ? kStep<T> : kStep<T> * a.w_row;
+#pragma unroll
+    for (int p = 0; p < WP; ++p) {
+        if (KCONTIG) {
+            const int n = n0 + (tid >> 3) + p * 32;
+            wp[p] = w + (i64)(n < a.ndim ? n : a.ndim - 1) * a.w_row + s_lo * kStep<T> + kcol;
+        } else {
+            const int g = tid + p * 256, n = n0 + (g % WTile::kPerRow) * kGran<T>;
+            wp[p] = w + (i64)(s_lo * kStep<T> + g / WTile::kPerRow) * a.w_row + (!VEC || n < a.ndim ? n : n0);
+        }
+    }
     struct Held { Granule x[XP], w[WP]; } held[kAhead<T>];
-    const auto fetch = [&](Held &h, int s) {
-        const int k0 = s * kStep<T>, kk = k0 + (tid & 7) * kGran<T>;
+    const int last = s_hi - 1;
+    const bool ragged = s_hi * kStep<T> > k_end;
+    const auto fetch = [&](Held &h, int s) {                    // (step after step: the pointers move along)
+        if (VEC && !(ragged && s == last)) {
 #pragma unroll
-        for (int p = 0; p < XP; ++p)
-            if (BM >= 32 || tid < BM * 8) h.x[p] = load_granule<T, VEC>(xrow[p] + kk, k_end - kk);
+            for (int p = 0; p < XP; ++p)
+                if (BM >= 32 || tid < BM * 8) h.x[p] = load_whole(xp[p]);
 #pragma unroll
-        for (int p = 0; p < WP; ++p) {
-            if (BN < 32 && tid >= BN * 8) continue;
-            if (KCONTIG) {
-                const int n = n0 + (tid >> 3) + p * 32;
-                h.w[p] = load_granule<T, VEC>(w + (i64)n * a.w_row + kk, n < a.ndim ? k_end - kk : 0);
-            } else {
-                const int g = tid + p * 256, k = k0 + g / WTile::kPerRow, n = n0 + (g % WTile::kPerRow) * kGran<T>;
-                h.w[p] = load_granule<T, VEC>(w + (i64)k * a.w_row + n, k < k_end ? a.ndim - n : 0);
+            for (int p = 0; p < WP; ++p)
+                if (BN >= 32 || tid < BN * 8) h.w[p] = load_whole(wp[p]);
+        } else {
+            const int left_k = k_end - s * kStep<T> - kcol;
+#pragma unroll
+            for (int p = 0; p < XP; ++p)
+                if (BM >= 32 || tid < BM * 8) h.x[p] = load_part(xp[p], left_k);
+#pragma unroll
+            for (int p = 0; p < WP; ++p) {
+                if (BN < 32 && tid >= BN * 8) continue;
+                if (KCONTIG) {
+                    h.w[p] = load_part(wp[p], left_k);
+                } else {
+                    const int g = tid + p * 256, n = n0 + (g % WTile::kPerRow) * kGran<T>;
+                    h.w[p] = load_part(wp[p], s * kStep<T> + g / WTile::kPerRow < k_end ? (VEC && n >= a.ndim ? kGran<T> : a.ndim - n) : 0);
+                }
             }
         }
+#pragma unroll
+        for (int p = 0; p < XP; ++p) xp[p] += kStep<T>;
+#pragma unroll
+        for (int p = 0; p < WP; ++p) wp[p] += w_step;
     };
     const auto put = [&](const Held &h, char *buf) {
 #pragma unroll
@@ -156,16 +206,16 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
     }
     if (s < n_steps) step(0);
 
-    // ---- results: lane l has elements 4 (l / 16) .. + 3 of the block's columns for row l % 16 of the block's rows
+    // ---- results: a lane has four columns of a block (result_col) of row lane % 16 of the block's rows
     const T *bias = a.bias && split == 0 ? (const T *)a.bias + (i64)e * a.bias_row : nullptr;
 #pragma unroll
     for (int i = 0; i < FA; ++i) {
-        const int n = n0 + (wn * FA + i) * 16 + (lane >> 4) * 4, avail = a.ndim - n;
+        const int n = n0 + (wn * FA + i) * 16, avail = a.ndim - n;
         A4 b = {0, 0, 0, 0};
         if (bias) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                if (c < avail) b[c] = (A)bias[n + c];
+                if (result_col<T>(lane >> 4, c) < avail) b[c] = (A)bias[n + result_col<T>(lane >> 4, c)];
         }
 #pragma unroll
         for (int j = 0; j < FB; ++j) {
@@ -174,10 +224,10 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
             const i64 p = list[m];
             A4 v = acc[i][j] + b;
             if (a.ws) {
-                store4((A *)a.ws + ((i64)split * a.P + p) * a.ndim + n, v, avail, a.out_vec);
+                store_block<T>((A *)a.ws + ((i64)split * a.P + p) * a.ndim + n, v, avail, a.out_vec);
             } else {
                 if (a.gates) v *= ((const A *)a.gates)[p];
-                store4((T *)a.out + p * a.out_stride + n, v, avail, a.out_vec);
+                store_block<T>((T *)a.out + p * a.out_stride + n, v, avail, a.out_vec);
             }
         }
     }
@@ -196,10 +246,10 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
     __shared__ __attribute__((aligned(128))) char lds[2][2 * BT * kStepBytes];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wo = wave % WO, wi = wave / WO;
-    const i64 out_tiles = (i64)a.i_tiles * a.o_tiles;
-    const i64 id = die_order((i64)a.bucket_first[a.K] * out_tiles);
+    const int out_tiles = a.i_tiles * a.o_tiles;
+    const int id = die_order(a.bucket_first[a.K] * out_tiles);
     if (id < 0) return;
-    const int chunk = (int)(id / out_tiles), tile = (int)(id % out_tiles);
+    const int chunk = id / out_tiles, tile = id % out_tiles;
     const int e = find_bucket(a.bucket_first, a.K, chunk);
     const int c = chunk - a.bucket_first[e], chunks = a.bucket_first[e + 1] - a.bucket_first[e];
     const int rows_per = 16 << a.level;
@@ -210,9 +260,12 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
     const bool want_db = a.db && i0 == 0;
 
     // a thread moves the same granule column of rows r, r + kRows, ...; both operands' rows go by the same index, read one
-    // step before its rows are asked for
+    // step before its rows are asked for.  As in rows_kernel, places outside read a neighbour (VEC); rows behind the last are
+    // zero in both operands.
     constexpr int kRows = 256 / Tile::kPerRow < kStep<T> ? 256 / Tile::kPerRow : kStep<T>;
     const int my_row = tid / Tile::kPerRow, my_col = (tid % Tile::kPerRow) * kGran<T>;
+    const T *in = (const T *)a.in + (!VEC || i0 + my_col < a.idim ? i0 + my_col : i0);
+    const T *dd = (const T *)a.d + (!VEC || o0 + my_col < a.odim ? o0 + my_col : o0);
     struct Held { Granule i[NP], o[NP]; A gate[NP]; } held[kAhead<T>];
     int at[NP];
     const auto look = [&](int s) {
@@ -223,24 +276,35 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
         }
     };
     const auto fetch = [&](Held &h, int s) {        // (at: the indices of step s; leaves those of s + 1)
-        if (kAll || tid < BT * 8) {
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                const bool on = s * kStep<T> + my_row + p * kRows < n_rows;
-                h.i[p] = load_granule<T, VEC>((const T *)a.in + (i64)((unsigned)at[p] / (unsigned)a.in_div) * a.in_stride + i0 + my_col,
-                                              on ? a.idim - i0 - my_col : 0);
-                h.o[p] = load_granule<T, VEC>((const T *)a.d + (i64)((unsigned)at[p] / (unsigned)a.d_div) * a.d_stride + o0 + my_col,
-                                              on ? a.odim - o0 - my_col : 0);
-                if (gates) h.gate[p] = on ? gates[at[p]] : (A)0;
+        for (int p = 0; p < NP; ++p) {
+            if (!kAll && tid >= BT * 8) continue;
+            const T *pi = in + (i64)divide(at[p], a.in_div) * a.in_stride, *po = dd + (i64)divide(at[p], a.d_div) * a.d_stride;
+            if (VEC) {
+                h.i[p] = load_whole(pi);
+                h.o[p] = load_whole(po);
+            } else {
+                h.i[p] = load_part(pi, a.idim - i0 - my_col);
+                h.o[p] = load_part(po, a.odim - o0 - my_col);
             }
+            if (gates) h.gate[p] = gates[at[p]];
         }
         look(s + 1);
     };
     A dsum[kGran<T>];
 #pragma unroll
     for (int j = 0; j < kGran<T>; ++j) dsum[j] = 0;
-    const auto put = [&](Held &h, char *buf) {
+    const int n_steps = (n_rows + kStep<T> - 1) / kStep<T>;     // (at least one: a chunk has rows)
+    const auto put = [&](Held &h, int s, char *buf) {
         if (!kAll && tid >= BT * 8) return;
+        if (s == n_steps - 1) {                                 // rows behind the last
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+                if (s * kStep<T> + my_row + p * kRows >= n_rows) {
+                    h.i[p].raw = h.o[p].raw = (v4i){0, 0, 0, 0};
+                    h.gate[p] = 0;
+                }
+        }
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             if (gates) {
@@ -248,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
 #pragma unroll
                 for (int j = 0; j < kGran<T>; ++j) {
                     const A v = (A)el[j] * h.gate[p];
-                    dsum[j] += v;
+                    if (want_db) dsum[j] += v;
                     el[j] = (T)v;
                 }
             } else if (want_db) {
@@ -281,11 +345,10 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
                 for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j]);
         }
     };
-    const int n_steps = (n_rows + kStep<T> - 1) / kStep<T>;     // (at least one: a chunk has rows)
     look(0);
     fetch(held[0], 0);
     if (kAhead<T> == 2 && n_steps > 1) fetch(held[kAhead<T> - 1], 1);
-    put(held[0], lds[0]);
+    put(held[0], 0, lds[0]);
     __syncthreads();
     int s = 0;
     const auto step = [&](int slot) {
@@ -295,7 +358,7 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
             if (s + 1 < n_steps) fetch(held[0], s + 1);
         }
         compute(lds[slot]);
-        if (s + 1 < n_steps) put(held[kAhead<T> == 2 ? 1 - slot : 0], lds[1 - slot]);
+        if (s + 1 < n_steps) put(held[kAhead<T> == 2 ? 1 - slot : 0], s + 1, lds[1 - slot]);
         __syncthreads();
         ++s;
     };
@@ -312,13 +375,13 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
     if (a.dw && wave < WO * WI) {
 #pragma unroll
         for (int i = 0; i < FA; ++i) {
-            const int o = o0 + (wo * FA + i) * 16 + (lane >> 4) * 4;
+            const int o = o0 + (wo * FA + i) * 16;
 #pragma unroll
             for (int j = 0; j < FB; ++j) {
                 const int r = i0 + (wi * FB + j) * 16 + (lane & 15);
                 if (r >= a.idim) continue;
-                if (slot) store4(slot + (i64)r * a.odim + o, acc[i][j], a.odim - o, o_vec);
-                else store4((T *)a.dw + ((i64)e * a.idim + r) * a.odim + o, acc[i][j], a.odim - o, o_vec);
+                if (slot) store_block<T>(slot + (i64)r * a.odim + o, acc[i][j], a.odim - o, o_vec);
+                else store_block<T>((T *)a.dw + ((i64)e * a.idim + r) * a.odim + o, acc[i][j], a.odim - o, o_vec);
             }
         }
     }

@@ -276,8 +276,8 @@ def test_route_gradient_against_differences():
 
 # ------------------------------------------------------------------------------------------ group_rows
 @gpu
-@pytest.mark.parametrize("shape,K", [((0,), 3), ((0,), 2000), ((1,), 1), ((5,), 8000), ((64,), 7), ((1000, 4), 64), ((8192,), 939), ((8192,), 940),
-                                     ((8193,), 3), ((40000,), 200), ((30011, 3), 3071), ((30011,), 3072), ((100003,), 8000), ((1000000,), 100)])
+@pytest.mark.parametrize("shape,K", [((0,), 3), ((0,), 2000), ((1,), 1), ((5,), 8000), ((64,), 7), ((1000, 4), 64), ((8192,), 939), ((8192,), 940), ((1024,), 50), ((1025,), 50),
+                                     ((8193,), 3), ((40000,), 200), ((30011, 3), 1779), ((30011,), 1780), ((30011, 3), 3199), ((30011,), 3200), ((100003,), 8000), ((1000000,), 100)])
 def test_group_rows(shape, K):
     from pybgmm_amd import ops
     g = torch.Generator().manual_seed(K + len(shape))
