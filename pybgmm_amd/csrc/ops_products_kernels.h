@@ -18,9 +18,11 @@ template <class T, class V> __device__ __forceinline__ void store4(T *p, const V
     }
 }
 
-// Steps of operands in flight in registers.  A 128 x 128 step of half precision is 1024 cycles of matrix instructions, less than
-// a load from memory takes under load: two.  Single and double precision spend 4096 on theirs: one.
-template <class T> constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;
+// Waves per SIMD.  The loads of the next step fly in registers while the LDS buffer is in use, one buffer and two barriers a
+// step instead of two and one: that a third workgroup fits a compute unit covers more latency (and the other two's
+// beginnings and ends) than a second buffer or a second step in flight (N = 1e6, D = 64 double: 316 -> 295 us; 64 experts of
+// 1024 x 2048, bfloat16: 197 -> 174 and 163 -> 134 us).
+template <class T, int TILE> constexpr int kWavesPerSimd = TILE >= 128 * 128 ? (sizeof(T) == 8 ? 2 : 3) : sizeof(T) == 8 && TILE >= 128 * 64 ? 3 : 4;
 
 // A lane's four results of a block of 16 columns of an output row (result_col); `avail` columns of the block exist.  S: what is
 // stored, T: the product's element type.
@@ -44,12 +46,12 @@ template <class T, class S, class V> __device__ __forceinline__ void store_block
 }
 
 template <class T, bool KCONTIG, bool VEC, int BM, int BN, int WN, int WM>
-__global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
+__global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(RowsArgs a) {
     typedef typename Acc<T>::type A;
     typedef typename Acc<T>::v4 A4;
     constexpr int FA = BN / WN / 16, FB = BM / WM / 16;
     constexpr int XP = (BM + 31) / 32, WP = (BN + 31) / 32;        // granules a thread moves per step
-    __shared__ __attribute__((aligned(128))) char lds[2][(BM + BN) * kStepBytes];
+    __shared__ __attribute__((aligned(128))) char lds[(BM + BN) * kStepBytes];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave % WN, wm = wave / WN;
 
@@ -107,7 +109,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
             wp[p] = w + (i64)(s_lo * kStep<T> + g / WTile::kPerRow) * a.w_row + (!VEC || n < a.ndim ? n : n0);
         }
     }
-    struct Held { Granule x[XP], w[WP]; } held[kAhead<T>];
+    struct Held { Granule x[XP], w[WP]; } held;
     const int last = s_hi - 1;
     const bool ragged = s_hi * kStep<T> > k_end;
     const auto fetch = [&](Held &h, int s) {                    // (step after step: the pointers move along)
@@ -180,31 +182,16 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
         }
     };
 
-    // step s: its operands are in lds[s & 1], those of s + 1 (and s + 2) on their way
-    const int n_steps = s_hi - s_lo;
-    if (n_steps > 0) {
-        fetch(held[0], s_lo);
-        if (kAhead<T> == 2 && n_steps > 1) fetch(held[kAhead<T> - 1], s_lo + 1);
-        put(held[0], lds[0]);
-    }
+    fetch(held, s_lo);                                          // (a split has at least one step)
+    put(held, lds);
     __syncthreads();
-    int s = 0;
-    const auto step = [&](int slot) {               // slot = s & 1, known at compile time
-        if (kAhead<T> == 2) {
-            if (s + 2 < n_steps) fetch(held[slot], s_lo + s + 2);
-        } else {
-            if (s + 1 < n_steps) fetch(held[0], s_lo + s + 1);
-        }
-        compute(lds[slot]);
-        if (s + 1 < n_steps) put(held[kAhead<T> == 2 ? 1 - slot : 0], lds[1 - slot]);
+    for (int s = s_lo; s < s_hi; ++s) {
+        if (s < last) fetch(held, s + 1);
+        compute(lds);
         __syncthreads();
-        ++s;
-    };
-    while (s + 1 < n_steps) {
-        step(0);
-        step(1);
+        if (s < last) put(held, lds);
+        __syncthreads();
     }
-    if (s < n_steps) step(0);
 
     // ---- results: a lane has four columns of a block (result_col) of row lane % 16 of the block's rows
     const T *bias = a.bias && split == 0 ? (const T *)a.bias + (i64)e * a.bias_row : nullptr;
@@ -236,14 +223,14 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs a) {
 // dW: the rows of a chunk are the contraction, both operands have it outermost (MTile).  Half precision: g d is rounded to
 // the operand type before the product (like the operands themselves), its column sums for db are not.
 template <class T, bool VEC, int BT, int WO, int WI>
-__global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
+__global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kernel(WeightArgs a) {
     typedef typename Acc<T>::type A;
     typedef typename Acc<T>::v4 A4;
     constexpr int FA = BT / WO / 16, FB = BT / WI / 16;
     constexpr int NP = (BT + 31) / 32;                          // granules of either operand a thread moves per step
     constexpr bool kAll = BT >= 32;                             // every thread moves some
     typedef MTile<T, BT> Tile;
-    __shared__ __attribute__((aligned(128))) char lds[2][2 * BT * kStepBytes];
+    __shared__ __attribute__((aligned(128))) char lds[2 * BT * kStepBytes];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wo = wave % WO, wi = wave / WO;
     const int out_tiles = a.i_tiles * a.o_tiles;
@@ -266,7 +253,7 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
     const int my_row = tid / Tile::kPerRow, my_col = (tid % Tile::kPerRow) * kGran<T>;
     const T *in = (const T *)a.in + (!VEC || i0 + my_col < a.idim ? i0 + my_col : i0);
     const T *dd = (const T *)a.d + (!VEC || o0 + my_col < a.odim ? o0 + my_col : o0);
-    struct Held { Granule i[NP], o[NP]; A gate[NP]; } held[kAhead<T>];
+    struct Held { Granule i[NP], o[NP]; A gate[NP]; } held;
     int at[NP];
     const auto look = [&](int s) {
 #pragma unroll
@@ -346,27 +333,16 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
         }
     };
     look(0);
-    fetch(held[0], 0);
-    if (kAhead<T> == 2 && n_steps > 1) fetch(held[kAhead<T> - 1], 1);
-    put(held[0], 0, lds[0]);
+    fetch(held, 0);
+    put(held, 0, lds);
     __syncthreads();
-    int s = 0;
-    const auto step = [&](int slot) {
-        if (kAhead<T> == 2) {
-            if (s + 2 < n_steps) fetch(held[slot], s + 2);
-        } else {
-            if (s + 1 < n_steps) fetch(held[0], s + 1);
-        }
-        compute(lds[slot]);
-        if (s + 1 < n_steps) put(held[kAhead<T> == 2 ? 1 - slot : 0], s + 1, lds[1 - slot]);
+    for (int s = 0; s < n_steps; ++s) {
+        if (s + 1 < n_steps) fetch(held, s + 1);
+        compute(lds);
         __syncthreads();
-        ++s;
-    };
-    while (s + 1 < n_steps) {
-        step(0);
-        step(1);
+        if (s + 1 < n_steps) put(held, s + 1, lds);
+        __syncthreads();
     }
-    if (s < n_steps) step(0);
 
     // a component with one chunk is finished here; several leave partial sums, added in the chunks' order by weight_reduce
     A *slot = nullptr;
@@ -388,7 +364,6 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(WeightArgs a) {
     if (!want_db) return;
     // column sums: a thread has those of its granule's columns over its own rows; the threads of a column add up in order
     A *sums = (A *)lds;                       // [kRows][BT]
-    __syncthreads();
     if (kAll || tid < BT * 8) {
 #pragma unroll
         for (int j = 0; j < kGran<T>; ++j) sums[my_row * BT + my_col + j] = dsum[j];
