@@ -53,14 +53,17 @@ BGMM_OPS_API const char *bgmm_ops_runtime_path(void);
  *   order    int32[P]      out: row indices sorted by (bucket, row)
  *   offsets  int32[K + 2]  out: bucket b holds order[offsets[b] .. offsets[b + 1])
  *   first    int32[BGMM_OPS_LEVELS][K + 2]  out: for tiles of 16 << level rows, how many tiles the buckets before b have
+ *   tiles    int32[bgmm_group_rows_tiles(P, K)][4]  out, 16-byte aligned: the tiles the products work by, {bucket, first place
+ *            in order, rows, 0}, bucket by bucket, {-1, ...} behind the last
  *   ws       bgmm_group_rows_ws(P, K) bytes
  */
 BGMM_OPS_API int64_t bgmm_group_rows_ws(int64_t P, int32_t K);
+BGMM_OPS_API int64_t bgmm_group_rows_tiles(int64_t P, int32_t K);
 BGMM_OPS_API int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int32_t *bucket, int32_t *order, int32_t *offsets,
-                                 int32_t *first, void *ws, int64_t ws_bytes, void *stream);
+                                 int32_t *first, int32_t *tiles, void *ws, int64_t ws_bytes, void *stream);
 
 /*
- * Rows times their own component's matrix: for every row p of component e (order / offsets / first: a grouping's)
+ * Rows times their own component's matrix: for every row p of component e (order / tiles: a grouping's)
  *     u_p = in[p / in_div] W_e + b_e
  * out != NULL: out[p] = g_p u_p, rounded once (rows of no component: zeros); splits must be 1.
  * ws != NULL: ws[s][p] = the part s of u_p, in the accumulator type (double for BGMM_F64, else float), not gated, bias in part
@@ -74,7 +77,7 @@ BGMM_OPS_API int bgmm_rows_product_splits(int32_t dtype, int64_t P, int32_t K, i
 BGMM_OPS_API int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_stride, int32_t in_div, const void *w, int64_t w_component,
                                    int64_t w_row, int32_t kcontig, const void *bias, int64_t bias_row, const void *gates, void *out,
                                    int64_t out_stride, void *ws, int32_t splits, int64_t P, int32_t K, int32_t kdim, int32_t ndim,
-                                   const int32_t *order, const int32_t *offsets, const int32_t *first, void *stream);
+                                   const int32_t *order, const int32_t *tiles, void *stream);
 
 /*
  * The weights' gradient: dW_e = sum over the rows p of component e of g_p in[p / in_div] (x) d[p / d_div], db_e = sum of

@@ -17,7 +17,6 @@ namespace {
 constexpr int kSmall = 8192;            // rows of the one-workgroup form
 constexpr int kWaves = 16;              // its waves
 constexpr int kSmallBuckets = 940;      // its buckets (K + 1): 16 histograms, the sizes and the sums fit 64 KB of LDS
-constexpr int kSegRows = 1024;          // rows of a segment (a wave's) of the three-launch form
 
 __device__ __forceinline__ int bucket_of(const int64_t *labels, i64 i, int K) {
     const int64_t z = labels[i];
@@ -102,20 +101,41 @@ template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows,
     }
 }
 
+struct Tiles { int4 *at; int n, level; };
+
+// The table of tiles from the sums that write_sums of this workgroup has left: a wave per bucket.
+__device__ __forceinline__ void write_tiles(int K, const int *size_of, const int *offsets, const int *first, Tiles t) {
+    const int *lv = first + (i64)t.level * (K + 2);
+    const int lg = 4 + t.level, nw = blockDim.x >> 6;
+    __syncthreads();
+    for (int b = threadIdx.x >> 6; b <= K; b += nw) {
+        const int n = size_of[b], t0 = lv[b], start = offsets[b];
+        for (int i = wave_lane(); i << lg < n; i += 64) t.at[t0 + i] = make_int4(b, start + (i << lg), n - (i << lg) < 1 << lg ? n - (i << lg) : 1 << lg, 0);
+    }
+    for (int i = lv[K + 1] + threadIdx.x; i < t.n; i += blockDim.x) t.at[i] = make_int4(-1, 0, 0, 0);
+}
+
 // A wave walks rows [lo, hi): cursor[b] moves by the rows of bucket b = bucket_at(i), write(i, b, place) sees every row's place.
 template <class L, class W>
 __device__ __forceinline__ void walk(i64 lo, i64 hi, int nbits, int *cursor, L bucket_at, W write) {
-    constexpr int kAhead = 4;
+    constexpr int kRound = 4;                   // rows of a lane per round; the next round's load flies meanwhile
     const int lane = wave_lane();
-    for (i64 i0 = lo; i0 < hi; i0 += 64 * kAhead) {
-        int bs[kAhead];
+    int next[kRound];
+    const auto load = [&](i64 i0) {
 #pragma unroll
-        for (int r = 0; r < kAhead; ++r) {
+        for (int r = 0; r < kRound; ++r) {
             const i64 i = i0 + r * 64 + lane;
-            bs[r] = i < hi ? bucket_at(i) : 0;
+            next[r] = i < hi ? bucket_at(i) : 0;
         }
+    };
+    if (lo < hi) load(lo);
+    for (i64 i0 = lo; i0 < hi; i0 += 64 * kRound) {
+        int bs[kRound];
 #pragma unroll
-        for (int r = 0; r < kAhead; ++r) {
+        for (int r = 0; r < kRound; ++r) bs[r] = next[r];
+        if (i0 + 64 * kRound < hi) load(i0 + 64 * kRound);
+#pragma unroll
+        for (int r = 0; r < kRound; ++r) {
             const i64 i = i0 + r * 64 + lane;
             const bool on = i < hi;
             const int b = bs[r];
@@ -130,7 +150,7 @@ __device__ __forceinline__ void walk(i64 lo, i64 hi, int nbits, int *cursor, L b
 }
 
 __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels, int P, int K, int nbits, int *bucket, int *order,
-                                                           int *offsets, int *first) {
+                                                           int *offsets, int *first, Tiles tiles) {
     extern __shared__ int lds[];
     const int B = K + 1, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
     int *hist = lds;                          // [waves][K + 1]
@@ -156,16 +176,17 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
         for (int j = 0; j < nw; ++j) hist[j * B + b] += start;
     });
     walk(lo, hi, nbits, hist + w * B, [&](i64 i) { return bucket_of(labels, i, K); }, [&](i64 i, int, int at) { order[at] = (int)i; });
+    write_tiles(K, sizes, offsets, first, tiles);
 }
 
 // within[segment][b]: the workgroup's earlier segments' rows of bucket b;  counts[workgroup][b]: all of its.
-__global__ void group_count(const int64_t *labels, i64 P, int K, int nbits, int nseg, int *bucket, int *within, int *counts) {
+__global__ void group_count(const int64_t *labels, i64 P, int K, int nbits, int seg, int nseg, int *bucket, int *within, int *counts) {
     extern __shared__ int lds[];
     const int B = K + 1, w = threadIdx.x >> 6, nw = blockDim.x >> 6, s = blockIdx.x * nw + w;
     int *hist = lds + w * B;
     for (int b = wave_lane(); b < B; b += 64) hist[b] = 0;
     __syncthreads();
-    const i64 lo = (i64)s * kSegRows < P ? (i64)s * kSegRows : P, hi = lo + kSegRows < P ? lo + kSegRows : P;
+    const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
     walk(lo, hi, nbits, hist, [&](i64 i) { return bucket_of(labels, i, K); }, [&](i64 i, int b, int) { bucket[i] = b; });
     __syncthreads();
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
@@ -204,15 +225,16 @@ __global__ void group_columns(int *counts, int nseg, int B, int *sizes) {
     if (wave_lane() == 0) sizes[b] = carry;
 }
 
-// The last workgroup writes the prefix sums instead.
-__global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int nseg, const int *within, const int *counts, const int *sizes,
-                              int *order, int *offsets, int *first) {
+// The last workgroup writes the prefix sums and the tiles instead.
+__global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int seg, int nseg, const int *within, const int *counts, const int *sizes,
+                              int *order, int *offsets, int *first, Tiles tiles) {
     extern __shared__ int lds[];
     const int nw = blockDim.x >> 6;
     const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * nw + w;
     int *start = lds + nw * B, *part = start + B;
     if (blockIdx.x == gridDim.x - 1) {
         write_sums(K, (int)P, sizes, offsets, first, part, [](int, int) {});
+        write_tiles(K, sizes, offsets, first, tiles);
         return;
     }
     block_scan(B, part, [&](int b) { return sizes[b]; }, [&](int b, int v) { start[b] = v + counts[(i64)blockIdx.x * B + b]; });
@@ -220,16 +242,17 @@ __global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int ns
     if (s < nseg)
         for (int b = wave_lane(); b < B; b += 64) cursor[b] = start[b] + within[(i64)s * B + b];
     __syncthreads();
-    const i64 lo = (i64)s * kSegRows < P ? (i64)s * kSegRows : P, hi = lo + kSegRows < P ? lo + kSegRows : P;
+    const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
     walk(lo, hi, nbits, cursor, [&](i64 i) { return bucket[i]; }, [&](i64 i, int, int at) { order[at] = (int)i; });
 }
 
-struct Split { int nseg, waves, groups; };
+struct Split { int seg, nseg, waves, groups; };
 
-// Segments per workgroup: eight while their histograms, the buckets' starts and the sums fit 64 KB of LDS.
+// Rows of a segment (a wave's): 1024, 256 where that would leave most of the chip idle.  Segments per workgroup: eight while their histograms, the buckets' starts and the sums fit 64 KB of LDS.
 Split split_of(i64 P, int K) {
     Split s;
-    s.nseg = (int)((P + kSegRows - 1) / kSegRows);
+    s.seg = P <= 131072 ? 256 : 1024;
+    s.nseg = (int)((P + s.seg - 1) / s.seg);
     s.waves = K + 1 <= 1780 ? 8 : K + 1 <= 3200 ? 4 : 1;
     s.groups = (s.nseg + s.waves - 1) / s.waves;
     return s;
@@ -245,29 +268,32 @@ extern "C" int64_t bgmm_group_rows_ws(int64_t P, int32_t K) {
     return 4 * ((int64_t)s.nseg + s.groups + 1) * (K + 1);
 }
 
+extern "C" int64_t bgmm_group_rows_tiles(int64_t P, int32_t K) { return P < 0 || K < 1 ? 0 : tiles_at_most(P, K); }
+
 extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int32_t *bucket, int32_t *order, int32_t *offsets,
-                               int32_t *first, void *ws, int64_t ws_bytes, void *stream) {
+                               int32_t *first, int32_t *tiles, void *ws, int64_t ws_bytes, void *stream) {
     if (P < 0 || P > 0x7fffffff - 65536) return ops_fail(BGMM_OPS_EINVAL, "group_rows: P = %lld rows (0 .. 2^31 - 65537)", (long long)P);
     if (K < 1) return ops_fail(BGMM_OPS_EINVAL, "group_rows: K = %d components", K);
     if (K > BGMM_OPS_MAX_COMPONENTS) return ops_fail(BGMM_OPS_EUNSUPPORTED, "group_rows: K = %d components (at most %d)", K, BGMM_OPS_MAX_COMPONENTS);
-    if (!offsets || !first || (P > 0 && (!labels || !bucket || !order))) return ops_fail(BGMM_OPS_EINVAL, "group_rows: a null pointer");
+    if (!offsets || !first || !tiles || ((uintptr_t)tiles & 15) || (P > 0 && (!labels || !bucket || !order))) return ops_fail(BGMM_OPS_EINVAL, "group_rows: a null pointer");
     if (ws_bytes < bgmm_group_rows_ws(P, K) || (bgmm_group_rows_ws(P, K) > 0 && !ws)) return ops_fail(BGMM_OPS_EINVAL, "group_rows: workspace too small");
     hipStream_t st = (hipStream_t)stream;
     const int B = K + 1;
+    const Tiles table = {(int4 *)tiles, (int)tiles_at_most(P, K), tile_level(P, K)};
     int nbits = 1;
     while ((1 << nbits) < B) ++nbits;
     if (small_form(P, K)) {
         const int waves = P <= 1024 ? 4 : kWaves;
         const size_t lds = sizeof(int) * ((size_t)(waves + 1) * B + kSums * waves);
-        group_small<<<1, 64 * waves, lds, st>>>(labels, (int)P, K, nbits, bucket, order, offsets, first);
+        group_small<<<1, 64 * waves, lds, st>>>(labels, (int)P, K, nbits, bucket, order, offsets, first, table);
         return ops_launched("group_rows");
     }
     const Split s = split_of(P, K);
     int *within = (int *)ws, *counts = within + (size_t)s.nseg * B, *sizes = counts + (size_t)s.groups * B;
     // (P = 0 with many components: no segment, but the sums over nothing and the empty offsets are still written)
-    if (s.groups > 0) group_count<<<s.groups, 64 * s.waves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, nbits, s.nseg, bucket, within, counts);
+    if (s.groups > 0) group_count<<<s.groups, 64 * s.waves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, nbits, s.seg, s.nseg, bucket, within, counts);
     group_columns<<<(B + 3) / 4, 256, 0, st>>>(counts, s.groups, B, sizes);
-    group_scatter<<<s.groups + 1, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + kSums * s.waves), st>>>(bucket, P, K, nbits, s.nseg, within, counts,
-                                                                                                                  sizes, order, offsets, first);
+    group_scatter<<<s.groups + 1, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + kSums * s.waves), st>>>(bucket, P, K, nbits, s.seg, s.nseg, within, counts,
+                                                                                                                  sizes, order, offsets, first, table);
     return ops_launched("group_rows");
 }

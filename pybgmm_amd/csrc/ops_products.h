@@ -41,19 +41,20 @@ template <> struct Elems<float> { static __device__ float *of(Granule &g) { retu
 template <> struct Elems<f16_t> { static __device__ f16_t *of(Granule &g) { return g.h; } };
 template <> struct Elems<bf16_t> { static __device__ bf16_t *of(Granule &g) { return g.b; } };
 
-template <class T> __device__ __forceinline__ void mma(typename Acc<T>::v4 &c, const Granule &a, const Granule &b);
-template <> __device__ __forceinline__ void mma<double>(v4d &c, const Granule &a, const Granule &b) {
-    c = __builtin_amdgcn_mfma_f64_16x16x4f64(a.d[0], b.d[0], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f64_16x16x4f64(a.d[1], b.d[1], c, 0, 0, 0);
+// The matrix instructions of one granule of each operand: kParts of them, each on a part of the granules.  A kernel runs part
+// s of all its accumulators before part s + 1 of any, so that no instruction waits for the one in front of it.
+template <class T> constexpr int kParts = sizeof(T) == 8 ? 2 : sizeof(T) == 4 ? 4 : 1;
+template <class T> __device__ __forceinline__ void mma(typename Acc<T>::v4 &c, const Granule &a, const Granule &b, int s);
+template <> __device__ __forceinline__ void mma<double>(v4d &c, const Granule &a, const Granule &b, int s) {
+    c = __builtin_amdgcn_mfma_f64_16x16x4f64(a.d[s], b.d[s], c, 0, 0, 0);
 }
-template <> __device__ __forceinline__ void mma<float>(v4f &c, const Granule &a, const Granule &b) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.f[s], b.f[s], c, 0, 0, 0);
+template <> __device__ __forceinline__ void mma<float>(v4f &c, const Granule &a, const Granule &b, int s) {
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.f[s], b.f[s], c, 0, 0, 0);
 }
-template <> __device__ __forceinline__ void mma<f16_t>(v4f &c, const Granule &a, const Granule &b) {
+template <> __device__ __forceinline__ void mma<f16_t>(v4f &c, const Granule &a, const Granule &b, int) {
     c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.vh, b.vh, c, 0, 0, 0);
 }
-template <> __device__ __forceinline__ void mma<bf16_t>(v4f &c, const Granule &a, const Granule &b) {
+template <> __device__ __forceinline__ void mma<bf16_t>(v4f &c, const Granule &a, const Granule &b, int) {
     c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.vb, b.vb, c, 0, 0, 0);
 }
 
@@ -141,18 +142,17 @@ struct Divisor {
 };
 __device__ __forceinline__ int divide(int n, Divisor d) { return (int)(((unsigned long long)(unsigned)n * d.m) >> d.s); }
 
-// Workgroups go round the eight dies in turn: number them so that a die gets a contiguous stretch, whose operands its own L2
-// then holds.  -1: no work.
-__device__ __forceinline__ int die_order(int useful) {
-    const int per = (useful + 7) >> 3, b = blockIdx.x;
-    const int i = (b & 7) * per + (b >> 3);
-    return (b >> 3) < per && i < useful ? i : -1;
+// Workgroups go round the eight dies in turn: number them so that a die gets runs of consecutive work, whose operands its own L2
+// then holds.  A permutation of 0 .. blocks - 1 (a multiple of 8 * run) that needs no load.
+__device__ __forceinline__ int die_order(int run) {
+    const int b = blockIdx.x, die = b & 7, at = b >> 3;
+    return (at / run * 8 + die) * run + at % run;
 }
 
 struct RowsArgs {
-    const int *bucket_first;        // the grouping's prefix sums for this tile size
-    const int *offsets, *order;
-    int K;
+    const int4 *tiles;              // the grouping's
+    const int *order;
+    int K, tile_blocks, run;        // blocks of eight tiles, consecutive workgroups on a die
     const void *in;                 // row src = p / in_div of `in`
     i64 in_stride;
     Divisor in_div;
@@ -172,7 +172,7 @@ struct RowsArgs {
 struct WeightArgs {
     const int *bucket_first;        // prefix sums for chunks of `chunk` rows
     const int *offsets, *order;
-    int K, level;
+    int K, level, run;
     const void *in;                 // row p / in_div
     i64 in_stride;
     Divisor in_div;

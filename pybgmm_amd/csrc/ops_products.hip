@@ -13,11 +13,16 @@ Divisor divisor(int d) {
 }
 i64 at_most(i64 a, i64 b) { return a < b ? a : b; }
 
-// Rows that share a component on average: up to 16 a tile of 16 rows, whose workgroup streams the weights with little else.
-bool small_tiles(i64 P, int K) { return P <= 16 * (i64)K; }
-int rows_tile(i64 P, int K) { return small_tiles(P, K) ? 16 : 128; }
-i64 rows_tiles(i64 P, int K, int tile) { return P / tile + at_most(K, P) + 1; }      // at most, the rows of no component included
 int cols_tile(bool small, int ndim) { return small ? 128 : ndim <= 16 ? 16 : ndim <= 64 ? 64 : 128; }
+
+// Workgroups for `useful` ones in runs per die (die_order): runs of up to 64, shorter where the dies would get less than eight.
+struct Grid { int run; i64 blocks; };
+Grid grid_of(i64 useful) {
+    Grid g = {64, 0};
+    while (g.run > 1 && useful < (i64)g.run * 64) g.run /= 2;
+    g.blocks = (useful + 8 * g.run - 1) / (8 * g.run) * (8 * g.run);
+    return g;
+}
 
 // Chunk of rows of the weights' gradient (a level of the grouping): as long as about a thousand workgroups remain, 256 ..
 // 32768 rows; a chunk leaves a tile of partial sums, which 256 rows of both operands outweigh.
@@ -43,7 +48,7 @@ extern "C" int bgmm_rows_product_splits(int32_t dtype, int64_t P, int32_t K, int
     if (check("rows_product_splits", dtype, P, K, kdim, ndim) != BGMM_OPS_OK || P == 0) return 1;
     const bool small = small_tiles(P, K);
     const int bn = cols_tile(small, ndim);
-    const i64 groups = rows_tiles(P, K, rows_tile(P, K)) * ((ndim + bn - 1) / bn);
+    const i64 groups = tiles_at_most(P, K) * ((ndim + bn - 1) / bn);
     const int steps = (kdim * size_of(dtype) + kStepBytes - 1) / kStepBytes;
     // (256 compute units: fill them twice over, but leave a part four steps to do)
     i64 s = at_most(512 / (groups > 0 ? groups : 1), steps / 4);
@@ -53,19 +58,19 @@ extern "C" int bgmm_rows_product_splits(int32_t dtype, int64_t P, int32_t K, int
 extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_stride, int32_t in_div, const void *w, int64_t w_component,
                                  int64_t w_row, int32_t kcontig, const void *bias, int64_t bias_row, const void *gates, void *out,
                                  int64_t out_stride, void *ws, int32_t splits, int64_t P, int32_t K, int32_t kdim, int32_t ndim,
-                                 const int32_t *order, const int32_t *offsets, const int32_t *first, void *stream) {
+                                 const int32_t *order, const int32_t *tiles, void *stream) {
     const int rc = check("rows_product", dtype, P, K, kdim, ndim);
     if (rc) return rc;
     if (P == 0) return BGMM_OPS_OK;
-    if (!in || !w || !order || !offsets || !first || !out == !ws) return ops_fail(BGMM_OPS_EINVAL, "rows_product: a null pointer (and exactly one of out, ws)");
+    if (!in || !w || !order || !tiles || !out == !ws) return ops_fail(BGMM_OPS_EINVAL, "rows_product: a null pointer (and exactly one of out, ws)");
     if (in_div < 1 || splits < 1 || (out && splits != 1) || in_stride < 0 || out_stride < 0)
         return ops_fail(BGMM_OPS_EINVAL, "rows_product: in_div %d, splits %d, strides %lld %lld", in_div, splits, (long long)in_stride, (long long)out_stride);
     const int S = size_of(dtype), E = 16 / S;
     const bool small = small_tiles(P, K);
-    const int bm = rows_tile(P, K), bn = cols_tile(small, ndim), level = small ? 0 : 3;
+    const int bn = cols_tile(small, ndim);
     RowsArgs a;
-    a.bucket_first = first + (size_t)level * (K + 2);
-    a.offsets = offsets;
+    a.tiles = (const int4 *)tiles;
+    a.tile_blocks = (int)(tiles_at_most(P, K) / 8);
     a.order = order;
     a.K = K;
     a.in = in;
@@ -88,9 +93,10 @@ extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_strid
     a.out_vec = ndim % 4 == 0 && (ws ? aligned(ws, 16) : out_stride % 4 == 0 && aligned(out, S == 2 ? 8 : 16));
     const bool vec = aligned(in, 16) && aligned(w, 16) && in_stride % E == 0 && w_component % E == 0 && w_row % E == 0 && kdim % E == 0 &&
                      (kcontig || ndim % E == 0);
-    const i64 blocks = (rows_tiles(P, K, bm) * a.n_tiles * splits + 7) & ~(i64)7;
-    if (blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "rows_product: %lld tiles", (long long)blocks);
-    return by_type(dtype, [&](auto *t) { return launch_rows<std::remove_pointer_t<decltype(t)>>(a, kcontig != 0, vec, small, blocks, (hipStream_t)stream); });
+    const Grid g = grid_of((i64)a.tile_blocks * 8 * a.n_tiles * splits);
+    if (g.blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "rows_product: %lld tiles", (long long)g.blocks);
+    a.run = g.run;
+    return by_type(dtype, [&](auto *t) { return launch_rows<std::remove_pointer_t<decltype(t)>>(a, kcontig != 0, vec, small, g.blocks, (hipStream_t)stream); });
 }
 
 extern "C" int64_t bgmm_weight_product_ws(int32_t dtype, int64_t P, int32_t K, int32_t idim, int32_t odim) {
@@ -134,9 +140,10 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
     a.i_tiles = (idim + t - 1) / t;
     a.o_tiles = (odim + t - 1) / t;
     const bool vec = aligned(in, 16) && aligned(d, 16) && in_stride % E == 0 && d_stride % E == 0 && idim % E == 0 && odim % E == 0;
-    const i64 blocks = P == 0 ? 0 : ((P / ((i64)16 << a.level) + at_most(K, P)) * a.i_tiles * a.o_tiles + 7) & ~(i64)7;
-    if (blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: %lld tiles", (long long)blocks);
-    return by_type(dtype, [&](auto *t_) { return launch_weight<std::remove_pointer_t<decltype(t_)>>(a, vec, blocks, (hipStream_t)stream); });
+    const Grid g = grid_of(P == 0 ? 0 : (P / ((i64)16 << a.level) + at_most(K, P)) * a.i_tiles * a.o_tiles);
+    if (g.blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: %lld tiles", (long long)g.blocks);
+    a.run = g.run;
+    return by_type(dtype, [&](auto *t_) { return launch_weight<std::remove_pointer_t<decltype(t_)>>(a, vec, g.blocks, (hipStream_t)stream); });
 }
 
 extern "C" int bgmm_combine(int32_t dtype, const void *ws, int32_t splits, int64_t rows, int32_t k, int32_t K, const int32_t *bucket,

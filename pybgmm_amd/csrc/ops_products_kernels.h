@@ -52,25 +52,22 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     constexpr int FA = BN / WN / 16, FB = BM / WM / 16;
     constexpr int XP = (BM + 31) / 32, WP = (BN + 31) / 32;        // granules a thread moves per step
     __shared__ __attribute__((aligned(128))) char lds[(BM + BN) * kStepBytes];
+    __shared__ int row_of[BM];      // what the results need is here before the products are done: rows, gates, bias
+    __shared__ A gate_of[BM];
+    __shared__ __attribute__((aligned(16))) A bias_of[BN];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave % WN, wm = wave / WN;
 
-    // ---- which tile: component by component, blocks of eight row tiles, within a block every column tile in turn
-    const int tiles = a.bucket_first[a.ws ? a.K : a.K + 1];
-    int id = die_order(tiles * a.n_tiles * a.splits);
-    if (id < 0) return;
-    const int split = id % a.splits;
-    id /= a.splits;
-    const int e = find_bucket(a.bucket_first, a.K + 1, id / a.n_tiles);
-    const int tile0 = a.bucket_first[e], my_tiles = a.bucket_first[e + 1] - tile0;
-    int local = id - tile0 * a.n_tiles;
+    // ---- which tile: blocks of eight row tiles, within a block every column tile (of every split) in turn
     constexpr int kBlock = 8;
-    const int blk = local / (kBlock * a.n_tiles);
-    local -= blk * kBlock * a.n_tiles;
-    const int in_block = my_tiles - blk * kBlock < kBlock ? my_tiles - blk * kBlock : kBlock;
-    const int nt = local / in_block, rt = blk * kBlock + local % in_block;
-    const int row0 = a.offsets[e] + rt * BM, left = a.offsets[e + 1] - row0, n_rows = left < BM ? left : BM;
-    const int *list = a.order + row0;
+    const int per_block = kBlock * a.n_tiles * a.splits;
+    const int id = die_order(a.run), blk = id / per_block, local = id - blk * per_block;
+    if (blk >= a.tile_blocks) return;
+    const int t = blk * kBlock + local % kBlock, rest = local / kBlock, nt = rest % a.n_tiles, split = rest / a.n_tiles;
+    const int4 tile = a.tiles[t];
+    const int e = tile.x, n_rows = tile.z;
+    if (e < 0 || (e == a.K && a.ws)) return;
+    const int *list = a.order + tile.y;
     const int n0 = nt * BN;
 
     if (e == a.K) {                 // rows of no component: zeros
@@ -92,10 +89,11 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     typedef MTile<T, BN> WTile;
     const int kcol = (tid & 7) * kGran<T>;
     const T *xp[XP], *wp[WP];
+    int pair[XP];
 #pragma unroll
     for (int p = 0; p < XP; ++p) {
         const int r = (tid >> 3) + p * 32;
-        xp[p] = (const T *)a.in + (i64)divide(list[r < n_rows ? r : n_rows - 1], a.in_div) * a.in_stride + s_lo * kStep<T> + kcol;
+        pair[p] = list[r < n_rows ? r : n_rows - 1];
     }
     const T *w = (const T *)a.w + (i64)e * a.w_component;
     const i64 w_step = KCONTIG ? kStep<T> : kStep<T> * a.w_row;
@@ -107,6 +105,17 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
         } else {
             const int g = tid + p * 256, n = n0 + (g % WTile::kPerRow) * kGran<T>;
             wp[p] = w + (i64)(s_lo * kStep<T> + g / WTile::kPerRow) * a.w_row + (!VEC || n < a.ndim ? n : n0);
+        }
+    }
+    A my_bias = 0;
+    if (tid < BN && a.bias && split == 0 && n0 + tid < a.ndim) my_bias = (A)((const T *)a.bias)[(i64)e * a.bias_row + n0 + tid];
+#pragma unroll
+    for (int p = 0; p < XP; ++p) {
+        xp[p] = (const T *)a.in + (i64)divide(pair[p], a.in_div) * a.in_stride + s_lo * kStep<T> + kcol;
+        const int r = (tid >> 3) + p * 32;
+        if ((tid & 7) == 0 && r < BM) {
+            row_of[r] = pair[p];
+            gate_of[r] = a.gates ? ((const A *)a.gates)[pair[p]] : (A)1;
         }
     }
     struct Held { Granule x[XP], w[WP]; } held;
@@ -176,13 +185,16 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
 #pragma unroll
             for (int j = 0; j < FB; ++j) fb[j] = KTile<T>::template read<false>(buf, wm * FB * 16 + j * 16, ks);
 #pragma unroll
-            for (int i = 0; i < FA; ++i)
+            for (int part = 0; part < kParts<T>; ++part)
 #pragma unroll
-                for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j]);
+                for (int i = 0; i < FA; ++i)
+#pragma unroll
+                    for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j], part);
         }
     };
 
     fetch(held, s_lo);                                          // (a split has at least one step)
+    if (tid < BN) bias_of[tid] = my_bias;
     put(held, lds);
     __syncthreads();
     for (int s = s_lo; s < s_hi; ++s) {
@@ -194,27 +206,23 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     }
 
     // ---- results: a lane has four columns of a block (result_col) of row lane % 16 of the block's rows
-    const T *bias = a.bias && split == 0 ? (const T *)a.bias + (i64)e * a.bias_row : nullptr;
 #pragma unroll
-    for (int i = 0; i < FA; ++i) {
-        const int n = n0 + (wn * FA + i) * 16, avail = a.ndim - n;
-        A4 b = {0, 0, 0, 0};
-        if (bias) {
+    for (int j = 0; j < FB; ++j) {
+        const int m = (wm * FB + j) * 16 + (lane & 15);
+        if (m >= n_rows) continue;
+        const i64 p = row_of[m];
+        const A gate = gate_of[m];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (result_col<T>(lane >> 4, c) < avail) b[c] = (A)bias[n + result_col<T>(lane >> 4, c)];
-        }
+        for (int i = 0; i < FA; ++i) {
+            const int c = (wn * FA + i) * 16, n = n0 + c;
+            A4 v = acc[i][j];
 #pragma unroll
-        for (int j = 0; j < FB; ++j) {
-            const int m = (wm * FB + j) * 16 + (lane & 15);
-            if (m >= n_rows) continue;
-            const i64 p = list[m];
-            A4 v = acc[i][j] + b;
+            for (int x = 0; x < 4; ++x) v[x] += bias_of[c + result_col<T>(lane >> 4, x)];
             if (a.ws) {
-                store_block<T>((A *)a.ws + ((i64)split * a.P + p) * a.ndim + n, v, avail, a.out_vec);
+                store_block<T>((A *)a.ws + ((i64)split * a.P + p) * a.ndim + n, v, a.ndim - n, a.out_vec);
             } else {
-                if (a.gates) v *= ((const A *)a.gates)[p];
-                store_block<T>((T *)a.out + p * a.out_stride + n, v, avail, a.out_vec);
+                v *= gate;
+                store_block<T>((T *)a.out + p * a.out_stride + n, v, a.ndim - n, a.out_vec);
             }
         }
     }
@@ -234,9 +242,8 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wo = wave % WO, wi = wave / WO;
     const int out_tiles = a.i_tiles * a.o_tiles;
-    const int id = die_order(a.bucket_first[a.K] * out_tiles);
-    if (id < 0) return;
-    const int chunk = id / out_tiles, tile = id % out_tiles;
+    const int id = die_order(a.run), chunk = id / out_tiles, tile = id % out_tiles;
+    if (chunk >= a.bucket_first[a.K]) return;
     const int e = find_bucket(a.bucket_first, a.K, chunk);
     const int c = chunk - a.bucket_first[e], chunks = a.bucket_first[e + 1] - a.bucket_first[e];
     const int rows_per = 16 << a.level;
@@ -327,9 +334,11 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
 #pragma unroll
             for (int j = 0; j < FB; ++j) fb[j] = Tile::template read<false>(buf, (wi * FB + j) * 16, ks);
 #pragma unroll
-            for (int i = 0; i < FA; ++i)
+            for (int part = 0; part < kParts<T>; ++part)
 #pragma unroll
-                for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j]);
+                for (int i = 0; i < FA; ++i)
+#pragma unroll
+                    for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j], part);
         }
     };
     look(0);

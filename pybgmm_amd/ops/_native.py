@@ -24,10 +24,11 @@ SIGNATURES = {
     "bgmm_ops_last_error": (ctypes.c_char_p, []),
     "bgmm_ops_runtime_path": (ctypes.c_char_p, []),
     "bgmm_group_rows_ws": (_i64, [_i64, _i32]),
-    "bgmm_group_rows": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "bgmm_group_rows_tiles": (_i64, [_i64, _i32]),
+    "bgmm_group_rows": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "bgmm_rows_product_splits": (_i32, [_i32, _i64, _i32, _i32, _i32]),
     "bgmm_rows_product": (_i32, [_i32, _vp, _i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _i32,
-                                 _vp, _vp, _vp, _vp]),
+                                 _vp, _vp, _vp]),
     "bgmm_weight_product_ws": (_i64, [_i32, _i64, _i32, _i32, _i32]),
     "bgmm_weight_product": (_i32, [_i32, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "bgmm_combine": (_i32, [_i32, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp]),

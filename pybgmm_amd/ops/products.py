@@ -77,7 +77,7 @@ def _product(x, x_stride, x_div, w, transposed, bias, gates, out, ws, splits, gr
     bias, bias_row = (None, 0) if bias is None else _row_stride(bias)
     nat.check(L.bgmm_rows_product(nat.DTYPES[x.dtype], nat.ptr(x), x_stride, x_div, nat.ptr(w), w_comp, w_row, int(in_contiguous != transposed),
                                   nat.ptr(bias), bias_row, nat.ptr(gates), nat.ptr(out), ndim, nat.ptr(ws), splits, P, groups.n_components,
-                                  kdim, ndim, nat.ptr(groups.order), nat.ptr(groups.offsets), nat.ptr(groups.first), nat.stream(x.device)))
+                                  kdim, ndim, nat.ptr(groups.order), nat.ptr(groups.tiles), nat.stream(x.device)))
 
 
 def _forward(x, weight, bias, gates, groups):

@@ -88,9 +88,9 @@ class RowGroups(object):
     bucket the rows of no component.  ``counts``: rows per component.  The tensors belong to the grouping: products read them.
     """
 
-    def __init__(self, labels_shape, n_components, bucket, order, offsets, first):
+    def __init__(self, labels_shape, n_components, bucket, order, offsets, first, tiles):
         self.labels_shape, self.n_components = tuple(labels_shape), n_components
-        self.bucket, self.order, self.offsets, self.first = bucket, order, offsets, first
+        self.bucket, self.order, self.offsets, self.first, self.tiles = bucket, order, offsets, first, tiles
         self.device = order.device
         self.n = self.labels_shape[0]
         self.k = self.labels_shape[1] if len(self.labels_shape) == 2 else 1
@@ -125,12 +125,11 @@ def group_rows(labels, n_components):
     dev = labels.device
     flat = labels.contiguous()
     n_first = nat.LEVELS * (K + 2)
-    ws_bytes = L.bgmm_group_rows_ws(P, K)
-    # one allocation: bucket [P], order [P], offsets [K + 2], first [levels][K + 2], workspace
-    store = torch.empty(2 * P + (K + 2) + n_first + ws_bytes // 4, dtype=torch.int32, device=dev)
-    bucket, order, offsets, first = store[:P], store[P:2 * P], store[2 * P:2 * P + K + 2], store[2 * P + K + 2:2 * P + K + 2 + n_first]
-    ws = store[2 * P + K + 2 + n_first:]
+    n_tiles, ws_bytes = L.bgmm_group_rows_tiles(P, K), L.bgmm_group_rows_ws(P, K)
+    # one allocation
+    tiles, bucket, order, offsets, first, ws = torch.empty(4 * n_tiles + 2 * P + K + 2 + n_first + ws_bytes // 4, dtype=torch.int32, device=dev).split(
+        [4 * n_tiles, P, P, K + 2, n_first, ws_bytes // 4])
     with nat.on(dev):
-        nat.check(L.bgmm_group_rows(nat.ptr(flat), P, K, nat.ptr(bucket), nat.ptr(order), nat.ptr(offsets), nat.ptr(first), nat.ptr(ws),
+        nat.check(L.bgmm_group_rows(nat.ptr(flat), P, K, nat.ptr(bucket), nat.ptr(order), nat.ptr(offsets), nat.ptr(first), nat.ptr(tiles), nat.ptr(ws),
                                     ws_bytes, nat.stream(dev)))
-    return RowGroups(labels.shape, K, bucket, order, offsets, first)
+    return RowGroups(labels.shape, K, bucket, order, offsets, first, tiles)

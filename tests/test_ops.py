@@ -62,7 +62,7 @@ def test_the_operators_bind_to_the_runtime_of_torch():
 def cpu_groups(shape, K):
     from pybgmm_amd import ops
     t = torch.zeros(4, dtype=torch.int32)
-    return ops.RowGroups(shape, K, t, t, t, t)
+    return ops.RowGroups(shape, K, t, t, t, t, t)
 
 
 def refused(code, call, *args, **kw):
@@ -144,12 +144,12 @@ def test_c_entry_points_refuse_before_they_launch():
     buf = ctypes.create_string_buffer(4096)
     p = ctypes.addressof(buf)
     calls = [
-        (-1, L.bgmm_group_rows(p, -1, 3, p, p, p, p, p, 0, None)),
-        (-1, L.bgmm_group_rows(p, 1 << 31, 3, p, p, p, p, p, 0, None)),
-        (-1, L.bgmm_group_rows(p, 5, 0, p, p, p, p, p, 0, None)),
-        (-5, L.bgmm_group_rows(p, 5, 8001, p, p, p, p, p, 0, None)),
-        (-1, L.bgmm_group_rows(None, 5, 3, p, p, p, p, p, 0, None)),
-        (-1, L.bgmm_group_rows(p, 100000, 3, p, p, p, p, p, 8, None)),
+        (-1, L.bgmm_group_rows(p, -1, 3, p, p, p, p, p, p, 0, None)),
+        (-1, L.bgmm_group_rows(p, 1 << 31, 3, p, p, p, p, p, p, 0, None)),
+        (-1, L.bgmm_group_rows(p, 5, 0, p, p, p, p, p, p, 0, None)),
+        (-5, L.bgmm_group_rows(p, 5, 8001, p, p, p, p, p, p, 0, None)),
+        (-1, L.bgmm_group_rows(None, 5, 3, p, p, p, p, p, p, 0, None)),
+        (-1, L.bgmm_group_rows(p, 100000, 3, p, p, p, p, p, p, 8, None)),
         (-1, L.bgmm_route(9, p, 4, 2, 4, 1, 1, p, p, None, None)),
         (-1, L.bgmm_route(1, p, 4, 2, 4, 5, 1, p, p, None, None)),
         (-5, L.bgmm_route(1, p, 64, 2, 64, 33, 1, p, p, None, None)),
@@ -159,10 +159,10 @@ def test_c_entry_points_refuse_before_they_launch():
         (-1, L.bgmm_verify_drafts(1, p, 4, 4, None, 4, 4, p, p, p, None, 1, 1, 4, p, p, None, 0, None)),
         (-1, L.bgmm_verify_drafts(1, p, 4, 4, p, 4, 4, p, p, p, None, 1, 1, 0, p, p, None, 0, None)),
         (-1, L.bgmm_verify_drafts(1, p, 4, 4, p, 4, 4, p, p, p, None, 1, 1, 5000, p, p, p, 8, None)),                 # workspace
-        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, p, 1, 8, 2, 4, 4, p, p, p, None)),     # out and ws
-        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 2, 8, 2, 4, 4, p, p, p, None)),  # splits without ws
-        (-1, L.bgmm_rows_product(1, p, 4, 0, p, 4, 4, 0, None, 0, None, p, 4, None, 1, 8, 2, 4, 4, p, p, p, None)),
-        (-1, L.bgmm_rows_product(4, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 1, 8, 2, 4, 4, p, p, p, None)),
+        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, p, 1, 8, 2, 4, 4, p, p, None)),     # out and ws
+        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 2, 8, 2, 4, 4, p, p, None)),  # splits without ws
+        (-1, L.bgmm_rows_product(1, p, 4, 0, p, 4, 4, 0, None, 0, None, p, 4, None, 1, 8, 2, 4, 4, p, p, None)),
+        (-1, L.bgmm_rows_product(4, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 1, 8, 2, 4, 4, p, p, None)),
         (-1, L.bgmm_weight_product(1, p, 4, 1, p, 4, 1, None, p, None, None, 0, 1 << 20, 2, 4, 4, p, p, p, None)),   # workspace
         (-1, L.bgmm_weight_product(1, None, 4, 1, p, 4, 1, None, p, None, None, 0, 8, 2, 4, 4, p, p, p, None)),
         (-1, L.bgmm_combine(1, p, 1, 4, 33, 2, p, None, p, 4, 4, None, None, 0, None, 0, None, 0, 1, 1, None)),
@@ -298,6 +298,10 @@ def test_group_rows(shape, K):
     for level in range(12):
         tiles = (size + (16 << level) - 1) // (16 << level)
         assert torch.equal(first[level], torch.cat([torch.zeros(1, dtype=torch.int64), tiles.cumsum(0)])), level
+    level = 0 if z.numel() <= 16 * K else 3
+    want = [[b, int(off[b]) + r, min(16 << level, int(size[b]) - r), 0] for b in range(K + 1) for r in range(0, int(size[b]), 16 << level)]
+    got = grp.tiles.view(-1, 4).cpu()
+    assert got[:len(want)].tolist() == want and bool((got[len(want):, 0] == -1).all())
 
 
 @gpu
