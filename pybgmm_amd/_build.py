@@ -1,14 +1,16 @@
 """
-Build libbgmm_hip.so and libbgmm_ops.so (hipcc, gfx950 only) in-tree next to their sources.
+Build libbgmm_hip.so, libbgmm_ops.so (hipcc, gfx950 only) and the operators' torch binding (g++) in-tree.
 
 The shared objects are git-ignored but travel to the GPU box with the gpurun
 snapshot.  ``build()`` is idempotent: it recompiles only sources newer than
 their objects.
 """
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -25,6 +27,7 @@ HEADERS = sorted(h for h in glob.glob(os.path.join(CSRC, "*.h")) if not os.path.
 OPS_LIB = os.path.join(HERE, "libbgmm_ops.so")
 OPS_SOURCES = ["ops_common.hip", "ops_groups.hip", "ops_products.hip", "ops_products_f64.hip", "ops_products_f32.hip",
                "ops_products_f16.hip", "ops_products_bf16.hip", "ops_route.hip", "ops_verify.hip"]
+OPS_BINDING = os.path.join(HERE, "ops", "_binding.so")          # what pybgmm_amd.ops imports: libbgmm_ops.so on torch tensors
 OPS_HEADERS = sorted(glob.glob(os.path.join(CSRC, "ops_*.h"))) + [os.path.join(INCLUDE, "bgmm_ops.h")]
 # -ffp-contract=off: the sufficient-statistics updates must round product and sum
 # separately (bit-identical m / S to the reference); hot loops call fma() explicitly.
@@ -50,10 +53,39 @@ def _stale(target, deps):
 
 
 def build(force=False, verbose=False, extra_flags=()):
-    """Both libraries; returns the path of libbgmm_hip.so."""
+    """Both libraries and the binding; returns the path of libbgmm_hip.so."""
     # -no-hip-rt: libbgmm_ops.so does not link a HIP runtime (include/bgmm_ops.h says which one it binds to)
-    _build_one(OPS_LIB, OPS_SOURCES, OPS_HEADERS, ["-no-hip-rt"], force, verbose, extra_flags)
+    _build_one(OPS_LIB, OPS_SOURCES, OPS_HEADERS, ["-no-hip-rt", "-Wl,-soname," + os.path.basename(OPS_LIB)], force, verbose, extra_flags)
+    _build_binding(force, verbose)
     return _build_one(LIB, SOURCES, HEADERS, [], force, verbose, extra_flags)
+
+
+def _build_binding(force, verbose):
+    """Host code against torch's headers and libraries; without torch there are no operators to bind."""
+    src = os.path.join(CSRC, "ops_torch.cpp")
+    if importlib.util.find_spec("torch") is None or not (force or _stale(OPS_BINDING, [src, OPS_HEADERS[-1]])):
+        return
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    rocm = os.path.dirname(os.path.dirname(hipcc()))
+    includes = include_paths() + [sysconfig.get_paths()["include"], os.path.join(rocm, "include"), "/opt/rocm/include"]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+    for p in includes:
+        cmd += ["-isystem", p]
+    cmd += [src, "-o", OPS_BINDING, "-L" + lib, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-L" + HERE, "-lbgmm_ops",
+            "-Wl,-rpath,$ORIGIN/..", "-Wl,--allow-shlib-undefined"]
+    _run(cmd, verbose)
+
+
+def _run(cmd, verbose):
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("%s failed:\n%s\n%s" % (os.path.basename(cmd[0]), " ".join(cmd), r.stdout))
+    return r.stdout
 
 
 def _build_one(lib, sources, headers, link_flags, force, verbose, extra_flags):
@@ -67,24 +99,16 @@ def _build_one(lib, sources, headers, link_flags, force, verbose, extra_flags):
         if force or _stale(o, [s] + headers):
             jobs.append([cc] + FLAGS + list(extra_flags) + ["-c", s, "-o", o])
 
-    def run(cmd):
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("hipcc failed:\n%s\n%s" % (" ".join(cmd), r.stdout))
-        return r.stdout
-
     if jobs:
         with ThreadPoolExecutor(max_workers=4) as ex:
-            outs = list(ex.map(run, jobs))
+            outs = list(ex.map(lambda cmd: _run(cmd, verbose), jobs))
         if verbose:
             for o in outs:
                 if o.strip():
                     print(o)
     objs = [os.path.join(objdir, s + ".o") for s in sources]
     if force or jobs or _stale(lib, objs):
-        run([cc, "--offload-arch=gfx950", "-shared", "-fPIC"] + link_flags + ["-o", lib] + objs)
+        _run([cc, "--offload-arch=gfx950", "-shared", "-fPIC"] + link_flags + ["-o", lib] + objs, verbose)
     return lib
 
 

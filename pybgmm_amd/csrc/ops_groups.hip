@@ -16,20 +16,21 @@ namespace {
 
 constexpr int kSmall = 8192;            // rows of the one-workgroup form
 constexpr int kWaves = 16;              // its waves
-constexpr int kSmallBuckets = 940;      // its buckets (K + 1): 16 histograms, the sizes and the sums fit 64 KB of LDS
+constexpr int kSmallBuckets = 890;      // its buckets (K + 1): 16 histograms, the sizes and the sums fit 64 KB of LDS
 
 __device__ __forceinline__ int bucket_of(const int64_t *labels, i64 i, int K) {
     const int64_t z = labels[i];
     return z >= 0 && z < K ? (int)z : K;
 }
 
-__device__ __forceinline__ int wave_incl_scan(int v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(v, o);
-        if (wave_lane() >= o) v += t;
-    }
-    return v;
+__device__ __forceinline__ int wave_incl_scan(int v) {         // rows of 16 lanes by row shifts, their totals by readlane
+    v += lane_move<0x111>(v);
+    v += lane_move<0x112>(v);
+    v += lane_move<0x114>(v);
+    v += lane_move<0x118>(v);
+    const int t0 = __builtin_amdgcn_readlane(v, 15), t1 = t0 + __builtin_amdgcn_readlane(v, 31), t2 = t1 + __builtin_amdgcn_readlane(v, 47);
+    const int row = wave_lane() >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? t0 : row == 2 ? t1 : t2);
 }
 
 // Exclusive sum of f(0 .. n-1) over the whole workgroup, handed to g(b, sum before b); returns the total.  `part` holds one
@@ -56,10 +57,10 @@ __device__ __forceinline__ int block_scan(int n, int *part, F f, G g) {
     return carry;
 }
 
-// All the prefix sums over buckets at once: offsets (handed to place(b, start)) and every level of tiles.  `part`:
-// kSums * waves ints.
+// All the prefix sums over buckets at once: offsets and every level of tiles; place(b, start, tiles of level `level` before b)
+// sees every bucket and b = K + 1, what is behind the last.  `part`: kSums * waves ints.
 constexpr int kSums = BGMM_OPS_LEVELS + 1;
-template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows, const int *size_of, int *offsets, int *first, int *part, P place) {
+template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows, const int *size_of, int *offsets, int *first, int level, int *part, P place) {
     const int nw = blockDim.x >> 6, w = threadIdx.x >> 6, B = K + 1;
     int carry[kSums];
 #pragma unroll
@@ -75,6 +76,7 @@ template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows,
             incl[l] = t - v;
         }
         __syncthreads();
+        int start = 0, tile = 0;
 #pragma unroll
         for (int l = 0; l < kSums; ++l) {
             int before = carry[l] + incl[l];
@@ -84,35 +86,36 @@ template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows,
                 carry[l] += t;
             }
             if (b < B) {
-                if (l == 0) {
-                    offsets[b] = before;
-                    place(b, before);
-                } else {
-                    first[(i64)(l - 1) * (K + 2) + b] = before;
-                }
+                if (l == 0) offsets[b] = start = before;
+                else first[(i64)(l - 1) * (K + 2) + b] = before;
+                if (l == level + 1) tile = before;
             }
         }
+        if (b < B) place(b, start, tile);
         __syncthreads();
     }
     if (threadIdx.x == 0) {
         offsets[B] = P_rows;
+        int tile = 0;
 #pragma unroll
-        for (int l = 1; l < kSums; ++l) first[(i64)(l - 1) * (K + 2) + B] = carry[l];
+        for (int l = 1; l < kSums; ++l) {
+            first[(i64)(l - 1) * (K + 2) + B] = carry[l];
+            if (l == level + 1) tile = carry[l];
+        }
+        place(B, P_rows, tile);
     }
 }
 
 struct Tiles { int4 *at; int n, level; };
 
-// The table of tiles from the sums that write_sums of this workgroup has left: a wave per bucket.
-__device__ __forceinline__ void write_tiles(int K, const int *size_of, const int *offsets, const int *first, Tiles t) {
-    const int *lv = first + (i64)t.level * (K + 2);
+// The table of tiles from a grouping's sums in LDS (starts and tile_starts: [K + 2]): a wave per bucket.
+__device__ __forceinline__ void write_tiles(int K, const int *starts, const int *tile_starts, Tiles t) {
     const int lg = 4 + t.level, nw = blockDim.x >> 6;
-    __syncthreads();
     for (int b = threadIdx.x >> 6; b <= K; b += nw) {
-        const int n = size_of[b], t0 = lv[b], start = offsets[b];
+        const int start = starts[b], n = starts[b + 1] - start, t0 = tile_starts[b];
         for (int i = wave_lane(); i << lg < n; i += 64) t.at[t0 + i] = make_int4(b, start + (i << lg), n - (i << lg) < 1 << lg ? n - (i << lg) : 1 << lg, 0);
     }
-    for (int i = lv[K + 1] + threadIdx.x; i < t.n; i += blockDim.x) t.at[i] = make_int4(-1, 0, 0, 0);
+    for (int i = tile_starts[K + 1] + threadIdx.x; i < t.n; i += blockDim.x) t.at[i] = make_int4(-1, 0, 0, 0);
 }
 
 // A wave walks rows [lo, hi): cursor[b] moves by the rows of bucket b = bucket_at(i), write(i, b, place) sees every row's place.
@@ -154,8 +157,9 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
     extern __shared__ int lds[];
     const int B = K + 1, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
     int *hist = lds;                          // [waves][K + 1]
-    int *sizes = hist + nw * B;               // [K + 1]
-    int *part = sizes + B;                    // [kSums * waves]
+    int *sizes = hist + nw * B;               // [K + 1], later the starts [K + 2]
+    int *tile_starts = sizes + B + 1;         // [K + 2]
+    int *part = tile_starts + B + 1;          // [kSums * waves]
     for (int j = threadIdx.x; j < nw * B; j += blockDim.x) hist[j] = 0;
     __syncthreads();
     const int per = ((P + nw - 1) / nw + 63) & ~63;
@@ -172,22 +176,31 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
         sizes[b] = s;
     }
     __syncthreads();
-    write_sums(K, P, sizes, offsets, first, part, [&](int b, int start) {
-        for (int j = 0; j < nw; ++j) hist[j * B + b] += start;
+    write_sums(K, P, sizes, offsets, first, tiles.level, part, [&](int b, int start, int tile) {
+        if (b < B)
+            for (int j = 0; j < nw; ++j) hist[j * B + b] += start;
+        sizes[b] = start;                     // (its own size has been read)
+        tile_starts[b] = tile;
     });
+    __syncthreads();
     walk(lo, hi, nbits, hist + w * B, [&](i64 i) { return bucket_of(labels, i, K); }, [&](i64 i, int, int at) { order[at] = (int)i; });
-    write_tiles(K, sizes, offsets, first, tiles);
+    write_tiles(K, sizes, tile_starts, tiles);
 }
 
 // within[segment][b]: the workgroup's earlier segments' rows of bucket b;  counts[workgroup][b]: all of its.
-__global__ void group_count(const int64_t *labels, i64 P, int K, int nbits, int seg, int nseg, int *bucket, int *within, int *counts) {
+__global__ void group_count(const int64_t *labels, i64 P, int K, int seg, int nseg, int *bucket, int *within, int *counts) {
     extern __shared__ int lds[];
     const int B = K + 1, w = threadIdx.x >> 6, nw = blockDim.x >> 6, s = blockIdx.x * nw + w;
     int *hist = lds + w * B;
     for (int b = wave_lane(); b < B; b += 64) hist[b] = 0;
     __syncthreads();
     const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
-    walk(lo, hi, nbits, hist, [&](i64 i) { return bucket_of(labels, i, K); }, [&](i64 i, int b, int) { bucket[i] = b; });
+#pragma unroll 4
+    for (i64 i = lo + wave_lane(); i < hi; i += 64) {           // (counts need no order)
+        const int b = bucket_of(labels, i, K);
+        atomicAdd(&hist[b], 1);
+        bucket[i] = b;
+    }
     __syncthreads();
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
         int sum = 0;
@@ -233,8 +246,13 @@ __global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int se
     const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * nw + w;
     int *start = lds + nw * B, *part = start + B;
     if (blockIdx.x == gridDim.x - 1) {
-        write_sums(K, (int)P, sizes, offsets, first, part, [](int, int) {});
-        write_tiles(K, sizes, offsets, first, tiles);
+        int *starts = lds, *tile_starts = starts + B + 1;       // (the sums' parts behind them)
+        write_sums(K, (int)P, sizes, offsets, first, tiles.level, tile_starts + B + 1, [&](int b, int at, int tile) {
+            starts[b] = at;
+            tile_starts[b] = tile;
+        });
+        __syncthreads();
+        write_tiles(K, starts, tile_starts, tiles);
         return;
     }
     block_scan(B, part, [&](int b) { return sizes[b]; }, [&](int b, int v) { start[b] = v + counts[(i64)blockIdx.x * B + b]; });
@@ -248,10 +266,10 @@ __global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int se
 
 struct Split { int seg, nseg, waves, groups; };
 
-// Rows of a segment (a wave's): 1024, 256 where that would leave most of the chip idle.  Segments per workgroup: eight while their histograms, the buckets' starts and the sums fit 64 KB of LDS.
+// Rows of a segment (a wave's): 512, 256 where that would leave most of the chip idle.  Segments per workgroup: eight while their histograms, the buckets' starts and the sums fit 64 KB of LDS.
 Split split_of(i64 P, int K) {
     Split s;
-    s.seg = P <= 131072 ? 256 : 1024;
+    s.seg = P <= 131072 ? 256 : 512;
     s.nseg = (int)((P + s.seg - 1) / s.seg);
     s.waves = K + 1 <= 1780 ? 8 : K + 1 <= 3200 ? 4 : 1;
     s.groups = (s.nseg + s.waves - 1) / s.waves;
@@ -284,16 +302,16 @@ extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int3
     while ((1 << nbits) < B) ++nbits;
     if (small_form(P, K)) {
         const int waves = P <= 1024 ? 4 : kWaves;
-        const size_t lds = sizeof(int) * ((size_t)(waves + 1) * B + kSums * waves);
+        const size_t lds = sizeof(int) * ((size_t)(waves + 2) * B + 2 + kSums * waves);
         group_small<<<1, 64 * waves, lds, st>>>(labels, (int)P, K, nbits, bucket, order, offsets, first, table);
         return ops_launched("group_rows");
     }
     const Split s = split_of(P, K);
     int *within = (int *)ws, *counts = within + (size_t)s.nseg * B, *sizes = counts + (size_t)s.groups * B;
     // (P = 0 with many components: no segment, but the sums over nothing and the empty offsets are still written)
-    if (s.groups > 0) group_count<<<s.groups, 64 * s.waves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, nbits, s.seg, s.nseg, bucket, within, counts);
+    if (s.groups > 0) group_count<<<s.groups, 64 * s.waves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, s.seg, s.nseg, bucket, within, counts);
     group_columns<<<(B + 3) / 4, 256, 0, st>>>(counts, s.groups, B, sizes);
-    group_scatter<<<s.groups + 1, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + kSums * s.waves), st>>>(bucket, P, K, nbits, s.seg, s.nseg, within, counts,
+    group_scatter<<<s.groups + 1, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + 2 + kSums * s.waves), st>>>(bucket, P, K, nbits, s.seg, s.nseg, within, counts,
                                                                                                                   sizes, order, offsets, first, table);
     return ops_launched("group_rows");
 }

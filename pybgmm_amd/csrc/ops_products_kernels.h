@@ -118,52 +118,53 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
             gate_of[r] = a.gates ? ((const A *)a.gates)[pair[p]] : (A)1;
         }
     }
-    struct Held { Granule x[XP], w[WP]; } held;
+    Granule gx[XP], gw[WP];
     const int last = s_hi - 1;
     const bool ragged = s_hi * kStep<T> > k_end;
-    const auto fetch = [&](Held &h, int s) {                    // (step after step: the pointers move along)
+    const auto fetch_rows = [&](int s) {      // (step after step: the pointers move along)
         if (VEC && !(ragged && s == last)) {
 #pragma unroll
             for (int p = 0; p < XP; ++p)
-                if (BM >= 32 || tid < BM * 8) h.x[p] = load_whole(xp[p]);
-#pragma unroll
-            for (int p = 0; p < WP; ++p)
-                if (BN >= 32 || tid < BN * 8) h.w[p] = load_whole(wp[p]);
+                if (BM >= 32 || tid < BM * 8) gx[p] = load_whole(xp[p]);
         } else {
             const int left_k = k_end - s * kStep<T> - kcol;
 #pragma unroll
             for (int p = 0; p < XP; ++p)
-                if (BM >= 32 || tid < BM * 8) h.x[p] = load_part(xp[p], left_k);
+                if (BM >= 32 || tid < BM * 8) gx[p] = load_part(xp[p], left_k);
+        }
+#pragma unroll
+        for (int p = 0; p < XP; ++p) xp[p] += kStep<T>;
+    };
+    const auto fetch_weights = [&](int s) {
+        if (VEC && !(ragged && s == last)) {
+#pragma unroll
+            for (int p = 0; p < WP; ++p)
+                if (BN >= 32 || tid < BN * 8) gw[p] = load_whole(wp[p]);
+        } else {
 #pragma unroll
             for (int p = 0; p < WP; ++p) {
                 if (BN < 32 && tid >= BN * 8) continue;
                 if (KCONTIG) {
-                    h.w[p] = load_part(wp[p], left_k);
+                    gw[p] = load_part(wp[p], k_end - s * kStep<T> - kcol);
                 } else {
                     const int g = tid + p * 256, n = n0 + (g % WTile::kPerRow) * kGran<T>;
-                    h.w[p] = load_part(wp[p], s * kStep<T> + g / WTile::kPerRow < k_end ? (VEC && n >= a.ndim ? kGran<T> : a.ndim - n) : 0);
+                    gw[p] = load_part(wp[p], s * kStep<T> + g / WTile::kPerRow < k_end ? (VEC && n >= a.ndim ? kGran<T> : a.ndim - n) : 0);
                 }
             }
         }
 #pragma unroll
-        for (int p = 0; p < XP; ++p) xp[p] += kStep<T>;
-#pragma unroll
         for (int p = 0; p < WP; ++p) wp[p] += w_step;
     };
-    const auto put = [&](const Held &h, char *buf) {
+    const auto put = [&]() {
 #pragma unroll
         for (int p = 0; p < XP; ++p)
-            if (BM >= 32 || tid < BM * 8) *(v4i *)(buf + KTile<T>::at((tid >> 3) + p * 32, tid & 7)) = h.x[p].raw;
-        char *wb = buf + BM * kStepBytes;
+            if (BM >= 32 || tid < BM * 8) *(v4i *)(lds + KTile<T>::at((tid >> 3) + p * 32, tid & 7)) = gx[p].raw;
+        char *wb = lds + BM * kStepBytes;
 #pragma unroll
         for (int p = 0; p < WP; ++p) {
             if (BN < 32 && tid >= BN * 8) continue;
-            if (KCONTIG) {
-                *(v4i *)(wb + KTile<T>::at((tid >> 3) + p * 32, tid & 7)) = h.w[p].raw;
-            } else {
-                const int g = tid + p * 256;
-                *(v4i *)(wb + WTile::at(g / WTile::kPerRow, g % WTile::kPerRow)) = h.w[p].raw;
-            }
+            const int x = tid + p * 256;
+            *(v4i *)(wb + (KCONTIG ? KTile<T>::at((tid >> 3) + p * 32, tid & 7) : WTile::at(x / WTile::kPerRow, x % WTile::kPerRow))) = gw[p].raw;
         }
     };
 
@@ -172,8 +173,8 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     for (int i = 0; i < FA; ++i)
 #pragma unroll
         for (int j = 0; j < FB; ++j) acc[i][j] = (A4){0, 0, 0, 0};
-    const auto compute = [&](const char *buf) {
-        const char *wb = buf + BM * kStepBytes;
+    const auto compute = [&]() {
+        const char *wb = lds + BM * kStepBytes;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             Granule fa[FA], fb[FB];
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
                 fa[i] = KCONTIG ? KTile<T>::template read<true>(wb, block, ks) : WTile::template read<true>(wb, block, ks);
             }
 #pragma unroll
-            for (int j = 0; j < FB; ++j) fb[j] = KTile<T>::template read<false>(buf, wm * FB * 16 + j * 16, ks);
+            for (int j = 0; j < FB; ++j) fb[j] = KTile<T>::template read<false>(lds, wm * FB * 16 + j * 16, ks);
 #pragma unroll
             for (int part = 0; part < kParts<T>; ++part)
 #pragma unroll
@@ -193,15 +194,19 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
         }
     };
 
-    fetch(held, s_lo);                                          // (a split has at least one step)
+    fetch_weights(s_lo);                                        // (a split has at least one step)
+    fetch_rows(s_lo);
     if (tid < BN) bias_of[tid] = my_bias;
-    put(held, lds);
+    put();
     __syncthreads();
-    for (int s = s_lo; s < s_hi; ++s) {
-        if (s < last) fetch(held, s + 1);
-        compute(lds);
+    for (int s = s_lo; s <= last; ++s) {
+        if (s < last) {
+            fetch_weights(s + 1);
+            fetch_rows(s + 1);
+        }
+        compute();
         __syncthreads();
-        if (s < last) put(held, lds);
+        if (s < last) put();
         __syncthreads();
     }
 

@@ -1,7 +1,8 @@
 """
-ctypes binding of libbgmm_ops.so (the C-ABI of include/bgmm_ops.h) for torch tensors.
+Loading of libbgmm_ops.so (the C-ABI of include/bgmm_ops.h) and of its torch binding.
 
-There is NO CPU fallback: tensors that are not on a HIP device are refused.
+There is NO CPU fallback: tensors that are not on a HIP device are refused, and a library that is missing and cannot be
+built raises.
 """
 import ctypes
 import os
@@ -9,15 +10,12 @@ import os
 import torch
 
 from .. import _build
-from .._lib import BGMMError
 
 _vp, _i32, _i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
 
 LEVELS = 12                 # tile sizes of a grouping (include/bgmm_ops.h: BGMM_OPS_LEVELS)
 MAX_COMPONENTS = 8000
 MAX_CHOSEN = 32
-
-DTYPES = {torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
 
 # every symbol include/bgmm_ops.h declares: name -> (restype, argtypes)
 SIGNATURES = {
@@ -64,62 +62,10 @@ def load():
     return L
 
 
-def check(rc):
-    if rc != 0:
-        raise BGMMError(rc, (_lib.bgmm_ops_last_error() or b"").decode())
-
-
-def refuse(message, *args, code=-1):
-    """An argument that an operator does not take: BGMM_EINVAL (or the code given), as the library's own."""
-    raise BGMMError(code, message % args)
-
-
-def require_tensors(what, **tensors):
-    for name, t in tensors.items():
-        if t is not None and not isinstance(t, torch.Tensor):
-            refuse("%s: %s is no torch tensor", what, name)
-
-
-def require_device(what, **tensors):
-    """All the tensors given (None: absent) on one HIP device; returns it."""
-    device = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        d = t.device
-        if d.type != "cuda":
-            refuse("%s: %s is on %s; the operators run on HIP devices only", what, name, d, code=-2)
-        if device is None:
-            device = d
-        elif d != device:
-            refuse("%s: %s is on %s, the others on %s", what, name, d, device)
-    return device
-
-
-class _Here(object):
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_here = _Here()
-
-
-def on(device):
-    """Context with `device` current (nothing to do, and nothing paid, where it is already)."""
-    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def acc_dtype(dtype):
-    """What products and sums of an element type are held in."""
-    return torch.float64 if dtype == torch.float64 else torch.float32
-
-
-def ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def stream(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def binding():
+    """The extension module with the operators (csrc/ops_torch.cpp)."""
+    if not os.path.exists(_build.OPS_BINDING):
+        _build.build()
+    load()                              # (first: it settles which HIP runtime the library binds to)
+    from . import _binding
+    return _binding

@@ -1,7 +1,7 @@
 """Drafted labels verified against exact probabilities from given uniforms (``verify_drafts``)."""
-import torch
+from ._native import binding
 
-from . import _native as nat
+_b = binding()
 
 
 def verify_drafts(target, draft, labels, u_accept, u_draw, lengths=None):
@@ -22,41 +22,4 @@ def verify_drafts(target, draft, labels, u_accept, u_draw, lengths=None):
 
     Returns ``(out, accepted)``: int64 (B, T + 1), the accepted labels, the drawn one, -1 behind; int64 (B,).
     """
-    what = "verify_drafts"
-    given = dict(target=target, draft=draft, labels=labels, u_accept=u_accept, u_draw=u_draw, lengths=lengths)
-    nat.require_tensors(what, **given)
-    if not (target.dim() == 3 and draft.dim() == 3):
-        nat.refuse("%s: target and draft have %d and %d axes, not 3", what, target.dim(), draft.dim())
-    B, T, V = draft.shape
-    if not (tuple(target.shape) == (B, T + 1, V)):
-        nat.refuse("%s: target is %s, draft %s", what, tuple(target.shape), tuple(draft.shape))
-    if not (V >= 1):
-        nat.refuse("%s: no labels", what)
-    if not (target.dtype in nat.DTYPES and draft.dtype == target.dtype):
-        nat.refuse("%s: target is %s, draft %s", what, target.dtype, draft.dtype)
-    if not (labels.dtype == torch.int64 and tuple(labels.shape) == (B, T)):
-        nat.refuse("%s: labels are %s %s", what, labels.dtype, tuple(labels.shape))
-    if not (u_accept.dtype == torch.float64 and tuple(u_accept.shape) == (B, T)):
-        nat.refuse("%s: u_accept is %s %s", what, u_accept.dtype, tuple(u_accept.shape))
-    if not (u_draw.dtype == torch.float64 and tuple(u_draw.shape) == (B,)):
-        nat.refuse("%s: u_draw is %s %s", what, u_draw.dtype, tuple(u_draw.shape))
-    if not (lengths is None or (lengths.dtype == torch.int64 and tuple(lengths.shape) == (B,))):
-        nat.refuse("%s: lengths have to be int64 (%d,)", what, B)
-    dev = nat.require_device(what, **given)
-    L = nat.load()
-    target, draft = _last_contiguous(target), _last_contiguous(draft)
-    labels, u_accept, u_draw = labels.contiguous(), u_accept.contiguous(), u_draw.contiguous()
-    lengths = None if lengths is None else lengths.contiguous()
-    out = torch.empty((B, T + 1), dtype=torch.int64, device=dev)
-    accepted = torch.empty((B,), dtype=torch.int64, device=dev)
-    ws_bytes = L.bgmm_verify_drafts_ws(B, V)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    with nat.on(dev):
-        nat.check(L.bgmm_verify_drafts(nat.DTYPES[target.dtype], nat.ptr(target), target.stride(0), target.stride(1), nat.ptr(draft), draft.stride(0),
-                                       draft.stride(1), nat.ptr(labels), nat.ptr(u_accept), nat.ptr(u_draw), nat.ptr(lengths), B, T, V,
-                                       nat.ptr(out), nat.ptr(accepted), nat.ptr(ws), ws_bytes, nat.stream(dev)))
-    return out, accepted
-
-
-def _last_contiguous(t):
-    return t if t.shape[2] == 1 or t.stride(2) == 1 else t.contiguous()
+    return _b.verify_drafts(target, draft, labels, u_accept, u_draw, lengths)
