@@ -38,6 +38,33 @@ int ops_launched(const char *what);         // the status of the launch just mad
 
 __device__ __forceinline__ int wave_lane() { return threadIdx.x & 63; }
 
+// N bytes (4, 8, 16 or 32) from or to memory as one access per 16, at whatever alignment p has.  (Through a vector of words: element
+// by element the compiler would put the pieces together again as it likes.)
+typedef unsigned words1 __attribute__((ext_vector_type(1)));
+typedef unsigned words2 __attribute__((ext_vector_type(2)));
+typedef unsigned words4 __attribute__((ext_vector_type(4)));
+template <int N> struct WordsOf { typedef words4 type; };
+template <> struct WordsOf<4> { typedef words1 type; };
+template <> struct WordsOf<8> { typedef words2 type; };
+template <class R> __device__ __forceinline__ R load_any(const void *p) {
+    constexpr int kEach = sizeof(R) < 16 ? (int)sizeof(R) : 16, kNum = (int)sizeof(R) / kEach;
+    typedef typename WordsOf<kEach>::type W;
+    struct __attribute__((packed, may_alias)) Loose { W w; };
+    struct All { W w[kNum]; } all;
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) all.w[i] = ((const Loose *)p)[i].w;
+    return __builtin_bit_cast(R, all);
+}
+template <class R> __device__ __forceinline__ void store_any(void *p, const R &r) {
+    constexpr int kEach = sizeof(R) < 16 ? (int)sizeof(R) : 16, kNum = (int)sizeof(R) / kEach;
+    typedef typename WordsOf<kEach>::type W;
+    struct __attribute__((packed, may_alias)) Loose { W w; };
+    struct All { W w[kNum]; };
+    const All all = __builtin_bit_cast(All, r);
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) ((Loose *)p)[i].w = all.w[i];
+}
+
 // Lanes of the wave whose `key` (bits 0 .. nbits-1) equals this lane's; inactive lanes are in no group.
 __device__ __forceinline__ unsigned long long wave_match(int key, int nbits, bool active) {
     unsigned long long m = __ballot(active);

@@ -161,10 +161,29 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
     int *tile_starts = sizes + B + 1;         // [K + 2]
     int *part = tile_starts + B + 1;          // [kSums * waves]
     for (int j = threadIdx.x; j < nw * B; j += blockDim.x) hist[j] = 0;
-    __syncthreads();
-    const int per = ((P + nw - 1) / nw + 63) & ~63;
+    // a wave's rows: at most kHeld rounds of 64; their buckets and places among the wave's own stay in registers
+    constexpr int kHeld = kSmall / (64 * kWaves);
+    const int per = ((P + nw - 1) / nw + 63) & ~63, lane = wave_lane();
     const int lo = w * per < P ? w * per : P, hi = lo + per < P ? lo + per : P;
-    walk(lo, hi, nbits, hist + w * B, [&](i64 i) { return bucket_of(labels, i, K); }, [&](i64 i, int b, int) { bucket[i] = b; });
+    int held_b[kHeld], held_at[kHeld];
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) {
+        const int i = lo + r * 64 + lane;
+        held_b[r] = i < hi ? bucket_of(labels, i, K) : -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) {
+        if (lo + r * 64 >= hi) break;
+        const int b = held_b[r];
+        const bool on = b >= 0;
+        const unsigned long long same = wave_match(b, nbits, on);
+        const int leader = on ? __ffsll((unsigned long long)same) - 1 : lane;
+        int at = 0;
+        if (on && leader == lane) at = atomicAdd(&hist[w * B + b], __popcll(same));
+        held_at[r] = __shfl(at, leader) + __popcll(same & ((1ull << lane) - 1));
+        if (on) bucket[lo + r * 64 + lane] = b;
+    }
     __syncthreads();
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
         int s = 0;
@@ -183,7 +202,9 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
         tile_starts[b] = tile;
     });
     __syncthreads();
-    walk(lo, hi, nbits, hist + w * B, [&](i64 i) { return bucket_of(labels, i, K); }, [&](i64 i, int, int at) { order[at] = (int)i; });
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r)
+        if (lo + r * 64 + lane < hi) order[hist[w * B + held_b[r]] + held_at[r]] = lo + r * 64 + lane;
     write_tiles(K, sizes, tile_starts, tiles);
 }
 
@@ -301,7 +322,7 @@ extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int3
     int nbits = 1;
     while ((1 << nbits) < B) ++nbits;
     if (small_form(P, K)) {
-        const int waves = P <= 1024 ? 4 : kWaves;
+        const int waves = P <= 2048 ? 4 : kWaves;
         const size_t lds = sizeof(int) * ((size_t)(waves + 2) * B + 2 + kSums * waves);
         group_small<<<1, 64 * waves, lds, st>>>(labels, (int)P, K, nbits, bucket, order, offsets, first, table);
         return ops_launched("group_rows");

@@ -116,7 +116,7 @@ template <class T, int WIDTH> struct MTile {
 // 16 bytes at p, at whatever alignment its elements have
 template <class T> __device__ __forceinline__ Granule load_whole(const T *p) {
     Granule g;
-    __builtin_memcpy(&g.raw, p, 16);
+    g.raw = load_any<v4i>(p);
     return g;
 }
 // 16 bytes at p of which the first `avail` elements exist; the rest become zero
@@ -166,7 +166,7 @@ struct RowsArgs {
     void *ws;                       // or, instead of out: accumulator type, [splits][P][n], neither gated nor rounded
     i64 P;
     int kdim, ndim, splits, n_tiles;
-    bool out_vec;
+    int w_safe;                     // rows k of any component in front of this have 16 bytes from any of their elements on
 };
 
 struct WeightArgs {
@@ -179,6 +179,7 @@ struct WeightArgs {
     const void *d;                  // row p / d_div
     i64 d_stride;
     Divisor d_div;
+    int in_safe, d_safe;            // rows in front of this have 16 bytes from any of their elements on
     const void *gates;
     void *dw, *db;                  // element type, [K][idim][odim] and [K][odim] (db may be null; dw too)
     void *ws;                       // accumulator type: a slot of idim * odim + odim per chunk of a component with several
@@ -205,7 +206,8 @@ struct CombineArgs {
     int d_div, ddim;
 };
 
-// One product with rows; `small`: tiles of 16 rows, else 128.  `kcontig`: the weights' contiguous axis is the contraction.
-template <class T> int launch_rows(const RowsArgs &a, bool kcontig, bool vec, bool small, i64 blocks, hipStream_t st);
-template <class T> int launch_weight(const WeightArgs &a, bool vec, i64 blocks, hipStream_t st);
-template <class T> int launch_combine(const CombineArgs &a, bool vec, hipStream_t st);
+// One product with rows; bm x bn: its tiles (16 x 128, 128 x 16, 64 or 128).  `kcontig`: the weights' contiguous axis is the
+// contraction.  The weights' gradient by tiles of bt x bt (16, 64 or 128).
+template <class T> int launch_rows(const RowsArgs &a, bool kcontig, int bm, int bn, i64 blocks, hipStream_t st);
+template <class T> int launch_weight(const WeightArgs &a, int bt, i64 blocks, hipStream_t st);
+template <class T> int launch_combine(const CombineArgs &a, hipStream_t st);

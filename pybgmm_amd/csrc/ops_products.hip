@@ -13,7 +13,21 @@ Divisor divisor(int d) {
 }
 i64 at_most(i64 a, i64 b) { return a < b ? a : b; }
 
-int cols_tile(bool small, int ndim) { return small ? 128 : ndim <= 16 ? 16 : ndim <= 64 ? 64 : 128; }
+// Of `rows` rows `stride` elements apart, the first how many have 16 bytes from their last element on: the rows behind them, up to
+// the last row's last element, hold the rest.
+int safe_rows(i64 rows, i64 stride, int size) {
+    if (stride < 1) return 0;
+    const i64 n = rows - (16 / size - 1 + stride - 1) / stride;
+    return n < 0 ? 0 : (int)n;
+}
+
+// Columns of a tile of a product with rows: 128 beside 16 rows; else as many as there are, 64 instead of 128 where that leaves
+// compute units without a workgroup (20011 rows, 33 components, 192 -> 77 single: 27 -> 18 us).
+int cols_tile(i64 P, int K, int ndim) {
+    if (small_tiles(P, K)) return 128;
+    if (ndim <= 64) return ndim <= 16 ? 16 : 64;
+    return tiles_at_most(P, K) * ((ndim + 127) / 128) < 512 ? 64 : 128;
+}
 
 // Workgroups for `useful` ones in runs per die (die_order): runs of up to 64, shorter where the dies would get less than eight.
 struct Grid { int run; i64 blocks; };
@@ -24,14 +38,15 @@ Grid grid_of(i64 useful) {
     return g;
 }
 
-// Chunk of rows of the weights' gradient (a level of the grouping): as long as about a thousand workgroups remain, 256 ..
-// 32768 rows; a chunk leaves a tile of partial sums, which 256 rows of both operands outweigh.
-int weight_level(i64 P, int K, int idim, int odim) {
-    const int t = idim <= 16 && odim <= 16 ? 16 : idim <= 64 && odim <= 64 ? 64 : 128;
-    const i64 tiles = (i64)((idim + t - 1) / t) * ((odim + t - 1) / t);
-    int level = 4;
-    while (level < BGMM_OPS_LEVELS - 1 && P / (16 << (level + 1)) * tiles >= 1024) ++level;
-    return level;
+// Tile of the weights' gradient (bt x bt) and chunk of rows (a level of the grouping): chunks as long as about a thousand
+// workgroups remain, 256 .. 32768 rows -- a chunk leaves a tile of partial sums, which 256 rows of both operands outweigh --,
+// and tiles of 64 where 128 would leave compute units idle even so.
+struct WeightTiles { int bt, level; };
+WeightTiles weight_tiles(i64 P, int idim, int odim) {
+    const auto tiles = [&](int t) { return (i64)((idim + t - 1) / t) * ((odim + t - 1) / t); };
+    WeightTiles w = {idim <= 16 && odim <= 16 ? 16 : (idim <= 64 && odim <= 64) || (P / 256 + 1) * tiles(128) < 512 ? 64 : 128, 4};
+    while (w.level < BGMM_OPS_LEVELS - 1 && P / (16 << (w.level + 1)) * tiles(w.bt) >= 1024) ++w.level;
+    return w;
 }
 
 int check(const char *what, int dtype, i64 P, int K, int a, int b) {
@@ -46,8 +61,7 @@ int check(const char *what, int dtype, i64 P, int K, int a, int b) {
 
 extern "C" int bgmm_rows_product_splits(int32_t dtype, int64_t P, int32_t K, int32_t kdim, int32_t ndim) {
     if (check("rows_product_splits", dtype, P, K, kdim, ndim) != BGMM_OPS_OK || P == 0) return 1;
-    const bool small = small_tiles(P, K);
-    const int bn = cols_tile(small, ndim);
+    const int bn = cols_tile(P, K, ndim);
     const i64 groups = tiles_at_most(P, K) * ((ndim + bn - 1) / bn);
     const int steps = (kdim * size_of(dtype) + kStepBytes - 1) / kStepBytes;
     // (256 compute units: fill them twice over, but leave a part four steps to do)
@@ -63,11 +77,9 @@ extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_strid
     if (rc) return rc;
     if (P == 0) return BGMM_OPS_OK;
     if (!in || !w || !order || !tiles || !out == !ws) return ops_fail(BGMM_OPS_EINVAL, "rows_product: a null pointer (and exactly one of out, ws)");
-    if (in_div < 1 || splits < 1 || (out && splits != 1) || in_stride < 0 || out_stride < 0)
+    if (in_div < 1 || splits < 1 || (out && splits != 1) || in_stride < 0 || out_stride < 0 || w_component < 0 || w_row < 0)
         return ops_fail(BGMM_OPS_EINVAL, "rows_product: in_div %d, splits %d, strides %lld %lld", in_div, splits, (long long)in_stride, (long long)out_stride);
-    const int S = size_of(dtype), E = 16 / S;
-    const bool small = small_tiles(P, K);
-    const int bn = cols_tile(small, ndim);
+    const int bm = small_tiles(P, K) ? 16 : 128, bn = cols_tile(P, K, ndim);
     RowsArgs a;
     a.tiles = (const int4 *)tiles;
     a.tile_blocks = (int)(tiles_at_most(P, K) / 8);
@@ -90,18 +102,16 @@ extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_strid
     a.ndim = ndim;
     a.splits = splits;
     a.n_tiles = (ndim + bn - 1) / bn;
-    a.out_vec = ndim % 4 == 0 && (ws ? aligned(ws, 16) : out_stride % 4 == 0 && aligned(out, S == 2 ? 8 : 16));
-    const bool vec = aligned(in, 16) && aligned(w, 16) && in_stride % E == 0 && w_component % E == 0 && w_row % E == 0 && kdim % E == 0 &&
-                     (kcontig || ndim % E == 0);
+    a.w_safe = safe_rows(kdim, w_row, size_of(dtype));
     const Grid g = grid_of((i64)a.tile_blocks * 8 * a.n_tiles * splits);
     if (g.blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "rows_product: %lld tiles", (long long)g.blocks);
     a.run = g.run;
-    return by_type(dtype, [&](auto *t) { return launch_rows<std::remove_pointer_t<decltype(t)>>(a, kcontig != 0, vec, small, g.blocks, (hipStream_t)stream); });
+    return by_type(dtype, [&](auto *t) { return launch_rows<std::remove_pointer_t<decltype(t)>>(a, kcontig != 0, bm, bn, g.blocks, (hipStream_t)stream); });
 }
 
 extern "C" int64_t bgmm_weight_product_ws(int32_t dtype, int64_t P, int32_t K, int32_t idim, int32_t odim) {
     if (check("weight_product_ws", dtype, P, K, idim, odim) != BGMM_OPS_OK) return 0;
-    const i64 rows = (i64)16 << weight_level(P, K, idim, odim);
+    const i64 rows = (i64)16 << weight_tiles(P, idim, odim).level;
     if (P <= rows) return 0;
     return (2 * P / rows + 2) * ((i64)idim * odim + odim) * acc_size(dtype);
 }
@@ -117,10 +127,10 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
     if (ws_bytes < bgmm_weight_product_ws(dtype, P, K, idim, odim) || (ws_bytes > 0 && (!ws || !aligned(ws, 16))))
         return ops_fail(BGMM_OPS_EINVAL, "weight_product: workspace of %lld bytes", (long long)ws_bytes);
     if (K > 65535) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: K = %d", K);
-    const int S = size_of(dtype), E = 16 / S;
-    const int t = idim <= 16 && odim <= 16 ? 16 : idim <= 64 && odim <= 64 ? 64 : 128;
+    const WeightTiles w = weight_tiles(P, idim, odim);
+    const int t = w.bt;
     WeightArgs a;
-    a.level = weight_level(P, K, idim, odim);
+    a.level = w.level;
     a.bucket_first = first + (size_t)a.level * (K + 2);
     a.offsets = offsets;
     a.order = order;
@@ -139,11 +149,12 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
     a.odim = odim;
     a.i_tiles = (idim + t - 1) / t;
     a.o_tiles = (odim + t - 1) / t;
-    const bool vec = aligned(in, 16) && aligned(d, 16) && in_stride % E == 0 && d_stride % E == 0 && idim % E == 0 && odim % E == 0;
+    a.in_safe = safe_rows(P / in_div, in_stride, size_of(dtype));
+    a.d_safe = safe_rows(P / d_div, d_stride, size_of(dtype));
     const Grid g = grid_of(P == 0 ? 0 : (P / ((i64)16 << a.level) + at_most(K, P)) * a.i_tiles * a.o_tiles);
     if (g.blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: %lld tiles", (long long)g.blocks);
     a.run = g.run;
-    return by_type(dtype, [&](auto *t_) { return launch_weight<std::remove_pointer_t<decltype(t_)>>(a, vec, g.blocks, (hipStream_t)stream); });
+    return by_type(dtype, [&](auto *t_) { return launch_weight<std::remove_pointer_t<decltype(t_)>>(a, t, g.blocks, (hipStream_t)stream); });
 }
 
 extern "C" int bgmm_combine(int32_t dtype, const void *ws, int32_t splits, int64_t rows, int32_t k, int32_t K, const int32_t *bucket,
@@ -176,9 +187,5 @@ extern "C" int bgmm_combine(int32_t dtype, const void *ws, int32_t splits, int64
     a.d_stride = d_stride;
     a.d_div = d_div < 1 ? 1 : d_div;
     a.ddim = ddim;
-    const int S = size_of(dtype);
-    const auto fours = [&](const void *p, i64 stride) { return !p || (stride % 4 == 0 && aligned(p, S == 2 ? 8 : 16)); };
-    const bool vec = dim % 4 == 0 && aligned(ws, 16) && fours(out, out_stride) &&
-                     (!dgates || (fours(in, in_stride) && (!bias || (ddim % 4 == 0 && fours(bias, bias_row) && fours(d, d_stride)))));
-    return by_type(dtype, [&](auto *t) { return launch_combine<std::remove_pointer_t<decltype(t)>>(a, vec, (hipStream_t)stream); });
+    return by_type(dtype, [&](auto *t) { return launch_combine<std::remove_pointer_t<decltype(t)>>(a, (hipStream_t)stream); });
 }

@@ -4,17 +4,17 @@
 
 template <class T> __device__ __forceinline__ float as_f32(T v) { return (float)v; }
 
-// Four consecutive elements of an output row from an accumulator; `avail` of them exist.
-template <class T, class V> __device__ __forceinline__ void store4(T *p, const V &v, int avail, bool vec) {
-    if (vec) {
-        struct alignas(sizeof(T) * 4 < 16 ? sizeof(T) * 4 : 16) Four { T e[4]; } o;
+// Consecutive elements of an output row from accumulators, as one store where all of them exist (at any alignment).
+template <int N, class T, class V> __device__ __forceinline__ void store_run(T *p, const V &v, int from, int avail) {
+    struct Run { T e[N]; } o;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o.e[i] = (T)v[i];
-        if (avail > 0) *(Four *)p = o;
+    for (int i = 0; i < N; ++i) o.e[i] = (T)v[from + i];
+    if (avail >= N) {
+        store_any(p, o);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < avail) p[i] = (T)v[i];
+        for (int i = 0; i < N; ++i)
+            if (i < avail) p[i] = o.e[i];
     }
 }
 
@@ -26,26 +26,17 @@ template <class T, int TILE> constexpr int kWavesPerSimd = TILE >= 128 * 128 ? (
 
 // A lane's four results of a block of 16 columns of an output row (result_col); `avail` columns of the block exist.  S: what is
 // stored, T: the product's element type.
-template <class T, class S, class V> __device__ __forceinline__ void store_block(S *p, const V &v, int avail, bool vec) {
+template <class T, class S, class V> __device__ __forceinline__ void store_block(S *p, const V &v, int avail) {
     const int q = wave_lane() >> 4;
     if constexpr (sizeof(T) == 8) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int c = result_col<T>(q, 2 * h);
-            if (vec) {
-                struct alignas(16) Two { S e[2]; } o = {{(S)v[2 * h], (S)v[2 * h + 1]}};
-                if (c < avail) *(Two *)(p + c) = o;
-            } else {
-                if (c < avail) p[c] = (S)v[2 * h];
-                if (c + 1 < avail) p[c + 1] = (S)v[2 * h + 1];
-            }
-        }
+        for (int h = 0; h < 2; ++h) store_run<2>(p + result_col<T>(q, 2 * h), v, 2 * h, avail - result_col<T>(q, 2 * h));
     } else {
-        store4(p + q * 4, v, avail - q * 4, vec);
+        store_run<4>(p + q * 4, v, 0, avail - q * 4);
     }
 }
 
-template <class T, bool KCONTIG, bool VEC, int BM, int BN, int WN, int WM>
+template <class T, bool KCONTIG, int BM, int BN, int WN, int WM>
 __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(RowsArgs a) {
     typedef typename Acc<T>::type A;
     typedef typename Acc<T>::v4 A4;
@@ -82,10 +73,11 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     const int s_lo = steps_all * split / a.splits, s_hi = steps_all * (split + 1) / a.splits;
     const int k_end = s_hi * kStep<T> < a.kdim ? s_hi * kStep<T> : a.kdim;
 
-    // What a thread moves: granule column tid % 8 of the rows tid / 8 + 32 p of a KTile, granules tid + 256 p of an MTile.  VEC:
-    // every granule is whole and aligned; places outside (rows behind the last, columns behind ndim) read a neighbour that
-    // exists, whose results are not stored, so that the loop has loads and additions only; behind k_end, in the last step of a
-    // contraction that is not whole steps, both operands become zero on their way to LDS.
+    // What a thread moves: granule column tid % 8 of the rows tid / 8 + 32 p of a KTile, granules tid + 256 p of an MTile.  16-byte
+    // loads at any alignment; places outside (rows behind the last, columns behind ndim) read a neighbour that exists, whose
+    // results are not stored, so that the loop has loads and additions only.  A step is careful where it has to be: the last one
+    // where the contraction is not whole steps (what is behind it becomes zero in both operands), and those where a granule
+    // across the end of a weight's row could be across the end of all weights.
     typedef MTile<T, BN> WTile;
     const int kcol = (tid & 7) * kGran<T>;
     const T *xp[XP], *wp[WP];
@@ -104,7 +96,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
             wp[p] = w + (i64)(n < a.ndim ? n : a.ndim - 1) * a.w_row + s_lo * kStep<T> + kcol;
         } else {
             const int g = tid + p * 256, n = n0 + (g % WTile::kPerRow) * kGran<T>;
-            wp[p] = w + (i64)(s_lo * kStep<T> + g / WTile::kPerRow) * a.w_row + (!VEC || n < a.ndim ? n : n0);
+            wp[p] = w + (i64)(s_lo * kStep<T> + g / WTile::kPerRow) * a.w_row + (n < a.ndim ? n : n0);
         }
     }
     A my_bias = 0;
@@ -121,8 +113,9 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     Granule gx[XP], gw[WP];
     const int last = s_hi - 1;
     const bool ragged = s_hi * kStep<T> > k_end;
+    const bool edge = !KCONTIG && a.ndim - n0 < BN && a.ndim % kGran<T> != 0;
     const auto fetch_rows = [&](int s) {      // (step after step: the pointers move along)
-        if (VEC && !(ragged && s == last)) {
+        if (!(ragged && s == last)) {
 #pragma unroll
             for (int p = 0; p < XP; ++p)
                 if (BM >= 32 || tid < BM * 8) gx[p] = load_whole(xp[p]);
@@ -136,7 +129,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
         for (int p = 0; p < XP; ++p) xp[p] += kStep<T>;
     };
     const auto fetch_weights = [&](int s) {
-        if (VEC && !(ragged && s == last)) {
+        if (!(ragged && s == last) && !(edge && (s + 1) * kStep<T> > a.w_safe)) {
 #pragma unroll
             for (int p = 0; p < WP; ++p)
                 if (BN >= 32 || tid < BN * 8) gw[p] = load_whole(wp[p]);
@@ -148,7 +141,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
                     gw[p] = load_part(wp[p], k_end - s * kStep<T> - kcol);
                 } else {
                     const int g = tid + p * 256, n = n0 + (g % WTile::kPerRow) * kGran<T>;
-                    gw[p] = load_part(wp[p], s * kStep<T> + g / WTile::kPerRow < k_end ? (VEC && n >= a.ndim ? kGran<T> : a.ndim - n) : 0);
+                    gw[p] = load_part(wp[p], s * kStep<T> + g / WTile::kPerRow < k_end ? a.ndim - (n < a.ndim ? n : n0) : 0);
                 }
             }
         }
@@ -224,10 +217,10 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
 #pragma unroll
             for (int x = 0; x < 4; ++x) v[x] += bias_of[c + result_col<T>(lane >> 4, x)];
             if (a.ws) {
-                store_block<T>((A *)a.ws + ((i64)split * a.P + p) * a.ndim + n, v, a.ndim - n, a.out_vec);
+                store_block<T>((A *)a.ws + ((i64)split * a.P + p) * a.ndim + n, v, a.ndim - n);
             } else {
                 v *= gate;
-                store_block<T>((T *)a.out + p * a.out_stride + n, v, a.ndim - n, a.out_vec);
+                store_block<T>((T *)a.out + p * a.out_stride + n, v, a.ndim - n);
             }
         }
     }
@@ -235,7 +228,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
 
 // dW: the rows of a chunk are the contraction, both operands have it outermost (MTile).  Half precision: g d is rounded to
 // the operand type before the product (like the operands themselves), its column sums for db are not.
-template <class T, bool VEC, int BT, int WO, int WI>
+template <class T, int BT, int WO, int WI>
 __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kernel(WeightArgs a) {
     typedef typename Acc<T>::type A;
     typedef typename Acc<T>::v4 A4;
@@ -259,12 +252,13 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
     const bool want_db = a.db && i0 == 0;
 
     // a thread moves the same granule column of rows r, r + kRows, ...; both operands' rows go by the same index, read one
-    // step before its rows are asked for.  As in rows_kernel, places outside read a neighbour (VEC); rows behind the last are
-    // zero in both operands.
+    // step before its rows are asked for.  As in rows_kernel, places outside read a neighbour; rows behind the last are
+    // zero in both operands, and a granule across the end of a row is read with care where no row is behind it.
     constexpr int kRows = 256 / Tile::kPerRow < kStep<T> ? 256 / Tile::kPerRow : kStep<T>;
     const int my_row = tid / Tile::kPerRow, my_col = (tid % Tile::kPerRow) * kGran<T>;
-    const T *in = (const T *)a.in + (!VEC || i0 + my_col < a.idim ? i0 + my_col : i0);
-    const T *dd = (const T *)a.d + (!VEC || o0 + my_col < a.odim ? o0 + my_col : o0);
+    const int i_col = i0 + my_col < a.idim ? i0 + my_col : i0, o_col = o0 + my_col < a.odim ? o0 + my_col : o0;
+    const T *in = (const T *)a.in + i_col, *dd = (const T *)a.d + o_col;
+    const int i_safe = a.idim - i_col < kGran<T> ? a.in_safe : 0x7fffffff, o_safe = a.odim - o_col < kGran<T> ? a.d_safe : 0x7fffffff;
     struct Held { Granule i[NP], o[NP]; A gate[NP]; } held;
     int at[NP];
     const auto look = [&](int s) {
@@ -274,19 +268,35 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
             at[p] = list[r < n_rows ? r : n_rows - 1];
         }
     };
+    const bool edge = a.idim - i0 < BT && a.idim % kGran<T> != 0, o_edge = a.odim - o0 < BT && a.odim % kGran<T> != 0;
     const auto fetch = [&](Held &h, int s) {        // (at: the indices of step s; leaves those of s + 1)
+        if (kAll || tid < BT * 8) {
+            int ri[NP], ro[NP];
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            if (!kAll && tid >= BT * 8) continue;
-            const T *pi = in + (i64)divide(at[p], a.in_div) * a.in_stride, *po = dd + (i64)divide(at[p], a.d_div) * a.d_stride;
-            if (VEC) {
-                h.i[p] = load_whole(pi);
-                h.o[p] = load_whole(po);
-            } else {
-                h.i[p] = load_part(pi, a.idim - i0 - my_col);
-                h.o[p] = load_part(po, a.odim - o0 - my_col);
+            for (int p = 0; p < NP; ++p) {
+                ri[p] = divide(at[p], a.in_div);
+                ro[p] = divide(at[p], a.d_div);
             }
-            if (gates) h.gate[p] = gates[at[p]];
+            if (!(edge || o_edge)) {
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    h.i[p] = load_whole(in + (i64)ri[p] * a.in_stride);
+                    h.o[p] = load_whole(dd + (i64)ro[p] * a.d_stride);
+                }
+            } else {
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    const T *pi = in + (i64)ri[p] * a.in_stride, *po = dd + (i64)ro[p] * a.d_stride;
+                    if (ri[p] < i_safe) h.i[p] = load_whole(pi);
+                    else h.i[p] = load_part(pi, a.idim - i_col);
+                    if (ro[p] < o_safe) h.o[p] = load_whole(po);
+                    else h.o[p] = load_part(po, a.odim - o_col);
+                }
+            }
+            if (gates) {
+#pragma unroll
+                for (int p = 0; p < NP; ++p) h.gate[p] = gates[at[p]];
+            }
         }
         look(s + 1);
     };
@@ -361,7 +371,6 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
     // a component with one chunk is finished here; several leave partial sums, added in the chunks' order by weight_reduce
     A *slot = nullptr;
     if (chunks > 1) slot = (A *)a.ws + ((((i64)a.offsets[e] * 2) >> (4 + a.level)) + c) * ((i64)a.idim * a.odim + a.odim);
-    const bool o_vec = (a.odim & 3) == 0;
     if (a.dw && wave < WO * WI) {
 #pragma unroll
         for (int i = 0; i < FA; ++i) {
@@ -370,8 +379,8 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
             for (int j = 0; j < FB; ++j) {
                 const int r = i0 + (wi * FB + j) * 16 + (lane & 15);
                 if (r >= a.idim) continue;
-                if (slot) store_block<T>(slot + (i64)r * a.odim + o, acc[i][j], a.odim - o, o_vec);
-                else store_block<T>((T *)a.dw + ((i64)e * a.idim + r) * a.odim + o, acc[i][j], a.odim - o, o_vec);
+                if (slot) store_block<T>(slot + (i64)r * a.odim + o, acc[i][j], a.odim - o);
+                else store_block<T>((T *)a.dw + ((i64)e * a.idim + r) * a.odim + o, acc[i][j], a.odim - o);
             }
         }
     }
@@ -403,17 +412,25 @@ template <class T> __global__ __launch_bounds__(256) void weight_reduce(WeightAr
         const bool is_w = j < n_w;
         if (is_w ? !a.dw : !a.db) continue;
         A v = 0;
-        for (int c = 0; c < chunks; ++c) v += slot[c * size + j];
+        int c = 0;
+        for (; c + 8 <= chunks; c += 8) {           // (eight loads in flight)
+            A t[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) t[q] = slot[(c + q) * size + j];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v += t[q];
+        }
+        for (; c < chunks; ++c) v += slot[c * size + j];
         if (is_w) ((T *)a.dw)[(i64)e * n_w + j] = (T)v;
         else ((T *)a.db)[(i64)e * a.odim + (j - n_w)] = (T)v;
     }
 }
 
-// Four elements of a row as accumulators; VEC: all there and aligned.
-template <class S, class A, bool VEC> __device__ __forceinline__ void load4(const S *p, int avail, A (&v)[4]) {
-    struct alignas(sizeof(S) * 4 < 16 ? sizeof(S) * 4 : 16) Four { S e[4]; };
-    if (VEC) {
-        const Four f = *(const Four *)p;
+// Four elements of a row as accumulators, at any alignment; behind the row's end zeros.
+template <class S, class A> __device__ __forceinline__ void load4(const S *p, int avail, A (&v)[4]) {
+    if (avail >= 4) {
+        struct Four { S e[4]; };
+        const Four f = load_any<Four>(p);
 #pragma unroll
         for (int x = 0; x < 4; ++x) v[x] = (A)f.e[x];
     } else {
@@ -423,28 +440,18 @@ template <class S, class A, bool VEC> __device__ __forceinline__ void load4(cons
 }
 
 // u_p, the sum of its parts
-template <class A, bool VEC> __device__ __forceinline__ void parts4(const A *src, i64 part, int splits, int avail, A (&u)[4]) {
-    load4<A, A, VEC>(src, avail, u);
-    int s = 1;
-    for (; s + 3 <= splits; s += 3) {               // (three more in flight at a time)
-        A t[3][4];
-#pragma unroll
-        for (int q = 0; q < 3; ++q) load4<A, A, VEC>(src + (s + q) * part, avail, t[q]);
-#pragma unroll
-        for (int q = 0; q < 3; ++q)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) u[x] += t[q][x];
-    }
-    for (; s < splits; ++s) {
+template <class A> __device__ __forceinline__ void parts4(const A *src, i64 part, int splits, int avail, A (&u)[4]) {
+    load4(src, avail, u);
+    for (int s = 1; s < splits; ++s) {
         A t[4];
-        load4<A, A, VEC>(src + s * part, avail, t);
+        load4(src + s * part, avail, t);
 #pragma unroll
         for (int x = 0; x < 4; ++x) u[x] += t[x];
     }
 }
 
 // out[i] = sum over j of g_ij u_ij, u_ij the sum of its splits: one thread per four elements.
-template <class T, bool VEC> __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
+template <class T> __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
     typedef typename Acc<T>::type A;
     const int quads = (a.dim + 3) >> 2;
     for (i64 t = (i64)blockIdx.x * 256 + threadIdx.x; t < a.rows * quads; t += (i64)gridDim.x * 256) {
@@ -455,17 +462,41 @@ template <class T, bool VEC> __global__ __launch_bounds__(256) void combine_kern
             const i64 p = i * a.k + j;
             if (a.bucket[p] >= a.K) continue;
             A u[4];
-            parts4<A, VEC>((const A *)a.ws + p * a.dim + c, a.P * a.dim, a.splits, avail, u);
+            parts4<A>((const A *)a.ws + p * a.dim + c, a.P * a.dim, a.splits, avail, u);
             const A g = a.gates ? ((const A *)a.gates)[p] : (A)1;
 #pragma unroll
             for (int x = 0; x < 4; ++x) v[x] += g * u[x];
         }
-        store4((T *)a.out + i * a.out_stride + c, v, avail, VEC);
+        store_run<4>((T *)a.out + i * a.out_stride + c, v, 0, avail);
     }
 }
 
-// The same with the gates' gradient in . u_ij + b . d_i: one wave per row.  KJ >= k.
-template <class T, int KJ, bool VEC> __global__ __launch_bounds__(256) void combine_gates_kernel(CombineArgs a) {
+// The same for few rows with many parts: sixteen lanes share the k x splits terms of four elements, so that they are all in
+// flight at once.
+template <class T> __global__ __launch_bounds__(256) void combine_parts_kernel(CombineArgs a) {
+    typedef typename Acc<T>::type A;
+    const int quads = (a.dim + 3) >> 2, lane = threadIdx.x & 15;
+    const i64 t = (i64)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const bool on = t < a.rows * quads;
+    const i64 i = on ? t / quads : 0;
+    const int c = on ? (int)(t - i * quads) * 4 : 0, avail = a.dim - c;
+    typename Acc<T>::v4 v = {0, 0, 0, 0};
+    for (int x = lane; x < a.k * a.splits; x += 16) {
+        const i64 p = i * a.k + x % a.k;
+        if (a.bucket[p] >= a.K) continue;
+        A u[4];
+        load4((const A *)a.ws + ((i64)(x / a.k) * a.P + p) * a.dim + c, avail, u);
+        const A g = a.gates ? ((const A *)a.gates)[p] : (A)1;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) v[y] += g * u[y];
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) v[y] = group_sum<16>((A)v[y]);
+    if (on && lane == 0) store_run<4>((T *)a.out + i * a.out_stride + c, v, 0, avail);
+}
+
+// With the gates' gradient in . u_ij + b . d_i: one wave per row.  KJ >= k.
+template <class T, int KJ> __global__ __launch_bounds__(256) void combine_gates_kernel(CombineArgs a) {
     typedef typename Acc<T>::type A;
     const int lane = wave_lane();
     const i64 i = (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -483,19 +514,19 @@ template <class T, int KJ, bool VEC> __global__ __launch_bounds__(256) void comb
         const int avail = a.dim - c;
         typename Acc<T>::v4 v = {0, 0, 0, 0};
         A x[4];
-        load4<T, A, VEC>(in + c, avail, x);
+        load4(in + c, avail, x);
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
             if (e[j] >= a.K) continue;
             A u[4];
-            parts4<A, VEC>((const A *)a.ws + (i * a.k + j) * a.dim + c, a.P * a.dim, a.splits, avail, u);
+            parts4<A>((const A *)a.ws + (i * a.k + j) * a.dim + c, a.P * a.dim, a.splits, avail, u);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 dot[j] += x[q] * u[q];
                 v[q] += g[j] * u[q];
             }
         }
-        if (a.out) store4((T *)a.out + i * a.out_stride + c, v, avail, VEC);
+        if (a.out) store_run<4>((T *)a.out + i * a.out_stride + c, v, 0, avail);
     }
     if (a.bias) {
         for (int c = lane * 4; c < a.ddim; c += 256) {
@@ -503,8 +534,8 @@ template <class T, int KJ, bool VEC> __global__ __launch_bounds__(256) void comb
             for (int j = 0; j < KJ; ++j)
                 if (e[j] < a.K) {
                     A b[4], d[4];
-                    load4<T, A, VEC>((const T *)a.bias + (i64)e[j] * a.bias_row + c, a.ddim - c, b);
-                    load4<T, A, VEC>((const T *)a.d + ((i * a.k + j) / a.d_div) * a.d_stride + c, a.ddim - c, d);
+                    load4((const T *)a.bias + (i64)e[j] * a.bias_row + c, a.ddim - c, b);
+                    load4((const T *)a.d + ((i * a.k + j) / a.d_div) * a.d_stride + c, a.ddim - c, d);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) dot[j] += b[q] * d[q];
                 }
@@ -513,60 +544,54 @@ template <class T, int KJ, bool VEC> __global__ __launch_bounds__(256) void comb
 #pragma unroll
     for (int j = 0; j < KJ; ++j) {
         if (j >= a.k) break;
-        A v = dot[j];
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        const A v = group_sum<64>(dot[j]);
         if (lane == 0) ((A *)a.dgates)[i * a.k + j] = v;
     }
 }
 
-template <class T, bool KCONTIG, bool VEC> static void rows_by_tile(const RowsArgs &a, bool small, i64 blocks, hipStream_t st) {
+template <class T, bool KCONTIG> static void rows_by_tile(const RowsArgs &a, int bm, int bn, i64 blocks, hipStream_t st) {
     const dim3 g((unsigned)blocks);
-    if (small) rows_kernel<T, KCONTIG, VEC, 16, 128, 4, 1><<<g, 256, 0, st>>>(a);
-    else if (a.ndim <= 16) rows_kernel<T, KCONTIG, VEC, 128, 16, 1, 4><<<g, 256, 0, st>>>(a);
-    else if (a.ndim <= 64) rows_kernel<T, KCONTIG, VEC, 128, 64, 2, 2><<<g, 256, 0, st>>>(a);
-    else rows_kernel<T, KCONTIG, VEC, 128, 128, 2, 2><<<g, 256, 0, st>>>(a);
+    if (bm == 16) rows_kernel<T, KCONTIG, 16, 128, 4, 1><<<g, 256, 0, st>>>(a);
+    else if (bn == 16) rows_kernel<T, KCONTIG, 128, 16, 1, 4><<<g, 256, 0, st>>>(a);
+    else if (bn == 64) rows_kernel<T, KCONTIG, 128, 64, 2, 2><<<g, 256, 0, st>>>(a);
+    else rows_kernel<T, KCONTIG, 128, 128, 2, 2><<<g, 256, 0, st>>>(a);
 }
 
-template <class T> int launch_rows(const RowsArgs &a, bool kcontig, bool vec, bool small, i64 blocks, hipStream_t st) {
-    if (kcontig) vec ? rows_by_tile<T, true, true>(a, small, blocks, st) : rows_by_tile<T, true, false>(a, small, blocks, st);
-    else vec ? rows_by_tile<T, false, true>(a, small, blocks, st) : rows_by_tile<T, false, false>(a, small, blocks, st);
+template <class T> int launch_rows(const RowsArgs &a, bool kcontig, int bm, int bn, i64 blocks, hipStream_t st) {
+    kcontig ? rows_by_tile<T, true>(a, bm, bn, blocks, st) : rows_by_tile<T, false>(a, bm, bn, blocks, st);
     return ops_launched("rows_product");
 }
 
-template <class T, bool VEC> static void weight_by_tile(const WeightArgs &a, i64 blocks, hipStream_t st) {
+template <class T> int launch_weight(const WeightArgs &a, int bt, i64 blocks, hipStream_t st) {
     const dim3 g((unsigned)blocks);
-    if (a.idim <= 16 && a.odim <= 16) weight_kernel<T, VEC, 16, 1, 1><<<g, 256, 0, st>>>(a);
-    else if (a.idim <= 64 && a.odim <= 64) weight_kernel<T, VEC, 64, 2, 2><<<g, 256, 0, st>>>(a);
-    else weight_kernel<T, VEC, 128, 2, 2><<<g, 256, 0, st>>>(a);
-}
-
-template <class T> int launch_weight(const WeightArgs &a, bool vec, i64 blocks, hipStream_t st) {
-    if (blocks > 0) vec ? weight_by_tile<T, true>(a, blocks, st) : weight_by_tile<T, false>(a, blocks, st);
+    if (blocks > 0) {
+        if (bt == 16) weight_kernel<T, 16, 1, 1><<<g, 256, 0, st>>>(a);
+        else if (bt == 64) weight_kernel<T, 64, 2, 2><<<g, 256, 0, st>>>(a);
+        else weight_kernel<T, 128, 2, 2><<<g, 256, 0, st>>>(a);
+    }
     const i64 size = (i64)a.idim * a.odim + a.odim;
     const i64 bx = (size + 1023) / 1024 < 256 ? (size + 1023) / 1024 : 256;
     weight_reduce<T><<<dim3((unsigned)bx, (unsigned)a.K), 256, 0, st>>>(a);
     return ops_launched("weight_product");
 }
 
-template <class T, bool VEC> static void combine_gates(const CombineArgs &a, hipStream_t st) {
-    const dim3 g((unsigned)((a.rows + 3) / 4));
-    if (a.k == 1) combine_gates_kernel<T, 1, VEC><<<g, 256, 0, st>>>(a);
-    else if (a.k == 2) combine_gates_kernel<T, 2, VEC><<<g, 256, 0, st>>>(a);
-    else if (a.k <= 4) combine_gates_kernel<T, 4, VEC><<<g, 256, 0, st>>>(a);
-    else if (a.k <= 8) combine_gates_kernel<T, 8, VEC><<<g, 256, 0, st>>>(a);
-    else combine_gates_kernel<T, 32, VEC><<<g, 256, 0, st>>>(a);
-}
-
-template <class T> int launch_combine(const CombineArgs &a, bool vec, hipStream_t st) {
+template <class T> int launch_combine(const CombineArgs &a, hipStream_t st) {
     if (a.rows == 0) return BGMM_OPS_OK;
     if (a.dgates) {
-        vec ? combine_gates<T, true>(a, st) : combine_gates<T, false>(a, st);
+        const dim3 g((unsigned)((a.rows + 3) / 4));
+        if (a.k == 1) combine_gates_kernel<T, 1><<<g, 256, 0, st>>>(a);
+        else if (a.k == 2) combine_gates_kernel<T, 2><<<g, 256, 0, st>>>(a);
+        else if (a.k <= 4) combine_gates_kernel<T, 4><<<g, 256, 0, st>>>(a);
+        else if (a.k <= 8) combine_gates_kernel<T, 8><<<g, 256, 0, st>>>(a);
+        else combine_gates_kernel<T, 32><<<g, 256, 0, st>>>(a);
     } else {
         const i64 threads = a.rows * ((a.dim + 3) / 4);
-        const i64 b = (threads + 255) / 256 < 65536 ? (threads + 255) / 256 : 65536;
-        if (vec) combine_kernel<T, true><<<dim3((unsigned)b), 256, 0, st>>>(a);
-        else combine_kernel<T, false><<<dim3((unsigned)b), 256, 0, st>>>(a);
+        if (a.splits > 1) {
+            combine_parts_kernel<T><<<dim3((unsigned)((threads + 15) / 16)), 256, 0, st>>>(a);
+        } else {
+            const i64 b = (threads + 255) / 256 < 65536 ? (threads + 255) / 256 : 65536;
+            combine_kernel<T><<<dim3((unsigned)b), 256, 0, st>>>(a);
+        }
     }
     return ops_launched("combine");
 }

@@ -126,8 +126,8 @@ template <class T> constexpr int kPack = 16 / (int)sizeof(T);
 
 // 16 bytes of a row at any alignment its elements have
 template <class T> __device__ __forceinline__ void load_pack(const T *p, T *v) {
-    struct alignas(16) Pack { T e[kPack<T>]; } k;
-    __builtin_memcpy(&k, p, 16);
+    struct Pack { T e[kPack<T>]; };
+    const Pack k = load_any<Pack>(p);
 #pragma unroll
     for (int j = 0; j < kPack<T>; ++j) v[j] = k.e[j];
 }

@@ -385,7 +385,7 @@ CASES = [
     # n, k, K, din, dout
     (1, 1, 1, 1, 1), (1, 4, 64, 256, 128), (3, 2, 5, 64, 64), (1, 2, 3, 2048, 40), (17, 1, 40, 96, 200), (130, 1, 3, 64, 64),
     (257, 2, 4, 130, 66), (1000, 1, 7, 16, 16), (999, 3, 6, 33, 5), (700, 1, 2, 128, 300), (2050, 1, 20, 192, 77), (5000, 2, 9, 72, 136),
-    (4000, 1, 1, 20, 16), (64, 8, 16, 513, 129),
+    (4000, 1, 1, 20, 16), (64, 8, 16, 513, 129), (300, 1, 2, 65, 1), (300, 1, 2, 1, 65), (2000, 1, 3, 129, 3),
 ]
 
 
