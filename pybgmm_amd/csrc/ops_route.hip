@@ -28,58 +28,91 @@ template <class A> __device__ __forceinline__ A neg_inf();
 template <> __device__ __forceinline__ float neg_inf<float>() { return -__builtin_inff(); }
 template <> __device__ __forceinline__ double neg_inf<double>() { return -__builtin_inf(); }
 
-// exp(x) for x <= 0: 2^k exp(r), |r| <= ln 2 / 2, k ln 2 taken off in two parts; the Taylor series to r^13 / 13! leaves
-// 4e-18.  Twenty instructions where the library's takes twice as many; below 1e-308 the result is zero.
-__device__ __forceinline__ double exp_of(double x) {
-    const double k = __builtin_rint(x * 1.4426950408889634074);
-    double r = __builtin_fma(k, -0x1.62e42fefa39efp-1, x);      // ln 2 rounded to 53 bits ...
-    r = __builtin_fma(k, -0x1.abc9e3b39803fp-56, r);            // ... and what it is short by
-    double y = 1.0 / 6227020800.0;
-    y = __builtin_fma(y, r, 1.0 / 479001600.0);
-    y = __builtin_fma(y, r, 1.0 / 39916800.0);
-    y = __builtin_fma(y, r, 1.0 / 3628800.0);
-    y = __builtin_fma(y, r, 1.0 / 362880.0);
-    y = __builtin_fma(y, r, 1.0 / 40320.0);
-    y = __builtin_fma(y, r, 1.0 / 5040.0);
-    y = __builtin_fma(y, r, 1.0 / 720.0);
-    y = __builtin_fma(y, r, 1.0 / 120.0);
-    y = __builtin_fma(y, r, 1.0 / 24.0);
-    y = __builtin_fma(y, r, 1.0 / 6.0);
-    y = __builtin_fma(y, r, 0.5);
-    y = __builtin_fma(y, r, 1.0);
-    y = __builtin_fma(y, r, 1.0);
-    return x > -708.0 ? __builtin_ldexp(y, (int)k) : 0.0;
+template <class A> __device__ __forceinline__ A largest();
+template <> __device__ __forceinline__ float largest<float>() { return __FLT_MAX__; }
+template <> __device__ __forceinline__ double largest<double>() { return __DBL_MAX__; }
+
+// Of two values the larger or smaller, the other one for a quiet NaN: one instruction each (the builtins put another in front of
+// every operand that quiets signalling NaNs; here that is done once, where the values are read).
+__device__ __forceinline__ double larger(double a, double b) {
+    double r;
+    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
 }
-// 2^(x log2 e) on the hardware's exponential, the rounding of the product made good to first order (its error alone is |x|
-// half steps); below 1e-38 the result is zero.
-__device__ __forceinline__ float exp_of(float x) {
-    const float t = x * 1.44269504f;
-    const float low = __builtin_fmaf(x, 1.44269504f, -t) + x * 1.92596303e-8f;
-    const float y = __builtin_amdgcn_exp2f(t);
-    return x > -87.0f ? __builtin_fmaf(y, low * 0.693147181f, y) : 0.0f;
+__device__ __forceinline__ float larger(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ double smaller(double a, double b) {
+    double r;
+    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ float smaller(float a, float b) {
+    float r;
+    asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
 }
 
-// exp(v - m) with v == m exactly 1, infinities included
-template <class A> __device__ __forceinline__ A ratio(A v, A m) { return v == m ? (A)1 : exp_of(v - m); }
+// y[q] = exp(x[q]) for x <= 0, N at once so that they share the constants' registers.  Double: 2^k exp(r), |r| <= ln 2 / 2, k ln 2
+// taken off in two parts; the Taylor series to r^13 / 13! leaves 4e-18.  About twenty instructions each where the library's
+// takes twice as many.  Arguments below -800, -inf among them, give zero by underflow.
+template <int N> __device__ __forceinline__ void exps(const double *x, double *y) {
+    constexpr double c[14] = {1.0, 1.0, 0.5, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800,
+                              1.0 / 39916800, 1.0 / 479001600, 1.0 / 6227020800};
+    double k[N], r[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        const double v = larger(x[q], -800.0);
+        k[q] = __builtin_rint(v * 1.4426950408889634074);
+        r[q] = __builtin_fma(k[q], -0x1.62e42fefa39efp-1, v);           // ln 2 rounded to 53 bits ...
+        r[q] = __builtin_fma(k[q], -0x1.abc9e3b39803fp-56, r[q]);       // ... and what it is short by
+        y[q] = c[13];
+    }
+#pragma unroll
+    for (int t = 12; t >= 0; --t)
+#pragma unroll
+        for (int q = 0; q < N; ++q) y[q] = __builtin_fma(y[q], r[q], c[t]);
+#pragma unroll
+    for (int q = 0; q < N; ++q) y[q] = __builtin_ldexp(y[q], (int)k[q]);
+}
+// Single: 2^(x log2 e) on the hardware's exponential, the rounding of the product made good to first order (its error alone is |x|
+// half steps); below e^-87 the result is zero.
+template <int N> __device__ __forceinline__ void exps(const float *x, float *y) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        const float v = larger(x[q], -100.0f);
+        const float t = v * 1.44269504f;
+        const float low = __builtin_fmaf(v, 1.44269504f, -t) + v * 1.92596303e-8f;
+        const float e = __builtin_amdgcn_exp2f(t);
+        y[q] = x[q] > -87.0f ? __builtin_fmaf(e, low * 0.693147181f, e) : 0.0f;
+    }
+}
 
-// What a thread gets of a row: granule `g` (E elements, E = 1 or 16 bytes' worth) of its row, -inf behind the end and for NaN.
-template <class T, int E, class A> __device__ __forceinline__ void load_logs(const T *row, int c, int K, A *v) {
-    if (E == 1) {
-        const A x = c < K ? (A)row[c] : neg_inf<A>();
-        v[0] = x > neg_inf<A>() ? x : neg_inf<A>();
-    } else {
-        struct alignas(16) Pack { T e[E]; };
-        if (c < K) {                                            // (K is whole granules)
-            const Pack p = *(const Pack *)(row + c);
+// exp(v - m) for v <= m, exactly 1 where they are equal; m = +inf: 1 for +inf, 0 for the others.  (m = -inf: 1 everywhere, for
+// callers that ask for no such row.)
+template <int N, class A> __device__ __forceinline__ void ratios(const A *v, A m, A *y) {
+    const A top = m < (A)largest<A>() ? m : (A)largest<A>();
+    A x[N];
 #pragma unroll
-            for (int q = 0; q < E; ++q) {
-                const A x = (A)p.e[q];
-                v[q] = x > neg_inf<A>() ? x : neg_inf<A>();
-            }
-        } else {
+    for (int q = 0; q < N; ++q) x[q] = smaller(v[q] - top, (A)0);
+    exps<N>(x, y);
+}
+template <class A> __device__ __forceinline__ A ratio(A v, A m) {
+    A y;
+    ratios<1>(&v, m, &y);
+    return y;
+}
+
+// Granule c / E of a row (E elements, E = 1 or 16 bytes' worth), -inf behind the end and for NaN.
+template <class T, int E, class A> __device__ __forceinline__ void load_logs(const T *row, int c, bool on, A *v) {
+    struct alignas(E == 1 ? sizeof(T) : 16) Pack { T e[E]; } p;
+    if (on) p = *(const Pack *)(row + c);
 #pragma unroll
-            for (int q = 0; q < E; ++q) v[q] = neg_inf<A>();
-        }
+    for (int q = 0; q < E; ++q) {
+        const A x = (A)p.e[q];
+        v[q] = on ? larger(neg_inf<A>(), larger(x, x)) : neg_inf<A>();
     }
 }
 
@@ -92,39 +125,52 @@ template <class T, int G, int NG, int E> __global__ __launch_bounds__(256) void 
     const i64 i = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
     const bool on = i < a.n;                                    // (rows behind the last: their lanes reduce along)
     const T *row = (const T *)a.l + (on ? i : 0) * a.stride;
+    constexpr int kBatch = NG * E % 7 == 0 ? 7 : NG * E % 8 == 0 ? 8 : NG * E % 4 == 0 ? 4 : 2;      // exponentials at once
     A v[NG * E];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) load_logs<T, E>(row, (g * G + lane) * E, a.K, v + g * E);
-    A top = neg_inf<A>(), mine = neg_inf<A>(), total = 0;
-    int mine_at = -1;
-    for (int r = 0; r < a.k; ++r) {
-        A m = v[0];
+    for (int g = 0; g < NG; ++g) {                              // (K is whole granules)
+        const int c = (g * G + lane) * E;
+        if ((g + 1) * G * E <= a.K) load_logs<T, E>(row, c, true, v + g * E);
+        else load_logs<T, E>(row, c, c < a.K, v + g * E);
+    }
+    A m;
+    int at;
+    const auto find = [&]() {
+        m = v[0];
 #pragma unroll
-        for (int q = 1; q < NG * E; ++q) m = v[q] > m ? v[q] : m;
-        m = group_reduce<G>(m, [](A x, A y) { return x > y ? x : y; });
-        int at = 0x7fffffff;
+        for (int q = 1; q < NG * E; ++q) m = larger(m, v[q]);
+        m = group_reduce<G>(m, [](A x, A y) { return larger(x, y); });
+        at = 0x7fffffff;
 #pragma unroll
         for (int q = NG * E - 1; q >= 0; --q) at = v[q] == m ? (q / E) * G * E + q % E : at;
         at = at == 0x7fffffff ? at : at + lane * E;
         at = group_reduce<G>(at, [](int x, int y) { return x < y ? x : y; });
-        if (r == 0) {
-            top = m;
-            if (!a.renormalise) {
+    };
+    find();
+    const A top = m;
+    A mine = m, total = 0;                                      // (every lane starts with the first; lane r takes round r's)
+    int mine_at = m > neg_inf<A>() ? at : -1;
+    if (!a.renormalise) {
 #pragma unroll
-                for (int q = 0; q < NG * E; ++q) total += v[q] > neg_inf<A>() ? ratio(v[q], top) : (A)0;
-                total = group_sum<G>(total);
-            }
+        for (int b = 0; b < NG * E; b += kBatch) {
+            A y[kBatch];
+            ratios<kBatch>(v + b, top, y);
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q) total += y[q];
         }
-        const bool some = m > neg_inf<A>();
-        if (lane == r) {
-            mine = m;
-            mine_at = some ? at : -1;
-        }
+        total = group_sum<G>(total);
+    }
+    for (int r = 1; r < a.k; ++r) {
         const int g = at / E, slot = g % G == lane ? (g / G) * E + at % E : -1;
 #pragma unroll
         for (int q = 0; q < NG * E; ++q) v[q] = q == slot ? neg_inf<A>() : v[q];
+        find();
+        if (lane == r) {
+            mine = m;
+            mine_at = m > neg_inf<A>() ? at : -1;
+        }
     }
-    const A e = mine_at >= 0 ? ratio(mine, top) : (A)0;
+    const A e = mine_at >= 0 && lane < a.k ? ratio(mine, top) : (A)0;
     if (a.renormalise) total = group_sum<G>(e);
     if (!on) return;
     if (lane < a.k) {

@@ -253,6 +253,21 @@ def test_route_forward_and_backward(dt, n, K, k, renormalise):
 
 
 @gpu
+@pytest.mark.parametrize("dt,bits,i", [(torch.float64, 0x7FF0000000000001, torch.int64), (torch.float32, 0x7F800001, torch.int32),
+                                       (torch.float16, 0x7C01, torch.int16), (torch.bfloat16, 0x7F81, torch.int16)], ids=str)
+def test_route_never_chooses_a_signalling_nan(dt, bits, i):
+    from pybgmm_amd import ops
+    raw = torch.linspace(-3, 2, 40, device="cuda").to(dt).repeat(5, 1)
+    raw.view(i)[:, 1::2] = bits
+    assert torch.isnan(raw[:, 1::2]).all()
+    labels, w = ops.route(raw, 3, renormalise=False)
+    assert labels.tolist() == [[38, 36, 34]] * 5
+    row = raw[0].cpu().double()
+    soft = torch.softmax(torch.where(torch.isnan(row), -math.inf, row), 0)[[38, 36, 34]]
+    assert torch.allclose(w.cpu().double(), soft.expand(5, 3), rtol=1e-5, atol=0)
+
+
+@gpu
 def test_route_rows_with_strides_and_no_rows():
     from pybgmm_amd import ops
     lw = route_rows(40, 96, torch.float32, 3).cuda()
