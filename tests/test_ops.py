@@ -401,6 +401,7 @@ CASES = [
     (1, 1, 1, 1, 1), (1, 4, 64, 256, 128), (3, 2, 5, 64, 64), (1, 2, 3, 2048, 40), (17, 1, 40, 96, 200), (130, 1, 3, 64, 64),
     (257, 2, 4, 130, 66), (1000, 1, 7, 16, 16), (999, 3, 6, 33, 5), (700, 1, 2, 128, 300), (2050, 1, 20, 192, 77), (5000, 2, 9, 72, 136),
     (4000, 1, 1, 20, 16), (64, 8, 16, 513, 129), (300, 1, 2, 65, 1), (300, 1, 2, 1, 65), (2000, 1, 3, 129, 3),
+    (3000, 1, 5, 8, 16), (2500, 2, 4, 16, 31), (900, 1, 60, 2, 2), (1500, 1, 3, 32, 9), (1, 1, 1, 16, 16),
 ]
 
 
@@ -452,6 +453,26 @@ def test_long_groups_are_split_and_joined(dt, rows, K, din, dout):
     close(dx, ref["x"][0], ref["x"][1], dout + 16)
     close(dw, *ref["w"], rows)
     close(db, *ref["b"], rows)
+
+
+@gpu
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n,k,K,din,dout", [(40000, 1, 20, 2, 2), (35001, 1, 30, 8, 5), (33000, 1, 12, 7, 8), (20000, 2, 9, 3, 4), (40000, 1, 1, 1, 1)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_many_thin_rows(dt, n, k, K, din, dout, gated):
+    from pybgmm_amd import ops
+    z, x, w, b, gt, g = product_case(n, k, K, din, dout, dt, n + din, flat=k == 1, gates=gated)
+    groups = ops.group_rows(z, K)
+    leaves = [t.requires_grad_() for t in (x, w, b, gt) if t is not None]
+    y = ops.grouped_matmul(x, w, groups, bias=b, gates=gt)
+    dy = torch.randn(y.shape, generator=g, device="cuda", dtype=torch.float64).to(dt)
+    grads = torch.autograd.grad(y, leaves, dy)
+    ref = products_ref(x.detach(), w.detach(), z.view(n, k), b.detach(), None if gt is None else gt.detach(), dy)
+    close(y.detach(), ref["y"][0].view(y.shape), ref["y"][1].view(y.shape), din + k + 16)
+    for name, got in zip("xwbg", grads):
+        want, mag = (t.view(got.shape) for t in ref[name])
+        close(got, want, mag, {"x": dout + k, "w": n * k, "b": n * k, "g": din + 2 * dout}[name] + 16,
+              operand=half_step(dt) * 1.001 if name == "w" and gated and dt.itemsize == 2 else 0.0)
 
 
 @gpu
