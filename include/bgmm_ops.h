@@ -37,7 +37,7 @@ enum { BGMM_F64 = 0, BGMM_F32 = 1, BGMM_F16 = 2, BGMM_BF16 = 3 };
 enum {
     BGMM_OPS_MAX_COMPONENTS = 8000,  /* components of a grouping                               */
     BGMM_OPS_MAX_CHOSEN = 32,        /* components chosen per row by bgmm_route                */
-    BGMM_OPS_LEVELS = 12             /* tile sizes of a grouping: 16, 32, ..., 32768 rows      */
+    BGMM_OPS_LEVELS = 8              /* chunk sizes of a grouping: 256, 512, ..., 32768 rows   */
 };
 
 BGMM_OPS_API const char *bgmm_ops_last_error(void);
@@ -52,7 +52,7 @@ BGMM_OPS_API const char *bgmm_ops_runtime_path(void);
  *   bucket   int32[P]      out: the label, or K
  *   order    int32[P]      out: row indices sorted by (bucket, row)
  *   offsets  int32[K + 2]  out: bucket b holds order[offsets[b] .. offsets[b + 1])
- *   first    int32[BGMM_OPS_LEVELS][K + 2]  out: for tiles of 16 << level rows, how many tiles the buckets before b have
+ *   first    int32[BGMM_OPS_LEVELS][K + 2]  out: in chunks of 256 << level rows, how many the buckets before b have
  *   tiles    int32[bgmm_group_rows_tiles(P, K)][4]  out, 16-byte aligned: the tiles the products work by, {bucket, first place
  *            in order, rows, 0}, bucket by bucket, {-1, ...} behind the last
  *   ws       bgmm_group_rows_ws(P, K) bytes

@@ -20,8 +20,8 @@ template <> struct Acc<double> { typedef double type; typedef v4d v4; };
 // The tiles of a grouping's products: 16 rows where components have up to 16 on average (their workgroups stream the weights with
 // little else), 128 beyond; at most this many, those of the rows of no component included, in whole blocks of eight.
 inline bool small_tiles(i64 P, int K) { return P <= 16 * (i64)K; }
-inline int tile_level(i64 P, int K) { return small_tiles(P, K) ? 0 : 3; }
-inline i64 tiles_at_most(i64 P, int K) { return ((P >> (4 + tile_level(P, K))) + (K < P ? K : P) + 8) & ~(i64)7; }
+inline int tile_log2(i64 P, int K) { return small_tiles(P, K) ? 4 : 7; }
+inline i64 tiles_at_most(i64 P, int K) { return ((P >> tile_log2(P, K)) + (K < P ? K : P) + 8) & ~(i64)7; }
 
 // f(a null pointer of the element type's own): the dispatch of the C entry points, whose checks know the four types
 template <class F> int by_type(int dtype, F f) {

@@ -1,7 +1,7 @@
 // Rows grouped by component: a stable counting sort of P labels into K + 1 buckets (bucket K: unassigned rows).
 //
 //   order = argsort(bucket, stable), offsets = exclusive sum of the bucket sizes,
-//   first[l][b] = sum over b' < b of ceil(size(b') / (16 << l))
+//   first[l][b] = sum over b' < b of ceil(size(b') / (256 << l)), and the table of tiles that the products work by
 //
 // Stable and without atomics across workgroups, so that a grouping is the same every time: the gradients that sum over a
 // group's rows in this order are too.  A wave owns a segment of consecutive rows and a histogram of its own in LDS; the 64
@@ -57,10 +57,10 @@ __device__ __forceinline__ int block_scan(int n, int *part, F f, G g) {
     return carry;
 }
 
-// All the prefix sums over buckets at once: offsets and every level of tiles; place(b, start, tiles of level `level` before b)
-// sees every bucket and b = K + 1, what is behind the last.  `part`: kSums * waves ints.
-constexpr int kSums = BGMM_OPS_LEVELS + 1;
-template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows, const int *size_of, int *offsets, int *first, int level, int *part, P place) {
+// All the prefix sums over buckets at once: offsets, every level's chunks, the tiles of 1 << tile_lg rows; place(b, start, tiles
+// before b) sees every bucket and b = K + 1, what is behind the last.  `part`: kSums * waves ints.
+constexpr int kSums = BGMM_OPS_LEVELS + 2;
+template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows, const int *size_of, int *offsets, int *first, int tile_lg, int *part, P place) {
     const int nw = blockDim.x >> 6, w = threadIdx.x >> 6, B = K + 1;
     int carry[kSums];
 #pragma unroll
@@ -70,47 +70,44 @@ template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows,
         int incl[kSums];
 #pragma unroll
         for (int l = 0; l < kSums; ++l) {
-            const int v = l == 0 ? size : (int)(((i64)size + (8 << l) - 1) >> (3 + l));
+            const int lg = l == 0 ? 0 : l == 1 ? tile_lg : 6 + l;
+            const int v = (int)(((i64)size + (1 << lg) - 1) >> lg);
             const int t = wave_incl_scan(v);
             if (wave_lane() == 63) part[l * nw + w] = t;
             incl[l] = t - v;
         }
         __syncthreads();
-        int start = 0, tile = 0;
+        int sum[kSums];
 #pragma unroll
         for (int l = 0; l < kSums; ++l) {
-            int before = carry[l] + incl[l];
+            sum[l] = carry[l] + incl[l];
             for (int j = 0; j < nw; ++j) {
                 const int t = part[l * nw + j];
-                if (j < w) before += t;
+                if (j < w) sum[l] += t;
                 carry[l] += t;
             }
-            if (b < B) {
-                if (l == 0) offsets[b] = start = before;
-                else first[(i64)(l - 1) * (K + 2) + b] = before;
-                if (l == level + 1) tile = before;
-            }
         }
-        if (b < B) place(b, start, tile);
+        if (b < B) {
+            offsets[b] = sum[0];
+#pragma unroll
+            for (int l = 2; l < kSums; ++l) first[(i64)(l - 2) * (K + 2) + b] = sum[l];
+            place(b, sum[0], sum[1]);
+        }
         __syncthreads();
     }
     if (threadIdx.x == 0) {
         offsets[B] = P_rows;
-        int tile = 0;
 #pragma unroll
-        for (int l = 1; l < kSums; ++l) {
-            first[(i64)(l - 1) * (K + 2) + B] = carry[l];
-            if (l == level + 1) tile = carry[l];
-        }
-        place(B, P_rows, tile);
+        for (int l = 2; l < kSums; ++l) first[(i64)(l - 2) * (K + 2) + B] = carry[l];
+        place(B, P_rows, carry[1]);
     }
 }
 
-struct Tiles { int4 *at; int n, level; };
+struct Tiles { int4 *at; int n, lg; };
 
 // The table of tiles from a grouping's sums in LDS (starts and tile_starts: [K + 2]): a wave per bucket.
 __device__ __forceinline__ void write_tiles(int K, const int *starts, const int *tile_starts, Tiles t) {
-    const int lg = 4 + t.level, nw = blockDim.x >> 6;
+    const int lg = t.lg, nw = blockDim.x >> 6;
     for (int b = threadIdx.x >> 6; b <= K; b += nw) {
         const int start = starts[b], n = starts[b + 1] - start, t0 = tile_starts[b];
         for (int i = wave_lane(); i << lg < n; i += 64) t.at[t0 + i] = make_int4(b, start + (i << lg), n - (i << lg) < 1 << lg ? n - (i << lg) : 1 << lg, 0);
@@ -195,7 +192,7 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
         sizes[b] = s;
     }
     __syncthreads();
-    write_sums(K, P, sizes, offsets, first, tiles.level, part, [&](int b, int start, int tile) {
+    write_sums(K, P, sizes, offsets, first, tiles.lg, part, [&](int b, int start, int tile) {
         if (b < B)
             for (int j = 0; j < nw; ++j) hist[j * B + b] += start;
         sizes[b] = start;                     // (its own size has been read)
@@ -268,7 +265,7 @@ __global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int se
     int *start = lds + nw * B, *part = start + B;
     if (blockIdx.x == gridDim.x - 1) {
         int *starts = lds, *tile_starts = starts + B + 1;       // (the sums' parts behind them)
-        write_sums(K, (int)P, sizes, offsets, first, tiles.level, tile_starts + B + 1, [&](int b, int at, int tile) {
+        write_sums(K, (int)P, sizes, offsets, first, tiles.lg, tile_starts + B + 1, [&](int b, int at, int tile) {
             starts[b] = at;
             tile_starts[b] = tile;
         });
@@ -318,7 +315,7 @@ extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int3
     if (ws_bytes < bgmm_group_rows_ws(P, K) || (bgmm_group_rows_ws(P, K) > 0 && !ws)) return ops_fail(BGMM_OPS_EINVAL, "group_rows: workspace too small");
     hipStream_t st = (hipStream_t)stream;
     const int B = K + 1;
-    const Tiles table = {(int4 *)tiles, (int)tiles_at_most(P, K), tile_level(P, K)};
+    const Tiles table = {(int4 *)tiles, (int)tiles_at_most(P, K), tile_log2(P, K)};
     int nbits = 1;
     while ((1 << nbits) < B) ++nbits;
     if (small_form(P, K)) {

@@ -44,8 +44,8 @@ Grid grid_of(i64 useful) {
 struct WeightTiles { int bt, level; };
 WeightTiles weight_tiles(i64 P, int idim, int odim) {
     const auto tiles = [&](int t) { return (i64)((idim + t - 1) / t) * ((odim + t - 1) / t); };
-    WeightTiles w = {idim <= 16 && odim <= 16 ? 16 : (idim <= 64 && odim <= 64) || (P / 256 + 1) * tiles(128) < 512 ? 64 : 128, 4};
-    while (w.level < BGMM_OPS_LEVELS - 1 && P / (16 << (w.level + 1)) * tiles(w.bt) >= 1024) ++w.level;
+    WeightTiles w = {idim <= 16 && odim <= 16 ? 16 : (idim <= 64 && odim <= 64) || (P / 256 + 1) * tiles(128) < 512 ? 64 : 128, 0};
+    while (w.level < BGMM_OPS_LEVELS - 1 && P / (256 << (w.level + 1)) * tiles(w.bt) >= 1024) ++w.level;
     return w;
 }
 
@@ -111,7 +111,7 @@ extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_strid
 
 extern "C" int64_t bgmm_weight_product_ws(int32_t dtype, int64_t P, int32_t K, int32_t idim, int32_t odim) {
     if (check("weight_product_ws", dtype, P, K, idim, odim) != BGMM_OPS_OK) return 0;
-    const i64 rows = (i64)16 << weight_tiles(P, idim, odim).level;
+    const i64 rows = (i64)256 << weight_tiles(P, idim, odim).level;
     if (P <= rows) return 0;
     return (2 * P / rows + 2) * ((i64)idim * odim + odim) * acc_size(dtype);
 }
@@ -151,7 +151,7 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
     a.o_tiles = (odim + t - 1) / t;
     a.in_safe = safe_rows(P / in_div, in_stride, size_of(dtype));
     a.d_safe = safe_rows(P / d_div, d_stride, size_of(dtype));
-    const Grid g = grid_of(P == 0 ? 0 : (P / ((i64)16 << a.level) + at_most(K, P)) * a.i_tiles * a.o_tiles);
+    const Grid g = grid_of(P == 0 ? 0 : (P / ((i64)256 << a.level) + at_most(K, P)) * a.i_tiles * a.o_tiles);
     if (g.blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: %lld tiles", (long long)g.blocks);
     a.run = g.run;
     return by_type(dtype, [&](auto *t_) { return launch_weight<std::remove_pointer_t<decltype(t_)>>(a, t, g.blocks, (hipStream_t)stream); });

@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
     if (chunk >= a.bucket_first[a.K]) return;
     const int e = find_bucket(a.bucket_first, a.K, chunk);
     const int c = chunk - a.bucket_first[e], chunks = a.bucket_first[e + 1] - a.bucket_first[e];
-    const int rows_per = 16 << a.level;
+    const int rows_per = 256 << a.level;
     const int row0 = a.offsets[e] + c * rows_per, left = a.offsets[e + 1] - row0, n_rows = left < rows_per ? left : rows_per;
     const int *list = a.order + row0;
     const int i0 = (tile % a.i_tiles) * BT, o0 = (tile / a.i_tiles) * BT;
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
 
     // a component with one chunk is finished here; several leave partial sums, added in the chunks' order by weight_reduce
     A *slot = nullptr;
-    if (chunks > 1) slot = (A *)a.ws + ((((i64)a.offsets[e] * 2) >> (4 + a.level)) + c) * ((i64)a.idim * a.odim + a.odim);
+    if (chunks > 1) slot = (A *)a.ws + ((((i64)a.offsets[e] * 2) >> (8 + a.level)) + c) * ((i64)a.idim * a.odim + a.odim);
     if (a.dw && wave < WO * WI) {
 #pragma unroll
         for (int i = 0; i < FA; ++i) {
@@ -407,7 +407,7 @@ template <class T> __global__ __launch_bounds__(256) void weight_reduce(WeightAr
     const int chunks = a.bucket_first[e + 1] - a.bucket_first[e];
     if (chunks == 1) return;
     const i64 n_w = (i64)a.idim * a.odim, size = n_w + a.odim;
-    const A *slot = (const A *)a.ws + (((i64)a.offsets[e] * 2) >> (4 + a.level)) * size;
+    const A *slot = (const A *)a.ws + (((i64)a.offsets[e] * 2) >> (8 + a.level)) * size;
     for (i64 j = (i64)blockIdx.x * 256 + threadIdx.x; j < size; j += (i64)gridDim.x * 256) {
         const bool is_w = j < n_w;
         if (is_w ? !a.dw : !a.db) continue;

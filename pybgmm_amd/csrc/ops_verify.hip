@@ -42,33 +42,39 @@ template <class T> __device__ __forceinline__ double weight(const T *p, const T 
     return r > 0 ? r : 0.0;
 }
 
-// The drafts accepted: the same for every lane of every wave that asks.
-template <class T> __device__ __forceinline__ int accepted_drafts(const VerifyArgs &a, i64 b, int *length) {
+// The drafts accepted: the same for every lane of every wave that asks.  Everything about the first 64 drafts is asked for at
+// once, the length too; *z0: the label that was drafted at this lane's place.
+template <class T> __device__ __forceinline__ int accepted_drafts(const VerifyArgs &a, i64 b, int *length, i64 *z0) {
     const int lane = wave_lane();
     i64 len = a.lengths ? a.lengths[b] : a.T;
-    len = len < 0 ? 0 : len > a.T ? a.T : len;
     const T *tgt = (const T *)a.target + b * a.target_b, *dft = (const T *)a.draft + b * a.draft_b;
     int acc = 0;
-    for (int t0 = 0; t0 < len; t0 += 64) {
+    *z0 = -1;
+    for (int t0 = 0; t0 < a.T; t0 += 64) {
         const int t = t0 + lane;
         bool ok = false;
-        if (t < len) {
+        if (t < a.T) {
             const i64 z = a.labels[b * a.T + t];
-            if (z >= 0 && z < a.V) ok = a.u_accept[b * a.T + t] * clean(dft[t * a.draft_t + z]) < clean(tgt[t * a.target_t + z]);
+            const double u = a.u_accept[b * a.T + t];
+            if (t0 == 0) *z0 = z;
+            if (z >= 0 && z < a.V) ok = u * clean(dft[t * a.draft_t + z]) < clean(tgt[t * a.target_t + z]);
         }
-        const unsigned long long bad = __ballot(!ok);       // (lanes behind the length end the run)
+        const unsigned long long bad = __ballot(!ok || t >= len);       // (the length ends the run)
         const int run = bad ? __ffsll(bad) - 1 : 64;
         acc += run;
         if (run < 64) break;
     }
+    len = len < 0 ? 0 : len > a.T ? a.T : len;
     *length = (int)len;
     return acc;
 }
 
 // One wave writes a sequence's results.
-__device__ __forceinline__ void write_labels(const VerifyArgs &a, i64 b, int acc, i64 drawn) {
-    for (int t = wave_lane(); t <= a.T; t += 64) a.out[b * (a.T + 1) + t] = t < acc ? a.labels[b * a.T + t] : t == acc ? drawn : -1;
-    if (wave_lane() == 0) a.accepted[b] = acc;
+__device__ __forceinline__ void write_labels(const VerifyArgs &a, i64 b, int acc, i64 drawn, i64 z0) {
+    const int lane = wave_lane();
+    if (lane <= a.T) a.out[b * (a.T + 1) + lane] = lane < acc ? z0 : lane == acc ? drawn : -1;
+    for (int t = lane + 64; t <= a.T; t += 64) a.out[b * (a.T + 1) + t] = t < acc ? a.labels[b * a.T + t] : t == acc ? drawn : -1;
+    if (lane == 0) a.accepted[b] = acc;
 }
 
 // ---- few labels: a wave per sequence, NV x 64 >= V
@@ -76,20 +82,29 @@ template <class T, int NV> __global__ __launch_bounds__(256) void verify_rows_ke
     const i64 b = (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (b >= a.B) return;
     const int lane = wave_lane();
+    const double u = a.u_draw[b];
     int len;
-    const int acc = accepted_drafts<T>(a, b, &len);
+    i64 z0;
+    const int acc = accepted_drafts<T>(a, b, &len, &z0);
     const T *p = (const T *)a.target + b * a.target_b + acc * a.target_t;
     const T *q = acc < len ? (const T *)a.draft + b * a.draft_b + acc * a.draft_t : nullptr;
     double w[NV], res[NV], total = 0;
+    if (q) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = j * 64 + lane;
+            w[j] = c < a.V ? (double)p[c] : 0.0;
+            res[j] = c < a.V ? (double)q[c] : 0.0;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) w[j] = j * 64 + lane < a.V ? (double)p[j * 64 + lane] : 0.0;
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = j * 64 + lane;
-        w[j] = c < a.V ? clean(p[c]) : 0.0;
-        res[j] = w[j];
-        if (q) {
-            const double r = w[j] - (c < a.V ? clean(q[c]) : 0.0);
-            res[j] = r > 0 ? r : 0.0;
-        }
+        w[j] = clean(w[j]);
+        const double r = q ? w[j] - clean(res[j]) : w[j];
+        res[j] = r > 0 ? r : 0.0;
         total += res[j];
     }
     total = group_sum<64>(total);
@@ -100,7 +115,7 @@ template <class T, int NV> __global__ __launch_bounds__(256) void verify_rows_ke
         for (int j = 0; j < NV; ++j) total += w[j];
         total = group_sum<64>(total);
     }
-    const double goal = a.u_draw[b] * total;
+    const double goal = u * total;
     double before = 0;
     i64 drawn = -1;
     bool found = false;
@@ -118,7 +133,7 @@ template <class T, int NV> __global__ __launch_bounds__(256) void verify_rows_ke
             before += lane_read(s, 63);
         }
     }
-    write_labels(a, b, acc, drawn);
+    write_labels(a, b, acc, drawn, z0);
 }
 
 // ---- many labels: chunks of a row
@@ -176,7 +191,8 @@ template <class T> __global__ __launch_bounds__(256) void verify_sums_kernel(Ver
     const i64 b = blockIdx.x / w.chunks;
     const int c = (int)(blockIdx.x % w.chunks);
     int len;
-    const int acc = accepted_drafts<T>(a, b, &len);
+    i64 z0;
+    const int acc = accepted_drafts<T>(a, b, &len, &z0);
     const T *p = (const T *)a.target + b * a.target_b + acc * a.target_t;
     const T *q = acc < len ? (const T *)a.draft + b * a.draft_b + acc * a.draft_t : nullptr;
     const i64 lo = c * w.chunk, hi = lo + w.chunk < a.V ? lo + w.chunk : a.V;
@@ -257,7 +273,7 @@ template <class T> __global__ __launch_bounds__(64 * kDrawWaves) void verify_dra
             }
         }
     }
-    if (wave == 0) write_labels(a, b, acc, drawn);
+    if (wave == 0) write_labels(a, b, acc, drawn, wave_lane() < a.T ? a.labels[b * a.T + wave_lane()] : -1);
 }
 
 // Labels per chunk: enough workgroups for the chip (two thousand), at least 4096.

@@ -13,7 +13,7 @@ from .. import _build
 
 _vp, _i32, _i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
 
-LEVELS = 12                 # tile sizes of a grouping (include/bgmm_ops.h: BGMM_OPS_LEVELS)
+LEVELS = 8                  # chunk sizes of a grouping (include/bgmm_ops.h: BGMM_OPS_LEVELS)
 MAX_COMPONENTS = 8000
 MAX_CHOSEN = 32
 

@@ -311,12 +311,12 @@ def test_group_rows(shape, K):
     assert torch.equal(grp.offsets.cpu().long(), off)
     assert torch.equal(grp.counts.cpu().long(), size[:K])
     assert grp.labels_shape == shape and grp.n_components == K
-    first = grp.first.view(12, K + 2).cpu().long()
-    for level in range(12):
-        tiles = (size + (16 << level) - 1) // (16 << level)
+    first = grp.first.view(8, K + 2).cpu().long()
+    for level in range(8):
+        tiles = (size + (256 << level) - 1) // (256 << level)
         assert torch.equal(first[level], torch.cat([torch.zeros(1, dtype=torch.int64), tiles.cumsum(0)])), level
-    level = 0 if z.numel() <= 16 * K else 3
-    want = [[b, int(off[b]) + r, min(16 << level, int(size[b]) - r), 0] for b in range(K + 1) for r in range(0, int(size[b]), 16 << level)]
+    rows = 16 if z.numel() <= 16 * K else 128
+    want = [[b, int(off[b]) + r, min(rows, int(size[b]) - r), 0] for b in range(K + 1) for r in range(0, int(size[b]), rows)]
     got = grp.tiles.view(-1, 4).cpu()
     assert got[:len(want)].tolist() == want and bool((got[len(want):, 0] == -1).all())
 
