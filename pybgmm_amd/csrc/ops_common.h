@@ -108,18 +108,36 @@ __device__ __forceinline__ double wave_scan_sum(double v) {
     return v + (row == 0 ? 0.0 : row == 1 ? t0 : row == 2 ? t1 : t2);
 }
 
-// Which bucket tile t belongs to: the last b in 0 .. n-1 with first[b] <= t (first is non-decreasing, first[0] = 0; t is
-// below first[n]).  64 candidates per probe: two probes up to 4096 buckets, three beyond.  Every wave of a workgroup
-// finds the same answer by itself.
-__device__ __forceinline__ int find_bucket(const int *first, int n, int t) {
-    int lo = 0, span = n;
-    while (span > 1) {
-        const int step = (span + 63) >> 6;
-        const int at = lo + wave_lane() * step;
-        const int v = (at < n && wave_lane() * step < span) ? first[at] : 0x7fffffff;
-        const int below = __popcll(__ballot(v <= t));
+// Which bucket chunk t belongs to: the last b in 0 .. n-1 with first[b] <= t (first is non-decreasing, first[0] = 0, first[n] what is
+// behind the last), with the bucket's and the next one's entries of `first` and `offsets`.  64 candidates per probe: one up
+// to 63 buckets, two up to 4032, three beyond; the last probe brings the entries with it, so that nothing waits for another
+// load.  Every wave of a workgroup finds the same answer by itself.  b < 0: t is behind the last.
+struct Bucket {
+    int b, first, next_first, offset, next_offset;
+};
+__device__ __forceinline__ Bucket find_bucket(const int *first, const int *offsets, int n, int t) {
+    const int lane = wave_lane();
+    int lo = 0, span = n + 1;                               // (entries 0 .. n)
+    while (span > 64) {
+        const int step = (span + 62) / 63;                  // (so that 64 probes overlap by one and the next entry is among them)
+        const int at = lo + lane * step;
+        const int v = lane * step < span ? first[at <= n ? at : n] : 0x7fffffff;
+        const int below = __popcll(__ballot(v <= t && at <= n));
         lo += (below - 1) * step;
-        span = step < n - lo ? step : n - lo;
+        span = step + 1 < n + 1 - lo ? step + 1 : n + 1 - lo;
     }
-    return __builtin_amdgcn_readfirstlane(lo);
+    const int at = lo + lane < n ? lo + lane : n;
+    const int v = first[at], o = offsets[at];
+    const int below = __popcll(__ballot(lane < span && v <= t));
+    Bucket r;
+    r.b = lo + below - 1;
+    if (r.b >= n) {
+        r.b = -1;
+        return r;
+    }
+    r.first = __builtin_amdgcn_readlane(v, below - 1);
+    r.offset = __builtin_amdgcn_readlane(o, below - 1);
+    r.next_first = __builtin_amdgcn_readlane(v, below);
+    r.next_offset = __builtin_amdgcn_readlane(o, below);
+    return r;
 }

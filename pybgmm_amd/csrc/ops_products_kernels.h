@@ -24,15 +24,84 @@ template <int N, class T, class V> __device__ __forceinline__ void store_run(T *
 // 1024 x 2048, bfloat16: 197 -> 174 and 163 -> 134 us).
 template <class T, int TILE> constexpr int kWavesPerSimd = TILE >= 128 * 128 ? (sizeof(T) == 8 ? 2 : 3) : sizeof(T) == 8 && TILE >= 128 * 64 ? 3 : 4;
 
-// A lane's four results of a block of 16 columns of an output row (result_col); `avail` columns of the block exist.  S: what is
-// stored, T: the product's element type.
-template <class T, class S, class V> __device__ __forceinline__ void store_block(S *p, const V &v, int avail) {
-    const int q = wave_lane() >> 4;
-    if constexpr (sizeof(T) == 8) {
+// A tile's results leave through LDS, so that a row's are one stretch of memory per store instruction: straight from the
+// accumulators a lane has 8 or 16 bytes of a row, an instruction sixteen pieces of it, and the address unit takes them one by
+// one (64 experts' gradients of 1024 x 2048, bfloat16: 237 -> 188 us; 1e6 rows of 64 doubles: 272 -> 264 us).  As many rows at
+// a time as the buffer of BYTES holds; a granule of a row goes to place ^ (row & 15).  A 128 x 128 tile of doubles would take
+// four rounds, which cost more than they save (2e6 rows: 1344 -> 1389 us): those leave directly, 64 bytes of a row together.
+// S: what is stored.  part(m, i, j): the four results of row m in block i of 16 columns, of the lane's own in block j of rows;
+// row(m): where row m begins (m below n_rows), of which `width` columns exist.
+template <class T, class S, int BYTES, int BM, int BN, int FA, int FB, class Part, class Row>
+__device__ __forceinline__ void store_tile(char *lds, int wn, int wm, int n_rows, int width, Part part, Row row) {
+    constexpr int kFit = BYTES / (BN * (int)sizeof(S));
+    constexpr int R = kFit >= BM ? BM : kFit >= 64 ? 64 : kFit >= 32 ? 32 : 16;
+    constexpr int G = BN * (int)sizeof(S) / 16, E = 16 / (int)sizeof(S), kMask = G < 16 ? G - 1 : 15;
+    static_assert(R * BN * (int)sizeof(S) <= BYTES && BM % R == 0, "a tile's results by whole rounds");
+    const int lane = wave_lane(), q = lane >> 4;
+    if constexpr (sizeof(S) == 8 && BM * BN >= 128 * 128) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) store_run<2>(p + result_col<T>(q, 2 * h), v, 2 * h, avail - result_col<T>(q, 2 * h));
-    } else {
-        store_run<4>(p + q * 4, v, 0, avail - q * 4);
+        for (int j = 0; j < FB; ++j) {
+            const int m = (wm * FB + j) * 16 + (lane & 15);
+            if (m >= n_rows) continue;
+            S *line = row(m);
+#pragma unroll
+            for (int i = 0; i < FA; ++i) {
+                const auto v = part(m, i, j);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int col = (wn * FA + i) * 16 + result_col<T>(q, 2 * h);
+                    store_run<2>(line + col, v, 2 * h, width - col);
+                }
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int r0 = 0; r0 < BM; r0 += R) {
+        if (r0 >= n_rows) break;
+        __syncthreads();                                        // (the buffer is free: of operands, or of the round before)
+#pragma unroll
+        for (int j = 0; j < FB; ++j) {
+            const int block = (wm * FB + j) * 16;
+            if (block < r0 || block >= r0 + R) continue;
+            const int m = block + (lane & 15) - r0;
+            char *line = lds + m * (G * 16);
+#pragma unroll
+            for (int i = 0; i < FA; ++i) {
+                const auto v = part(m + r0, i, j);
+                const int c = (wn * FA + i) * 16;
+                if constexpr (sizeof(T) == 8) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int col = c + result_col<T>(q, 2 * h);
+                        struct alignas(16) Run { S e[2]; } o = {{(S)v[2 * h], (S)v[2 * h + 1]}};
+                        *(Run *)(line + (((col / E) ^ (m & kMask)) << 4)) = o;
+                    }
+                } else {
+                    const int col = c + q * 4;
+                    struct alignas(sizeof(S) == 2 ? 8 : 16) Run { S e[4]; } o = {{(S)v[0], (S)v[1], (S)v[2], (S)v[3]}};
+                    *(Run *)(line + (((col / E) ^ (m & kMask)) << 4) + col % E * (int)sizeof(S)) = o;
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x0 = 0; x0 < R * G; x0 += 256) {
+            const int x = x0 + threadIdx.x, m = x / G, g = x % G;
+            if ((R * G) % 256 != 0 && x >= R * G) continue;
+            if (m + r0 >= n_rows) continue;
+            struct alignas(16) Run { S e[E]; };
+            const Run o = *(const Run *)(lds + m * (G * 16) + ((g ^ (m & kMask)) << 4));
+            S *p = row(m + r0) + g * E;
+            const int avail = width - g * E;
+            if (avail >= E) {
+                store_any(p, o);
+            } else {
+#pragma unroll
+                for (int c = 0; c < E; ++c)
+                    if (c < avail) p[c] = o.e[c];
+            }
+        }
     }
 }
 
@@ -203,26 +272,22 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
         __syncthreads();
     }
 
-    // ---- results: a lane has four columns of a block (result_col) of row lane % 16 of the block's rows
+    // ---- results
+    constexpr int kBytes = (BM + BN) * kStepBytes;
+    const auto biased = [&](int i, int j) {
+        A4 v = acc[i][j];
 #pragma unroll
-    for (int j = 0; j < FB; ++j) {
-        const int m = (wm * FB + j) * 16 + (lane & 15);
-        if (m >= n_rows) continue;
-        const i64 p = row_of[m];
-        const A gate = gate_of[m];
-#pragma unroll
-        for (int i = 0; i < FA; ++i) {
-            const int c = (wn * FA + i) * 16, n = n0 + c;
-            A4 v = acc[i][j];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) v[x] += bias_of[c + result_col<T>(lane >> 4, x)];
-            if (a.ws) {
-                store_block<T>((A *)a.ws + ((i64)split * a.P + p) * a.ndim + n, v, a.ndim - n);
-            } else {
-                v *= gate;
-                store_block<T>((T *)a.out + p * a.out_stride + n, v, a.ndim - n);
-            }
-        }
+        for (int x = 0; x < 4; ++x) v[x] += bias_of[(wn * FA + i) * 16 + result_col<T>(lane >> 4, x)];
+        return v;
+    };
+    if (a.ws) {
+        A *ws = (A *)a.ws + (i64)split * a.P * a.ndim + n0;
+        store_tile<T, A, kBytes, BM, BN, FA, FB>(lds, wn, wm, n_rows, a.ndim - n0, [&](int, int i, int j) { return biased(i, j); },
+                                                 [&](int m) { return ws + (i64)row_of[m] * a.ndim; });
+    } else {
+        T *out = (T *)a.out + n0;
+        store_tile<T, T, kBytes, BM, BN, FA, FB>(lds, wn, wm, n_rows, a.ndim - n0, [&](int m, int i, int j) { return biased(i, j) * gate_of[m]; },
+                                                 [&](int m) { return out + (i64)row_of[m] * a.out_stride; });
     }
 }
 
@@ -241,11 +306,11 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
     const int wo = wave % WO, wi = wave / WO;
     const int out_tiles = a.i_tiles * a.o_tiles;
     const int id = die_order(a.run), chunk = id / out_tiles, tile = id % out_tiles;
-    if (chunk >= a.bucket_first[a.K]) return;
-    const int e = find_bucket(a.bucket_first, a.K, chunk);
-    const int c = chunk - a.bucket_first[e], chunks = a.bucket_first[e + 1] - a.bucket_first[e];
+    const Bucket at_b = find_bucket(a.bucket_first, a.offsets, a.K, chunk);
+    if (at_b.b < 0) return;
+    const int e = at_b.b, c = chunk - at_b.first, chunks = at_b.next_first - at_b.first;
     const int rows_per = 256 << a.level;
-    const int row0 = a.offsets[e] + c * rows_per, left = a.offsets[e + 1] - row0, n_rows = left < rows_per ? left : rows_per;
+    const int row0 = at_b.offset + c * rows_per, left = at_b.next_offset - row0, n_rows = left < rows_per ? left : rows_per;
     const int *list = a.order + row0;
     const int i0 = (tile % a.i_tiles) * BT, o0 = (tile / a.i_tiles) * BT;
     const A *gates = (const A *)a.gates;
@@ -370,23 +435,23 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
 
     // a component with one chunk is finished here; several leave partial sums, added in the chunks' order by weight_reduce
     A *slot = nullptr;
-    if (chunks > 1) slot = (A *)a.ws + ((((i64)a.offsets[e] * 2) >> (8 + a.level)) + c) * ((i64)a.idim * a.odim + a.odim);
-    if (a.dw && wave < WO * WI) {
-#pragma unroll
-        for (int i = 0; i < FA; ++i) {
-            const int o = o0 + (wo * FA + i) * 16;
-#pragma unroll
-            for (int j = 0; j < FB; ++j) {
-                const int r = i0 + (wi * FB + j) * 16 + (lane & 15);
-                if (r >= a.idim) continue;
-                if (slot) store_block<T>(slot + (i64)r * a.odim + o, acc[i][j], a.odim - o);
-                else store_block<T>((T *)a.dw + ((i64)e * a.idim + r) * a.odim + o, acc[i][j], a.odim - o);
-            }
+    if (chunks > 1) slot = (A *)a.ws + ((((i64)at_b.offset * 2) >> (8 + a.level)) + c) * ((i64)a.idim * a.odim + a.odim);
+    if (a.dw) {
+        constexpr int kBytes = 2 * BT * kStepBytes;
+        const int n_i = a.idim - i0 < BT ? a.idim - i0 : BT, w_o = WO * WI < 4 && wave >= WO * WI ? 0 : wo, w_i = WO * WI < 4 && wave >= WO * WI ? BT : wi;
+        const auto part = [&](int, int i, int j) { return acc[i][j]; };         // (waves without a part of the tile: none of its rows)
+        if (slot) {
+            A *to = slot + (i64)i0 * a.odim + o0;
+            store_tile<T, A, kBytes, BT, BT, FA, FB>(lds, w_o, w_i, n_i, a.odim - o0, part, [&](int m) { return to + (i64)m * a.odim; });
+        } else {
+            T *to = (T *)a.dw + ((i64)e * a.idim + i0) * a.odim + o0;
+            store_tile<T, T, kBytes, BT, BT, FA, FB>(lds, w_o, w_i, n_i, a.odim - o0, part, [&](int m) { return to + (i64)m * a.odim; });
         }
     }
     if (!want_db) return;
     // column sums: a thread has those of its granule's columns over its own rows; the threads of a column add up in order
     A *sums = (A *)lds;                       // [kRows][BT]
+    __syncthreads();
     if (kAll || tid < BT * 8) {
 #pragma unroll
         for (int j = 0; j < kGran<T>; ++j) sums[my_row * BT + my_col + j] = dsum[j];
