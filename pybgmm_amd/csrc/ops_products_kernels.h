@@ -235,6 +235,8 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     for (int i = 0; i < FA; ++i)
 #pragma unroll
         for (int j = 0; j < FB; ++j) acc[i][j] = (A4){0, 0, 0, 0};
+    // a wave whose part of the tile lies behind the last column or row multiplies nothing
+    const bool busy = n0 + wn * FA * 16 < a.ndim && wm * FB * 16 < n_rows;
     const auto compute = [&]() {
         const char *wb = lds + BM * kStepBytes;
 #pragma unroll
@@ -266,7 +268,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
             fetch_weights(s + 1);
             fetch_rows(s + 1);
         }
-        compute();
+        if (busy) compute();
         __syncthreads();
         if (s < last) put();
         __syncthreads();
@@ -634,8 +636,9 @@ template <class T> int launch_weight(const WeightArgs &a, int bt, i64 blocks, hi
         else if (bt == 64) weight_kernel<T, 64, 2, 2><<<g, 256, 0, st>>>(a);
         else weight_kernel<T, 128, 2, 2><<<g, 256, 0, st>>>(a);
     }
-    const i64 size = (i64)a.idim * a.odim + a.odim;
-    const i64 bx = (size + 1023) / 1024 < 256 ? (size + 1023) / 1024 : 256;
+    // (most components have one chunk and nothing to add up: about 4096 workgroups in all)
+    const i64 size = (i64)a.idim * a.odim + a.odim, most = 4096 / a.K > 4 ? 4096 / a.K : 4;
+    const i64 bx = (size + 255) / 256 < most ? (size + 255) / 256 : most;
     weight_reduce<T><<<dim3((unsigned)bx, (unsigned)a.K), 256, 0, st>>>(a);
     return ops_launched("weight_product");
 }
