@@ -147,7 +147,7 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
     a.ws = ws;
     a.idim = idim;
     a.odim = odim;
-    a.i_tiles = (idim + t - 1) / t;
+    a.i_tiles = dw ? (idim + t - 1) / t : 1;        // (the bias's sums come with the first)
     a.o_tiles = (odim + t - 1) / t;
     a.in_safe = safe_rows(P / in_div, in_stride, size_of(dtype));
     a.d_safe = safe_rows(P / d_div, d_stride, size_of(dtype));
