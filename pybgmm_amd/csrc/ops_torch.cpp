@@ -3,12 +3,14 @@
 // host (5 us here, twice that and more through ctypes and a Python autograd function) is what the small calls are made of.
 #include <torch/extension.h>
 
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cstdarg>
 #include <cstdio>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
 
 #include "../../include/bgmm_ops.h"
 
@@ -71,6 +73,9 @@ struct Device {
 void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor given(const Maybe &t) { return t ? *t : Tensor(); }
+// What the kernels read is the memory, so a view that torch negates on reading (the imaginary part of a conjugate) becomes values.
+Tensor values(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor packed(const Tensor &t) { return values(t).contiguous(); }
 
 // A (n, d) tensor as rows: the tensor itself if its last axis is contiguous, a copy otherwise.
 struct Rows {
@@ -79,6 +84,7 @@ struct Rows {
 };
 Rows rows_of(Tensor t) {
     if (!t.defined()) return {};
+    t = values(t);
     if (t.dim() == 3) t = t.reshape({-1, t.size(2)});               // (a view where the strides allow it)
     if ((t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < 0)) t = t.contiguous();
     return {t, t.size(0) > 1 ? t.stride(0) : t.size(1)};
@@ -86,6 +92,36 @@ Rows rows_of(Tensor t) {
 
 void first_order_only(const char *what) {
     if (at::GradMode::is_enabled()) refuse(BGMM_OPS_EUNSUPPORTED, "%s: differentiable once (no create_graph)", what);
+}
+
+// Whether gradients are wanted of any of a call's tensors (undefined ones: absent), and whether the call can give them.
+// Under capture, a node of the graph behind them that belongs to the default stream -- a leaf's too, while an eager graph that
+// was made there lives -- would draw the default stream into the capture in backward, which ends the process there; refused here.
+bool differentiable(const char *what, std::initializer_list<Tensor> inputs) {
+    bool any = false;
+    for (const Tensor &t : inputs) {
+        if (!t.defined()) continue;
+        if (t._fw_grad(0).defined()) refuse(BGMM_OPS_EUNSUPPORTED, "%s: no forward-mode derivatives", what);
+        any = any || t.requires_grad();
+    }
+    if (!any || !at::GradMode::is_enabled()) return false;
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return true;
+    std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+    std::unordered_set<const torch::autograd::Node *> seen;
+    const auto visit = [&](const std::shared_ptr<torch::autograd::Node> &f) {
+        if (f && seen.insert(f.get()).second) todo.push_back(f);
+    };
+    for (const Tensor &t : inputs)
+        if (t.defined() && t.requires_grad()) visit(t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t));
+    while (!todo.empty()) {
+        const auto f = todo.back();
+        todo.pop_back();
+        const auto s = f->stream();
+        if (s && s->id() == 0)
+            refuse(BGMM_OPS_EUNSUPPORTED, "%s: captured with gradients, but %s belongs to an eager graph of the default stream (free that graph, detach, or capture under no_grad)", what, f->name().c_str());
+        for (const auto &edge : f->next_edges()) visit(edge.function);
+    }
+    return true;
 }
 
 // ------------------------------------------------------------------------------------------ groupings
@@ -125,7 +161,7 @@ Groups group_rows(const Tensor &labels, int64_t components) {
     if (labels.numel() > 0x7fffffff - 65536) refuse(BGMM_OPS_EUNSUPPORTED, "%s: %lld labels (at most 2^31 - 65537)", what, (long long)labels.numel());
     Device dev{what};
     dev("labels", labels);
-    const Tensor flat = labels.contiguous();
+    const Tensor flat = packed(labels);
     const c10::OptionalDeviceGuard guard(labels.device());
     auto g = std::make_shared<RowGroups>(labels.sizes().vec(), components, at::empty({RowGroups::size(labels.numel(), components)}, labels.options().dtype(at::kInt)));
     check(bgmm_group_rows(g->P ? flat.data_ptr<int64_t>() : nullptr, g->P, (int32_t)g->K, g->bucket(), g->order(), g->offsets(), g->first(), g->tiles(), g->ws(),
@@ -174,7 +210,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
         const at::ScalarType dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
         const c10::OptionalDeviceGuard guard(labels.device());
         const Rows lw = renormalise ? Rows() : rows_of(saved[2]);
-        const Tensor d = grads[1].contiguous();
+        const Tensor d = packed(grads[1]);
         Tensor out = at::empty({labels.size(0), K}, labels.options().dtype(dtype));
         check(bgmm_route_backward(type_of(dtype), ptr(lw.t), lw.stride, labels.size(0), (int32_t)K, (int32_t)k, renormalise, (int64_t *)ptr(labels), ptr(weights),
                                   renormalise ? nullptr : ptr(saved[3]), ptr(d), ptr(out), stream_of(labels)));
@@ -191,7 +227,8 @@ std::tuple<Tensor, Tensor> route(const Tensor &lw, int64_t k, bool renormalise) 
     if (lw.size(1) > 0x7fffffff) refuse(BGMM_OPS_EUNSUPPORTED, "%s: %lld components", what, (long long)lw.size(1));
     Device dev{what};
     dev("log_weights", lw);
-    if (at::GradMode::is_enabled() && lw.requires_grad()) {
+    const c10::OptionalDeviceGuard guard(lw.device());
+    if (differentiable(what, {lw})) {
         const variable_list r = RouteFunction::apply(lw, k, renormalise);
         return {r[0], r[1]};
     }
@@ -206,7 +243,8 @@ struct Matrices {
     int64_t component, row;
     bool in_contiguous;
 };
-Matrices matrices_of(const Tensor &w) {
+Matrices matrices_of(const Tensor &stored) {
+    const Tensor w = values(stored);
     const int64_t s0 = w.stride(0), s1 = w.stride(1), s2 = w.stride(2);
     if (s0 >= 0 && s1 >= 0 && (s2 == 1 || w.size(2) == 1)) return {w, s0, s1, false};
     if (s0 >= 0 && s2 >= 0 && (s1 == 1 || w.size(1) == 1)) return {w, s0, s2, true};
@@ -232,7 +270,7 @@ Tensor matmul_forward(const Tensor &x_in, const Tensor &weight, const RowGroups 
     Tensor y = at::empty(shape, x_in.options());
     if (g.P == 0) return y;
     const Rows x = rows_of(x_in), bias = rows_of(bias_in);
-    const Tensor gates = gated ? gates_in.contiguous() : gates_in;
+    const Tensor gates = gated ? packed(gates_in) : gates_in;
     const int splits = bgmm_rows_product_splits(type, g.P, (int32_t)g.K, (int32_t)d_in, (int32_t)d_out);
     if (splits == 1 && !(gated && g.k > 1)) {
         product(g, x, x_div, matrices_of(weight), false, bias, gates, y, Tensor(), 1);
@@ -267,7 +305,7 @@ struct MatmulFunction : torch::autograd::Function<MatmulFunction> {
         const bool has_b = bias_in.defined(), has_g = saved[3].defined();
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(2),
                    need_g = has_g && ctx->needs_input_grad(2 + has_b);
-        const Tensor gates = has_g ? saved[3].contiguous() : Tensor();
+        const Tensor gates = has_g ? packed(saved[3]) : Tensor();
         const Rows x = rows_of(x_in), d = rows_of(grads[0]);
         const int64_t d_div = has_g ? g.k : 1;
         void *st = stream_of(x_in);
@@ -322,13 +360,14 @@ Tensor grouped_matmul(const Tensor &x, const Tensor &weight, const Groups &g, co
     dev("bias", b);
     dev("gates", gt);
     dev("the grouping", g->store);
-    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad()) || (gt.defined() && gt.requires_grad())))
+    const c10::OptionalDeviceGuard guard(x.device());
+    if (differentiable(what, {x, weight, b, gt}))
         return MatmulFunction::apply(x, weight, bias, gates, g);
     return matmul_forward(x, weight, *g, b, gt);
 }
 
 // ------------------------------------------------------------------------------------------ verify_drafts
-Tensor last_contiguous(const Tensor &t) { return t.size(2) == 1 || t.stride(2) == 1 ? t : t.contiguous(); }
+Tensor last_contiguous(const Tensor &t) { return t.size(2) == 1 || t.stride(2) == 1 ? values(t) : packed(t); }
 
 std::tuple<Tensor, Tensor> verify_drafts(const Tensor &target_in, const Tensor &draft_in, const Tensor &labels, const Tensor &u_accept, const Tensor &u_draw,
                                          const Maybe &lengths_in) {
@@ -356,8 +395,8 @@ std::tuple<Tensor, Tensor> verify_drafts(const Tensor &target_in, const Tensor &
     dev("u_draw", u_draw);
     dev("lengths", len_in);
     const c10::OptionalDeviceGuard guard(target_in.device());
-    const Tensor p = last_contiguous(target_in), q = last_contiguous(draft_in), z = labels.contiguous(), ua = u_accept.contiguous(), ud = u_draw.contiguous();
-    const Tensor len = len_in.defined() ? len_in.contiguous() : len_in;
+    const Tensor p = last_contiguous(target_in), q = last_contiguous(draft_in), z = packed(labels), ua = packed(u_accept), ud = packed(u_draw);
+    const Tensor len = len_in.defined() ? packed(len_in) : len_in;
     Tensor out = at::empty({B, T + 1}, labels.options()), accepted = at::empty({B}, labels.options());
     const int64_t bytes = bgmm_verify_drafts_ws(B, V);
     const Tensor ws = bytes ? at::empty({bytes}, labels.options().dtype(at::kByte)) : Tensor();
@@ -379,7 +418,12 @@ PYBIND11_MODULE(_binding, m) {
         }
     });
     py::class_<RowGroups, Groups>(m, "RowGroups")
-        .def(py::init<std::vector<int64_t>, int64_t, Tensor>(), py::arg("labels_shape"), py::arg("n_components"), py::arg("store"))
+        .def(py::init([](std::vector<int64_t> shape, int64_t components, Tensor store) {
+                 // (what the kernels follow is group_rows' own work)
+                 if (!store.device().is_cpu()) refuse(BGMM_OPS_EDEVICE, "RowGroups: a grouping on a device comes from group_rows");
+                 return std::make_shared<RowGroups>(std::move(shape), components, store);
+             }),
+             py::arg("labels_shape"), py::arg("n_components"), py::arg("store"))
         .def_static("store_size", &RowGroups::size)
         .def_property_readonly("labels_shape", [](const RowGroups &g) { return py::tuple(py::cast(g.shape)); })
         .def_readonly("n_components", &RowGroups::K)

@@ -888,3 +888,146 @@ def test_diagonal_components_have_no_factors():
     mm = CRPMM(X, NIW(np.zeros(3), 0.1, 5, np.ones(3)), 1.0, None, assignments="rand", K=2, covariance_type="diag")
     with pytest.raises(NotImplementedError):
         mm.posterior_labels(X)
+
+
+# ------------------------------------------------------------------------------------------ what the documentation allows or refuses
+@gpu
+def test_weights_and_their_gradients_beyond_32_bits_of_elements():
+    """Three matrices of 2^30 elements: the last begins at element 2^31.  Small integers, so every result is exact."""
+    from pybgmm_amd import ops
+    d = 1 << 15
+    w = torch.zeros(3, d, d, device="cuda", dtype=torch.float16)
+    w[2, d - 1, d - 1], w[2, 0, 5], w[1, 7, d - 1] = 3, 2, 1
+    x = torch.zeros(5, d, device="cuda", dtype=torch.float16)
+    x[:, d - 1], x[:, 0], x[:, 7] = 1, torch.arange(5, device="cuda", dtype=torch.float16), 4
+    w.requires_grad_()
+    z = torch.tensor([2, 0, 2, 1, 2], device="cuda")
+    y = ops.grouped_matmul(x, w, ops.group_rows(z, 3))
+    want = torch.zeros_like(y)
+    want[[0, 2, 4], d - 1], want[3, d - 1] = 3, 4
+    want[[0, 2, 4], 5] = 2 * torch.tensor([0, 2, 4], device="cuda", dtype=torch.float16)
+    assert torch.equal(y, want)
+    dy = torch.zeros_like(y)
+    dy[:, d - 2] = 1
+    dw, = torch.autograd.grad(y, w, dy)
+    for e, rows in enumerate(([1], [3], [0, 2, 4])):
+        assert torch.equal(dw[e, :, d - 2], x.detach()[rows].sum(0))
+    assert int(torch.count_nonzero(dw)) == int(torch.count_nonzero(dw[:, :, d - 2]))
+
+
+@gpu
+def test_a_label_is_compared_in_64_bits():
+    from pybgmm_amd import ops
+    z = torch.tensor([1, (1 << 32) + 1, -(1 << 32), (1 << 62), 0], device="cuda")
+    g = ops.group_rows(z, 2)
+    assert g.counts.tolist() == [1, 1]
+    x = torch.ones(5, 3, device="cuda")
+    y = ops.grouped_matmul(x, torch.ones(2, 3, 2, device="cuda"), g)
+    assert y[:, 0].tolist() == [3, 0, 0, 0, 3]
+    p = torch.ones(2, 2, 2, device="cuda")
+    out, acc = ops.verify_drafts(p, p[:, :1], torch.tensor([[(1 << 32) + 1], [1]], device="cuda"), torch.zeros(2, 1, device="cuda", dtype=torch.float64),
+                                 torch.full((2,), 0.75, device="cuda", dtype=torch.float64))
+    assert acc.tolist() == [0, 1] and out.tolist() == [[1, -1], [1, 1]]
+
+
+@gpu
+def test_views_that_are_negated_on_reading():
+    """The imaginary part of a conjugate shares the memory of the number; the operators see its values."""
+    from pybgmm_amd import ops
+    g = torch.Generator("cuda").manual_seed(5)
+
+    def neg(t):
+        return torch.complex(torch.zeros_like(t), -t).conj().imag
+    lw = torch.randn(40, 6, device="cuda", dtype=torch.float64, generator=g)
+    x = torch.randn(40, 6, device="cuda", dtype=torch.float64, generator=g)
+    w = torch.randn(6, 6, 5, device="cuda", dtype=torch.float64, generator=g)
+    b = torch.randn(6, 5, device="cuda", dtype=torch.float64, generator=g)
+    assert neg(lw).is_neg() and torch.equal(neg(lw), lw)
+    labels, gates = ops.route(lw, 2)
+    for a, c in zip((labels, gates), ops.route(neg(lw), 2)):
+        assert torch.equal(a, c)
+    groups = ops.group_rows(labels, 6)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b, gates)]
+    views = [t.clone().requires_grad_() for t in (x, w, b, gates)]
+    y = ops.grouped_matmul(leaves[0], leaves[1], groups, bias=leaves[2], gates=leaves[3])
+    y2 = ops.grouped_matmul(neg(views[0]), neg(views[1]), groups, bias=neg(views[2]), gates=neg(views[3]))
+    assert torch.equal(y, y2)
+    dy = torch.randn_like(y)
+    for a, c in zip(torch.autograd.grad(y, leaves, dy), torch.autograd.grad(y2, views, neg(dy))):
+        assert torch.equal(a, c)
+    p = torch.rand(3, 3, 9, device="cuda", dtype=torch.float64, generator=g)
+    u = torch.rand(3, 2, device="cuda", dtype=torch.float64, generator=g)
+    z = torch.tensor([[1, 2], [3, 4], [8, 0]], device="cuda")
+    want = ops.verify_drafts(p, p[:, 1:].contiguous(), z, u, u[:, 0].contiguous())
+    got = ops.verify_drafts(neg(p), neg(p[:, 1:].contiguous()), z, neg(u), neg(u[:, 0].contiguous()))
+    assert all(torch.equal(a, c) for a, c in zip(want, got))
+
+
+@gpu
+def test_derivatives_that_are_refused():
+    from pybgmm_amd import ops
+    from pybgmm_amd._lib import BGMMError
+    lw = torch.randn(8, 4, device="cuda", requires_grad=True)
+    x = torch.randn(8, 3, device="cuda", requires_grad=True)
+    w = torch.randn(4, 3, 2, device="cuda", requires_grad=True)
+    labels, gates = ops.route(lw, 2)
+    y = ops.grouped_matmul(x, w, ops.group_rows(labels, 4), gates=gates)
+    for out, leaf in ((gates, lw), (y, w)):
+        with pytest.raises(RuntimeError, match="differentiable once"):          # (reported by torch's engine)
+            torch.autograd.grad(out.sum(), leaf, create_graph=True, retain_graph=True)
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        dual = fw.make_dual(lw.detach(), torch.ones_like(lw))
+        with pytest.raises(BGMMError) as e:
+            ops.route(dual, 2)
+        assert e.value.code == -5
+        with pytest.raises(BGMMError) as e:
+            ops.grouped_matmul(fw.make_dual(x.detach(), torch.ones_like(x)), w.detach(), ops.group_rows(labels, 4))
+        assert e.value.code == -5
+
+
+@gpu
+def test_a_captured_step_is_refused_while_an_eager_graph_of_its_leaves_lives():
+    """Made on the default stream, that graph's leaves would draw it into the capture in backward."""
+    from pybgmm_amd import ops
+    from pybgmm_amd._lib import BGMMError
+    t, k, K = layer_inputs(n=120)
+    leaves = [a.clone().requires_grad_() for a in t]
+    dy = torch.randn(120, 12, device="cuda", dtype=torch.float64)
+    y = layer(*leaves, k, K)                                        # lives
+    want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    x, w = torch.randn(6, 3, device="cuda"), torch.randn(2, 3, 2, device="cuda", requires_grad=True)
+    groups = ops.group_rows(torch.tensor([0, 1, 1, 0, -1, 1], device="cuda"), 2)
+    kept = w * 2
+    torch.cuda.synchronize()
+    with pytest.raises(BGMMError) as e:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            dy.add(1.0)
+            layer(*leaves, k, K)
+    assert e.value.code == -5 and "default stream" in str(e.value)
+    with pytest.raises(BGMMError) as e:                             # the leaf, and a product behind it
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            dy.add(1.0)
+            ops.grouped_matmul(x, w, groups)
+    assert e.value.code == -5
+    with pytest.raises(BGMMError) as e:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            dy.add(1.0)
+            ops.grouped_matmul(x, kept, groups)
+    assert e.value.code == -5
+    with torch.no_grad():                                           # without gradients it is an ordinary capture
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            again = layer(*leaves, k, K)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, y)
+    del y, kept
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(layer(*leaves, k, K), leaves, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
