@@ -17,8 +17,9 @@ typedef double v4d __attribute__((ext_vector_type(4)));
 template <class T> struct Acc { typedef float type; typedef v4f v4; };
 template <> struct Acc<double> { typedef double type; typedef v4d v4; };
 
-// The tiles of a grouping's products: 16 rows where components have up to 16 on average (their workgroups stream the weights with
-// little else), 128 beyond; at most this many, those of the rows of no component included, in whole blocks of eight.
+// The tiles of a grouping's products: 16 rows where components have up to 16 on average, 128 beyond (1000 components, 64 x 64 double,
+// 16 rows each: 18 us against 24 with 128; 64 experts, 1024 x 1024 bfloat16, bound by their weights' 134 MB: 16 rows each 26 and
+// 25 us, 64 rows each 45 and 27 us).  At most this many, those of the rows of no component included, in whole blocks of eight.
 inline bool small_tiles(i64 P, int K) { return P <= 16 * (i64)K; }
 inline int tile_log2(i64 P, int K) { return small_tiles(P, K) ? 4 : 7; }
 inline i64 tiles_at_most(i64 P, int K) { return ((P >> tile_log2(P, K)) + (K < P ? K : P) + 8) & ~(i64)7; }

@@ -7,16 +7,21 @@
 // group's rows in this order are too.  A wave owns a segment of consecutive rows and a histogram of its own in LDS; the 64
 // rows it looks at together find their equals with one ballot per label bit.
 //
-// Up to kSmall rows one workgroup does everything in one launch (a single served row pays one launch, not three).  Beyond:
-// histograms per segment and workgroup, an exclusive sum over the workgroups per bucket, the scatter -- bound by the
-// latency of the segments' dependent LDS steps, not by the 20 P bytes that move.
+// Up to 4096 rows one workgroup does everything in one launch (64 components, one row 4 us, 4096 rows 9.4 us; in three launches 9
+// and 10.4 us).  Beyond: histograms per segment and workgroup, an exclusive sum over the workgroups per bucket, the scatter (1e6
+// rows, 100 components: 17 us) -- bound by the latency of the launches and of the segments' dependent LDS steps, not by the
+// 20 P bytes that move (4 us).
 #include "ops_common.h"
 
 namespace {
 
-constexpr int kSmall = 8192;            // rows of the one-workgroup form
-constexpr int kWaves = 16;              // its waves
-constexpr int kSmallBuckets = 890;      // its buckets (K + 1): 16 histograms, the sizes and the sums fit 64 KB of LDS
+constexpr int kSums = BGMM_OPS_LEVELS + 2;      // sums over buckets: offsets, tiles, chunks of every level
+// The one-workgroup form: up to 512 rows for each of its 8 waves with rows, 4 of them where 8 histograms, the sizes and the sums
+// would not fit 64 KB of LDS; the sums over buckets have a wave each.
+constexpr int kWaves = 8, kHeld = 8;    // (rounds of 64 rows)
+int small_waves(int K) { return K + 1 <= 1480 ? kWaves : K + 1 <= 2300 ? 4 : 0; }
+bool small_form(i64 P, int K) { return P <= small_waves(K) * 64 * kHeld && small_waves(K) > 0; }
+constexpr int kManyWaves = 8;           // waves of a workgroup of the other form
 
 __device__ __forceinline__ int bucket_of(const int64_t *labels, i64 i, int K) {
     const int64_t z = labels[i];
@@ -57,60 +62,63 @@ __device__ __forceinline__ int block_scan(int n, int *part, F f, G g) {
     return carry;
 }
 
-// All the prefix sums over buckets at once: offsets, every level's chunks, the tiles of 1 << tile_lg rows; place(b, start, tiles
-// before b) sees every bucket and b = K + 1, what is behind the last.  `part`: kSums * waves ints.
-constexpr int kSums = BGMM_OPS_LEVELS + 2;
-template <class P> __device__ __forceinline__ void write_sums(int K, int P_rows, const int *size_of, int *offsets, int *first, int tile_lg, int *part, P place) {
-    const int nw = blockDim.x >> 6, w = threadIdx.x >> 6, B = K + 1;
-    int carry[kSums];
+// All the prefix sums over buckets: offsets (sum 0), the tiles of 1 << tile_lg rows (1), every level's chunks.  Each sum is one
+// wave's, 64 buckets at a time without a barrier (four rows, 2000 components: 12 us, 68 with a barrier per round over all sums
+// and a wave per bucket in write_tiles).  start(b, ...) and tile(b, ...) see sums 0 and 1 of every bucket and of b = K + 1, what is
+// behind the last.
+template <class S, class T> __device__ __forceinline__ void write_sums(int K, const int *size_of, int *offsets, int *first, int tile_lg, S start, T tile) {
+    constexpr int kRounds = 4;                  // loads in flight
+    const int nw = blockDim.x >> 6, lane = wave_lane(), B = K + 1;
+    for (int l = threadIdx.x >> 6; l < kSums; l += nw) {
+        const int lg = l == 0 ? 0 : l == 1 ? tile_lg : 6 + l;
+        const auto emit = [&](int b, int sum) {
+            if (l == 0) {
+                offsets[b] = sum;
+                start(b, sum);
+            } else if (l == 1) {
+                tile(b, sum);
+            } else {
+                first[(i64)(l - 2) * (K + 2) + b] = sum;
+            }
+        };
+        int carry = 0;
+        for (int b0 = 0; b0 < B; b0 += 64 * kRounds) {
+            int v[kRounds];
 #pragma unroll
-    for (int l = 0; l < kSums; ++l) carry[l] = 0;
-    for (int base = 0; base < B; base += blockDim.x) {
-        const int b = base + threadIdx.x, size = b < B ? size_of[b] : 0;
-        int incl[kSums];
+            for (int r = 0; r < kRounds; ++r) {
+                const int b = b0 + r * 64 + lane;
+                v[r] = b < B ? size_of[b] : 0;
+            }
 #pragma unroll
-        for (int l = 0; l < kSums; ++l) {
-            const int lg = l == 0 ? 0 : l == 1 ? tile_lg : 6 + l;
-            const int v = (int)(((i64)size + (1 << lg) - 1) >> lg);
-            const int t = wave_incl_scan(v);
-            if (wave_lane() == 63) part[l * nw + w] = t;
-            incl[l] = t - v;
-        }
-        __syncthreads();
-        int sum[kSums];
-#pragma unroll
-        for (int l = 0; l < kSums; ++l) {
-            sum[l] = carry[l] + incl[l];
-            for (int j = 0; j < nw; ++j) {
-                const int t = part[l * nw + j];
-                if (j < w) sum[l] += t;
-                carry[l] += t;
+            for (int r = 0; r < kRounds; ++r) {
+                const int b = b0 + r * 64 + lane, n = (int)(((i64)v[r] + (1 << lg) - 1) >> lg), incl = wave_incl_scan(n);
+                if (b < B) emit(b, carry + incl - n);
+                carry += __builtin_amdgcn_readlane(incl, 63);
             }
         }
-        if (b < B) {
-            offsets[b] = sum[0];
-#pragma unroll
-            for (int l = 2; l < kSums; ++l) first[(i64)(l - 2) * (K + 2) + b] = sum[l];
-            place(b, sum[0], sum[1]);
-        }
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        offsets[B] = P_rows;
-#pragma unroll
-        for (int l = 2; l < kSums; ++l) first[(i64)(l - 2) * (K + 2) + B] = carry[l];
-        place(B, P_rows, carry[1]);
+        if (lane == 0) emit(B, carry);
     }
 }
 
 struct Tiles { int4 *at; int n, lg; };
 
-// The table of tiles from a grouping's sums in LDS (starts and tile_starts: [K + 2]): a wave per bucket.
+// The table of tiles from a grouping's sums in LDS (starts and tile_starts: [K + 2]): a lane per bucket, the wave together for a
+// bucket of more than four tiles.
 __device__ __forceinline__ void write_tiles(int K, const int *starts, const int *tile_starts, Tiles t) {
-    const int lg = t.lg, nw = blockDim.x >> 6;
-    for (int b = threadIdx.x >> 6; b <= K; b += nw) {
-        const int start = starts[b], n = starts[b + 1] - start, t0 = tile_starts[b];
-        for (int i = wave_lane(); i << lg < n; i += 64) t.at[t0 + i] = make_int4(b, start + (i << lg), n - (i << lg) < 1 << lg ? n - (i << lg) : 1 << lg, 0);
+    const int lg = t.lg, nw = blockDim.x >> 6, w = threadIdx.x >> 6, lane = wave_lane();
+    const auto write = [&](int b, int start, int n, int t0, int i) { t.at[t0 + i] = make_int4(b, start + (i << lg), n - (i << lg) < 1 << lg ? n - (i << lg) : 1 << lg, 0); };
+    for (int b0 = w; b0 <= K; b0 += 64 * nw) {
+        const int b = b0 + lane * nw;
+        const bool on = b <= K;
+        const int start = on ? starts[b] : 0, n = on ? starts[b + 1] - start : 0, t0 = on ? tile_starts[b] : 0;
+        const bool many = n > 4 << lg;
+        if (!many)
+            for (int i = 0; i << lg < n; ++i) write(b, start, n, t0, i);
+        for (unsigned long long left = __ballot(many); left; left &= left - 1) {
+            const int l = __ffsll(left) - 1;
+            const int lb = b0 + l * nw, ls = __builtin_amdgcn_readlane(start, l), ln = __builtin_amdgcn_readlane(n, l), lt = __builtin_amdgcn_readlane(t0, l);
+            for (int i = lane; i << lg < ln; i += 64) write(lb, ls, ln, lt, i);
+        }
     }
     for (int i = tile_starts[K + 1] + threadIdx.x; i < t.n; i += blockDim.x) t.at[i] = make_int4(-1, 0, 0, 0);
 }
@@ -149,19 +157,18 @@ __device__ __forceinline__ void walk(i64 lo, i64 hi, int nbits, int *cursor, L b
     }
 }
 
-__global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels, int P, int K, int nbits, int *bucket, int *order,
+__global__ __launch_bounds__(64 * kSums) void group_small(const int64_t *labels, int P, int K, int nbits, int waves, int *bucket, int *order,
                                                            int *offsets, int *first, Tiles tiles) {
     extern __shared__ int lds[];
-    const int B = K + 1, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    const int B = K + 1, w = threadIdx.x >> 6;
     int *hist = lds;                          // [waves][K + 1]
-    int *sizes = hist + nw * B;               // [K + 1], later the starts [K + 2]
-    int *tile_starts = sizes + B + 1;         // [K + 2]
-    int *part = tile_starts + B + 1;          // [kSums * waves]
-    for (int j = threadIdx.x; j < nw * B; j += blockDim.x) hist[j] = 0;
+    int *sizes = hist + waves * B;            // [K + 1]
+    int *starts = sizes + B;                  // [K + 2]
+    int *tile_starts = starts + B + 1;        // [K + 2]
+    for (int j = threadIdx.x; j < waves * B; j += blockDim.x) hist[j] = 0;
     // a wave's rows: at most kHeld rounds of 64; their buckets and places among the wave's own stay in registers
-    constexpr int kHeld = kSmall / (64 * kWaves);
-    const int per = ((P + nw - 1) / nw + 63) & ~63, lane = wave_lane();
-    const int lo = w * per < P ? w * per : P, hi = lo + per < P ? lo + per : P;
+    const int per = ((P + waves - 1) / waves + 63) & ~63, lane = wave_lane();
+    const int lo = w * per < P ? w * per : P, hi = lo + per < P ? lo + per : P;       // (none for the waves behind them: waves * per >= P)
     int held_b[kHeld], held_at[kHeld];
 #pragma unroll
     for (int r = 0; r < kHeld; ++r) {
@@ -183,38 +190,36 @@ __global__ __launch_bounds__(64 * kWaves) void group_small(const int64_t *labels
     }
     __syncthreads();
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
-        int s = 0;
-        for (int j = 0; j < nw; ++j) {
-            const int n = hist[j * B + b];
-            hist[j * B + b] = s;
-            s += n;
+        int n[kWaves], s = 0;
+#pragma unroll
+        for (int j = 0; j < kWaves; ++j) n[j] = j < waves ? hist[j * B + b] : 0;
+#pragma unroll
+        for (int j = 0; j < kWaves; ++j) {
+            if (j < waves) hist[j * B + b] = s;
+            s += n[j];
         }
         sizes[b] = s;
     }
     __syncthreads();
-    write_sums(K, P, sizes, offsets, first, tiles.lg, part, [&](int b, int start, int tile) {
-        if (b < B)
-            for (int j = 0; j < nw; ++j) hist[j * B + b] += start;
-        sizes[b] = start;                     // (its own size has been read)
-        tile_starts[b] = tile;
-    });
+    write_sums(K, sizes, offsets, first, tiles.lg, [&](int b, int sum) { starts[b] = sum; }, [&](int b, int sum) { tile_starts[b] = sum; });
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kHeld; ++r)
-        if (lo + r * 64 + lane < hi) order[hist[w * B + held_b[r]] + held_at[r]] = lo + r * 64 + lane;
-    write_tiles(K, sizes, tile_starts, tiles);
+        if (lo + r * 64 + lane < hi) order[starts[held_b[r]] + hist[w * B + held_b[r]] + held_at[r]] = lo + r * 64 + lane;
+    write_tiles(K, starts, tile_starts, tiles);
 }
 
+// `waves` segments per workgroup (1, 4 or 8), of as many waves each as its kManyWaves allow.
 // within[segment][b]: the workgroup's earlier segments' rows of bucket b;  counts[workgroup][b]: all of its.
-__global__ void group_count(const int64_t *labels, i64 P, int K, int seg, int nseg, int *bucket, int *within, int *counts) {
+__global__ void group_count(const int64_t *labels, i64 P, int K, int seg, int nseg, int waves, int *bucket, int *within, int *counts) {
     extern __shared__ int lds[];
-    const int B = K + 1, w = threadIdx.x >> 6, nw = blockDim.x >> 6, s = blockIdx.x * nw + w;
-    int *hist = lds + w * B;
-    for (int b = wave_lane(); b < B; b += 64) hist[b] = 0;
+    const int B = K + 1, w = threadIdx.x >> 6, parts = kManyWaves / waves, s0 = blockIdx.x * waves, s = s0 + w % waves;
+    int *hist = lds + w % waves * B;
+    for (int b = threadIdx.x; b < waves * B; b += blockDim.x) lds[b] = 0;
     __syncthreads();
     const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
 #pragma unroll 4
-    for (i64 i = lo + wave_lane(); i < hi; i += 64) {           // (counts need no order)
+    for (i64 i = lo + w / waves * 64 + wave_lane(); i < hi; i += 64 * parts) {          // (counts need no order)
         const int b = bucket_of(labels, i, K);
         atomicAdd(&hist[b], 1);
         bucket[i] = b;
@@ -222,8 +227,8 @@ __global__ void group_count(const int64_t *labels, i64 P, int K, int seg, int ns
     __syncthreads();
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
         int sum = 0;
-        for (int j = 0; j < nw; ++j) {
-            if (blockIdx.x * nw + j < nseg) within[(i64)(blockIdx.x * nw + j) * B + b] = sum;
+        for (int j = 0; j < waves; ++j) {
+            if (s0 + j < nseg) within[(i64)(s0 + j) * B + b] = sum;
             sum += lds[j * B + b];
         }
         counts[(i64)blockIdx.x * B + b] = sum;
@@ -256,28 +261,28 @@ __global__ void group_columns(int *counts, int nseg, int B, int *sizes) {
     if (wave_lane() == 0) sizes[b] = carry;
 }
 
-// The last workgroup writes the prefix sums and the tiles instead.
-__global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int seg, int nseg, const int *within, const int *counts, const int *sizes,
-                              int *order, int *offsets, int *first, Tiles tiles) {
+// The first `waves` waves of a workgroup have a segment each; the last workgroup writes the prefix sums and the tiles instead.
+__global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int seg, int nseg, int waves, const int *within, const int *counts,
+                              const int *sizes, int *order, int *offsets, int *first, Tiles tiles) {
     extern __shared__ int lds[];
-    const int nw = blockDim.x >> 6;
-    const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * nw + w;
-    int *start = lds + nw * B, *part = start + B;
+    const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * waves + w;
     if (blockIdx.x == gridDim.x - 1) {
-        int *starts = lds, *tile_starts = starts + B + 1;       // (the sums' parts behind them)
-        write_sums(K, (int)P, sizes, offsets, first, tiles.lg, tile_starts + B + 1, [&](int b, int at, int tile) {
-            starts[b] = at;
-            tile_starts[b] = tile;
-        });
+        int *starts = lds, *tile_starts = starts + B + 1;
+        write_sums(K, sizes, offsets, first, tiles.lg, [&](int b, int sum) { starts[b] = sum; }, [&](int b, int sum) { tile_starts[b] = sum; });
         __syncthreads();
         write_tiles(K, starts, tile_starts, tiles);
         return;
     }
+    int *start = lds + waves * B, *part = start + B;
     block_scan(B, part, [&](int b) { return sizes[b]; }, [&](int b, int v) { start[b] = v + counts[(i64)blockIdx.x * B + b]; });
-    int *cursor = lds + w * B;
-    if (s < nseg)
-        for (int b = wave_lane(); b < B; b += 64) cursor[b] = start[b] + within[(i64)s * B + b];
+    const int v = w % waves, parts = kManyWaves / waves;
+    if (blockIdx.x * waves + v < nseg) {
+#pragma unroll 4
+        for (int b = w / waves * 64 + wave_lane(); b < B; b += 64 * parts) lds[v * B + b] = start[b] + within[(i64)(blockIdx.x * waves + v) * B + b];
+    }
     __syncthreads();
+    if (w >= waves) return;
+    int *cursor = lds + w * B;
     const i64 lo = (i64)s * seg < P ? (i64)s * seg : P, hi = lo + seg < P ? lo + seg : P;
     walk(lo, hi, nbits, cursor, [&](i64 i) { return bucket[i]; }, [&](i64 i, int, int at) { order[at] = (int)i; });
 }
@@ -293,8 +298,6 @@ Split split_of(i64 P, int K) {
     s.groups = (s.nseg + s.waves - 1) / s.waves;
     return s;
 }
-
-bool small_form(i64 P, int K) { return P <= kSmall && K + 1 <= kSmallBuckets; }
 
 }  // namespace
 
@@ -319,17 +322,16 @@ extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int3
     int nbits = 1;
     while ((1 << nbits) < B) ++nbits;
     if (small_form(P, K)) {
-        const int waves = P <= 2048 ? 4 : kWaves;
-        const size_t lds = sizeof(int) * ((size_t)(waves + 2) * B + 2 + kSums * waves);
-        group_small<<<1, 64 * waves, lds, st>>>(labels, (int)P, K, nbits, bucket, order, offsets, first, table);
+        const int waves = small_waves(K);
+        group_small<<<1, 64 * kSums, sizeof(int) * ((size_t)(waves + 3) * B + 2), st>>>(labels, (int)P, K, nbits, waves, bucket, order, offsets, first, table);
         return ops_launched("group_rows");
     }
     const Split s = split_of(P, K);
     int *within = (int *)ws, *counts = within + (size_t)s.nseg * B, *sizes = counts + (size_t)s.groups * B;
     // (P = 0 with many components: no segment, but the sums over nothing and the empty offsets are still written)
-    if (s.groups > 0) group_count<<<s.groups, 64 * s.waves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, s.seg, s.nseg, bucket, within, counts);
+    if (s.groups > 0) group_count<<<s.groups, 64 * kManyWaves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, s.seg, s.nseg, s.waves, bucket, within, counts);
     group_columns<<<(B + 3) / 4, 256, 0, st>>>(counts, s.groups, B, sizes);
-    group_scatter<<<s.groups + 1, 64 * s.waves, sizeof(int) * ((size_t)(s.waves + 1) * B + 2 + kSums * s.waves), st>>>(bucket, P, K, nbits, s.seg, s.nseg, within, counts,
-                                                                                                                  sizes, order, offsets, first, table);
+    group_scatter<<<s.groups + 1, 64 * kManyWaves, sizeof(int) * ((size_t)(s.waves + 1) * B + 2 + kManyWaves), st>>>(
+        bucket, P, K, nbits, s.seg, s.nseg, s.waves, within, counts, sizes, order, offsets, first, table);
     return ops_launched("group_rows");
 }

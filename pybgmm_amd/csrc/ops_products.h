@@ -10,7 +10,7 @@
 // 16x16x4 (single) or two 16x16x4 (double) matrix instructions: where an instruction takes fewer elements than a lane has
 // read, its k-th element is not the k-th of the row but the same permutation holds for both operands, which a sum does
 // not see.  The weights are the instruction's row operand and the data rows its columns: a lane then holds four consecutive
-// elements of one output row, and stores them as one vector.
+// elements of one output row (two pairs in double precision), which go to LDS as one vector and from there to memory by rows.
 //
 // LDS layouts (both without bank conflicts on the operand reads, by XOR on the 16-byte granule):
 //   KTile: rows along the contraction, [row][8 granules], granule ^ (row & 7); read 16 bytes per lane.

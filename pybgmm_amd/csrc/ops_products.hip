@@ -5,7 +5,6 @@ namespace {
 
 int size_of(int dtype) { return dtype == BGMM_F64 ? 8 : dtype == BGMM_F32 ? 4 : 2; }
 int acc_size(int dtype) { return dtype == BGMM_F64 ? 8 : 4; }
-bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 Divisor divisor(int d) {
     int lg = 0;
     while ((1ll << lg) < d) ++lg;
@@ -21,8 +20,9 @@ int safe_rows(i64 rows, i64 stride, int size) {
     return n < 0 ? 0 : (int)n;
 }
 
-// Columns of a tile of a product with rows: 128 beside 16 rows; else as many as there are, 64 instead of 128 where that leaves
-// compute units without a workgroup (20011 rows, 33 components, 192 -> 77 single: 27 -> 18 us).
+// Columns of a tile of a product with rows: 128 beside 16 rows; else as many as there are, 64 instead of 128 where that would leave
+// compute units without a workgroup (20011 rows, 33 components, 192 -> 77 single: 23.1 -> 21.5 us; 2000 rows, 4 components,
+// 256 -> 512 bfloat16: 8.0 -> 6.3 us).
 int cols_tile(i64 P, int K, int ndim) {
     if (small_tiles(P, K)) return 128;
     if (ndim <= 64) return ndim <= 16 ? 16 : 64;
@@ -39,8 +39,9 @@ Grid grid_of(i64 useful) {
 }
 
 // Tile of the weights' gradient (bt x bt) and chunk of rows (a level of the grouping): chunks as long as about a thousand
-// workgroups remain, 256 .. 32768 rows -- a chunk leaves a tile of partial sums, which 256 rows of both operands outweigh --,
-// and tiles of 64 where 128 would leave compute units idle even so.
+// workgroups remain, 256 .. 32768 rows -- a chunk leaves a tile of partial sums, which 256 rows of both operands outweigh --
+// (forward and this, 1e6 rows, 4 components of 64 x 64 single: 338 us with chunks of 256, 302 us), and tiles of 64 where 128
+// would leave compute units idle even so (20011 rows, 33 components, 192 x 77: 61.5 -> 53.1 us).
 struct WeightTiles { int bt, level; };
 WeightTiles weight_tiles(i64 P, int idim, int odim) {
     const auto tiles = [&](int t) { return (i64)((idim + t - 1) / t) * ((odim + t - 1) / t); };
@@ -62,10 +63,12 @@ int check(const char *what, int dtype, i64 P, int K, int a, int b) {
 extern "C" int bgmm_rows_product_splits(int32_t dtype, int64_t P, int32_t K, int32_t kdim, int32_t ndim) {
     if (check("rows_product_splits", dtype, P, K, kdim, ndim) != BGMM_OPS_OK || P == 0) return 1;
     const int bn = cols_tile(P, K, ndim);
-    const i64 groups = tiles_at_most(P, K) * ((ndim + bn - 1) / bn);
+    const i64 groups = ((P >> tile_log2(P, K)) + at_most(K, P)) * ((ndim + bn - 1) / bn);
     const int steps = (kdim * size_of(dtype) + kStepBytes - 1) / kStepBytes;
-    // (256 compute units: fill them twice over, but leave a part four steps to do)
-    i64 s = at_most(512 / (groups > 0 ? groups : 1), steps / 4);
+    // Few rows leave compute units idle while a few stream the weights: the contraction in parts, as many workgroups as the compute
+    // units hold of either tile, but a part has four steps to do (bfloat16, one row of 4 experts of 64, 2048 -> 1024: 29.6 -> 8.6
+    // us; of one, 4096 -> 4096: 57 -> 17 us, 33.5 MB of weights).
+    i64 s = at_most((small_tiles(P, K) ? 1024 : 512) / groups, steps / 4);
     return (int)(s < 1 ? 1 : at_most(s, 16));
 }
 
@@ -124,7 +127,7 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
     if (!dw && !db) return BGMM_OPS_OK;
     if (!offsets || !first || (P > 0 && (!in || !d || !order))) return ops_fail(BGMM_OPS_EINVAL, "weight_product: a null pointer");
     if (in_div < 1 || d_div < 1 || in_stride < 0 || d_stride < 0) return ops_fail(BGMM_OPS_EINVAL, "weight_product: divisors %d %d, strides %lld %lld", in_div, d_div, (long long)in_stride, (long long)d_stride);
-    if (ws_bytes < bgmm_weight_product_ws(dtype, P, K, idim, odim) || (ws_bytes > 0 && (!ws || !aligned(ws, 16))))
+    if (ws_bytes < bgmm_weight_product_ws(dtype, P, K, idim, odim) || (ws_bytes > 0 && (!ws || ((uintptr_t)ws & 15))))
         return ops_fail(BGMM_OPS_EINVAL, "weight_product: workspace of %lld bytes", (long long)ws_bytes);
     if (K > 65535) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: K = %d", K);
     const WeightTiles w = weight_tiles(P, idim, odim);

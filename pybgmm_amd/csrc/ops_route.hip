@@ -183,7 +183,8 @@ template <class T, int G, int NG, int E> __global__ __launch_bounds__(256) void 
     }
 }
 
-// Any K and k: one wave per row, which is read again for every chosen component (from the caches).
+// Any K and k: one wave per row, which is read again for every chosen component (from the caches).  (n = 1e6, K = 200, k = 4,
+// double: 1512 us, in registers 359; 1e5 x 64 bfloat16: 73 and 10 us.)
 template <class T> __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     typedef typename Acc<T>::type A;
     const int lane = wave_lane();
@@ -324,6 +325,7 @@ extern "C" int bgmm_route(int32_t dtype, const void *log_weights, int64_t stride
     return by_type(dtype, [&](auto *t) {
         typedef std::remove_pointer_t<decltype(t)> T;
         constexpr int E = 16 / (int)sizeof(T);
+        // 16 bytes a load where rows begin on them, else an element (n = 1e6, K = 200, double: 299 and 411 us; 1e5 x 64 bfloat16: 10.3, 11.4)
         const bool vec = ((uintptr_t)log_weights & 15) == 0 && stride % E == 0 && K % E == 0;
         if (!(vec ? route_in_registers<T, E>(a, st) : route_in_registers<T, 1>(a, st))) route_kernel<T><<<g, 256, 0, st>>>(a);
         return ops_launched("route");

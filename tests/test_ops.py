@@ -293,7 +293,8 @@ def test_route_gradient_against_differences():
 # ------------------------------------------------------------------------------------------ group_rows
 @gpu
 @pytest.mark.parametrize("shape,K", [((0,), 3), ((0,), 2000), ((1,), 1), ((5,), 8000), ((64,), 7), ((1000, 4), 64), ((8192,), 889), ((8192,), 890), ((1024,), 50), ((1025,), 50),
-                                     ((8193,), 3), ((40000,), 200), ((30011, 3), 1779), ((30011,), 1780), ((30011, 3), 3199), ((30011,), 3200), ((100003,), 8000), ((1000000,), 100)])
+                                     ((8193,), 3), ((40000,), 200), ((30011, 3), 1779), ((30011,), 1780), ((30011, 3), 3199), ((30011,), 3200), ((100003,), 8000), ((1000000,), 100),
+                                     ((4096,), 64), ((4097,), 64), ((513, 7), 20), ((4096,), 1479), ((2048,), 1480), ((2049,), 1480), ((2048,), 2299), ((300, 2), 2300), ((6000,), 2)])
 def test_group_rows(shape, K):
     from pybgmm_amd import ops
     g = torch.Generator().manual_seed(K + len(shape))
