@@ -66,10 +66,11 @@ extern "C" int bgmm_rows_product_splits(int32_t dtype, int64_t P, int32_t K, int
     const i64 groups = ((P >> tile_log2(P, K)) + at_most(K, P)) * ((ndim + bn - 1) / bn);
     const int steps = (kdim * size_of(dtype) + kStepBytes - 1) / kStepBytes;
     // Few rows leave compute units idle while a few stream the weights: the contraction in parts, as many workgroups as the compute
-    // units hold of either tile, but a part has four steps to do (bfloat16, one row of 4 experts of 64, 2048 -> 1024: 29.6 -> 8.6
-    // us; of one, 4096 -> 4096: 57 -> 17 us, 33.5 MB of weights).
-    i64 s = at_most((small_tiles(P, K) ? 1024 : 512) / groups, steps / 4);
-    return (int)(s < 1 ? 1 : at_most(s, 16));
+    // units hold of either tile, but a part has four steps to do, and the steps saved outweigh adding the parts up.  (bfloat16,
+    // one row of 4 experts of 64, 2048 -> 1024: 29.6 -> 8.6 us; one row, 4096 -> 4096: 57 -> 17 us, 33.5 MB of weights; 5000
+    // rows, 8 components, 1024 -> 64, twelve steps saved: 12.7 -> 11.8 us; but 20000 rows, 32, 768 -> 64, six: 13.0 -> 16.6 us.)
+    const i64 s = at_most(at_most((small_tiles(P, K) ? 1024 : 512) / groups, steps / 4), 16);
+    return s > 1 && steps - steps / s >= 8 ? (int)s : 1;
 }
 
 extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_stride, int32_t in_div, const void *w, int64_t w_component,

@@ -490,8 +490,17 @@ template <class T> __global__ __launch_bounds__(256) void weight_reduce(WeightAr
     const int chunks = a.bucket_first[e + 1] - a.bucket_first[e];
     if (chunks == 1) return;
     const i64 n_w = (i64)a.idim * a.odim, size = n_w + a.odim;
+    if (chunks == 0 && a.dw) {
+        struct Run { T e[kGran<T>]; } zeros;
+#pragma unroll
+        for (int q = 0; q < kGran<T>; ++q) zeros.e[q] = (T)0.0f;
+        T *dw = (T *)a.dw + (i64)e * n_w;
+        const i64 whole = n_w / kGran<T>;
+        for (i64 g = (i64)blockIdx.x * 256 + threadIdx.x; g < whole; g += (i64)gridDim.x * 256) store_any(dw + g * kGran<T>, zeros);
+        if (blockIdx.x == 0 && threadIdx.x < n_w - whole * kGran<T>) dw[whole * kGran<T> + threadIdx.x] = (T)0.0f;
+    }
     const A *slot = (const A *)a.ws + (((i64)a.offsets[e] * 2) >> (8 + a.level)) * size;
-    for (i64 j = (i64)blockIdx.x * 256 + threadIdx.x; j < size; j += (i64)gridDim.x * 256) {
+    for (i64 j = (chunks == 0 ? n_w : 0) + (i64)blockIdx.x * 256 + threadIdx.x; j < size; j += (i64)gridDim.x * 256) {
         const bool is_w = j < n_w;
         if (is_w ? !a.dw : !a.db) continue;
         A v = 0;
@@ -554,8 +563,9 @@ template <class T> __global__ __launch_bounds__(256) void combine_kernel(Combine
     }
 }
 
-// The same for few rows with many parts: sixteen lanes share the k x splits terms of four elements, so that they are all in
-// flight at once (one row of 4 experts, 2048 -> 1024 bfloat16, product and sum: 16.7 -> 8.8 us).
+// The same for few results of many parts: sixteen lanes share the k x splits terms of four elements, so that they are all in
+// flight at once (product and sum, one row of 4 experts, 2048 -> 1024 bfloat16: 16.7 -> 8.8 us, 600 rows, 4096 -> 128 single: 22.6
+// -> 19.1 us; but 300 rows, 2048 -> 1024 bfloat16: 17.8 -> 18.3 us).
 template <class T> __global__ __launch_bounds__(256) void combine_parts_kernel(CombineArgs a) {
     typedef typename Acc<T>::type A;
     const int quads = (a.dim + 3) >> 2, lane = threadIdx.x & 15;
@@ -582,53 +592,53 @@ template <class T> __global__ __launch_bounds__(256) void combine_parts_kernel(C
 template <class T, int KJ> __global__ __launch_bounds__(256) void combine_gates_kernel(CombineArgs a) {
     typedef typename Acc<T>::type A;
     const int lane = wave_lane();
-    const i64 i = (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= a.rows) return;
-    A dot[KJ], g[KJ];
-    int e[KJ];
-#pragma unroll
-    for (int j = 0; j < KJ; ++j) {
-        dot[j] = 0;
-        e[j] = j < a.k ? a.bucket[i * a.k + j] : a.K;
-        g[j] = e[j] < a.K ? ((const A *)a.gates)[i * a.k + j] : (A)0;
-    }
-    const T *in = (const T *)a.in + i * a.in_stride;
-    for (int c = lane * 4; c < a.dim; c += 256) {
-        const int avail = a.dim - c;
-        typename Acc<T>::v4 v = {0, 0, 0, 0};
-        A x[4];
-        load4(in + c, avail, x);
+    for (i64 i = (i64)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.rows; i += (i64)gridDim.x * 4) {
+        A dot[KJ], g[KJ];
+        int e[KJ];
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
-            if (e[j] >= a.K) continue;
-            A u[4];
-            parts4<A>((const A *)a.ws + (i * a.k + j) * a.dim + c, a.P * a.dim, a.splits, avail, u);
+            dot[j] = 0;
+            e[j] = j < a.k ? a.bucket[i * a.k + j] : a.K;
+            g[j] = e[j] < a.K ? ((const A *)a.gates)[i * a.k + j] : (A)0;
+        }
+        const T *in = (const T *)a.in + i * a.in_stride;
+        for (int c = lane * 4; c < a.dim; c += 256) {
+            const int avail = a.dim - c;
+            typename Acc<T>::v4 v = {0, 0, 0, 0};
+            A x[4];
+            load4(in + c, avail, x);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                dot[j] += x[q] * u[q];
-                v[q] += g[j] * u[q];
+            for (int j = 0; j < KJ; ++j) {
+                if (e[j] >= a.K) continue;
+                A u[4];
+                parts4<A>((const A *)a.ws + (i * a.k + j) * a.dim + c, a.P * a.dim, a.splits, avail, u);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    dot[j] += x[q] * u[q];
+                    v[q] += g[j] * u[q];
+                }
+            }
+            if (a.out) store_run<4>((T *)a.out + i * a.out_stride + c, v, 0, avail);
+        }
+        if (a.bias) {
+            for (int c = lane * 4; c < a.ddim; c += 256) {
+#pragma unroll
+                for (int j = 0; j < KJ; ++j)
+                    if (e[j] < a.K) {
+                        A b[4], d[4];
+                        load4((const T *)a.bias + (i64)e[j] * a.bias_row + c, a.ddim - c, b);
+                        load4((const T *)a.d + ((i * a.k + j) / a.d_div) * a.d_stride + c, a.ddim - c, d);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) dot[j] += b[q] * d[q];
+                    }
             }
         }
-        if (a.out) store_run<4>((T *)a.out + i * a.out_stride + c, v, 0, avail);
-    }
-    if (a.bias) {
-        for (int c = lane * 4; c < a.ddim; c += 256) {
 #pragma unroll
-            for (int j = 0; j < KJ; ++j)
-                if (e[j] < a.K) {
-                    A b[4], d[4];
-                    load4((const T *)a.bias + (i64)e[j] * a.bias_row + c, a.ddim - c, b);
-                    load4((const T *)a.d + ((i * a.k + j) / a.d_div) * a.d_stride + c, a.ddim - c, d);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) dot[j] += b[q] * d[q];
-                }
+        for (int j = 0; j < KJ; ++j) {
+            if (j >= a.k) break;
+            const A v = group_sum<64>(dot[j]);
+            if (lane == 0) ((A *)a.dgates)[i * a.k + j] = v;
         }
-    }
-#pragma unroll
-    for (int j = 0; j < KJ; ++j) {
-        if (j >= a.k) break;
-        const A v = group_sum<64>(dot[j]);
-        if (lane == 0) ((A *)a.dgates)[i * a.k + j] = v;
     }
 }
 
@@ -662,7 +672,7 @@ template <class T> int launch_weight(const WeightArgs &a, int bt, i64 blocks, hi
 template <class T> int launch_combine(const CombineArgs &a, hipStream_t st) {
     if (a.rows == 0) return BGMM_OPS_OK;
     if (a.dgates) {
-        const dim3 g((unsigned)((a.rows + 3) / 4));
+        const dim3 g((unsigned)((a.rows + 3) / 4 < (1 << 22) ? (a.rows + 3) / 4 : 1 << 22));
         if (a.k == 1) combine_gates_kernel<T, 1><<<g, 256, 0, st>>>(a);
         else if (a.k == 2) combine_gates_kernel<T, 2><<<g, 256, 0, st>>>(a);
         else if (a.k <= 4) combine_gates_kernel<T, 4><<<g, 256, 0, st>>>(a);
@@ -670,7 +680,7 @@ template <class T> int launch_combine(const CombineArgs &a, hipStream_t st) {
         else combine_gates_kernel<T, 32><<<g, 256, 0, st>>>(a);
     } else {
         const i64 threads = a.rows * ((a.dim + 3) / 4);
-        if (a.splits > 1) {
+        if (a.splits > 1 && threads < 32768) {
             combine_parts_kernel<T><<<dim3((unsigned)((threads + 15) / 16)), 256, 0, st>>>(a);
         } else {
             const i64 b = (threads + 255) / 256 < 65536 ? (threads + 255) / 256 : 65536;

@@ -183,54 +183,117 @@ template <class T, int G, int NG, int E> __global__ __launch_bounds__(256) void 
     }
 }
 
-// Any K and k: one wave per row, which is read again for every chosen component (from the caches).  (n = 1e6, K = 200, k = 4,
-// double: 1512 us, in registers 359; 1e5 x 64 bfloat16: 73 and 10 us.)
-template <class T> __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+// Longer rows: a workgroup of W waves per row.  HELD: its threads have the row in registers as above, 16 elements each (up to 4096
+// and 16384 components); else it is read again for every chosen component, the next one being the largest behind the last
+// in the order.  A round's W maxima meet in LDS, in one of two places in turn, so that it takes one barrier.  (single precision,
+// 10000 rows of 8000, k = 4: 250 us, one row 8 us, 1000 rows of 100000, k = 2: 294 us; a wave per row took 417, 86 and 2232.)
+template <class T, int W, bool HELD, int E> __global__ __launch_bounds__(64 * W) void route_wide_kernel(RouteArgs a) {
     typedef typename Acc<T>::type A;
-    const int lane = wave_lane();
-    const i64 i = (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= a.n) return;
-    const T *row = (const T *)a.l + i * a.stride;
-    A top = neg_inf<A>(), last = 0, mine = neg_inf<A>();
-    int last_at = -1, mine_at = -1;
-    for (int j = 0; j < a.k; ++j) {
-        A best = neg_inf<A>();
-        int at = 0x7fffffff;
-        for (int c = lane; c < a.K; c += 64) {
-            const A v = (A)row[c];
-            const bool after = j == 0 || v < last || (v == last && c > last_at);
-            if (after && v > best) { best = v; at = c; }
-        }
+    constexpr int NG = 16 / E, N = 64 * W;
+    __shared__ A top_of[2][W], sum_of[W];
+    __shared__ int at_of[2][W];
+    const int lane = wave_lane(), w = threadIdx.x >> 6;
+    int turn = 0;
+    for (i64 i = blockIdx.x; i < a.n; i += gridDim.x) {
+        const T *row = (const T *)a.l + i * a.stride;
+        A v[HELD ? 16 : 1];
+        if constexpr (HELD) {
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const A ov = __shfl_xor(best, o);
-            const int oa = __shfl_xor(at, o);
-            if (ov > best || (ov == best && oa < at)) { best = ov; at = oa; }
+            for (int g = 0; g < NG; ++g) {                      // (K is whole granules)
+                const int c = (g * N + threadIdx.x) * E;
+                load_logs<T, E>(row, c, c < a.K, v + g * E);
+            }
         }
-        if (best == neg_inf<A>()) break;
-        if (j == 0) top = best;
-        if (lane == j) { mine = best; mine_at = at; }
-        last = best;
-        last_at = at;
-    }
-    A total = 0;
-    if (a.renormalise) {
-        total = mine_at >= 0 ? ratio(mine, top) : (A)0;
-    } else if (top > neg_inf<A>()) {
-        for (int c = lane; c < a.K; c += 64) {
-            const A v = (A)row[c];
-            if (v > neg_inf<A>()) total += ratio(v, top);
-        }
-    }
+        A m = neg_inf<A>(), last = 0;
+        int at = -1;
+        const auto find = [&](bool first) {
+            A best = neg_inf<A>();
+            int mine = 0x7fffffff;
+            if constexpr (HELD) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-    if (lane < a.k) {
-        a.labels[i * a.k + lane] = mine_at;
-        ((A *)a.weights)[i * a.k + lane] = mine_at >= 0 ? ratio(mine, top) / total : (A)0;
-    }
-    if (a.stats && lane == 0) {
-        ((A *)a.stats)[2 * i] = top;
-        ((A *)a.stats)[2 * i + 1] = total;
+                for (int q = 0; q < 16; ++q) best = larger(best, v[q]);
+                best = group_reduce<64>(best, [](A x, A y) { return larger(x, y); });
+#pragma unroll
+                for (int q = 15; q >= 0; --q) mine = v[q] == best ? ((q / E) * N + (int)threadIdx.x) * E + q % E : mine;
+            } else {
+#pragma unroll 4
+                for (int c = threadIdx.x; c < a.K; c += N) {
+                    A x;
+                    load_logs<T, 1>(row, c, true, &x);
+                    const bool after = first || x < last || (x == last && c > at);
+                    mine = after && x > best ? c : mine;
+                    best = after && x > best ? x : best;
+                }
+                const A own = best;
+                best = group_reduce<64>(best, [](A x, A y) { return larger(x, y); });
+                mine = own == best ? mine : 0x7fffffff;
+            }
+            mine = group_reduce<64>(mine, [](int x, int y) { return x < y ? x : y; });
+            if (lane == 0) {
+                top_of[turn][w] = best;
+                at_of[turn][w] = mine;
+            }
+            __syncthreads();
+            const A t = top_of[turn][lane % W];
+            m = group_reduce<16>(t, [](A x, A y) { return larger(x, y); });
+            at = group_reduce<16>(t == m ? at_of[turn][lane % W] : 0x7fffffff, [](int x, int y) { return x < y ? x : y; });
+            last = m;
+            turn ^= 1;
+        };
+        find(true);
+        const A top = m;
+        A chosen = neg_inf<A>(), total = 0;
+        int chosen_at = -1;
+        if (top > neg_inf<A>()) {
+            if (!a.renormalise) {
+                if constexpr (HELD) {
+#pragma unroll
+                    for (int b = 0; b < 16; b += 4) {
+                        A y[4];
+                        ratios<4>(v + b, top, y);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) total += y[q];
+                    }
+                } else {
+                    for (int c = threadIdx.x; c < a.K; c += N) {
+                        A x;
+                        load_logs<T, 1>(row, c, true, &x);
+                        total += ratio(x, top);
+                    }
+                }
+                total = group_sum<64>(total);
+                if (lane == 0) sum_of[w] = total;
+                __syncthreads();
+                total = 0;
+#pragma unroll
+                for (int j = 0; j < W; ++j) total += sum_of[j];
+            }
+            for (int r = 0;;) {
+                if (lane == r) {
+                    chosen = m;
+                    chosen_at = at;
+                }
+                if (++r == a.k) break;
+                if constexpr (HELD) {
+                    const int g = at / E, slot = g % N == (int)threadIdx.x ? (g / N) * E + at % E : -1;
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) v[q] = q == slot ? neg_inf<A>() : v[q];
+                }
+                find(false);
+                if (!(m > neg_inf<A>())) break;                 // (no other; the same for every wave)
+            }
+        }
+        const A e = chosen_at >= 0 ? ratio(chosen, top) : (A)0;
+        if (a.renormalise) total = group_sum<64>(e);
+        if (w != 0) continue;
+        if (lane < a.k) {
+            a.labels[i * a.k + lane] = chosen_at;
+            ((A *)a.weights)[i * a.k + lane] = chosen_at >= 0 ? e / total : (A)0;
+        }
+        if (a.stats && lane == 0) {
+            ((A *)a.stats)[2 * i] = top;
+            ((A *)a.stats)[2 * i + 1] = total;
+        }
     }
 }
 
@@ -284,8 +347,8 @@ template <class T> __global__ __launch_bounds__(256) void route_backward_kernel(
     }
 }
 
-// The register form for this K and k, or false.  G: 8 lanes up to 16 elements each, then 16, 32, 64; at least k.
-template <class T, int G, int E> bool route_by_size(const RouteArgs &a, hipStream_t st) {
+// The form for this K and k: 8 lanes up to 16 elements each, then 16, 32, 64 -- at least k --, then workgroups.
+template <class T, int G, int E> void route_by_size(const RouteArgs &a, hipStream_t st) {
     const int need = (a.K + G * E - 1) / (G * E);
     constexpr int kMost = 16 / E;
     const dim3 g((unsigned)((a.n + 256 / G - 1) / (256 / G)));
@@ -293,15 +356,20 @@ template <class T, int G, int E> bool route_by_size(const RouteArgs &a, hipStrea
     else if (need <= kMost / 2) route_rows_kernel<T, G, (kMost + 1) / 2, E><<<g, 256, 0, st>>>(a);
     else if (need <= (kMost * 7 + 7) / 8 && kMost > 4) route_rows_kernel<T, G, (kMost * 7 + 7) / 8, E><<<g, 256, 0, st>>>(a);
     else route_rows_kernel<T, G, kMost, E><<<g, 256, 0, st>>>(a);
-    return true;
 }
-template <class T, int E> bool route_in_registers(const RouteArgs &a, hipStream_t st) {
-    if (a.K <= 8 * 16 && a.k <= 8) return route_by_size<T, 8, E>(a, st);
-    if (a.K <= 16 * 16 && a.k <= 16) return route_by_size<T, 16, E>(a, st);
-    if (a.K <= 32 * 16) return route_by_size<T, 32, E>(a, st);
-    if (a.K <= 64 * 16) return route_by_size<T, 64, E>(a, st);
-    return false;
+template <class T, int E> void route_by_width(const RouteArgs &a, hipStream_t st) {
+    const dim3 g((unsigned)(a.n < (1 << 20) ? a.n : 1 << 20));
+    if (a.K <= 8 * 16 && a.k <= 8) route_by_size<T, 8, E>(a, st);
+    else if (a.K <= 16 * 16 && a.k <= 16) route_by_size<T, 16, E>(a, st);
+    else if (a.K <= 32 * 16) route_by_size<T, 32, E>(a, st);
+    else if (a.K <= 64 * 16) route_by_size<T, 64, E>(a, st);
+    else if (a.K <= 4096) route_wide_kernel<T, 4, true, E><<<g, 256, 0, st>>>(a);
+    else if (a.K <= 16384) route_wide_kernel<T, 16, true, E><<<g, 1024, 0, st>>>(a);
+    else route_wide_kernel<T, 16, false, 1><<<g, 1024, 0, st>>>(a);
 }
+
+// Rows of a launch: a launch's threads are counted in 32 bits.
+constexpr i64 kRowsAtOnce = (i64)1 << 25;
 
 int check(const char *what, int dtype, i64 n, int K, int k, i64 stride) {
     if (dtype < BGMM_F64 || dtype > BGMM_BF16) return ops_fail(BGMM_OPS_EINVAL, "%s: element type %d", what, dtype);
@@ -319,15 +387,18 @@ extern "C" int bgmm_route(int32_t dtype, const void *log_weights, int64_t stride
     const int rc = check("route", dtype, n, K, k, stride);
     if (rc || n == 0) return rc;
     if (!log_weights || !labels || !weights) return ops_fail(BGMM_OPS_EINVAL, "route: a null pointer");
-    RouteArgs a = {log_weights, stride, n, K, k, renormalise != 0, labels, weights, stats, nullptr, nullptr};
-    const dim3 g((unsigned)((n + 3) / 4));
     const hipStream_t st = (hipStream_t)stream;
     return by_type(dtype, [&](auto *t) {
         typedef std::remove_pointer_t<decltype(t)> T;
         constexpr int E = 16 / (int)sizeof(T);
         // 16 bytes a load where rows begin on them, else an element (n = 1e6, K = 200, double: 299 and 411 us; 1e5 x 64 bfloat16: 10.3, 11.4)
         const bool vec = ((uintptr_t)log_weights & 15) == 0 && stride % E == 0 && K % E == 0;
-        if (!(vec ? route_in_registers<T, E>(a, st) : route_in_registers<T, 1>(a, st))) route_kernel<T><<<g, 256, 0, st>>>(a);
+        typedef typename Acc<T>::type A;
+        for (i64 i = 0; i < n; i += kRowsAtOnce) {
+            const RouteArgs a = {(const T *)log_weights + i * stride, stride, n - i < kRowsAtOnce ? n - i : kRowsAtOnce, K, k, renormalise != 0, labels + i * k,
+                                 (A *)weights + i * k, stats ? (A *)stats + 2 * i : nullptr, nullptr, nullptr};
+            vec ? route_by_width<T, E>(a, st) : route_by_width<T, 1>(a, st);
+        }
         return ops_launched("route");
     });
 }
@@ -339,13 +410,18 @@ extern "C" int bgmm_route_backward(int32_t dtype, const void *log_weights, int64
     if (rc || n == 0) return rc;
     if (!labels || !weights || !dweights || !dlog_weights || (!renormalise && (!log_weights || !stats)))
         return ops_fail(BGMM_OPS_EINVAL, "route_backward: a null pointer");
-    RouteArgs a = {log_weights, stride, n, K, k, renormalise != 0, (int64_t *)labels, (void *)weights, (void *)stats, dweights, dlog_weights};
     // rows of a workgroup: about 8192 elements, a multiple of eight (so that stretches of any K start on 16 bytes)
     int rows = 8;
     while (rows < kBackRows && (i64)rows * K < 8192) rows *= 2;
-    const dim3 g((unsigned)((n + rows - 1) / rows));
     return by_type(dtype, [&](auto *t) {
-        route_backward_kernel<std::remove_pointer_t<decltype(t)>><<<g, 256, 0, (hipStream_t)stream>>>(a, rows);
+        typedef std::remove_pointer_t<decltype(t)> T;
+        typedef typename Acc<T>::type A;
+        for (i64 i = 0; i < n; i += kRowsAtOnce) {
+            const i64 m = n - i < kRowsAtOnce ? n - i : kRowsAtOnce;
+            const RouteArgs a = {log_weights ? (const T *)log_weights + i * stride : nullptr, stride, m, K, k, renormalise != 0, (int64_t *)labels + i * k,
+                                 (A *)weights + i * k, stats ? (A *)stats + 2 * i : nullptr, (const A *)dweights + i * k, (T *)dlog_weights + i * K};
+            route_backward_kernel<T><<<dim3((unsigned)((m + rows - 1) / rows)), 256, 0, (hipStream_t)stream>>>(a, rows);
+        }
         return ops_launched("route_backward");
     });
 }

@@ -377,6 +377,7 @@ std::tuple<Tensor, Tensor> verify_drafts(const Tensor &target_in, const Tensor &
     if (target_in.size(0) != B || target_in.size(1) != T + 1 || target_in.size(2) != V)
         refuse(BGMM_OPS_EINVAL, "%s: target is %s, draft %s", what, shape_of(target_in).c_str(), shape_of(draft_in).c_str());
     if (V < 1) refuse(BGMM_OPS_EINVAL, "%s: no labels", what);
+    if (T > (1 << 20)) refuse(BGMM_OPS_EUNSUPPORTED, "%s: %lld drafts (at most 2^20)", what, (long long)T);
     const int type = type_of(what, "target", target_in);
     if (draft_in.scalar_type() != target_in.scalar_type()) refuse(BGMM_OPS_EINVAL, "%s: target is %s, draft %s", what, c10::toString(target_in.scalar_type()), c10::toString(draft_in.scalar_type()));
     const auto wants = [&](const char *name, const Tensor &t, at::ScalarType type, at::IntArrayRef shape) {

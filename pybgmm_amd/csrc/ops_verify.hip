@@ -233,9 +233,8 @@ template <class F> __device__ __forceinline__ int pick(int n, F sum_of, double g
     return last;
 }
 
-constexpr int kDrawWaves = 16;
-template <class T> __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyArgs a, VerifyWs w) {
-    __shared__ double part[kDrawWaves];
+template <class T, int W> __global__ __launch_bounds__(64 * W) void verify_draw_kernel(VerifyArgs a, VerifyWs w) {
+    __shared__ double part[W];
     const i64 b = blockIdx.x;
     const int acc = w.acc[b], len = w.len[b], wave = threadIdx.x >> 6;
     const T *p = (const T *)a.target + b * a.target_b + acc * a.target_t;
@@ -255,9 +254,9 @@ template <class T> __global__ __launch_bounds__(64 * kDrawWaves) void verify_dra
     const int c = pick(w.chunks, [&](int j) { return sums[2 * j + which]; }, goal, &before);
     i64 drawn = -1;
     if (c >= 0) {
-        // sixteen parts of the chunk, one per wave; then 64 labels at a time
+        // a part of the chunk per wave; then 64 labels at a time
         const i64 lo = c * w.chunk, hi = lo + w.chunk < a.V ? lo + w.chunk : a.V;
-        const i64 len1 = ((hi - lo + kDrawWaves - 1) / kDrawWaves + 63) & ~(i64)63;
+        const i64 len1 = ((hi - lo + W - 1) / W + 63) & ~(i64)63;
         const i64 lo1 = lo + wave * len1 < hi ? lo + wave * len1 : hi, hi1 = lo1 + len1 < hi ? lo1 + len1 : hi;
         double r, s;
         sum_span(p, q, lo1, hi1, wave_lane(), 64, &r, &s);
@@ -265,7 +264,7 @@ template <class T> __global__ __launch_bounds__(64 * kDrawWaves) void verify_dra
         if (wave_lane() == 0) part[wave] = r;
         __syncthreads();
         if (wave == 0) {
-            const int k = pick(kDrawWaves, [&](int j) { return part[j]; }, goal, &before);
+            const int k = pick(W, [&](int j) { return part[j]; }, goal, &before);
             if (k >= 0) {
                 const i64 lo2 = lo + k * len1, hi2 = lo2 + len1 < hi ? lo2 + len1 : hi;
                 const int j = pick((int)(hi2 - lo2), [&](int x) { return weight(p, q, lo2 + x); }, goal, &before);
@@ -324,7 +323,9 @@ extern "C" int bgmm_verify_drafts(int32_t dtype, const void *target, int64_t tar
         else if (few_labels(V)) verify_rows_kernel<E, 16><<<g, 256, 0, st>>>(a);
         else {
             verify_sums_kernel<E><<<dim3((unsigned)(B * w.chunks)), 256, 0, st>>>(a, w);
-            verify_draw_kernel<E><<<dim3((unsigned)B), 64 * kDrawWaves, 0, st>>>(a, w);
+            // few sequences: more waves for the latency of each (5000 sequences of 2000 singles: 38 us with 4, 68 with 16)
+            if (B > 512) verify_draw_kernel<E, 4><<<dim3((unsigned)B), 256, 0, st>>>(a, w);
+            else verify_draw_kernel<E, 16><<<dim3((unsigned)B), 1024, 0, st>>>(a, w);
         }
         return ops_launched("verify_drafts");
     });

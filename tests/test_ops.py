@@ -227,7 +227,8 @@ def route_rows(n, K, dt, seed):
 
 @gpu
 @pytest.mark.parametrize("dt", TYPES, ids=str)
-@pytest.mark.parametrize("n,K,k", [(1, 1, 1), (1, 200, 4), (7, 2, 2), (33, 64, 6), (65, 100, 1), (20, 129, 8), (9, 1000, 32), (5, 5000, 3), (300, 17, 17)])
+@pytest.mark.parametrize("n,K,k", [(1, 1, 1), (1, 200, 4), (7, 2, 2), (33, 64, 6), (65, 100, 1), (20, 129, 8), (9, 1000, 32), (5, 5000, 3), (300, 17, 17),
+                                   (3, 1025, 32), (5, 4096, 8), (4, 4097, 3), (2, 16384, 32), (3, 16385, 5), (2, 40001, 2)])
 @pytest.mark.parametrize("renormalise", [True, False])
 def test_route_forward_and_backward(dt, n, K, k, renormalise):
     from pybgmm_amd import ops
@@ -615,7 +616,7 @@ def verify_on_gpu(*args):
 
 @gpu
 @pytest.mark.parametrize("dt", TYPES, ids=str)
-@pytest.mark.parametrize("B,T,V", [(1, 1, 1), (1, 0, 7), (3, 4, 2), (50, 8, 20), (40, 3, 200), (5, 70, 33), (9, 2, 256), (7, 2, 999), (6, 2, 1025), (4, 5, 5003), (2, 3, 20000), (1, 1, 70001), (3, 2, 65536), (3, 2, 65537), (130, 1, 3001)])
+@pytest.mark.parametrize("B,T,V", [(1, 1, 1), (1, 0, 7), (3, 4, 2), (50, 8, 20), (40, 3, 200), (5, 70, 33), (9, 2, 256), (7, 2, 999), (6, 2, 1025), (4, 5, 5003), (2, 3, 20000), (1, 1, 70001), (3, 2, 65536), (3, 2, 65537), (130, 1, 3001), (513, 1, 1100)])
 def test_verify_drafts(dt, B, T, V):
     args = verify_case(B, T, V, dt, B * V + T)
     want = verify_ref(*args)
@@ -1032,3 +1033,38 @@ def test_a_captured_step_is_refused_while_an_eager_graph_of_its_leaves_lives():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@gpu
+def test_route_of_more_rows_than_a_launch_takes():
+    from pybgmm_amd import ops
+    n = (1 << 25) + 5
+    lw = torch.randint(-8, 8, (n, 3), device="cuda", dtype=torch.int8).to(torch.bfloat16).requires_grad_()
+    for renormalise in (True, False):
+        labels, weights = ops.route(lw, 1, renormalise)
+        # (the first of equal ones, exactly: small integers)
+        key = lw.detach() * 4 - torch.arange(3, device="cuda", dtype=torch.bfloat16)
+        assert torch.equal(labels[:, 0], key.argmax(1))
+        grad, = torch.autograd.grad(weights.sum(), lw)
+        if renormalise:
+            assert bool((weights == 1).all()) and not bool(grad.any())
+            continue
+        p = torch.softmax(lw.detach().float(), 1)
+        top = p.gather(1, labels)
+        # (softmax in 32 bits on either side: a few units of 2^-24 each; the gradient is rounded to bfloat16, 2^-8 of at most 1/4)
+        assert float((weights - top).abs().max()) < 2e-6
+        want = top * (torch.nn.functional.one_hot(labels[:, 0], 3) - p)
+        assert float((grad.float() - want).abs().max()) < 2.0 ** -8 / 4 + 2e-6
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=str)
+def test_a_large_batch_draws_as_its_parts_do(dt):
+    """Batches of more than 512 sequences and smaller ones take the sums of a chunk in different parts."""
+    from pybgmm_amd import ops
+    args = [a.cuda() for a in verify_case(600, 2, 9001, dt, 11)]
+    out, acc = ops.verify_drafts(*args[:5], lengths=args[5])
+    for i in range(0, 600, 120):
+        part = [a[i:i + 120] for a in args]
+        o, c = ops.verify_drafts(*part[:5], lengths=part[5])
+        assert torch.equal(o, out[i:i + 120]) and torch.equal(c, acc[i:i + 120])
