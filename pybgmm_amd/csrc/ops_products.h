@@ -134,6 +134,13 @@ template <class T> __device__ __forceinline__ Granule load_part(const T *p, int 
     return g;
 }
 
+// elements `avail` and behind zeroed
+template <class T> __device__ __forceinline__ void keep(Granule &g, int avail) {
+    T *e = Elems<T>::of(g);
+#pragma unroll
+    for (int j = 0; j < kGran<T>; ++j) e[j] = j < avail ? e[j] : (T)0.0f;
+}
+
 // n / d for n < 2^31 by one multiplication: (n m) >> s with m = floor(2^s / d) + 1, s = 31 + ceil(log2 d).  The error
 // n (m - 2^s / d) / 2^s is below n / 2^s <= 1 / d, so the quotient is exact.
 struct Divisor {
@@ -166,7 +173,8 @@ struct RowsArgs {
     void *ws;                       // or, instead of out: accumulator type, [splits][P][n], neither gated nor rounded
     i64 P;
     int kdim, ndim, splits, n_tiles;
-    int w_safe;                     // rows k of any component in front of this have 16 bytes from any of their elements on
+    int in_safe;                    // rows of `in` in front of this have 16 bytes from any of their elements on
+    int w_safe;                     // rows of a component's matrix likewise (along w_row)
 };
 
 struct WeightArgs {

@@ -106,7 +106,8 @@ extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_strid
     a.ndim = ndim;
     a.splits = splits;
     a.n_tiles = (ndim + bn - 1) / bn;
-    a.w_safe = safe_rows(kdim, w_row, size_of(dtype));
+    a.in_safe = safe_rows(P / in_div, in_stride, size_of(dtype));
+    a.w_safe = safe_rows(kcontig ? ndim : kdim, w_row, size_of(dtype));
     const Grid g = grid_of((i64)a.tile_blocks * 8 * a.n_tiles * splits);
     if (g.blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "rows_product: %lld tiles", (long long)g.blocks);
     a.run = g.run;
