@@ -214,8 +214,8 @@ struct CombineArgs {
     int d_div, ddim;
 };
 
-// One product with rows; bm x bn: its tiles (16 x 128, 128 x 16, 64 or 128).  `kcontig`: the weights' contiguous axis is the
-// contraction.  The weights' gradient by tiles of bt x bt (16, 64 or 128).
+// One product with rows; bm x bn: its tiles (16 x 128, 128 x 16, 32, 64 or 128).  `kcontig`: the weights' contiguous axis is the
+// contraction.  The weights' gradient by tiles of bi x bo (16, 64 or 128 each, but not 16 x 64 nor 64 x 16).
 template <class T> int launch_rows(const RowsArgs &a, bool kcontig, int bm, int bn, i64 blocks, hipStream_t st);
-template <class T> int launch_weight(const WeightArgs &a, int bt, i64 blocks, hipStream_t st);
+template <class T> int launch_weight(const WeightArgs &a, int bi, int bo, i64 blocks, hipStream_t st);
 template <class T> int launch_combine(const CombineArgs &a, hipStream_t st);

@@ -20,12 +20,13 @@ int safe_rows(i64 rows, i64 stride, int size) {
     return n < 0 ? 0 : (int)n;
 }
 
-// Columns of a tile of a product with rows: 128 beside 16 rows; else as many as there are, 64 instead of 128 where that would leave
+// Columns of a tile of a product with rows: 128 beside 16 rows; else the next of 16, 32, 64, 128 (1e6 rows, 32 -> 32 double: 147 us
+// with 64, 113 with 32), 64 instead of 128 where that would leave
 // compute units without a workgroup (20011 rows, 33 components, 192 -> 77 single: 23.1 -> 21.5 us; 2000 rows, 4 components,
 // 256 -> 512 bfloat16: 8.0 -> 6.3 us).
 int cols_tile(i64 P, int K, int ndim) {
     if (small_tiles(P, K)) return 128;
-    if (ndim <= 64) return ndim <= 16 ? 16 : 64;
+    if (ndim <= 64) return ndim <= 16 ? 16 : ndim <= 32 ? 32 : 64;
     return tiles_at_most(P, K) * ((ndim + 127) / 128) < 512 ? 64 : 128;
 }
 
@@ -38,15 +39,19 @@ Grid grid_of(i64 useful) {
     return g;
 }
 
-// Tile of the weights' gradient (bt x bt) and chunk of rows (a level of the grouping): chunks as long as about a thousand
+// Tile of the weights' gradient (bi x bo) and chunk of rows (a level of the grouping): chunks as long as about a thousand
 // workgroups remain, 256 .. 32768 rows -- a chunk leaves a tile of partial sums, which 256 rows of both operands outweigh --
 // (forward and this, 1e6 rows, 4 components of 64 x 64 single: 338 us with chunks of 256, 302 us), and tiles of 64 where 128
 // would leave compute units idle even so (20011 rows, 33 components, 192 x 77: 61.5 -> 53.1 us).
-struct WeightTiles { int bt, level; };
+// An axis of up to 16 or 64 gets a tile of that width (forward and this, 114804 rows, 905 x 16 double: 773 us with 128 x 128, 379;
+// 1e6 rows, 128 x 10 single: 457 and 277 us).
+struct WeightTiles { int bi, bo, level; };
 WeightTiles weight_tiles(i64 P, int idim, int odim) {
-    const auto tiles = [&](int t) { return (i64)((idim + t - 1) / t) * ((odim + t - 1) / t); };
-    WeightTiles w = {idim <= 16 && odim <= 16 ? 16 : (idim <= 64 && odim <= 64) || (P / 256 + 1) * tiles(128) < 512 ? 64 : 128, 0};
-    while (w.level < BGMM_OPS_LEVELS - 1 && P / (256 << (w.level + 1)) * tiles(w.bt) >= 1024) ++w.level;
+    const auto tiles = [&](int ti, int to) { return (i64)((idim + ti - 1) / ti) * ((odim + to - 1) / to); };
+    const auto width = [](int d) { return d <= 16 ? 16 : d <= 64 ? 64 : 128; };
+    WeightTiles w = {width(idim), width(odim), 0};
+    if (w.bi + w.bo == 80 || (w.bi + w.bo > 80 && (P / 256 + 1) * tiles(w.bi, w.bo) < 512)) w.bi = w.bo = 64;
+    while (w.level < BGMM_OPS_LEVELS - 1 && P / (256 << (w.level + 1)) * tiles(w.bi, w.bo) >= 1024) ++w.level;
     return w;
 }
 
@@ -133,7 +138,6 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
         return ops_fail(BGMM_OPS_EINVAL, "weight_product: workspace of %lld bytes", (long long)ws_bytes);
     if (K > 65535) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: K = %d", K);
     const WeightTiles w = weight_tiles(P, idim, odim);
-    const int t = w.bt;
     WeightArgs a;
     a.level = w.level;
     a.bucket_first = first + (size_t)a.level * (K + 2);
@@ -152,14 +156,14 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
     a.ws = ws;
     a.idim = idim;
     a.odim = odim;
-    a.i_tiles = dw ? (idim + t - 1) / t : 1;        // (the bias's sums come with the first)
-    a.o_tiles = (odim + t - 1) / t;
+    a.i_tiles = dw ? (idim + w.bi - 1) / w.bi : 1;        // (the bias's sums come with the first)
+    a.o_tiles = (odim + w.bo - 1) / w.bo;
     a.in_safe = safe_rows(P / in_div, in_stride, size_of(dtype));
     a.d_safe = safe_rows(P / d_div, d_stride, size_of(dtype));
     const Grid g = grid_of(P == 0 ? 0 : (P / ((i64)256 << a.level) + at_most(K, P)) * a.i_tiles * a.o_tiles);
     if (g.blocks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: %lld tiles", (long long)g.blocks);
     a.run = g.run;
-    return by_type(dtype, [&](auto *t_) { return launch_weight<std::remove_pointer_t<decltype(t_)>>(a, t, g.blocks, (hipStream_t)stream); });
+    return by_type(dtype, [&](auto *t_) { return launch_weight<std::remove_pointer_t<decltype(t_)>>(a, w.bi, w.bo, g.blocks, (hipStream_t)stream); });
 }
 
 extern "C" int bgmm_combine(int32_t dtype, const void *ws, int32_t splits, int64_t rows, int32_t k, int32_t K, const int32_t *bucket,

@@ -1,5 +1,5 @@
 #include "ops_products_kernels.h"
 
 template int launch_rows<float>(const RowsArgs &, bool, int, int, i64, hipStream_t);
-template int launch_weight<float>(const WeightArgs &, int, i64, hipStream_t);
+template int launch_weight<float>(const WeightArgs &, int, int, i64, hipStream_t);
 template int launch_combine<float>(const CombineArgs &, hipStream_t);

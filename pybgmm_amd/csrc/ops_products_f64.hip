@@ -1,5 +1,5 @@
 #include "ops_products_kernels.h"
 
 template int launch_rows<double>(const RowsArgs &, bool, int, int, i64, hipStream_t);
-template int launch_weight<double>(const WeightArgs &, int, i64, hipStream_t);
+template int launch_weight<double>(const WeightArgs &, int, int, i64, hipStream_t);
 template int launch_combine<double>(const CombineArgs &, hipStream_t);

@@ -349,15 +349,17 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
 // 64 experts of 1024 x 2048 from 16384 rows, bfloat16: 190 us, 360 TFLOP/s.  A component's 256 rows are four steps, so the time is
 // what four steps do not hide: finding the chunk, its rows and the first loads (a quarter, alone), and the results' stores (4 MB
 // for 1.5 MB of operands; a third).
-template <class T, int BT, int WO, int WI>
-__global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kernel(WeightArgs a) {
+template <class T, int BI, int BO, int WO, int WI>
+__global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kernel(WeightArgs a) {
     typedef typename Acc<T>::type A;
     typedef typename Acc<T>::v4 A4;
-    constexpr int FA = BT / WO / 16, FB = BT / WI / 16;
-    constexpr int NP = (BT + 31) / 32;                          // granules of either operand a thread moves per step
-    constexpr bool kAll = BT >= 32;                             // every thread moves some
-    typedef MTile<T, BT> Tile;
-    __shared__ __attribute__((aligned(128))) char lds[2 * BT * kStepBytes];
+    constexpr int FA = BO / WO / 16, FB = BI / WI / 16;
+    constexpr int NI = (BI + 31) / 32, NO = (BO + 31) / 32;     // granules of either operand a thread moves per step
+    constexpr bool kAllI = BI >= 32, kAllO = BO >= 32, kSame = BI == BO;        // every thread moves some; the same rows of both
+    typedef MTile<T, BI> ITile;
+    typedef MTile<T, BO> OTile;
+    __shared__ __attribute__((aligned(128))) char lds[(BI + BO) * kStepBytes];
+    char *const lds_o = lds + BI * kStepBytes;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wo = wave % WO, wi = wave / WO;
     const int out_tiles = a.i_tiles * a.o_tiles;
@@ -368,62 +370,80 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
     const int rows_per = 256 << a.level;
     const int row0 = at_b.offset + c * rows_per, left = at_b.next_offset - row0, n_rows = left < rows_per ? left : rows_per;
     const int *list = a.order + row0;
-    const int i0 = (tile % a.i_tiles) * BT, o0 = (tile / a.i_tiles) * BT;
+    const int i0 = (tile % a.i_tiles) * BI, o0 = (tile / a.i_tiles) * BO;
     const A *gates = (const A *)a.gates;
     const bool want_db = a.db && i0 == 0;
 
-    // a thread moves the same granule column of rows r, r + kRows, ...; both operands' rows go by the same index, read one
-    // step before its rows are asked for.  As in rows_kernel, places outside read a neighbour; rows behind the last are
+    // a thread moves the same granule column of rows r, r + kRows, ...; an operand's rows go by indices read one step
+    // before its rows are asked for (the same ones for both in square tiles).  As in rows_kernel, places outside read a neighbour; rows behind the last are
     // zero in both operands, and a granule across the end of a row is read with care where no row is behind it.
-    constexpr int kRows = 256 / Tile::kPerRow < kStep<T> ? 256 / Tile::kPerRow : kStep<T>;
-    const int my_row = tid / Tile::kPerRow, my_col = (tid % Tile::kPerRow) * kGran<T>;
-    const int i_col = i0 + my_col < a.idim ? i0 + my_col : i0, o_col = o0 + my_col < a.odim ? o0 + my_col : o0;
+    constexpr int kRowsI = 256 / ITile::kPerRow < kStep<T> ? 256 / ITile::kPerRow : kStep<T>;
+    constexpr int kRowsO = 256 / OTile::kPerRow < kStep<T> ? 256 / OTile::kPerRow : kStep<T>;
+    const int i_row = tid / ITile::kPerRow, i_at = tid % ITile::kPerRow, o_row = tid / OTile::kPerRow, o_at = tid % OTile::kPerRow;
+    const int i_col = i0 + i_at * kGran<T> < a.idim ? i0 + i_at * kGran<T> : i0, o_col = o0 + o_at * kGran<T> < a.odim ? o0 + o_at * kGran<T> : o0;
     const T *in = (const T *)a.in + i_col, *dd = (const T *)a.d + o_col;
     const int i_safe = a.idim - i_col < kGran<T> ? a.in_safe : 0x7fffffff, o_safe = a.odim - o_col < kGran<T> ? a.d_safe : 0x7fffffff;
-    struct Held { Granule i[NP], o[NP]; A gate[NP]; } held;
-    int at[NP];
+    struct Held { Granule i[NI], o[NO]; A gate[NO]; } held;
+    int at_i[NI], at_o[NO];
     const auto look = [&](int s) {
+        if (!kSame) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            const int r = s * kStep<T> + my_row + p * kRows;
-            at[p] = list[r < n_rows ? r : n_rows - 1];
+            for (int p = 0; p < NI; ++p) {
+                const int r = s * kStep<T> + i_row + p * kRowsI;
+                at_i[p] = list[r < n_rows ? r : n_rows - 1];
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < NO; ++p) {
+            const int r = s * kStep<T> + o_row + p * kRowsO;
+            at_o[p] = list[r < n_rows ? r : n_rows - 1];
         }
     };
-    const bool edge = a.idim - i0 < BT && a.idim % kGran<T> != 0, o_edge = a.odim - o0 < BT && a.odim % kGran<T> != 0;
-    const auto fetch = [&](Held &h, int s) {        // (at: the indices of step s; leaves those of s + 1)
-        if (kAll || tid < BT * 8) {
-            int ri[NP], ro[NP];
+    const bool edge = (a.idim - i0 < BI && a.idim % kGran<T> != 0) || (a.odim - o0 < BO && a.odim % kGran<T> != 0);
+    const auto fetch = [&](Held &h, int s) {        // (at_i, at_o: the indices of step s; leaves those of s + 1)
+        int ri[NI], ro[NO];
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                ri[p] = divide(at[p], a.in_div);
-                ro[p] = divide(at[p], a.d_div);
+        for (int p = 0; p < NI; ++p) ri[p] = divide(kSame ? at_o[p] : at_i[p], a.in_div);
+#pragma unroll
+        for (int p = 0; p < NO; ++p) ro[p] = divide(at_o[p], a.d_div);
+        bool careful = false;
+        if (edge) {
+#pragma unroll
+            for (int p = 0; p < NI; ++p) careful = careful || ri[p] >= i_safe;
+#pragma unroll
+            for (int p = 0; p < NO; ++p) careful = careful || ro[p] >= o_safe;
+            careful = __any(careful);
+        }
+        if (!careful) {
+            if (kAllI || tid < BI * 8) {
+#pragma unroll
+                for (int p = 0; p < NI; ++p) h.i[p] = load_whole(in + (i64)ri[p] * a.in_stride);
             }
-            bool careful = false;
-            if (edge || o_edge) {
+            if (kAllO || tid < BO * 8) {
 #pragma unroll
-                for (int p = 0; p < NP; ++p) careful = careful || ri[p] >= i_safe || ro[p] >= o_safe;
-                careful = __any(careful);
+                for (int p = 0; p < NO; ++p) h.o[p] = load_whole(dd + (i64)ro[p] * a.d_stride);
             }
-            if (!careful) {
+        } else {
+            if (kAllI || tid < BI * 8) {
 #pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    h.i[p] = load_whole(in + (i64)ri[p] * a.in_stride);
-                    h.o[p] = load_whole(dd + (i64)ro[p] * a.d_stride);
-                }
-            } else {
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    const T *pi = in + (i64)ri[p] * a.in_stride, *po = dd + (i64)ro[p] * a.d_stride;
+                for (int p = 0; p < NI; ++p) {
+                    const T *pi = in + (i64)ri[p] * a.in_stride;
                     if (ri[p] < i_safe) h.i[p] = load_whole(pi);
                     else h.i[p] = load_part(pi, a.idim - i_col);
+                }
+            }
+            if (kAllO || tid < BO * 8) {
+#pragma unroll
+                for (int p = 0; p < NO; ++p) {
+                    const T *po = dd + (i64)ro[p] * a.d_stride;
                     if (ro[p] < o_safe) h.o[p] = load_whole(po);
                     else h.o[p] = load_part(po, a.odim - o_col);
                 }
             }
-            if (gates) {
+        }
+        if (gates && (kAllO || tid < BO * 8)) {
 #pragma unroll
-                for (int p = 0; p < NP; ++p) h.gate[p] = gates[at[p]];
-            }
+            for (int p = 0; p < NO; ++p) h.gate[p] = gates[at_o[p]];
         }
         look(s + 1);
     };
@@ -432,32 +452,38 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
     for (int j = 0; j < kGran<T>; ++j) dsum[j] = 0;
     const int n_steps = (n_rows + kStep<T> - 1) / kStep<T>;     // (at least one: a chunk has rows)
     const auto put = [&](Held &h, int s) {
-        if (!kAll && tid >= BT * 8) return;
         if (s == n_steps - 1) {                                 // rows behind the last
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
-                if (s * kStep<T> + my_row + p * kRows >= n_rows) {
-                    h.i[p].raw = h.o[p].raw = (v4i){0, 0, 0, 0};
+            for (int p = 0; p < NI; ++p)
+                if (s * kStep<T> + i_row + p * kRowsI >= n_rows) h.i[p].raw = (v4i){0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < NO; ++p)
+                if (s * kStep<T> + o_row + p * kRowsO >= n_rows) {
+                    h.o[p].raw = (v4i){0, 0, 0, 0};
                     h.gate[p] = 0;
                 }
         }
+        if (kAllO || tid < BO * 8) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            if (gates) {
+            for (int p = 0; p < NO; ++p) {
                 T *el = Elems<T>::of(h.o[p]);
+                if (gates) {
 #pragma unroll
-                for (int j = 0; j < kGran<T>; ++j) {
-                    const A v = (A)el[j] * h.gate[p];
-                    if (want_db) dsum[j] += v;
-                    el[j] = (T)v;
+                    for (int j = 0; j < kGran<T>; ++j) {
+                        const A v = (A)el[j] * h.gate[p];
+                        if (want_db) dsum[j] += v;
+                        el[j] = (T)v;
+                    }
+                } else if (want_db) {
+#pragma unroll
+                    for (int j = 0; j < kGran<T>; ++j) dsum[j] += (A)el[j];
                 }
-            } else if (want_db) {
-                T *el = Elems<T>::of(h.o[p]);
-#pragma unroll
-                for (int j = 0; j < kGran<T>; ++j) dsum[j] += (A)el[j];
+                *(v4i *)(lds_o + OTile::at(o_row + p * kRowsO, o_at)) = h.o[p].raw;
             }
-            *(v4i *)(lds + Tile::at(my_row + p * kRows, tid % Tile::kPerRow)) = h.i[p].raw;
-            *(v4i *)(lds + BT * kStepBytes + Tile::at(my_row + p * kRows, tid % Tile::kPerRow)) = h.o[p].raw;
+        }
+        if (kAllI || tid < BI * 8) {
+#pragma unroll
+            for (int p = 0; p < NI; ++p) *(v4i *)(lds + ITile::at(i_row + p * kRowsI, i_at)) = h.i[p].raw;
         }
     };
 
@@ -472,9 +498,9 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
         for (int ks = 0; ks < 2; ++ks) {
             Granule fa[FA], fb[FB];
 #pragma unroll
-            for (int i = 0; i < FA; ++i) fa[i] = Tile::template read<true>(lds + BT * kStepBytes, (wo * FA + i) * 16, ks);
+            for (int i = 0; i < FA; ++i) fa[i] = OTile::template read<true>(lds_o, (wo * FA + i) * 16, ks);
 #pragma unroll
-            for (int j = 0; j < FB; ++j) fb[j] = Tile::template read<false>(lds, (wi * FB + j) * 16, ks);
+            for (int j = 0; j < FB; ++j) fb[j] = ITile::template read<false>(lds, (wi * FB + j) * 16, ks);
 #pragma unroll
             for (int part = 0; part < kParts<T>; ++part)
 #pragma unroll
@@ -499,29 +525,29 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BT * BT>)) void weight_kerne
     A *slot = nullptr;
     if (chunks > 1) slot = (A *)a.ws + ((((i64)at_b.offset * 2) >> (8 + a.level)) + c) * ((i64)a.idim * a.odim + a.odim);
     if (a.dw) {
-        constexpr int kBytes = 2 * BT * kStepBytes;
-        const int n_i = a.idim - i0 < BT ? a.idim - i0 : BT, w_o = WO * WI < 4 && wave >= WO * WI ? 0 : wo, w_i = WO * WI < 4 && wave >= WO * WI ? BT : wi;
+        constexpr int kBytes = (BI + BO) * kStepBytes;
+        const int n_i = a.idim - i0 < BI ? a.idim - i0 : BI, w_o = WO * WI < 4 && wave >= WO * WI ? 0 : wo, w_i = WO * WI < 4 && wave >= WO * WI ? BI : wi;
         const auto part = [&](int, int i, int j) { return acc[i][j]; };         // (waves without a part of the tile: none of its rows)
         if (slot) {
             A *to = slot + (i64)i0 * a.odim + o0;
-            store_tile<T, A, kBytes, BT, BT, FA, FB>(lds, w_o, w_i, n_i, a.odim - o0, part, [&](int m) { return to + (i64)m * a.odim; });
+            store_tile<T, A, kBytes, BI, BO, FA, FB>(lds, w_o, w_i, n_i, a.odim - o0, part, [&](int m) { return to + (i64)m * a.odim; });
         } else {
             T *to = (T *)a.dw + ((i64)e * a.idim + i0) * a.odim + o0;
-            store_tile<T, T, kBytes, BT, BT, FA, FB>(lds, w_o, w_i, n_i, a.odim - o0, part, [&](int m) { return to + (i64)m * a.odim; });
+            store_tile<T, T, kBytes, BI, BO, FA, FB>(lds, w_o, w_i, n_i, a.odim - o0, part, [&](int m) { return to + (i64)m * a.odim; });
         }
     }
     if (!want_db) return;
     // column sums: a thread has those of its granule's columns over its own rows; the threads of a column add up in order
-    A *sums = (A *)lds;                       // [kRows][BT]
+    A *sums = (A *)lds;                       // [kRowsO][BO]
     __syncthreads();
-    if (kAll || tid < BT * 8) {
+    if (kAllO || tid < BO * 8) {
 #pragma unroll
-        for (int j = 0; j < kGran<T>; ++j) sums[my_row * BT + my_col + j] = dsum[j];
+        for (int j = 0; j < kGran<T>; ++j) sums[o_row * BO + o_at * kGran<T> + j] = dsum[j];
     }
     __syncthreads();
-    for (int n = tid; n < BT && o0 + n < a.odim; n += 256) {
+    for (int n = tid; n < BO && o0 + n < a.odim; n += 256) {
         A v = 0;
-        for (int r = 0; r < kRows; ++r) v += sums[r * BT + n];
+        for (int r = 0; r < kRowsO; ++r) v += sums[r * BO + n];
         if (slot) slot[(i64)a.idim * a.odim + o0 + n] = v;
         else ((T *)a.db)[(i64)e * a.odim + o0 + n] = (T)v;
     }
@@ -691,6 +717,7 @@ template <class T, bool KCONTIG> static void rows_by_tile(const RowsArgs &a, int
     const dim3 g((unsigned)blocks);
     if (bm == 16) rows_kernel<T, KCONTIG, 16, 128, 4, 1><<<g, 256, 0, st>>>(a);
     else if (bn == 16) rows_kernel<T, KCONTIG, 128, 16, 1, 4><<<g, 256, 0, st>>>(a);
+    else if (bn == 32) rows_kernel<T, KCONTIG, 128, 32, 1, 4><<<g, 256, 0, st>>>(a);
     else if (bn == 64) rows_kernel<T, KCONTIG, 128, 64, 2, 2><<<g, 256, 0, st>>>(a);
     else rows_kernel<T, KCONTIG, 128, 128, 2, 2><<<g, 256, 0, st>>>(a);
 }
@@ -700,12 +727,16 @@ template <class T> int launch_rows(const RowsArgs &a, bool kcontig, int bm, int 
     return ops_launched("rows_product");
 }
 
-template <class T> int launch_weight(const WeightArgs &a, int bt, i64 blocks, hipStream_t st) {
+template <class T> int launch_weight(const WeightArgs &a, int bi, int bo, i64 blocks, hipStream_t st) {
     const dim3 g((unsigned)blocks);
     if (blocks > 0) {
-        if (bt == 16) weight_kernel<T, 16, 1, 1><<<g, 256, 0, st>>>(a);
-        else if (bt == 64) weight_kernel<T, 64, 2, 2><<<g, 256, 0, st>>>(a);
-        else weight_kernel<T, 128, 2, 2><<<g, 256, 0, st>>>(a);
+        if (bi == 16 && bo == 16) weight_kernel<T, 16, 16, 1, 1><<<g, 256, 0, st>>>(a);
+        else if (bi == 16) weight_kernel<T, 16, 128, 4, 1><<<g, 256, 0, st>>>(a);
+        else if (bo == 16) weight_kernel<T, 128, 16, 1, 4><<<g, 256, 0, st>>>(a);
+        else if (bi == 64 && bo == 64) weight_kernel<T, 64, 64, 2, 2><<<g, 256, 0, st>>>(a);
+        else if (bi == 64) weight_kernel<T, 64, 128, 2, 2><<<g, 256, 0, st>>>(a);
+        else if (bo == 64) weight_kernel<T, 128, 64, 2, 2><<<g, 256, 0, st>>>(a);
+        else weight_kernel<T, 128, 128, 2, 2><<<g, 256, 0, st>>>(a);
     }
     // (most components have one chunk and nothing to add up: about 4096 workgroups in all)
     const i64 size = (i64)a.idim * a.odim + a.odim, most = 4096 / a.K > 4 ? 4096 / a.K : 4;

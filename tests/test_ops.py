@@ -404,6 +404,8 @@ CASES = [
     (257, 2, 4, 130, 66), (1000, 1, 7, 16, 16), (999, 3, 6, 33, 5), (700, 1, 2, 128, 300), (2050, 1, 20, 192, 77), (5000, 2, 9, 72, 136),
     (4000, 1, 1, 20, 16), (64, 8, 16, 513, 129), (300, 1, 2, 65, 1), (300, 1, 2, 1, 65), (2000, 1, 3, 129, 3),
     (3000, 1, 5, 8, 16), (2500, 2, 4, 16, 31), (900, 1, 60, 2, 2), (1500, 1, 3, 32, 9), (1, 1, 1, 16, 16),
+    (1100, 1, 4, 17, 32), (1300, 2, 5, 32, 17), (800, 1, 3, 29, 23), (600, 1, 2, 300, 24), (900, 2, 4, 31, 1),
+    (70000, 1, 30, 150, 12), (70000, 1, 30, 12, 150), (40000, 2, 9, 140, 40), (70000, 1, 30, 40, 140), (5000, 1, 4, 16, 60), (5000, 1, 4, 60, 16),
 ]
 
 
