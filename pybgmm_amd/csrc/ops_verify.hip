@@ -11,10 +11,10 @@
 // fewer bits are exact there, so that a draw depends on the order of the sum in the last bits of the total only.
 //
 // Bound by reading one row of the target (and of the draft) per sequence, and for a few sequences by the latency of the chain
-// label -> its probabilities -> the row.  Up to 1024 labels a wave has a sequence and its row in registers, one launch.  Beyond,
+// label -> its probabilities -> the row.  Up to 2048 labels a wave has a sequence and its row in registers, one launch.  Beyond,
 // a workgroup sums a chunk of a row (16-byte loads, however the row is aligned), so that one sequence already fills many
 // compute units, and a second launch finds the chunk that holds the draw and reads only that again.  20000 sequences of 200 doubles:
-// 16.5 us, 3.5 TB/s; 256 of 131072 bfloat16: 33 us, 3.7 TB/s; one of 50000 singles: 9 us, the chain of loads twice.
+// 16.2 us, 3.5 TB/s; 256 of 131072 bfloat16: 33 us, 3.7 TB/s; one of 50000 singles: 9 us, the chain of loads twice.
 #include "ops_common.h"
 
 namespace {
@@ -78,76 +78,116 @@ __device__ __forceinline__ void write_labels(const VerifyArgs &a, i64 b, int acc
     if (lane == 0) a.accepted[b] = acc;
 }
 
-// ---- few labels: a wave per sequence, NV x 64 >= V
-template <class T, int NV> __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
+// 16 bytes of a row at any alignment its elements have
+template <class T> constexpr int kPack = 16 / (int)sizeof(T);
+template <class T, int E = kPack<T>> __device__ __forceinline__ void load_pack(const T *p, T *v) {
+    if constexpr (E == 1) {
+        *v = *p;
+    } else {
+        struct Pack { T e[E]; };
+        const Pack k = load_any<Pack>(p);
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = k.e[j];
+    }
+}
+
+// The row's packs of this lane, NG x 64 of them in all (V >= E).  One that reaches over the row's end is read where it ends with the
+// row, so that no load has a branch around it ...
+template <class T, int NG, int E> __device__ __forceinline__ void load_row(const T *p, int V, T *v) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const int c = (g * 64 + wave_lane()) * E;
+        load_pack<T, E>(p + (c + E <= V ? c : V - E), v + g * E);
+    }
+}
+// ... and shifted to its place here, zeros behind it (apart, so that a second row is asked for before the first one is waited for).
+template <class T, int NG, int E> __device__ __forceinline__ void end_row(int V, T *v) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        if ((g + 1) * 64 * E <= V) continue;
+        const int behind = (g * 64 + wave_lane()) * E + E - V;
+        if constexpr (E == 1) {
+            if (behind > 0) v[g] = (T)0.0f;
+        } else {
+            struct Pack { T e[E]; } k;
+#pragma unroll
+            for (int j = 0; j < E; ++j) k.e[j] = v[g * E + j];
+            unsigned __int128 bits = __builtin_bit_cast(unsigned __int128, k);
+            if (behind > 0) bits = behind < E ? bits >> (behind * 8 * (int)sizeof(T)) : 0;
+            k = __builtin_bit_cast(Pack, bits);
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[g * E + j] = k.e[j];
+        }
+    }
+}
+
+// ---- few labels: a wave per sequence has its row in registers, NG packs a lane.  The sums run over a lane's pack, then over the lanes.
+template <class T, int NG, int E> __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     const i64 b = (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (b >= a.B) return;
-    const int lane = wave_lane();
+    const int lane = wave_lane(), V = (int)a.V;
     const double u = a.u_draw[b];
     int len;
     i64 z0;
     const int acc = accepted_drafts<T>(a, b, &len, &z0);
-    const T *p = (const T *)a.target + b * a.target_b + acc * a.target_t;
-    const T *q = acc < len ? (const T *)a.draft + b * a.draft_b + acc * a.draft_t : nullptr;
-    double w[NV], res[NV], total = 0;
-    if (q) {
+    const bool has_q = acc < len;
+    T p[NG * E], q[NG * E];
+    load_row<T, NG, E>((const T *)a.target + b * a.target_b + acc * a.target_t, V, p);
+    if (has_q) load_row<T, NG, E>((const T *)a.draft + b * a.draft_b + acc * a.draft_t, V, q);
+    end_row<T, NG, E>(V, p);
+    if (has_q) end_row<T, NG, E>(V, q);
+    double res[NG * E], total = 0;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = j * 64 + lane;
-            w[j] = c < a.V ? (double)p[c] : 0.0;
-            res[j] = c < a.V ? (double)q[c] : 0.0;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) w[j] = j * 64 + lane < a.V ? (double)p[j * 64 + lane] : 0.0;
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        w[j] = clean(w[j]);
-        const double r = q ? w[j] - clean(res[j]) : w[j];
+    for (int j = 0; j < NG * E; ++j) {
+        const double r = has_q ? clean(p[j]) - clean(q[j]) : clean(p[j]);
         res[j] = r > 0 ? r : 0.0;
         total += res[j];
     }
     total = group_sum<64>(total);
-    const bool use_p = !(total > 0);
-    if (use_p && q) {
+    if (has_q && !(total > 0)) {
         total = 0;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) total += w[j];
+        for (int j = 0; j < NG * E; ++j) {
+            res[j] = clean(p[j]);
+            total += res[j];
+        }
         total = group_sum<64>(total);
     }
     const double goal = u * total;
     double before = 0;
-    i64 drawn = -1;
+    int drawn = -1;
     bool found = false;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        if (found || j * 64 >= a.V) continue;
-        const double x = use_p ? w[j] : res[j];
+    for (int g = 0; g < NG; ++g) {
+        if (found || g * 64 * E >= V) continue;
+        double x = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) x += res[g * E + j];
         const double s = wave_scan_sum(x);
         const unsigned long long pos = __ballot(x > 0), hit = __ballot(x > 0 && before + s > goal);
-        if (hit) {
-            drawn = j * 64 + __ffsll(hit) - 1;
-            found = true;
-        } else {
-            if (pos) drawn = j * 64 + 63 - __clzll(pos);        // (rounding: the last one with any weight)
-            before += lane_read(s, 63);
+        if (hit | pos) {
+            // in the lane that has it: the first of its pack beyond the goal (else, by rounding, the last one with any weight)
+            double at = before + (s - x);
+            int mine = -1;
+            bool over = false;
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                at += res[g * E + j];
+                if (!over && res[g * E + j] > 0) {
+                    mine = j;
+                    over = at > goal;
+                }
+            }
+            const int l = hit ? __ffsll(hit) - 1 : 63 - __clzll(pos);
+            drawn = (g * 64 + l) * E + __builtin_amdgcn_readlane(mine, l);
+            found = hit != 0;
         }
+        before += lane_read(s, 63);
     }
     write_labels(a, b, acc, drawn, z0);
 }
 
 // ---- many labels: chunks of a row
-template <class T> constexpr int kPack = 16 / (int)sizeof(T);
-
-// 16 bytes of a row at any alignment its elements have
-template <class T> __device__ __forceinline__ void load_pack(const T *p, T *v) {
-    struct Pack { T e[kPack<T>]; };
-    const Pack k = load_any<Pack>(p);
-#pragma unroll
-    for (int j = 0; j < kPack<T>; ++j) v[j] = k.e[j];
-}
-
 // Sums of max(0, p - q) (p where q is null) and of p over [lo, hi) by `n` threads, this one the `me`-th.
 template <class T> __device__ __forceinline__ void sum_span(const T *p, const T *q, i64 lo, i64 hi, int me, int n, double *res, double *all) {
     constexpr int E = kPack<T>;
@@ -282,8 +322,18 @@ i64 chunk_of(i64 B, i64 V) {
     while (chunk < 32768 && B * ((V + chunk - 1) / chunk) > 4096) chunk *= 2;
     return chunk;
 }
-// A wave has the row in registers (20000 sequences of 200 doubles: 18 us, by chunks 170; of 1000 singles: 59 and 207; one: 6.6 and 7.1).
-bool few_labels(i64 V) { return V <= 1024; }
+// A wave has the row in registers, by packs of 16 bytes beyond 256 labels (20000 sequences of 200 bfloat16: 21.5 us by packs, 18.3
+// one by one; of 1000 singles: 30 by packs, 59 one by one, 207 by chunks; 5000 of 2000 singles: 23, 38 by chunks; one: 6.6 and 8.5).
+bool few_labels(i64 V) { return V <= 2048; }
+template <class T> void verify_few(const VerifyArgs &a, hipStream_t st) {
+    constexpr int E = kPack<T>;
+    const dim3 g((unsigned)((a.B + 3) / 4));
+    if (a.V <= 64) verify_rows_kernel<T, 1, 1><<<g, 256, 0, st>>>(a);
+    else if (a.V <= 256) verify_rows_kernel<T, 4, 1><<<g, 256, 0, st>>>(a);
+    else if (a.V <= 512) verify_rows_kernel<T, 8 / E, E><<<g, 256, 0, st>>>(a);
+    else if (a.V <= 1024) verify_rows_kernel<T, 16 / E, E><<<g, 256, 0, st>>>(a);
+    else verify_rows_kernel<T, 32 / E, E><<<g, 256, 0, st>>>(a);
+}
 
 }  // namespace
 
@@ -318,11 +368,9 @@ extern "C" int bgmm_verify_drafts(int32_t dtype, const void *target, int64_t tar
     }
     return by_type(dtype, [&](auto *t) {
         typedef std::remove_pointer_t<decltype(t)> E;
-        const dim3 g((unsigned)((B + 3) / 4));
-        if (V <= 64) verify_rows_kernel<E, 1><<<g, 256, 0, st>>>(a);
-        else if (V <= 256) verify_rows_kernel<E, 4><<<g, 256, 0, st>>>(a);
-        else if (few_labels(V)) verify_rows_kernel<E, 16><<<g, 256, 0, st>>>(a);
-        else {
+        if (few_labels(V)) {
+            verify_few<E>(a, st);
+        } else {
             verify_sums_kernel<E><<<dim3((unsigned)(B * w.chunks)), 256, 0, st>>>(a, w);
             // few sequences: more waves for the latency of each (5000 sequences of 2000 singles: 38 us with 4, 68 with 16)
             if (B > 512) verify_draw_kernel<E, 4><<<dim3((unsigned)B), 256, 0, st>>>(a, w);

@@ -618,7 +618,7 @@ def verify_on_gpu(*args):
 
 @gpu
 @pytest.mark.parametrize("dt", TYPES, ids=str)
-@pytest.mark.parametrize("B,T,V", [(1, 1, 1), (1, 0, 7), (3, 4, 2), (50, 8, 20), (40, 3, 200), (5, 70, 33), (9, 2, 256), (7, 2, 999), (6, 2, 1025), (4, 5, 5003), (2, 3, 20000), (1, 1, 70001), (3, 2, 65536), (3, 2, 65537), (130, 1, 3001), (513, 1, 1100)])
+@pytest.mark.parametrize("B,T,V", [(1, 1, 1), (1, 0, 7), (3, 4, 2), (50, 8, 20), (40, 3, 200), (5, 70, 33), (9, 2, 256), (7, 2, 999), (6, 2, 1025), (4, 5, 5003), (2, 3, 20000), (1, 1, 70001), (3, 2, 65536), (3, 2, 65537), (130, 1, 3001), (513, 1, 1100), (9, 3, 129), (9, 3, 257), (9, 2, 511), (9, 2, 513), (5, 2, 2048), (5, 2, 2049)])
 def test_verify_drafts(dt, B, T, V):
     args = verify_case(B, T, V, dt, B * V + T)
     want = verify_ref(*args)
