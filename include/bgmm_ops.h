@@ -71,13 +71,18 @@ BGMM_OPS_API int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, in
  *   dtype        of in, W, bias, out; products of half precision types accumulate in 32 bits
  *   W            element (k, n) of component e at e * w_component + k * w_row + n (kcontig 0) or + n * w_row + k (kcontig 1)
  *   bias         [K][ndim] with row stride bias_row, or NULL;  gates  accumulator type [P], or NULL
+ *   dots         [P][bgmm_rows_product_dots(...)] in the accumulator type, or NULL: parts of dot_in[p / dot_div] . u_p (ungated, without
+ *                bias), which bgmm_gate_gradient adds up; out and ws may then both be NULL
+ * Operands' rows are read by 16 bytes: up to 15 bytes behind a row's end, where another row follows, whose values do not matter.
  * bgmm_rows_product_splits: how many parts serve a product well (1: write `out`).
  */
 BGMM_OPS_API int bgmm_rows_product_splits(int32_t dtype, int64_t P, int32_t K, int32_t kdim, int32_t ndim);
 BGMM_OPS_API int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_stride, int32_t in_div, const void *w, int64_t w_component,
                                    int64_t w_row, int32_t kcontig, const void *bias, int64_t bias_row, const void *gates, void *out,
-                                   int64_t out_stride, void *ws, int32_t splits, int64_t P, int32_t K, int32_t kdim, int32_t ndim,
-                                   const int32_t *order, const int32_t *tiles, void *stream);
+                                   int64_t out_stride, void *ws, int32_t splits, const void *dot_in, int64_t dot_stride, int32_t dot_div,
+                                   void *dots, int64_t P, int32_t K, int32_t kdim, int32_t ndim, const int32_t *order, const int32_t *tiles,
+                                   void *stream);
+BGMM_OPS_API int bgmm_rows_product_dots(int32_t dtype, int64_t P, int32_t K, int32_t kdim, int32_t ndim, int32_t splits);
 
 /*
  * The weights' gradient: dW_e = sum over the rows p of component e of g_p in[p / in_div] (x) d[p / d_div], db_e = sum of
@@ -98,6 +103,14 @@ BGMM_OPS_API int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_s
 BGMM_OPS_API int bgmm_combine(int32_t dtype, const void *ws, int32_t splits, int64_t rows, int32_t k, int32_t K, const int32_t *bucket,
                               const void *gates, void *out, int64_t out_stride, int32_t dim, void *dgates, const void *in, int64_t in_stride,
                               const void *bias, int64_t bias_row, const void *d, int64_t d_stride, int32_t d_div, int32_t ddim, void *stream);
+
+/*
+ * The gates' gradient dgates[p] = sum of dots[p] + bias_e . d[p / d_div] (bias NULL: without it; rows of no component: zero), dots what
+ * the product of d with the transposed weights left (dot_in: the rows that the forward pass multiplied).
+ */
+BGMM_OPS_API int bgmm_gate_gradient(int32_t dtype, const void *dots, int32_t n_dots, int64_t P, int32_t K, const int32_t *bucket, const void *bias,
+                                    int64_t bias_row, const void *d, int64_t d_stride, int32_t d_div, int32_t ddim, void *dgates,
+                                    void *stream);
 
 /*
  * The k most probable components of every row of log weights [n][K] (row stride `stride`): ordered by (log weight descending,

@@ -2,7 +2,8 @@
 //
 //   rows      out[p] = in[src(p)] W_e (+ b_e) for the rows p of component e           forward, and the rows' gradient
 //   weight    dW_e = sum over the rows of e of g_p in[src(p)] (x) d[dst(p)], db_e      the weights' gradient
-//   combine   sums over a row's k components and over split contractions, the gates' gradient
+//   combine   sums over a row's k components and over split contractions
+//   gates     dg_p = in[src(p)] . (W_e d[p]) + b_e . d[p]: the first part falls off the rows' gradient, whose tiles hold W_e d[p]
 //
 // Tiles.  A workgroup of four waves owns a tile of one component's rows (found in the grouping's prefix sums) times a tile of
 // the other axis and walks the contraction in steps of 128 bytes per row: 64 half, 32 single or 16 double precision elements,
@@ -171,6 +172,11 @@ struct RowsArgs {
     void *out;                      // element type, row p at p * out_stride
     i64 out_stride;
     void *ws;                       // or, instead of out: accumulator type, [splits][P][n], neither gated nor rounded
+    const void *dot_in;             // with dots: row p / dot_div, ndim elements
+    i64 dot_stride;
+    Divisor dot_div;
+    void *dots;                     // accumulator type, [P][n_dots]: the parts of dot_in . u_p, ungated; or null
+    int n_dots;
     i64 P;
     int kdim, ndim, splits, n_tiles;
     int in_safe;                    // rows of `in` in front of this have 16 bytes from any of their elements on
@@ -214,8 +220,23 @@ struct CombineArgs {
     int d_div, ddim;
 };
 
+struct GatesArgs {
+    const int *bucket;              // [P]
+    int K, n_dots;
+    i64 P;
+    const void *dots;               // accumulator type, [P][n_dots]
+    const void *bias;               // [K], row stride bias_row, or null
+    i64 bias_row;
+    const void *d;                  // with bias: row p / d_div, ddim elements
+    i64 d_stride;
+    Divisor d_div;
+    int ddim;
+    void *dgates;                   // accumulator type, [P]
+};
+
 // One product with rows; bm x bn: its tiles (16 x 128, 128 x 16, 32, 64 or 128).  `kcontig`: the weights' contiguous axis is the
 // contraction.  The weights' gradient by tiles of bi x bo (16, 64 or 128 each, but not 16 x 64 nor 64 x 16).
 template <class T> int launch_rows(const RowsArgs &a, bool kcontig, int bm, int bn, i64 blocks, hipStream_t st);
 template <class T> int launch_weight(const WeightArgs &a, int bi, int bo, i64 blocks, hipStream_t st);
 template <class T> int launch_combine(const CombineArgs &a, hipStream_t st);
+template <class T> int launch_gates(const GatesArgs &a, hipStream_t st);

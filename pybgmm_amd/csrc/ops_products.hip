@@ -78,14 +78,22 @@ extern "C" int bgmm_rows_product_splits(int32_t dtype, int64_t P, int32_t K, int
     return s > 1 && steps - steps / s >= 8 ? (int)s : 1;
 }
 
+extern "C" int bgmm_rows_product_dots(int32_t dtype, int64_t P, int32_t K, int32_t kdim, int32_t ndim, int32_t splits) {
+    if (check("rows_product_dots", dtype, P, K, kdim, ndim) != BGMM_OPS_OK || splits < 1) return 0;
+    const int bn = cols_tile(P, K, ndim);
+    return splits * ((ndim + bn - 1) / bn) * (small_tiles(P, K) ? 4 : bn >= 64 ? 2 : 1);       // (waves side by side along a tile's columns)
+}
+
 extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_stride, int32_t in_div, const void *w, int64_t w_component,
                                  int64_t w_row, int32_t kcontig, const void *bias, int64_t bias_row, const void *gates, void *out,
-                                 int64_t out_stride, void *ws, int32_t splits, int64_t P, int32_t K, int32_t kdim, int32_t ndim,
-                                 const int32_t *order, const int32_t *tiles, void *stream) {
+                                 int64_t out_stride, void *ws, int32_t splits, const void *dot_in, int64_t dot_stride, int32_t dot_div, void *dots,
+                                 int64_t P, int32_t K, int32_t kdim, int32_t ndim, const int32_t *order, const int32_t *tiles, void *stream) {
     const int rc = check("rows_product", dtype, P, K, kdim, ndim);
     if (rc) return rc;
     if (P == 0) return BGMM_OPS_OK;
-    if (!in || !w || !order || !tiles || !out == !ws) return ops_fail(BGMM_OPS_EINVAL, "rows_product: a null pointer (and exactly one of out, ws)");
+    if (!in || !w || !order || !tiles || (out && ws) || (!out && !ws && !dots) || (dots && !dot_in))
+        return ops_fail(BGMM_OPS_EINVAL, "rows_product: a null pointer (one of out and ws, or neither with dots)");
+    if (dots && (dot_stride < 0 || dot_div < 1)) return ops_fail(BGMM_OPS_EINVAL, "rows_product: stride %lld, divisor %d of the rows of dots", (long long)dot_stride, dot_div);
     if (in_div < 1 || splits < 1 || (out && splits != 1) || in_stride < 0 || out_stride < 0 || w_component < 0 || w_row < 0)
         return ops_fail(BGMM_OPS_EINVAL, "rows_product: in_div %d, splits %d, strides %lld %lld", in_div, splits, (long long)in_stride, (long long)out_stride);
     const int bm = small_tiles(P, K) ? 16 : 128, bn = cols_tile(P, K, ndim);
@@ -106,6 +114,11 @@ extern "C" int bgmm_rows_product(int32_t dtype, const void *in, int64_t in_strid
     a.out = out;
     a.out_stride = out_stride;
     a.ws = ws;
+    a.dot_in = dot_in;
+    a.dot_stride = dot_stride;
+    a.dot_div = divisor(dots ? dot_div : 1);
+    a.dots = dots;
+    a.n_dots = bgmm_rows_product_dots(dtype, P, K, kdim, ndim, splits);
     a.P = P;
     a.kdim = kdim;
     a.ndim = ndim;
@@ -197,4 +210,15 @@ extern "C" int bgmm_combine(int32_t dtype, const void *ws, int32_t splits, int64
     a.d_div = d_div < 1 ? 1 : d_div;
     a.ddim = ddim;
     return by_type(dtype, [&](auto *t) { return launch_combine<std::remove_pointer_t<decltype(t)>>(a, (hipStream_t)stream); });
+}
+
+extern "C" int bgmm_gate_gradient(int32_t dtype, const void *dots, int32_t n_dots, int64_t P, int32_t K, const int32_t *bucket, const void *bias,
+                                  int64_t bias_row, const void *d, int64_t d_stride, int32_t d_div, int32_t ddim, void *dgates, void *stream) {
+    const int rc = check("gate_gradient", dtype, P, K, n_dots, 1);
+    if (rc) return rc;
+    if (P == 0) return BGMM_OPS_OK;
+    if (!dots || !bucket || !dgates || (bias && (!d || d_div < 1 || ddim < 1 || d_stride < 0 || bias_row < 0)))
+        return ops_fail(BGMM_OPS_EINVAL, "gate_gradient: a null pointer, or a bias with a size or stride that is none");
+    const GatesArgs a = {bucket, K, n_dots, P, dots, bias, bias_row, d, d_stride, divisor(bias ? d_div : 1), ddim, dgates};
+    return by_type(dtype, [&](auto *t) { return launch_gates<std::remove_pointer_t<decltype(t)>>(a, (hipStream_t)stream); });
 }

@@ -3,3 +3,4 @@
 template int launch_rows<f16_t>(const RowsArgs &, bool, int, int, i64, hipStream_t);
 template int launch_weight<f16_t>(const WeightArgs &, int, int, i64, hipStream_t);
 template int launch_combine<f16_t>(const CombineArgs &, hipStream_t);
+template int launch_gates<f16_t>(const GatesArgs &, hipStream_t);

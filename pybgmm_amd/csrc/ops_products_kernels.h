@@ -18,6 +18,20 @@ template <int N, class T, class V> __device__ __forceinline__ void store_run(T *
     }
 }
 
+// N elements of a row as accumulators, at any alignment; behind the row's end zeros.
+template <int N, class S, class A> __device__ __forceinline__ void load_few(const S *p, int avail, A (&v)[N]) {
+    if (avail >= N) {
+        struct Few { S e[N]; };
+        const Few f = load_any<Few>(p);
+#pragma unroll
+        for (int x = 0; x < N; ++x) v[x] = (A)f.e[x];
+    } else {
+#pragma unroll
+        for (int x = 0; x < N; ++x) v[x] = x < avail ? (A)p[x] : (A)0;
+    }
+}
+template <class S, class A> __device__ __forceinline__ void load4(const S *p, int avail, A (&v)[4]) { load_few<4>(p, avail, v); }
+
 // Waves per SIMD.  The loads of the next step fly in registers while the LDS buffer is in use, one buffer and two barriers a
 // step instead of two and one: that a third workgroup fits a compute unit covers more latency (and the other two's
 // beginnings and ends) than a second buffer or a second step in flight (N = 1e6, D = 64 double: 316 -> 295 us; 64 experts of
@@ -134,7 +148,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     const int t = blk * kBlock + local % kBlock, rest = local / kBlock, nt = rest % a.n_tiles, split = rest / a.n_tiles;
     const int4 tile = a.tiles[t];
     const int e = tile.x, n_rows = tile.z;
-    if (e < 0 || (e == a.K && a.ws)) return;
+    if (e < 0 || (e == a.K && !a.out)) return;
     const int *list = a.order + tile.y;
     const int n0 = nt * BN;
 
@@ -333,11 +347,37 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
         for (int x = 0; x < 4; ++x) v[x] += bias_of[(wn * FA + i) * 16 + result_col<T>(lane >> 4, x)];
         return v;
     };
+    if (a.dots) {
+        // the gates' gradient wants in . u: each wave's columns of a row, added up by gates_kernel
+#pragma unroll
+        for (int j = 0; j < FB; ++j) {
+            const int m = (wm * FB + j) * 16 + (lane & 15);
+            A s = 0;
+            if (m < n_rows) {
+                const T *x = (const T *)a.dot_in + (i64)divide(row_of[m], a.dot_div) * a.dot_stride + n0;
+#pragma unroll
+                for (int i = 0; i < FA; ++i) {
+                    constexpr int kRun = sizeof(T) == 8 ? 2 : 4;        // consecutive columns among a lane's four results
+#pragma unroll
+                    for (int h = 0; h < 4; h += kRun) {
+                        const int col = (wn * FA + i) * 16 + result_col<T>(lane >> 4, h), avail = a.ndim - n0 - col;
+                        A v[kRun];
+                        load_few<kRun>(x + col, avail, v);
+#pragma unroll
+                        for (int y = 0; y < kRun; ++y) s += y < avail ? acc[i][j][h + y] * v[y] : (A)0;
+                    }
+                }
+            }
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            if (m < n_rows && lane < 16) ((A *)a.dots)[(i64)row_of[m] * a.n_dots + (split * a.n_tiles + nt) * WN + wn] = s;
+        }
+    }
     if (a.ws) {
         A *ws = (A *)a.ws + (i64)split * a.P * a.ndim + n0;
         store_tile<T, A, kBytes, BM, BN, FA, FB>(lds, wn, wm, n_rows, a.ndim - n0, [&](int, int i, int j) { return biased(i, j); },
                                                  [&](int m) { return ws + (i64)row_of[m] * a.ndim; });
-    } else {
+    } else if (a.out) {
         T *out = (T *)a.out + n0;
         store_tile<T, T, kBytes, BM, BN, FA, FB>(lds, wn, wm, n_rows, a.ndim - n0, [&](int m, int i, int j) { return biased(i, j) * gate_of[m]; },
                                                  [&](int m) { return out + (i64)row_of[m] * a.out_stride; });
@@ -588,19 +628,6 @@ template <class T> __global__ __launch_bounds__(256) void weight_reduce(WeightAr
     }
 }
 
-// Four elements of a row as accumulators, at any alignment; behind the row's end zeros.
-template <class S, class A> __device__ __forceinline__ void load4(const S *p, int avail, A (&v)[4]) {
-    if (avail >= 4) {
-        struct Four { S e[4]; };
-        const Four f = load_any<Four>(p);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = (A)f.e[x];
-    } else {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = x < avail ? (A)p[x] : (A)0;
-    }
-}
-
 // u_p, the sum of its parts
 template <class A> __device__ __forceinline__ void parts4(const A *src, i64 part, int splits, int avail, A (&u)[4]) {
     load4(src, avail, u);
@@ -713,6 +740,32 @@ template <class T, int KJ> __global__ __launch_bounds__(256) void combine_gates_
     }
 }
 
+// The gates' gradient where a row has one product: the parts of in . u_p that the product left, and b_e . d: sixteen lanes per row.
+template <class T> __global__ __launch_bounds__(256) void gates_kernel(GatesArgs a) {
+    typedef typename Acc<T>::type A;
+    const int lane = threadIdx.x & 15;
+    for (i64 p0 = (i64)blockIdx.x * 16; p0 < a.P; p0 += (i64)gridDim.x * 16) {
+        const i64 p = p0 + (threadIdx.x >> 4);
+        const int e = p < a.P ? a.bucket[p] : a.K;
+        A s = 0;
+        if (e < a.K) {
+            for (int c = lane; c < a.n_dots; c += 16) s += ((const A *)a.dots)[p * a.n_dots + c];
+            if (a.bias) {
+                const T *b = (const T *)a.bias + (i64)e * a.bias_row, *d = (const T *)a.d + divide((int)p, a.d_div) * a.d_stride;
+                for (int c = lane * 4; c < a.ddim; c += 64) {
+                    A x[4], y[4];
+                    load4(b + c, a.ddim - c, x);
+                    load4(d + c, a.ddim - c, y);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) s += x[q] * y[q];
+                }
+            }
+        }
+        s = group_sum<16>(s);
+        if (p < a.P && lane == 0) ((A *)a.dgates)[p] = s;
+    }
+}
+
 template <class T, bool KCONTIG> static void rows_by_tile(const RowsArgs &a, int bm, int bn, i64 blocks, hipStream_t st) {
     const dim3 g((unsigned)blocks);
     if (bm == 16) rows_kernel<T, KCONTIG, 16, 128, 4, 1><<<g, 256, 0, st>>>(a);
@@ -764,4 +817,10 @@ template <class T> int launch_combine(const CombineArgs &a, hipStream_t st) {
         }
     }
     return ops_launched("combine");
+}
+
+template <class T> int launch_gates(const GatesArgs &a, hipStream_t st) {
+    const i64 b = (a.P + 15) / 16 < 65536 ? (a.P + 15) / 16 : 65536;
+    gates_kernel<T><<<dim3((unsigned)b), 256, 0, st>>>(a);
+    return ops_launched("gate_gradient");
 }

@@ -25,11 +25,13 @@ SIGNATURES = {
     "bgmm_group_rows_tiles": (_i64, [_i64, _i32]),
     "bgmm_group_rows": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "bgmm_rows_product_splits": (_i32, [_i32, _i64, _i32, _i32, _i32]),
-    "bgmm_rows_product": (_i32, [_i32, _vp, _i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _i32,
-                                 _vp, _vp, _vp]),
+    "bgmm_rows_product_dots": (_i32, [_i32, _i64, _i32, _i32, _i32, _i32]),
+    "bgmm_rows_product": (_i32, [_i32, _vp, _i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i64, _i32, _vp,
+                                 _i64, _i32, _i32, _i32, _vp, _vp, _vp]),
     "bgmm_weight_product_ws": (_i64, [_i32, _i64, _i32, _i32, _i32]),
     "bgmm_weight_product": (_i32, [_i32, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "bgmm_combine": (_i32, [_i32, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp]),
+    "bgmm_gate_gradient": (_i32, [_i32, _vp, _i32, _i64, _i32, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp]),
     "bgmm_route": (_i32, [_i32, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "bgmm_route_backward": (_i32, [_i32, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "bgmm_verify_drafts": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i64, _vp, _vp, _vp, _i64, _vp]),

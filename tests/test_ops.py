@@ -160,14 +160,20 @@ def test_c_entry_points_refuse_before_they_launch():
         (-1, L.bgmm_verify_drafts(1, p, 4, 4, None, 4, 4, p, p, p, None, 1, 1, 4, p, p, None, 0, None)),
         (-1, L.bgmm_verify_drafts(1, p, 4, 4, p, 4, 4, p, p, p, None, 1, 1, 0, p, p, None, 0, None)),
         (-1, L.bgmm_verify_drafts(1, p, 4, 4, p, 4, 4, p, p, p, None, 1, 1, 5000, p, p, p, 8, None)),                 # workspace
-        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, p, 1, 8, 2, 4, 4, p, p, None)),     # out and ws
-        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 2, 8, 2, 4, 4, p, p, None)),  # splits without ws
-        (-1, L.bgmm_rows_product(1, p, 4, 0, p, 4, 4, 0, None, 0, None, p, 4, None, 1, 8, 2, 4, 4, p, p, None)),
-        (-1, L.bgmm_rows_product(4, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 1, 8, 2, 4, 4, p, p, None)),
+        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, p, 1, None, 0, 1, None, 8, 2, 4, 4, p, p, None)),     # out and ws
+        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 2, None, 0, 1, None, 8, 2, 4, 4, p, p, None)),  # splits without ws
+        (-1, L.bgmm_rows_product(1, p, 4, 0, p, 4, 4, 0, None, 0, None, p, 4, None, 1, None, 0, 1, None, 8, 2, 4, 4, p, p, None)),
+        (-1, L.bgmm_rows_product(4, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 1, None, 0, 1, None, 8, 2, 4, 4, p, p, None)),
         (-1, L.bgmm_weight_product(1, p, 4, 1, p, 4, 1, None, p, None, None, 0, 1 << 20, 2, 4, 4, p, p, p, None)),   # workspace
         (-1, L.bgmm_weight_product(1, None, 4, 1, p, 4, 1, None, p, None, None, 0, 8, 2, 4, 4, p, p, p, None)),
+        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, None, 4, None, 1, None, 0, 1, None, 8, 2, 4, 4, p, p, None)),   # no result
+        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, None, 4, None, 1, None, 4, 1, p, 8, 2, 4, 4, p, p, None)),      # dots without rows
+        (-1, L.bgmm_rows_product(1, p, 4, 1, p, 4, 4, 0, None, 0, None, None, 4, None, 1, p, 4, 0, p, 8, 2, 4, 4, p, p, None)),
         (-1, L.bgmm_combine(1, p, 1, 4, 33, 2, p, None, p, 4, 4, None, None, 0, None, 0, None, 0, 1, 1, None)),
         (-1, L.bgmm_combine(1, p, 1, 4, 1, 2, p, None, p, 4, 4, p, p, 4, None, 0, None, 0, 1, 1, None)),             # dgates without gates
+        (-1, L.bgmm_gate_gradient(1, p, 0, 4, 2, p, None, 0, None, 0, 1, 1, p, None)),
+        (-1, L.bgmm_gate_gradient(1, p, 2, 4, 2, p, p, 4, None, 0, 1, 4, p, None)),                                   # a bias without d
+        (-1, L.bgmm_gate_gradient(5, p, 2, 4, 2, p, None, 0, None, 0, 1, 1, p, None)),
     ]
     for i, (want, got) in enumerate(calls):
         assert got == want, (i, got)
