@@ -204,6 +204,7 @@ struct CombineArgs {
     const int *bucket;              // [rows * k]
     int K, k, splits;
     i64 rows, P;
+    i64 first;                      // (of a launch's rows)
     const void *ws;                 // [splits][P][dim]
     const void *gates;              // [rows * k] or null
     void *out;                      // [rows], stride out_stride

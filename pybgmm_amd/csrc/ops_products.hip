@@ -195,6 +195,7 @@ extern "C" int bgmm_combine(int32_t dtype, const void *ws, int32_t splits, int64
     a.splits = splits;
     a.rows = rows;
     a.P = rows * k;
+    a.first = 0;
     a.ws = ws;
     a.gates = gates;
     a.out = out;

@@ -690,53 +690,53 @@ template <class T> __global__ __launch_bounds__(256) void combine_parts_kernel(C
 template <class T, int KJ> __global__ __launch_bounds__(256) void combine_gates_kernel(CombineArgs a) {
     typedef typename Acc<T>::type A;
     const int lane = wave_lane();
-    for (i64 i = (i64)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.rows; i += (i64)gridDim.x * 4) {
-        A dot[KJ], g[KJ];
-        int e[KJ];
+    const i64 i = a.first + (i64)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= a.rows) return;
+    A dot[KJ], g[KJ];
+    int e[KJ];
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) {
+        dot[j] = 0;
+        e[j] = j < a.k ? a.bucket[i * a.k + j] : a.K;
+        g[j] = e[j] < a.K ? ((const A *)a.gates)[i * a.k + j] : (A)0;
+    }
+    const T *in = (const T *)a.in + i * a.in_stride;
+    for (int c = lane * 4; c < a.dim; c += 256) {
+        const int avail = a.dim - c;
+        typename Acc<T>::v4 v = {0, 0, 0, 0};
+        A x[4];
+        load4(in + c, avail, x);
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
-            dot[j] = 0;
-            e[j] = j < a.k ? a.bucket[i * a.k + j] : a.K;
-            g[j] = e[j] < a.K ? ((const A *)a.gates)[i * a.k + j] : (A)0;
+            if (e[j] >= a.K) continue;
+            A u[4];
+            parts4<A>((const A *)a.ws + (i * a.k + j) * a.dim + c, a.P * a.dim, a.splits, avail, u);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                dot[j] += x[q] * u[q];
+                v[q] += g[j] * u[q];
+            }
         }
-        const T *in = (const T *)a.in + i * a.in_stride;
-        for (int c = lane * 4; c < a.dim; c += 256) {
-            const int avail = a.dim - c;
-            typename Acc<T>::v4 v = {0, 0, 0, 0};
-            A x[4];
-            load4(in + c, avail, x);
+        if (a.out) store_run<4>((T *)a.out + i * a.out_stride + c, v, 0, avail);
+    }
+    if (a.bias) {
+        for (int c = lane * 4; c < a.ddim; c += 256) {
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                if (e[j] >= a.K) continue;
-                A u[4];
-                parts4<A>((const A *)a.ws + (i * a.k + j) * a.dim + c, a.P * a.dim, a.splits, avail, u);
+            for (int j = 0; j < KJ; ++j)
+                if (e[j] < a.K) {
+                    A b[4], d[4];
+                    load4((const T *)a.bias + (i64)e[j] * a.bias_row + c, a.ddim - c, b);
+                    load4((const T *)a.d + ((i * a.k + j) / a.d_div) * a.d_stride + c, a.ddim - c, d);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    dot[j] += x[q] * u[q];
-                    v[q] += g[j] * u[q];
+                    for (int q = 0; q < 4; ++q) dot[j] += b[q] * d[q];
                 }
-            }
-            if (a.out) store_run<4>((T *)a.out + i * a.out_stride + c, v, 0, avail);
         }
-        if (a.bias) {
-            for (int c = lane * 4; c < a.ddim; c += 256) {
+    }
 #pragma unroll
-                for (int j = 0; j < KJ; ++j)
-                    if (e[j] < a.K) {
-                        A b[4], d[4];
-                        load4((const T *)a.bias + (i64)e[j] * a.bias_row + c, a.ddim - c, b);
-                        load4((const T *)a.d + ((i * a.k + j) / a.d_div) * a.d_stride + c, a.ddim - c, d);
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) dot[j] += b[q] * d[q];
-                    }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) {
-            if (j >= a.k) break;
-            const A v = group_sum<64>(dot[j]);
-            if (lane == 0) ((A *)a.dgates)[i * a.k + j] = v;
-        }
+    for (int j = 0; j < KJ; ++j) {
+        if (j >= a.k) break;
+        const A v = group_sum<64>(dot[j]);
+        if (lane == 0) ((A *)a.dgates)[i * a.k + j] = v;
     }
 }
 
@@ -801,12 +801,18 @@ template <class T> int launch_weight(const WeightArgs &a, int bi, int bo, i64 bl
 template <class T> int launch_combine(const CombineArgs &a, hipStream_t st) {
     if (a.rows == 0) return BGMM_OPS_OK;
     if (a.dgates) {
-        const dim3 g((unsigned)((a.rows + 3) / 4 < (1 << 22) ? (a.rows + 3) / 4 : 1 << 22));
-        if (a.k == 1) combine_gates_kernel<T, 1><<<g, 256, 0, st>>>(a);
-        else if (a.k == 2) combine_gates_kernel<T, 2><<<g, 256, 0, st>>>(a);
-        else if (a.k <= 4) combine_gates_kernel<T, 4><<<g, 256, 0, st>>>(a);
-        else if (a.k <= 8) combine_gates_kernel<T, 8><<<g, 256, 0, st>>>(a);
-        else combine_gates_kernel<T, 32><<<g, 256, 0, st>>>(a);
+        // (a launch's threads are counted in 32 bits; a loop over rows in the kernel instead: 8192 rows of 2 x 1024 51 us, 37)
+        constexpr i64 kAtOnce = (i64)1 << 25;
+        CombineArgs b = a;
+        for (b.first = 0; b.first < a.rows; b.first += kAtOnce) {
+            const i64 n = a.rows - b.first < kAtOnce ? a.rows - b.first : kAtOnce;
+            const dim3 g((unsigned)((n + 3) / 4));
+            if (a.k == 1) combine_gates_kernel<T, 1><<<g, 256, 0, st>>>(b);
+            else if (a.k == 2) combine_gates_kernel<T, 2><<<g, 256, 0, st>>>(b);
+            else if (a.k <= 4) combine_gates_kernel<T, 4><<<g, 256, 0, st>>>(b);
+            else if (a.k <= 8) combine_gates_kernel<T, 8><<<g, 256, 0, st>>>(b);
+            else combine_gates_kernel<T, 32><<<g, 256, 0, st>>>(b);
+        }
     } else {
         const i64 threads = a.rows * ((a.dim + 3) / 4);
         if (a.splits > 1 && threads < 32768) {
