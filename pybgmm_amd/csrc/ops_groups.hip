@@ -7,10 +7,11 @@
 // group's rows in this order are too.  A wave owns a segment of consecutive rows and a histogram of its own in LDS; the 64
 // rows it looks at together find their equals with one ballot per label bit.
 //
-// Up to 4096 rows one workgroup does everything in one launch (64 components, one row 4 us, 4096 rows 9.4 us; in three launches 9
-// and 10.4 us).  Beyond: histograms per segment and workgroup, an exclusive sum over the workgroups per bucket, the scatter (1e6
-// rows, 100 components: 17 us) -- bound by the latency of the launches and of the segments' dependent LDS steps, not by the
-// 20 P bytes that move (4 us).
+// Up to 4096 rows one workgroup does everything in one launch (64 components, one row 4 us, 2048 rows 6.5, 4096 rows 9.4 us; in several
+// launches 9, 8.5 and 8.7; 4096 rows of 1400 components 17 and 23).  Beyond: histograms per segment and workgroup, an exclusive
+// sum over the workgroups per bucket -- by the scatter itself where they are few --, the scatter (20000 rows 9 us, 1e6 rows
+// of 100 components 17 us): bound by the latency of the launches and of the segments' dependent LDS steps, not by the 20 P
+// bytes that move (4 us).
 #include "ops_common.h"
 
 namespace {
@@ -262,19 +263,38 @@ __global__ void group_columns(int *counts, int nseg, int B, int *sizes) {
 }
 
 // The first `waves` waves of a workgroup have a segment each; the last workgroup writes the prefix sums and the tiles instead.
-__global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int seg, int nseg, int waves, const int *within, const int *counts,
+// sizes null: counts holds the workgroups' own counts, `groups` of them, which every workgroup adds up for itself.
+__global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int seg, int nseg, int waves, int groups, const int *within, const int *counts,
                               const int *sizes, int *order, int *offsets, int *first, Tiles tiles) {
     extern __shared__ int lds[];
-    const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * waves + w;
+    const int B = K + 1, w = threadIdx.x >> 6, s = blockIdx.x * waves + w, me = blockIdx.x;
+    int before = 0;
+    const auto total = [&](int b) {             // (before: of the workgroups in front of this one)
+        int sum = 0;
+        before = 0;
+#pragma unroll 8
+        for (int g = 0; g < groups; ++g) {
+            const int n = counts[(i64)g * B + b];
+            before += g < me ? n : 0;
+            sum += n;
+        }
+        return sum;
+    };
     if (blockIdx.x == gridDim.x - 1) {
         int *starts = lds, *tile_starts = starts + B + 1;
+        if (!sizes) {
+            int *own = tile_starts + B + 1;
+            for (int b = threadIdx.x; b < B; b += blockDim.x) own[b] = total(b);
+            __syncthreads();
+            sizes = own;
+        }
         write_sums(K, sizes, offsets, first, tiles.lg, [&](int b, int sum) { starts[b] = sum; }, [&](int b, int sum) { tile_starts[b] = sum; });
         __syncthreads();
         write_tiles(K, starts, tile_starts, tiles);
         return;
     }
     int *start = lds + waves * B, *part = start + B;
-    block_scan(B, part, [&](int b) { return sizes[b]; }, [&](int b, int v) { start[b] = v + counts[(i64)blockIdx.x * B + b]; });
+    block_scan(B, part, [&](int b) { return sizes ? sizes[b] : total(b); }, [&](int b, int v) { start[b] = v + (sizes ? counts[(i64)me * B + b] : before); });
     const int v = w % waves, parts = kManyWaves / waves;
     if (blockIdx.x * waves + v < nseg) {
 #pragma unroll 4
@@ -287,6 +307,9 @@ __global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int se
     walk(lo, hi, nbits, cursor, [&](i64 i) { return bucket[i]; }, [&](i64 i, int, int at) { order[at] = (int)i; });
 }
 
+// Up to so many workgroups each of the scatter's adds up the counts itself (20011 rows 10.5 -> 8.7 us, 65536 rows 11.0 -> 9.5; 131072
+// rows, 64 workgroups, 1000 components: 18.1 with the sums in a launch of their own, 19.2; 1e6 rows, 245: 16.5 and 23.7).
+constexpr int kFewGroups = 32;
 struct Split { int seg, nseg, waves, groups; };
 
 // Rows of a segment (a wave's): 512, 256 where that would leave most of the chip idle.  Segments per workgroup: eight while their histograms, the buckets' starts and the sums fit 64 KB of LDS.
@@ -330,8 +353,9 @@ extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int3
     int *within = (int *)ws, *counts = within + (size_t)s.nseg * B, *sizes = counts + (size_t)s.groups * B;
     // (P = 0 with many components: no segment, but the sums over nothing and the empty offsets are still written)
     if (s.groups > 0) group_count<<<s.groups, 64 * kManyWaves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, s.seg, s.nseg, s.waves, bucket, within, counts);
-    group_columns<<<(B + 3) / 4, 256, 0, st>>>(counts, s.groups, B, sizes);
+    const bool columns = s.groups > kFewGroups || s.waves < 8;
+    if (columns) group_columns<<<(B + 3) / 4, 256, 0, st>>>(counts, s.groups, B, sizes);
     group_scatter<<<s.groups + 1, 64 * kManyWaves, sizeof(int) * ((size_t)(s.waves + 1) * B + 2 + kManyWaves), st>>>(
-        bucket, P, K, nbits, s.seg, s.nseg, s.waves, within, counts, sizes, order, offsets, first, table);
+        bucket, P, K, nbits, s.seg, s.nseg, s.waves, s.groups, within, counts, columns ? sizes : nullptr, order, offsets, first, table);
     return ops_launched("group_rows");
 }
