@@ -1,8 +1,8 @@
 """
 Build libbgmm_hip.so, libbgmm_ops.so (hipcc, gfx950 only) and the operators' torch binding (g++) in-tree.
 
-The shared objects are git-ignored but travel to the GPU box with the gpurun
-snapshot.  ``build()`` is idempotent: it recompiles only sources newer than
+The shared objects are git-ignored and go with the tree where it is copied.
+``build()`` is idempotent: it recompiles only sources newer than
 their objects.
 """
 import glob
