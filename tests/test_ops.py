@@ -1076,3 +1076,58 @@ def test_a_large_batch_draws_as_its_parts_do(dt):
         part = [a[i:i + 120] for a in args]
         o, c = ops.verify_drafts(*part[:5], lengths=part[5])
         assert torch.equal(o, out[i:i + 120]) and torch.equal(c, acc[i:i + 120])
+
+
+@gpu
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n,k,K,din,dout", [(300, 1, 5, 37, 21), (300, 2, 4, 64, 16), (5, 2, 3, 7, 9), (2000, 1, 6, 130, 67)])
+def test_broadcast_operands(dt, n, k, K, din, dout):
+    """Operands of stride zero give what their copies give, and the gradients of what was broadcast are sums."""
+    from pybgmm_amd import ops
+    z, x, w, b, gt, g = product_case(n, k, K, din, dout, dt, 3 * n + din)
+    groups = ops.group_rows(z, K)
+    gt = torch.nan_to_num(gt)
+    one_row, one_matrix, one_line = torch.randn(1, din, generator=g, device="cuda").to(dt), w[:1].clone(), w[:1, :1].clone()
+    cases = [(one_row.expand(n, din), w, b, gt), (x, one_matrix.expand(K, din, dout), b, gt), (x, one_line.expand(K, din, dout), b[:1].expand(K, dout), gt),
+             (x, w, b[:, :1].expand(K, dout), gt[:1].expand(n, k)), (x, w[:, :1].expand(K, din, dout).transpose(1, 2).contiguous().transpose(1, 2), b, gt)]
+    dy = torch.randn(n, 1, generator=g, device="cuda").to(dt).expand(n, dout)
+    for case in cases:
+        views = [t.detach().requires_grad_() for t in case]
+        copies = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for t in case]
+        if case is cases[4]:
+            copies[1] = case[1].detach().clone(memory_format=torch.preserve_format).requires_grad_()
+        y, y2 = (ops.grouped_matmul(t[0], t[1], groups, bias=t[2], gates=t[3]) for t in (views, copies))
+        assert torch.equal(y, y2) or (torch.isnan(y) == torch.isnan(y2)).all() and torch.equal(torch.nan_to_num(y), torch.nan_to_num(y2))
+        for a, c in zip(torch.autograd.grad(y, views, dy), torch.autograd.grad(y2, copies, dy.contiguous())):
+            assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(c))
+    leaf = one_row.clone().requires_grad_()
+    y = ops.grouped_matmul(leaf.expand(n, din), w, groups, bias=b, gates=gt)
+    full = one_row.expand(n, din).clone().requires_grad_()
+    y2 = ops.grouped_matmul(full, w, groups, bias=b, gates=gt)
+    got, = torch.autograd.grad(y, leaf, dy)
+    rows, = torch.autograd.grad(y2, full, dy)
+    assert torch.equal(got, rows.sum(0, keepdim=True))
+
+
+@gpu
+def test_the_same_label_in_every_place_and_one_grouping_for_two_products():
+    from pybgmm_amd import ops
+    g = torch.Generator("cuda").manual_seed(9)
+    z = torch.full((130, 3), 2, device="cuda")
+    groups = ops.group_rows(z, 4)
+    x = torch.randn(130, 19, device="cuda", dtype=torch.float64, generator=g, requires_grad=True)
+    w = torch.randn(4, 19, 6, device="cuda", dtype=torch.float64, generator=g, requires_grad=True)
+    gates = torch.rand(130, 3, device="cuda", dtype=torch.float64, generator=g, requires_grad=True)
+    y = ops.grouped_matmul(x, w, groups, gates=gates)
+    want = (x @ w[2]) * gates.sum(1, keepdim=True)
+    tol = dict(rtol=1e-12, atol=1e-12)                  # (19 products of about one, 3 of them added: a few hundred steps of 2^-53)
+    assert torch.allclose(y, want, **tol)
+    dy = torch.randn_like(y)
+    for a, c in zip(torch.autograd.grad(y, (x, w, gates), dy), torch.autograd.grad(want, (x, w, gates), dy)):
+        assert torch.allclose(a, c, rtol=1e-11, atol=1e-11)      # (dW: 390 terms)
+    w2 = torch.randn(4, 6, 19, device="cuda", dtype=torch.float64, generator=g)
+    with torch.no_grad():
+        h = ops.grouped_matmul(x, w, groups)                     # a row per label, straight into the next product
+        out = ops.grouped_matmul(h, w2, groups, gates=gates)
+        assert tuple(h.shape) == (130, 3, 6)
+        assert torch.allclose(out, ((x @ w[2]) @ w2[2]) * gates.sum(1, keepdim=True), rtol=1e-11, atol=1e-11)
