@@ -61,13 +61,15 @@ def build(force=False, verbose=False, extra_flags=()):
 
 
 def _build_binding(force, verbose):
-    """Host code against torch's headers and libraries; without torch there are no operators to bind."""
+    """Host code against torch's headers and libraries; without torch, or with one that has no HIP, there are no operators to bind."""
     src = os.path.join(CSRC, "ops_torch.cpp")
     if importlib.util.find_spec("torch") is None or not (force or _stale(OPS_BINDING, [src, OPS_HEADERS[-1]])):
         return
     import torch
     from torch.utils.cpp_extension import include_paths
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    if not os.path.exists(os.path.join(lib, "libc10_hip.so")):
+        return
     rocm = os.path.dirname(os.path.dirname(hipcc()))
     includes = include_paths() + [sysconfig.get_paths()["include"], os.path.join(rocm, "include"), "/opt/rocm/include"]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
