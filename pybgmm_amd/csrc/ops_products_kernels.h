@@ -384,13 +384,27 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     }
 }
 
-// dW: the rows of a chunk are the contraction, both operands have it outermost (MTile).  Half precision: g d is rounded to
-// the operand type before the product (like the operands themselves), its column sums for db are not.
-// 64 experts of 1024 x 2048 from 16384 rows, bfloat16: 190 us, 360 TFLOP/s.  A component's 256 rows are four steps, so the time is
+// A number as two of bfloat16, which has its range: the upper half of its bits, and the rest rounded to 8 bits (2^-15 of the number
+// at most is lost) with 2^-20 of the number on top, so that it is of the number's sign and zero only with it: an infinite operand
+// stays infinite against either.  Infinities and NaN are themselves in both.
+__device__ __forceinline__ void two_pieces(float v, bf16_t &high, bf16_t &low) {
+    const float h = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+    high = (bf16_t)h;
+    low = (bf16_t)(__builtin_fabsf(v) < __builtin_inff() ? __builtin_fmaf(v, 0x1p-20f, v - h) : v);
+}
+
+// dW: the rows of a chunk are the contraction, both operands have it outermost (MTile).
+// PIECES, the gates of 16-bit types: g d in 16 bits would be a rounding more than the operands have, and in half precision it leaves
+// the range (a gate of 1e-4 times a gradient of 1e-4 is zero there).  It goes into the product as two of bfloat16, the rows in half
+// precision too (11 bits are whole in two): two or four products of pieces in one accumulator, 2^-15 of a term lost.  Forward and this,
+// 16384 rows of 64 experts, 1024 x 2048: bfloat16 330 us with g d rounded, 380 in pieces (25 the second product, 25 to make them),
+// half precision 334 and 530.
+// 64 experts of 1024 x 2048 from 16384 rows, bfloat16: 190 us, 360 TFLOP/s, without pieces.  A component's 256 rows are four steps, so the time is
 // what four steps do not hide: finding the chunk, its rows and the first loads (a quarter, alone), and the results' stores (4 MB
 // for 1.5 MB of operands; a third).
-template <class T, int BI, int BO, int WO, int WI>
+template <class T, int BI, int BO, int WO, int WI, bool PIECES>
 __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kernel(WeightArgs a) {
+    static_assert(!PIECES || sizeof(T) == 2, "pieces of 16 bits");
     typedef typename Acc<T>::type A;
     typedef typename Acc<T>::v4 A4;
     constexpr int FA = BO / WO / 16, FB = BI / WI / 16;
@@ -398,8 +412,11 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kerne
     constexpr bool kAllI = BI >= 32, kAllO = BO >= 32, kSame = BI == BO;        // every thread moves some; the same rows of both
     typedef MTile<T, BI> ITile;
     typedef MTile<T, BO> OTile;
-    __shared__ __attribute__((aligned(128))) char lds[(BI + BO) * kStepBytes];
-    char *const lds_o = lds + BI * kStepBytes;
+    constexpr bool kHalves = PIECES && std::is_same_v<T, f16_t>;       // the rows in pieces, too
+    typedef std::conditional_t<PIECES, bf16_t, T> M;                    // what is multiplied
+    constexpr int kBytes = (BI + BO + (PIECES ? BO : 0) + (kHalves ? BI : 0)) * kStepBytes;
+    __shared__ __attribute__((aligned(128))) char lds[kBytes];
+    char *const lds_o = lds + BI * kStepBytes, *const low_o = lds_o + BO * kStepBytes, *const low_i = low_o + BO * kStepBytes;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wo = wave % WO, wi = wave / WO;
     const int out_tiles = a.i_tiles * a.o_tiles;
@@ -507,7 +524,16 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kerne
 #pragma unroll
             for (int p = 0; p < NO; ++p) {
                 T *el = Elems<T>::of(h.o[p]);
-                if (gates) {
+                if constexpr (PIECES) {
+                    Granule low;
+#pragma unroll
+                    for (int j = 0; j < kGran<T>; ++j) {
+                        const A v = (A)el[j] * h.gate[p];
+                        if (want_db) dsum[j] += v;
+                        two_pieces(v, h.o[p].b[j], low.b[j]);
+                    }
+                    *(v4i *)(low_o + OTile::at(o_row + p * kRowsO, o_at)) = low.raw;
+                } else if (gates) {
 #pragma unroll
                     for (int j = 0; j < kGran<T>; ++j) {
                         const A v = (A)el[j] * h.gate[p];
@@ -523,7 +549,15 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kerne
         }
         if (kAllI || tid < BI * 8) {
 #pragma unroll
-            for (int p = 0; p < NI; ++p) *(v4i *)(lds + ITile::at(i_row + p * kRowsI, i_at)) = h.i[p].raw;
+            for (int p = 0; p < NI; ++p) {
+                if constexpr (kHalves) {
+                    Granule low;
+#pragma unroll
+                    for (int j = 0; j < kGran<T>; ++j) two_pieces((float)h.i[p].h[j], h.i[p].b[j], low.b[j]);
+                    *(v4i *)(low_i + ITile::at(i_row + p * kRowsI, i_at)) = low.raw;
+                }
+                *(v4i *)(lds + ITile::at(i_row + p * kRowsI, i_at)) = h.i[p].raw;
+            }
         }
     };
 
@@ -538,15 +572,23 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kerne
         for (int ks = 0; ks < 2; ++ks) {
             Granule fa[FA], fb[FB];
 #pragma unroll
-            for (int i = 0; i < FA; ++i) fa[i] = OTile::template read<true>(lds_o, (wo * FA + i) * 16, ks);
+            for (int turn = (PIECES ? 2 : 1) * (kHalves ? 2 : 1) - 1; turn >= 0; --turn) {          // (the small products first)
+                const bool low = turn & 1, rows_low = turn >> 1;
+                if (turn == (kHalves ? 3 : PIECES ? 1 : 0) || (kHalves && turn == 1)) {
 #pragma unroll
-            for (int j = 0; j < FB; ++j) fb[j] = ITile::template read<false>(lds, (wi * FB + j) * 16, ks);
+                    for (int j = 0; j < FB; ++j) fb[j] = ITile::template read<false>(rows_low ? low_i : lds, (wi * FB + j) * 16, ks);
+                }
 #pragma unroll
-            for (int part = 0; part < kParts<T>; ++part)
+                for (int i = 0; i < FA; ++i) fa[i] = OTile::template read<true>(low ? low_o : lds_o, (wo * FA + i) * 16, ks);
 #pragma unroll
-                for (int i = 0; i < FA; ++i)
+                for (int part = 0; part < kParts<T>; ++part)
 #pragma unroll
-                    for (int j = 0; j < FB; ++j) mma<T>(acc[i][j], fa[i], fb[j], part);
+                    for (int i = 0; i < FA; ++i)
+#pragma unroll
+                        for (int j = 0; j < FB; ++j) mma<M>(acc[i][j], fa[i], fb[j], part);
+                // (the next turn's operands in these ones' registers: 123 spilled with all at once)
+                if (PIECES) __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
     look(0);
@@ -565,7 +607,6 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kerne
     A *slot = nullptr;
     if (chunks > 1) slot = (A *)a.ws + ((((i64)at_b.offset * 2) >> (8 + a.level)) + c) * ((i64)a.idim * a.odim + a.odim);
     if (a.dw) {
-        constexpr int kBytes = (BI + BO) * kStepBytes;
         const int n_i = a.idim - i0 < BI ? a.idim - i0 : BI, w_o = WO * WI < 4 && wave >= WO * WI ? 0 : wo, w_i = WO * WI < 4 && wave >= WO * WI ? BI : wi;
         const auto part = [&](int, int i, int j) { return acc[i][j]; };         // (waves without a part of the tile: none of its rows)
         if (slot) {
@@ -780,17 +821,19 @@ template <class T> int launch_rows(const RowsArgs &a, bool kcontig, int bm, int 
     return ops_launched("rows_product");
 }
 
-template <class T> int launch_weight(const WeightArgs &a, int bi, int bo, i64 blocks, hipStream_t st) {
+template <class T, bool PIECES> static void weight_by_tile(const WeightArgs &a, int bi, int bo, i64 blocks, hipStream_t st) {
     const dim3 g((unsigned)blocks);
-    if (blocks > 0) {
-        if (bi == 16 && bo == 16) weight_kernel<T, 16, 16, 1, 1><<<g, 256, 0, st>>>(a);
-        else if (bi == 16) weight_kernel<T, 16, 128, 4, 1><<<g, 256, 0, st>>>(a);
-        else if (bo == 16) weight_kernel<T, 128, 16, 1, 4><<<g, 256, 0, st>>>(a);
-        else if (bi == 64 && bo == 64) weight_kernel<T, 64, 64, 2, 2><<<g, 256, 0, st>>>(a);
-        else if (bi == 64) weight_kernel<T, 64, 128, 2, 2><<<g, 256, 0, st>>>(a);
-        else if (bo == 64) weight_kernel<T, 128, 64, 2, 2><<<g, 256, 0, st>>>(a);
-        else weight_kernel<T, 128, 128, 2, 2><<<g, 256, 0, st>>>(a);
-    }
+    if (bi == 16 && bo == 16) weight_kernel<T, 16, 16, 1, 1, PIECES><<<g, 256, 0, st>>>(a);
+    else if (bi == 16) weight_kernel<T, 16, 128, 4, 1, PIECES><<<g, 256, 0, st>>>(a);
+    else if (bo == 16) weight_kernel<T, 128, 16, 1, 4, PIECES><<<g, 256, 0, st>>>(a);
+    else if (bi == 64 && bo == 64) weight_kernel<T, 64, 64, 2, 2, PIECES><<<g, 256, 0, st>>>(a);
+    else if (bi == 64) weight_kernel<T, 64, 128, 2, 2, PIECES><<<g, 256, 0, st>>>(a);
+    else if (bo == 64) weight_kernel<T, 128, 64, 2, 2, PIECES><<<g, 256, 0, st>>>(a);
+    else weight_kernel<T, 128, 128, 2, 2, PIECES><<<g, 256, 0, st>>>(a);
+}
+
+template <class T> int launch_weight(const WeightArgs &a, int bi, int bo, i64 blocks, hipStream_t st) {
+    if (blocks > 0) a.gates && sizeof(T) == 2 ? weight_by_tile<T, sizeof(T) == 2>(a, bi, bo, blocks, st) : weight_by_tile<T, false>(a, bi, bo, blocks, st);
     // (most components have one chunk and nothing to add up: about 4096 workgroups in all)
     const i64 size = (i64)a.idim * a.odim + a.odim, most = 4096 / a.K > 4 ? 4096 / a.K : 4;
     const i64 bx = (size + 255) / 256 < most ? (size + 255) / 256 : most;

@@ -1131,3 +1131,62 @@ def test_the_same_label_in_every_place_and_one_grouping_for_two_products():
         out = ops.grouped_matmul(h, w2, groups, gates=gates)
         assert tuple(h.shape) == (130, 3, 6)
         assert torch.allclose(out, ((x @ w[2]) @ w2[2]) * gates.sum(1, keepdim=True), rtol=1e-11, atol=1e-11)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("n,k,K,din,dout", [(700, 1, 3, 16, 16), (900, 2, 4, 130, 136), (2100, 1, 2, 24, 200), (1500, 2, 3, 200, 12), (800, 1, 3, 64, 60), (3000, 1, 2, 40, 70)])
+@pytest.mark.parametrize("gate,d_size,x_size", [(1.0, 1.0, 1.0), (1e-4, 1e-4, 3e4), (1e-3, 1e-4, 3e4), (100.0, 1000.0, 1e-3), (1e30, 1e-3, 1.0)])
+def test_gates_of_any_size_in_the_weights_gradient(dt, n, k, K, din, dout, gate, d_size, x_size):
+    """
+    Gates times gradients that 16 bits cannot hold (nothing of 1e-4 x 1e-4 is left in half precision, 100 x 1000 is infinite there), next
+    to ordinary ones.  The product takes g d as two bfloat16 numbers, which lose at most 2^-15 of it (the first has 8 bits, the rest is
+    rounded to 8: 2^-7 2^-8) and carry 2^-20 too much, in half precision x likewise (whose 11 bits are whole in two): 2^-14 of a term
+    covers both; 32-bit sums of a component's own rows (two to four products a term), and the result's own rounding.
+    """
+    from pybgmm_amd import ops
+    if gate == 1e30 and dt == torch.float16:
+        gate, x_size = 1e-30, 1e4                                           # (a result of zero: nothing may become infinite or NaN)
+    g = torch.Generator("cuda").manual_seed(n + din)
+
+    def rand(*s):
+        sign = torch.randint(0, 2, s, generator=g, device="cuda") * 2 - 1
+        return (torch.rand(*s, generator=g, device="cuda", dtype=torch.float64) + 0.5) * sign
+    z = torch.randint(0, K, (n, k), generator=g, device="cuda")
+    z[5] = -1
+    x, dy = (rand(n, din) * x_size).to(dt), (rand(n, dout) * d_size).to(dt)
+    w = rand(K, din, dout).to(dt).requires_grad_()
+    gates = (rand(n, k) * gate).float()
+    groups = ops.group_rows(z, K)
+    got, = torch.autograd.grad(ops.grouped_matmul(x, w, groups, gates=gates), w, dy)
+    bits, top = half_step(dt), torch.finfo(dt).max
+    smallest = torch.finfo(dt).tiny * bits                                  # half of the type's smallest step
+    for e in range(K):
+        i, j = torch.nonzero(z == e, as_tuple=True)
+        gd = gates[i, j].double()[:, None] * dy[i].double()
+        want, mag = (a.t().contiguous() @ b for a, b in ((x[i].double(), gd), (x[i].double().abs(), gd.abs())))
+        tol = (2.0 ** -14 + 2.0 ** -24 * (4 * i.numel() + 8)) * mag
+        fits = want.abs() + tol < top
+        off = (got[e].double() - want).abs()
+        assert bool((off <= tol + bits * (want.abs() + tol) + smallest)[fits].all()), float((off / mag)[fits].max())
+        assert fits.float().mean() > 0.9 and not torch.isnan(got[e]).any()
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=str)
+def test_infinite_and_undefined_gates_and_gradients_stay_in_their_columns(dt):
+    from pybgmm_amd import ops
+    n, K, din, dout = 300, 2, 40, 33
+    z = torch.arange(n, device="cuda") % K
+    x, dy = torch.full((n, din), 1.5, device="cuda", dtype=dt), torch.ones(n, dout, device="cuda", dtype=dt)
+    dy[4, 3], dy[7, 5], dy[6, 8] = math.inf, math.nan, -math.inf            # components 0, 1, 0
+    x[12, 11] = math.inf
+    w = torch.zeros(K, din, dout, device="cuda", dtype=dt, requires_grad=True)
+    gates = torch.full((n,), 0.5, device="cuda")
+    got, = torch.autograd.grad(ops.grouped_matmul(x, w, ops.group_rows(z, K), gates=gates), w, dy)
+    want = torch.full((K, din, dout), 1.5 * 0.5 * n / K, device="cuda", dtype=torch.float64)
+    want[0, :, 3], want[1, :, 5], want[0, :, 8] = math.inf, math.nan, -math.inf
+    want[0, 11] = math.inf
+    want[0, 11, 8] = math.nan
+    ok = (got.double() == want) | (torch.isnan(got) & torch.isnan(want)) | ((got.double() - want).abs() <= 112.5 * half_step(dt))
+    assert bool(ok.all())
