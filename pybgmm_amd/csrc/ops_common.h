@@ -37,6 +37,9 @@ template <class F> int by_type(int dtype, F f) {
 int ops_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 int ops_launched(const char *what);         // the status of the launch just made
 
+// Threads of a launch: they are counted in 32 bits.  What needs more is launched in parts.
+constexpr i64 kThreadsAtOnce = (i64)1 << 31;
+
 __device__ __forceinline__ int wave_lane() { return threadIdx.x & 63; }
 
 // N bytes (4, 8, 16 or 32) from or to memory as one access per 16, at whatever alignment p has.  (Through a vector of words: element

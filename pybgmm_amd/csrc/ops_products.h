@@ -151,9 +151,10 @@ struct Divisor {
 __device__ __forceinline__ int divide(int n, Divisor d) { return (int)(((unsigned long long)(unsigned)n * d.m) >> d.s); }
 
 // Workgroups go round the eight dies in turn: number them so that a die gets runs of consecutive work, whose operands its own L2
-// then holds.  A permutation of 0 .. blocks - 1 (a multiple of 8 * run) that needs no load.
-__device__ __forceinline__ int die_order(int run) {
-    const int b = blockIdx.x, die = b & 7, at = b >> 3;
+// then holds.  A permutation of 0 .. blocks - 1 (a multiple of 8 * run) that needs no load; first: of a launch's part of them, such a
+// multiple too.
+__device__ __forceinline__ int die_order(int run, int first) {
+    const int b = first + blockIdx.x, die = b & 7, at = b >> 3;
     return (at / run * 8 + die) * run + at % run;
 }
 
@@ -161,6 +162,7 @@ struct RowsArgs {
     const int4 *tiles;              // the grouping's
     const int *order;
     int K, tile_blocks, run;        // blocks of eight tiles, consecutive workgroups on a die
+    int first;                      // of a launch's workgroups
     const void *in;                 // row src = p / in_div of `in`
     i64 in_stride;
     Divisor in_div;
@@ -186,7 +188,7 @@ struct RowsArgs {
 struct WeightArgs {
     const int *bucket_first;        // prefix sums for chunks of `chunk` rows
     const int *offsets, *order;
-    int K, level, run;
+    int K, level, run, first;       // (run, first: as above)
     const void *in;                 // row p / in_div
     i64 in_stride;
     Divisor in_div;

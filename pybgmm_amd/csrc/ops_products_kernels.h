@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
     // ---- which tile: blocks of eight row tiles, within a block every column tile (of every split) in turn
     constexpr int kBlock = 8;
     const int per_block = kBlock * a.n_tiles * a.splits;
-    const int id = die_order(a.run), blk = id / per_block, local = id - blk * per_block;
+    const int id = die_order(a.run, a.first), blk = id / per_block, local = id - blk * per_block;
     if (blk >= a.tile_blocks) return;
     const int t = blk * kBlock + local % kBlock, rest = local / kBlock, nt = rest % a.n_tiles, split = rest / a.n_tiles;
     const int4 tile = a.tiles[t];
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kerne
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wo = wave % WO, wi = wave / WO;
     const int out_tiles = a.i_tiles * a.o_tiles;
-    const int id = die_order(a.run), chunk = id / out_tiles, tile = id % out_tiles;
+    const int id = die_order(a.run, a.first), chunk = id / out_tiles, tile = id % out_tiles;
     const Bucket at_b = find_bucket(a.bucket_first, a.offsets, a.K, chunk);
     if (at_b.b < 0) return;
     const int e = at_b.b, c = chunk - at_b.first, chunks = at_b.next_first - at_b.first;
@@ -807,6 +807,15 @@ template <class T> __global__ __launch_bounds__(256) void gates_kernel(GatesArgs
     }
 }
 
+// Workgroups of 256 in as many launches as they take.
+template <class Args, class F> static void in_parts(Args a, i64 blocks, F launch) {
+    constexpr i64 kEach = kThreadsAtOnce / 256;
+    for (i64 b = 0; b < blocks; b += kEach) {
+        a.first = (int)b;
+        launch(a, blocks - b < kEach ? blocks - b : kEach);
+    }
+}
+
 template <class T, bool KCONTIG> static void rows_by_tile(const RowsArgs &a, int bm, int bn, i64 blocks, hipStream_t st) {
     const dim3 g((unsigned)blocks);
     if (bm == 16) rows_kernel<T, KCONTIG, 16, 128, 4, 1><<<g, 256, 0, st>>>(a);
@@ -817,7 +826,9 @@ template <class T, bool KCONTIG> static void rows_by_tile(const RowsArgs &a, int
 }
 
 template <class T> int launch_rows(const RowsArgs &a, bool kcontig, int bm, int bn, i64 blocks, hipStream_t st) {
-    kcontig ? rows_by_tile<T, true>(a, bm, bn, blocks, st) : rows_by_tile<T, false>(a, bm, bn, blocks, st);
+    in_parts(a, blocks, [&](const RowsArgs &part, i64 n) {
+        kcontig ? rows_by_tile<T, true>(part, bm, bn, n, st) : rows_by_tile<T, false>(part, bm, bn, n, st);
+    });
     return ops_launched("rows_product");
 }
 
@@ -833,7 +844,9 @@ template <class T, bool PIECES> static void weight_by_tile(const WeightArgs &a, 
 }
 
 template <class T> int launch_weight(const WeightArgs &a, int bi, int bo, i64 blocks, hipStream_t st) {
-    if (blocks > 0) a.gates && sizeof(T) == 2 ? weight_by_tile<T, sizeof(T) == 2>(a, bi, bo, blocks, st) : weight_by_tile<T, false>(a, bi, bo, blocks, st);
+    in_parts(a, blocks, [&](const WeightArgs &part, i64 n) {
+        a.gates && sizeof(T) == 2 ? weight_by_tile<T, sizeof(T) == 2>(part, bi, bo, n, st) : weight_by_tile<T, false>(part, bi, bo, n, st);
+    });
     // (most components have one chunk and nothing to add up: about 4096 workgroups in all)
     const i64 size = (i64)a.idim * a.odim + a.odim, most = 4096 / a.K > 4 ? 4096 / a.K : 4;
     const i64 bx = (size + 255) / 256 < most ? (size + 255) / 256 : most;

@@ -26,6 +26,7 @@ struct VerifyArgs {
     const double *u_accept, *u_draw;        // [B][T], [B]
     const int64_t *lengths;                 // [B], or null: T
     int B, T;
+    int first;                              // of a launch's sequences
     i64 V;
     int64_t *out, *accepted;                // [B][T + 1], [B]
 };
@@ -229,7 +230,7 @@ struct VerifyWs {
 
 template <class T> __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a, VerifyWs w) {
     __shared__ double part[4][2];
-    const i64 b = blockIdx.x / w.chunks;
+    const i64 b = a.first + blockIdx.x / w.chunks;
     const int c = (int)(blockIdx.x % w.chunks);
     int len;
     i64 z0;
@@ -276,7 +277,7 @@ template <class F> __device__ __forceinline__ int pick(int n, F sum_of, double g
 
 template <class T, int W> __global__ __launch_bounds__(64 * W) void verify_draw_kernel(VerifyArgs a, VerifyWs w) {
     __shared__ double part[W];
-    const i64 b = blockIdx.x;
+    const i64 b = a.first + blockIdx.x;
     const int acc = w.acc[b], len = w.len[b], wave = threadIdx.x >> 6;
     const T *p = (const T *)a.target + b * a.target_b + acc * a.target_t;
     const T *q = acc < len ? (const T *)a.draft + b * a.draft_b + acc * a.draft_t : nullptr;
@@ -355,7 +356,7 @@ extern "C" int bgmm_verify_drafts(int32_t dtype, const void *target, int64_t tar
         return ops_fail(BGMM_OPS_EINVAL, "verify_drafts: a null pointer");
     const i64 need = bgmm_verify_drafts_ws(B, V);
     if (ws_bytes < need || (need > 0 && (!ws || ((uintptr_t)ws & 7)))) return ops_fail(BGMM_OPS_EINVAL, "verify_drafts: workspace of %lld bytes", (long long)ws_bytes);
-    const VerifyArgs a = {target, draft, target_b, target_t, draft_b, draft_t, labels, u_accept, u_draw, lengths, (int)B, T, V, out, accepted};
+    VerifyArgs a = {target, draft, target_b, target_t, draft_b, draft_t, labels, u_accept, u_draw, lengths, (int)B, T, 0, V, out, accepted};
     const hipStream_t st = (hipStream_t)stream;
     VerifyWs w = {};
     if (need > 0) {
@@ -364,17 +365,23 @@ extern "C" int bgmm_verify_drafts(int32_t dtype, const void *target, int64_t tar
         w.sums = (double *)ws;
         w.acc = (int *)(w.sums + B * w.chunks * 2);
         w.len = w.acc + B;
-        if (B * w.chunks > 0x7fffffff) return ops_fail(BGMM_OPS_EUNSUPPORTED, "verify_drafts: %lld chunks", (long long)(B * w.chunks));
     }
     return by_type(dtype, [&](auto *t) {
         typedef std::remove_pointer_t<decltype(t)> E;
         if (few_labels(V)) {
             verify_few<E>(a, st);
         } else {
-            verify_sums_kernel<E><<<dim3((unsigned)(B * w.chunks)), 256, 0, st>>>(a, w);
+            // (a sequence has at most 2^19 chunks)
+            const auto parts = [&](i64 each, auto launch) {
+                for (i64 b = 0; b < B; b += each) {
+                    a.first = (int)b;
+                    launch((unsigned)(B - b < each ? B - b : each));
+                }
+            };
+            parts(kThreadsAtOnce / 256 / w.chunks, [&](unsigned n) { verify_sums_kernel<E><<<dim3(n * (unsigned)w.chunks), 256, 0, st>>>(a, w); });
             // few sequences: more waves for the latency of each (5000 sequences of 2000 singles: 38 us with 4, 68 with 16)
-            if (B > 512) verify_draw_kernel<E, 4><<<dim3((unsigned)B), 256, 0, st>>>(a, w);
-            else verify_draw_kernel<E, 16><<<dim3((unsigned)B), 1024, 0, st>>>(a, w);
+            if (B > 512) parts(kThreadsAtOnce / 256, [&](unsigned n) { verify_draw_kernel<E, 4><<<dim3(n), 256, 0, st>>>(a, w); });
+            else parts(B, [&](unsigned n) { verify_draw_kernel<E, 16><<<dim3(n), 1024, 0, st>>>(a, w); });
         }
         return ops_launched("verify_drafts");
     });

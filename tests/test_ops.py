@@ -1190,3 +1190,35 @@ def test_infinite_and_undefined_gates_and_gradients_stay_in_their_columns(dt):
     want[0, 11, 8] = math.nan
     ok = (got.double() == want) | (torch.isnan(got) & torch.isnan(want)) | ((got.double() - want).abs() <= 112.5 * half_step(dt))
     assert bool(ok.all())
+
+
+@gpu
+def test_more_sequences_than_a_launch_takes():
+    """2^24 sequences, the most a call takes: with 256 threads each they are more threads than a launch counts."""
+    from pybgmm_amd import ops
+    B, V = 1 << 24, 2049
+    p = torch.randint(0, 4, (V,), device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    u = (torch.arange(B, device="cuda", dtype=torch.float64) * 48271 % B) / B
+    none = torch.empty(B, 0, dtype=torch.int64, device="cuda")
+    out, acc = ops.verify_drafts(p.to(torch.bfloat16).expand(B, 1, V), torch.empty(B, 0, V, device="cuda", dtype=torch.bfloat16), none, none.double(), u)
+    total = p.double().cumsum(0)                                            # (whole numbers: the same in any order)
+    assert not acc.any() and torch.equal(out[:, 0], torch.searchsorted(total, u * total[-1], right=True))
+
+
+@gpu
+def test_more_tiles_than_a_launch_takes():
+    """8000 components times 2094 tiles of columns: more workgroups of 256 than a launch counts threads for, in every product."""
+    from pybgmm_amd import ops
+    K, dout = 8000, 268032
+    g = torch.Generator("cuda").manual_seed(4)
+    z = torch.randperm(K, device="cuda", generator=g)
+    x = torch.randint(-8, 9, (K, 1), device="cuda", generator=g).to(torch.bfloat16).requires_grad_()
+    w = torch.randint(-8, 9, (1, 1, dout), device="cuda", generator=g).to(torch.bfloat16).expand(K, 1, dout).requires_grad_()
+    y = ops.grouped_matmul(x, w, ops.group_rows(z, K))
+    assert torch.equal(y.detach(), x.detach() * w.detach()[0])              # (products of small integers: exact)
+    dy = torch.randint(-1, 2, (K, 1), device="cuda", generator=g).to(torch.bfloat16)
+    dx, dw = torch.autograd.grad(y, (x, w), dy.expand(K, dout))
+    del y
+    assert torch.equal(dw[z, 0], (x.detach() * dy).expand(K, dout))
+    want = dy.double() * w.detach()[0].double().sum()
+    assert bool(((dx.double() - want).abs() <= 2.0 ** -8 * want.abs()).all())           # (268000 terms of at most 8: exact in 32 bits)
