@@ -28,10 +28,6 @@ template <class A> __device__ __forceinline__ A neg_inf();
 template <> __device__ __forceinline__ float neg_inf<float>() { return -__builtin_inff(); }
 template <> __device__ __forceinline__ double neg_inf<double>() { return -__builtin_inf(); }
 
-template <class A> __device__ __forceinline__ A largest();
-template <> __device__ __forceinline__ float largest<float>() { return __FLT_MAX__; }
-template <> __device__ __forceinline__ double largest<double>() { return __DBL_MAX__; }
-
 // Of two values the larger or smaller, the other one for a quiet NaN: one instruction each (the builtins put another in front of
 // every operand that quiets signalling NaNs; here that is done once, where the values are read).
 __device__ __forceinline__ double larger(double a, double b) {
@@ -90,13 +86,12 @@ template <int N> __device__ __forceinline__ void exps(const float *x, float *y) 
     }
 }
 
-// exp(v - m) for v <= m, exactly 1 where they are equal; m = +inf: 1 for +inf, 0 for the others.  (m = -inf: 1 everywhere, for
-// callers that ask for no such row.)
+// exp(v - m) for v <= m, exactly 1 where they are equal: also where both are infinite, whose difference is NaN and the smaller of that
+// and 0 is 0.  m = +inf: 0 for the others.  (m = -inf: 1 everywhere, for callers that ask for no such row.)
 template <int N, class A> __device__ __forceinline__ void ratios(const A *v, A m, A *y) {
-    const A top = m < (A)largest<A>() ? m : (A)largest<A>();
     A x[N];
 #pragma unroll
-    for (int q = 0; q < N; ++q) x[q] = smaller(v[q] - top, (A)0);
+    for (int q = 0; q < N; ++q) x[q] = smaller(v[q] - m, (A)0);
     exps<N>(x, y);
 }
 template <class A> __device__ __forceinline__ A ratio(A v, A m) {

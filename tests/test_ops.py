@@ -1222,3 +1222,26 @@ def test_more_tiles_than_a_launch_takes():
     assert torch.equal(dw[z, 0], (x.detach() * dy).expand(K, dout))
     want = dy.double() * w.detach()[0].double().sum()
     assert bool(((dx.double() - want).abs() <= 2.0 ** -8 * want.abs()).all())           # (268000 terms of at most 8: exact in 32 bits)
+
+
+@gpu
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n,K", [(9, 7), (5, 64), (3, 1000), (2, 5000), (2, 20001)])
+@pytest.mark.parametrize("renormalise", [True, False])
+def test_the_largest_number_beside_infinity_has_no_weight(dt, n, K, renormalise):
+    """exp(v - inf) is zero for every finite v, the type's largest among them; several infinite ones share the weight."""
+    from pybgmm_amd import ops
+    lw = torch.zeros(n, K, dtype=dt, device="cuda")
+    lw[:, 1], lw[:, 3], lw[:, 5] = torch.finfo(dt).max, math.inf, torch.finfo(dt).min
+    lw[0, 6] = math.inf
+    lw.requires_grad_()
+    labels, weights = ops.route(lw, 4, renormalise)
+    want = torch.tensor([[1.0, 0, 0, 0]] * n, dtype=weights.dtype, device="cuda")
+    want[0, :2] = 0.5
+    assert torch.equal(weights.detach(), want)
+    assert torch.equal(labels[1:, :3].cpu(), torch.tensor([[3, 1, 0]] * (n - 1))) and labels[0, :3].tolist() == [3, 6, 1]
+    up = torch.arange(1.0, 5.0, dtype=weights.dtype, device="cuda").expand(n, 4).contiguous()
+    grad, = torch.autograd.grad(weights, lw, up)
+    want = torch.zeros(n, K, dtype=dt, device="cuda")
+    want[0, 3], want[0, 6] = -0.25, 0.25                                  # 0.5 (1 - 1.5), 0.5 (2 - 1.5)
+    assert torch.equal(grad, want)
