@@ -48,6 +48,7 @@ class IGMM(GMM):
         self._rng = rng
         self._nprng = np.random if nprng is None else nprng
         self._lease = None              # the generators' states while a sampler loop runs (utils/rng.py: DeviceLease)
+        self._power = None              # the last sweep's exponent
 
         if isinstance(assignments, str):
             if assignments == "rand":
@@ -119,20 +120,25 @@ class IGMM(GMM):
         """log p(X, z) (igmm.py:199-215), evaluated on the device."""
         return self.components._ctx.log_marg()
 
-    def posterior_labels(self, X, k=1):
+    def posterior_labels(self, X, k=1, power=None):
         """
         The ``k`` most probable labels of new points and their posterior probabilities, given the current components: the
         weights of one visit of the sampler (igmm/crpmm.py:68-75), ``log n_k + log predictive`` for every component and
         ``log alpha + log prior predictive`` for label K, "a component of its own".  Full covariance.  (extension)
 
-        X : n x D array, or a float64 tensor on this model's GPU.  Returns ``(labels, weights)``, n x k, of X's kind,
-        ordered by probability; the weights are shares of the whole posterior.  (``pybgmm_amd.ops.route``)
+        X : n x D array, or a float64 tensor on this model's GPU.
+        power : exponent of the powered samplers' visits, ``power * log n_k`` (igmm/pcrpmm.py:105-108); default: that of the
+          last sweep this model ran, 1 where it was not powered or there was none.
+        Returns ``(labels, weights)``, n x k, of X's kind, ordered by probability; the weights are shares of the whole
+        posterior.  (``pybgmm_amd.ops.route``)
         """
         import torch
         from .. import ops
         x, back = self.components._on_device(X)
         K = self.components.K
-        prior = np.log(np.concatenate([self.components.counts[:K].astype(np.float64), [self.alpha]]))
+        if power is None:
+            power = 1.0 if self._power is None else self._power
+        prior = np.append(power * np.log(self.components.counts[:K].astype(np.float64)), np.log(self.alpha))
         log_weights = self.components.log_predictive(x) + torch.from_numpy(prior).to(x.device)
         labels, weights = ops.route(log_weights, k, renormalise=False)
         return back(labels), back(weights)
@@ -180,6 +186,7 @@ class IGMM(GMM):
 
     def _sweep(self, order=None, power=None):
         """One device sweep fed from the caller's random streams."""
+        self._power = power
         ctx = self.components._ctx
         if order is _rng.STAGED:        # (drawn on the device and already in place: _draw_order)
             order = None

@@ -1245,3 +1245,45 @@ def test_the_largest_number_beside_infinity_has_no_weight(dt, n, K, renormalise)
     want = torch.zeros(n, K, dtype=dt, device="cuda")
     want[0, 3], want[0, 6] = -0.25, 0.25                                  # 0.5 (1 - 1.5), 0.5 (2 - 1.5)
     assert torch.equal(grad, want)
+
+
+@gpu
+@pytest.mark.parametrize("cls,fit,powered", [("CRPMM", {}, False), ("PCRPMM", dict(n_power=1.4), True), ("PCRPMM", dict(n_power=1.4, flag_power=False), False),
+                                             ("PCRPMM", dict(n_power=1.4, power_burnin=9), False), ("ADAPCRPMM", dict(r_up=1.6, adapcrp_perct=0.5, adapcrp_burnin=-1), True),
+                                             ("ADAPCRPMM", dict(flag_adapcrp=False), False)])
+def test_posterior_labels_weigh_as_the_last_sweep_did(cls, fit, powered):
+    """The visit's weights, n_k ** power times the predictive and alpha times the prior's, normalised, for every sampler's own power."""
+    import random
+    import numpy as np
+    from pybgmm_amd import igmm
+    from pybgmm_amd.prior import NIW
+    from pybgmm_amd.utils import gendata
+    random.seed(4)
+    np.random.seed(4)
+    X, _ = gendata.synth_mixture(400, 3, 3, seed=5, mu_scale=1.5)
+    seen = []
+
+    class Watched(getattr(igmm, cls)):
+        def _sweep(self, order=None, power=None):
+            seen.append(power)
+            super()._sweep(order=order, power=power)
+    mm = Watched(X, NIW(np.zeros(3), 0.05, 6, np.eye(3)), 0.7, None, assignments="rand", K=5)
+    comp = mm.components
+
+    def weights(power):
+        lw = np.append(np.log(comp.counts[:comp.K] ** power), np.log(mm.alpha)) + np.array([np.append(comp.log_post_pred(i), comp.log_prior(i)) for i in range(30)])
+        p = np.exp(lw - lw.max(1, keepdims=True))
+        return p / p.sum(1, keepdims=True)
+
+    def check(expected, **kw):
+        labels, w = mm.posterior_labels(X[:30], k=comp.K + 1, **kw)
+        # (64-bit predictives of two routes, as in the comparison of the densities themselves: 1e-9 of each logarithm)
+        np.testing.assert_allclose(np.take_along_axis(w, np.argsort(labels, axis=1), 1), weights(expected), rtol=1e-7, atol=1e-12)
+    check(1.0)                                                      # no sweep yet
+    mm.collapsed_gibbs_sampler(4, np.zeros(400, dtype=int), **fit)
+    power = 1.0 if seen[-1] is None else seen[-1]
+    assert (power > 1.1) == powered
+    check(power)
+    check(2.5, power=2.5)
+    if powered:
+        assert np.abs(weights(power) - weights(1.0)).max() > 1e-3           # (the power matters to these points)
