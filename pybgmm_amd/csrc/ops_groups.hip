@@ -211,7 +211,7 @@ __global__ __launch_bounds__(64 * kSums) void group_small(const int64_t *labels,
 }
 
 // `waves` segments per workgroup (1, 4 or 8), of as many waves each as its kManyWaves allow.
-// within[segment][b]: the workgroup's earlier segments' rows of bucket b;  counts[workgroup][b]: all of its.
+// within[segment][b]: the workgroup's earlier segments' rows of bucket b (null: a workgroup has one);  counts[workgroup][b]: all of its.
 __global__ void group_count(const int64_t *labels, i64 P, int K, int seg, int nseg, int waves, int *bucket, int *within, int *counts) {
     extern __shared__ int lds[];
     const int B = K + 1, w = threadIdx.x >> 6, parts = kManyWaves / waves, s0 = blockIdx.x * waves, s = s0 + w % waves;
@@ -229,7 +229,7 @@ __global__ void group_count(const int64_t *labels, i64 P, int K, int seg, int ns
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
         int sum = 0;
         for (int j = 0; j < waves; ++j) {
-            if (s0 + j < nseg) within[(i64)(s0 + j) * B + b] = sum;
+            if (within && s0 + j < nseg) within[(i64)(s0 + j) * B + b] = sum;
             sum += lds[j * B + b];
         }
         counts[(i64)blockIdx.x * B + b] = sum;
@@ -298,7 +298,7 @@ __global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int se
     const int v = w % waves, parts = kManyWaves / waves;
     if (blockIdx.x * waves + v < nseg) {
 #pragma unroll 4
-        for (int b = w / waves * 64 + wave_lane(); b < B; b += 64 * parts) lds[v * B + b] = start[b] + within[(i64)(blockIdx.x * waves + v) * B + b];
+        for (int b = w / waves * 64 + wave_lane(); b < B; b += 64 * parts) lds[v * B + b] = start[b] + (within ? within[(i64)(blockIdx.x * waves + v) * B + b] : 0);
     }
     __syncthreads();
     if (w >= waves) return;
@@ -311,11 +311,17 @@ __global__ void group_scatter(const int *bucket, i64 P, int K, int nbits, int se
 // rows, 64 workgroups, 1000 components: 18.1 with the sums in a launch of their own, 19.2; 1e6 rows, 245: 16.5 and 23.7).
 constexpr int kFewGroups = 32;
 struct Split { int seg, nseg, waves, groups; };
+i64 within_of(const Split &s) { return s.waves > 1 ? s.nseg : 0; }          // histograms in `within`
 
-// Rows of a segment (a wave's): 512, 256 where that would leave most of the chip idle.  Segments per workgroup: eight while their histograms, the buckets' starts and the sums fit 64 KB of LDS.
+// Rows of a segment (a wave's): 512, 256 where that would leave most of the chip idle; more, up to the number of buckets, where the
+// histograms in memory would be 8 MB and more (4 MB of few rows), so that they are no larger than that and the rows' indices (1e6 rows
+// of 8000 components: 395 us and 125 MB with 512, 128 us with 4096, 140 us with 8192; of 3500: 169, 74 us with 2048, 77 with 4096; 4e6 of
+// 8000: 1740, 325 us with 4096, 207 with 8192; 1e5 of 8000: 128, 87 us with 1024, 125 with 8192; but 8192 rows of 8000: 78, 92 with 2048).
+// Segments per workgroup: eight while their histograms, the buckets' starts and the sums fit 64 KB of LDS.
 Split split_of(i64 P, int K) {
     Split s;
     s.seg = P <= 131072 ? 256 : 512;
+    while (s.seg <= K && (P + s.seg - 1) / s.seg * (K + 1) > (P <= 131072 ? 1 << 20 : 1 << 21)) s.seg *= 2;
     s.nseg = (int)((P + s.seg - 1) / s.seg);
     s.waves = K + 1 <= 1780 ? 8 : K + 1 <= 3200 ? 4 : 1;
     s.groups = (s.nseg + s.waves - 1) / s.waves;
@@ -327,7 +333,7 @@ Split split_of(i64 P, int K) {
 extern "C" int64_t bgmm_group_rows_ws(int64_t P, int32_t K) {
     if (P < 0 || K < 1 || small_form(P, K)) return 0;
     const Split s = split_of(P, K);
-    return 4 * ((int64_t)s.nseg + s.groups + 1) * (K + 1);
+    return 4 * (within_of(s) + s.groups + 1) * (K + 1);
 }
 
 extern "C" int64_t bgmm_group_rows_tiles(int64_t P, int32_t K) { return P < 0 || K < 1 ? 0 : tiles_at_most(P, K); }
@@ -350,7 +356,7 @@ extern "C" int bgmm_group_rows(const int64_t *labels, int64_t P, int32_t K, int3
         return ops_launched("group_rows");
     }
     const Split s = split_of(P, K);
-    int *within = (int *)ws, *counts = within + (size_t)s.nseg * B, *sizes = counts + (size_t)s.groups * B;
+    int *within = s.waves > 1 ? (int *)ws : nullptr, *counts = (int *)ws + (size_t)within_of(s) * B, *sizes = counts + (size_t)s.groups * B;
     // (P = 0 with many components: no segment, but the sums over nothing and the empty offsets are still written)
     if (s.groups > 0) group_count<<<s.groups, 64 * kManyWaves, sizeof(int) * (size_t)s.waves * B, st>>>(labels, P, K, s.seg, s.nseg, s.waves, bucket, within, counts);
     const bool columns = s.groups > kFewGroups || s.waves < 8;

@@ -128,7 +128,7 @@ bool differentiable(const char *what, std::initializer_list<Tensor> inputs) {
 struct RowGroups {
     std::vector<int64_t> shape;             // the labels'
     int64_t n, k, P, K, n_tiles;
-    Tensor store;                           // int32: tiles [n_tiles][4], bucket [P], order [P], offsets [K + 2], first [levels][K + 2], workspace
+    Tensor store;                           // int32: tiles [n_tiles][4], bucket [P], order [P], offsets [K + 2], first [levels][K + 2]
 
     RowGroups(std::vector<int64_t> s, int64_t components, Tensor st) : shape(std::move(s)), K(components), store(std::move(st)) {
         n = shape.at(0);
@@ -138,14 +138,13 @@ struct RowGroups {
         if (store.scalar_type() != at::kInt || store.dim() != 1 || store.numel() < size(P, K)) refuse(BGMM_OPS_EINVAL, "RowGroups: the store does not fit");
     }
     static int64_t size(int64_t P, int64_t K) {
-        return 4 * bgmm_group_rows_tiles(P, (int32_t)K) + 2 * P + (BGMM_OPS_LEVELS + 1) * (K + 2) + bgmm_group_rows_ws(P, (int32_t)K) / 4;
+        return 4 * bgmm_group_rows_tiles(P, (int32_t)K) + 2 * P + (BGMM_OPS_LEVELS + 1) * (K + 2);
     }
     int32_t *tiles() const { return store.numel() ? store.data_ptr<int32_t>() : nullptr; }
     int32_t *bucket() const { return tiles() + 4 * n_tiles; }
     int32_t *order() const { return bucket() + P; }
     int32_t *offsets() const { return order() + P; }
     int32_t *first() const { return offsets() + K + 2; }
-    int32_t *ws() const { return first() + BGMM_OPS_LEVELS * (K + 2); }
     Tensor part(int64_t at, int64_t size) const { return store.narrow(0, at, size); }
 };
 typedef std::shared_ptr<RowGroups> Groups;
@@ -164,8 +163,10 @@ Groups group_rows(const Tensor &labels, int64_t components) {
     const Tensor flat = packed(labels);
     const c10::OptionalDeviceGuard guard(labels.device());
     auto g = std::make_shared<RowGroups>(labels.sizes().vec(), components, at::empty({RowGroups::size(labels.numel(), components)}, labels.options().dtype(at::kInt)));
-    check(bgmm_group_rows(g->P ? flat.data_ptr<int64_t>() : nullptr, g->P, (int32_t)g->K, g->bucket(), g->order(), g->offsets(), g->first(), g->tiles(), g->ws(),
-                          bgmm_group_rows_ws(g->P, (int32_t)g->K), stream_of(labels)));
+    const int64_t bytes = bgmm_group_rows_ws(g->P, (int32_t)g->K);
+    const Tensor ws = bytes ? at::empty({bytes}, labels.options().dtype(at::kByte)) : Tensor();
+    check(bgmm_group_rows(g->P ? flat.data_ptr<int64_t>() : nullptr, g->P, (int32_t)g->K, g->bucket(), g->order(), g->offsets(), g->first(), g->tiles(), ptr(ws), bytes,
+                          stream_of(labels)));
     return g;
 }
 

@@ -1287,3 +1287,30 @@ def test_posterior_labels_weigh_as_the_last_sweep_did(cls, fit, powered):
     check(2.5, power=2.5)
     if powered:
         assert np.abs(weights(power) - weights(1.0)).max() > 1e-3           # (the power matters to these points)
+
+
+def test_a_groupings_memory_is_its_rows_and_components():
+    """The workspace does not grow with rows times components, and a grouping keeps none of it."""
+    from pybgmm_amd import ops
+    from pybgmm_amd.ops import _native as nat
+    L = nat.load()
+    for P in (0, 1, 4096, 4097, 131072, 131073, 1000000, 10**7, 10**9, 2**31 - 65537):
+        for K in (1, 100, 511, 512, 900, 1779, 1780, 3199, 3200, 8000):
+            # 4 bytes for each of at most 2^21 or P + K + 1 counts of segments, a quarter as many of workgroups, one per bucket and their remainders
+            assert L.bgmm_group_rows_ws(P, K) <= 5 * max(1 << 21, P + K + 1) + 12 * (K + 1), (P, K)
+            assert ops.RowGroups.store_size(P, K) == 4 * L.bgmm_group_rows_tiles(P, K) + 2 * P + 9 * (K + 2)
+
+
+@gpu
+@pytest.mark.parametrize("P,K", [(131072, 8000), (131073, 8000), (262144, 3199), (300001, 3200), (1200000, 8000), (270000, 7999), (4300000, 511), (2200000, 1023)])
+def test_groupings_of_long_segments(P, K):
+    from pybgmm_amd import ops
+    g = torch.Generator("cuda").manual_seed(P)
+    z = (torch.rand(P, device="cuda", generator=g) ** 3 * (K + 1)).long() - 1
+    grp = ops.group_rows(z, K)
+    bucket = torch.where(z >= 0, z, torch.full_like(z, K))
+    assert torch.equal(grp.order.long(), torch.argsort(bucket, stable=True))
+    size = torch.bincount(bucket, minlength=K + 1)
+    assert torch.equal(grp.counts.long(), size[:K]) and torch.equal(grp.offsets[1:].long(), size.cumsum(0))
+    again = ops.group_rows(z, K)
+    assert all(torch.equal(getattr(grp, a), getattr(again, a)) for a in ("order", "offsets", "first", "tiles", "bucket"))
