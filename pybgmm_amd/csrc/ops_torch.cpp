@@ -438,6 +438,8 @@ PYBIND11_MODULE(_binding, m) {
              }),
              py::arg("labels_shape"), py::arg("n_components"), py::arg("store"))
         .def_static("store_size", &RowGroups::size)
+        .def("record_stream", [](const RowGroups &g, const py::object &stream) { py::cast(g.store).attr("record_stream")(stream); }, py::arg("stream"),
+             "What Tensor.record_stream is for a tensor: this grouping's memory is not used again before the work queued on `stream` is done.")
         .def_property_readonly("labels_shape", [](const RowGroups &g) { return py::tuple(py::cast(g.shape)); })
         .def_readonly("n_components", &RowGroups::K)
         .def_readonly("n", &RowGroups::n)

@@ -27,6 +27,7 @@ def group_rows(labels, n_components):
     Returns a ``RowGroups`` for any number of ``grouped_matmul`` calls: ``labels_shape``, ``n_components``; ``order`` int32, flat
     label indices sorted by (component, index), those of no component last; ``offsets`` int32 (n_components + 2,), component e
     holds ``order[offsets[e]:offsets[e + 1]]``, the last bucket the rows of no component; ``counts``, rows per component.  The
-    products read them: they are not for writing.
+    products read them: they are not for writing.  For products on another stream than the one it was made on, that stream has to
+    wait for this one, and ``record_stream(stream)`` keeps the grouping's memory until they are done, as a tensor's does.
     """
     return _b.group_rows(labels, n_components)

@@ -1314,3 +1314,28 @@ def test_groupings_of_long_segments(P, K):
     assert torch.equal(grp.counts.long(), size[:K]) and torch.equal(grp.offsets[1:].long(), size.cumsum(0))
     again = ops.group_rows(z, K)
     assert all(torch.equal(getattr(grp, a), getattr(again, a)) for a in ("order", "offsets", "first", "tiles", "bucket"))
+
+
+@gpu
+def test_a_grouping_recorded_on_another_stream_keeps_its_memory():
+    from pybgmm_amd import ops
+    z = torch.randint(0, 7, (3000000,), device="cuda")
+    x, w = torch.randn(3000000, 4, device="cuda"), torch.randn(7, 4, 4, device="cuda")
+    want = ops.grouped_matmul(x, w, ops.group_rows(z, 7))
+    groups = ops.group_rows(z, 7)
+    at = groups.tiles.data_ptr()
+    size = ops.RowGroups.store_size(3000000, 7)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200000000)                                # (cycles: about 0.1 s)
+        y = ops.grouped_matmul(x, w, groups)
+    groups.record_stream(side)
+    del groups
+    others = [torch.full((size,), 1 << 20, dtype=torch.int32, device="cuda") for _ in range(4)]
+    assert not side.query()                                         # (the product still waits)
+    assert at not in [t.data_ptr() for t in others]
+    side.synchronize()
+    assert torch.equal(y, want)
+    with pytest.raises(RuntimeError):                                # (as Tensor.record_stream)
+        ops.group_rows(z, 7).record_stream(3)
