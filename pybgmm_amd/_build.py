@@ -54,22 +54,37 @@ def _stale(target, deps):
 
 def build(force=False, verbose=False, extra_flags=()):
     """Both libraries and the binding; returns the path of libbgmm_hip.so."""
-    # -no-hip-rt: libbgmm_ops.so does not link a HIP runtime (include/bgmm_ops.h says which one it binds to)
-    _build_one(OPS_LIB, OPS_SOURCES, OPS_HEADERS, ["-no-hip-rt", "-Wl,-soname," + os.path.basename(OPS_LIB)], force, verbose, extra_flags)
-    _build_binding(force, verbose)
+    path = build_sampler(force, verbose, extra_flags)
+    build_ops(force, verbose, extra_flags)
+    return path
+
+
+def build_sampler(force=False, verbose=False, extra_flags=()):
+    """libbgmm_hip.so alone: the samplers need neither g++ nor torch."""
     return _build_one(LIB, SOURCES, HEADERS, [], force, verbose, extra_flags)
 
 
+def build_ops(force=False, verbose=False, extra_flags=()):
+    """libbgmm_ops.so and, where there is a torch with HIP, the binding."""
+    # -no-hip-rt: libbgmm_ops.so does not link a HIP runtime (include/bgmm_ops.h says which one it binds to)
+    _build_one(OPS_LIB, OPS_SOURCES, OPS_HEADERS, ["-no-hip-rt", "-Wl,-soname," + os.path.basename(OPS_LIB)], force, verbose, extra_flags)
+    _build_binding(force, verbose)
+
+
+def bindable():
+    """Whether there is a torch with HIP: without one there are no operators to bind, nor ``pybgmm_amd.ops``."""
+    spec = importlib.util.find_spec("torch")
+    return spec is not None and bool(spec.origin) and os.path.exists(os.path.join(os.path.dirname(spec.origin), "lib", "libc10_hip.so"))
+
+
 def _build_binding(force, verbose):
-    """Host code against torch's headers and libraries; without torch, or with one that has no HIP, there are no operators to bind."""
+    """Host code against torch's headers and libraries."""
     src = os.path.join(CSRC, "ops_torch.cpp")
-    if importlib.util.find_spec("torch") is None or not (force or _stale(OPS_BINDING, [src, OPS_HEADERS[-1]])):
+    if not bindable() or not (force or _stale(OPS_BINDING, [src, OPS_HEADERS[-1]])):
         return
     import torch
     from torch.utils.cpp_extension import include_paths
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    if not os.path.exists(os.path.join(lib, "libc10_hip.so")):
-        return
     rocm = os.path.dirname(os.path.dirname(hipcc()))
     includes = include_paths() + [sysconfig.get_paths()["include"], os.path.join(rocm, "include"), "/opt/rocm/include"]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",

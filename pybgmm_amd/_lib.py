@@ -121,7 +121,7 @@ def load(build_if_missing=True):
         if not build_if_missing:
             raise OSError("libbgmm_hip.so not built: run `python __graft_entry__.py` "
                           "(there is no CPU fallback)")
-        _build.build()
+        _build.build_sampler()
     L = ctypes.CDLL(path)
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(L, name)

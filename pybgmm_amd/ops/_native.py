@@ -47,7 +47,7 @@ def load():
     if _lib is not None:
         return _lib
     if not os.path.exists(_build.OPS_LIB):
-        _build.build()
+        _build.build_ops()
     # The library links no HIP runtime.  libbgmm_hip.so may have brought the system's into the process; streams and device
     # pointers of one runtime mean nothing to the other, so torch's copy is made visible first and the binding is checked.
     runtime = os.path.join(os.path.dirname(torch.__file__), "lib", "libamdhip64.so")
@@ -67,7 +67,7 @@ def load():
 def binding():
     """The extension module with the operators (csrc/ops_torch.cpp)."""
     if not os.path.exists(_build.OPS_BINDING):
-        _build.build()
+        _build.build_ops()
     load()                              # (first: it settles which HIP runtime the library binds to)
     from . import _binding
     return _binding

@@ -1,0 +1,67 @@
+"""What the build makes, from what, and in which order (no compiler runs here)."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+from pybgmm_amd import _build
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def made(monkeypatch, fails=None):
+    """Records what a build makes; `fails`: a target whose compiler fails."""
+    log = []
+
+    def one(lib, *args):
+        log.append(lib)
+        return lib
+
+    def run(cmd, verbose):
+        log.append(cmd[cmd.index("-o") + 1])
+        if log[-1] == fails:
+            raise RuntimeError("no compiler")
+    monkeypatch.setattr(_build, "_build_one", one)
+    monkeypatch.setattr(_build, "_run", run)
+    return log
+
+
+def test_a_binding_that_cannot_be_built_leaves_the_samplers_library(monkeypatch):
+    log = made(monkeypatch, fails=_build.OPS_BINDING)
+    monkeypatch.setattr(_build, "_stale", lambda target, deps: True)
+    with pytest.raises(RuntimeError):
+        _build.build()
+    assert log[0] == _build.LIB
+
+
+def test_a_missing_library_is_built_by_itself(monkeypatch, tmp_path):
+    from pybgmm_amd import _lib
+    log = made(monkeypatch)
+    monkeypatch.setattr(_lib, "_lib", None)
+    missing = str(tmp_path / "libbgmm_hip.so")
+    monkeypatch.setattr(_build, "LIB", missing)
+    with pytest.raises(OSError):                # (nothing was really built)
+        _lib.load()
+    assert log == [missing]
+
+
+@pytest.mark.parametrize("without", ["torch", "hip"])
+def test_the_entry_point_builds_without_a_torch_that_has_hip(without, tmp_path):
+    """In a process of its own: no torch at all, or one without HIP."""
+    code = """if 1:
+        import sys
+        if %r == "torch":
+            sys.modules["torch"] = None
+        else:
+            sys.path.insert(0, %r)
+        import __graft_entry__ as entry
+        from pybgmm_amd import _build
+        _build.build = lambda *a, **k: _build.LIB
+        entry.build()
+        assert "pybgmm_amd.ops" not in sys.modules
+    """ % (without, str(tmp_path))
+    os.makedirs(str(tmp_path / "torch" / "lib"))
+    (tmp_path / "torch" / "__init__.py").write_text("raise ImportError('a torch without HIP')")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert r.returncode == 0, r.stdout
