@@ -6,6 +6,7 @@ The shared objects are git-ignored and go with the tree where it is copied.
 their objects.
 """
 import glob
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -28,6 +29,7 @@ OPS_LIB = os.path.join(HERE, "libbgmm_ops.so")
 OPS_SOURCES = ["ops_common.hip", "ops_groups.hip", "ops_products.hip", "ops_products_f64.hip", "ops_products_f32.hip",
                "ops_products_f16.hip", "ops_products_bf16.hip", "ops_route.hip", "ops_verify.hip"]
 OPS_BINDING = os.path.join(HERE, "ops", "_binding.so")          # what pybgmm_amd.ops imports: libbgmm_ops.so on torch tensors
+BOUND_TO = os.path.join(CSRC, "_obj", "binding_torch.txt")      # the torch that the binding was built for
 OPS_HEADERS = sorted(glob.glob(os.path.join(CSRC, "ops_*.h"))) + [os.path.join(INCLUDE, "bgmm_ops.h")]
 # -ffp-contract=off: the sufficient-statistics updates must round product and sum
 # separately (bit-identical m / S to the reference); hot loops call fma() explicitly.
@@ -80,7 +82,7 @@ def bindable():
 def _build_binding(force, verbose):
     """Host code against torch's headers and libraries."""
     src = os.path.join(CSRC, "ops_torch.cpp")
-    if not bindable() or not (force or _stale(OPS_BINDING, [src, OPS_HEADERS[-1]])):
+    if not bindable() or not (force or _stale(OPS_BINDING, [src, OPS_HEADERS[-1]]) or _bound_to() != _torch_here()):
         return
     import torch
     from torch.utils.cpp_extension import include_paths
@@ -94,6 +96,20 @@ def _build_binding(force, verbose):
     cmd += [src, "-o", OPS_BINDING, "-L" + lib, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-L" + HERE, "-lbgmm_ops",
             "-Wl,-rpath,$ORIGIN/..", "-Wl,--allow-shlib-undefined"]
     _run(cmd, verbose)
+    with open(BOUND_TO, "w") as f:
+        f.write(_torch_here())
+
+
+def _torch_here():
+    """Which torch a binding built now is for: its C++ interface differs between versions."""
+    return "%s %s" % (importlib.metadata.version("torch"), importlib.util.find_spec("torch").origin)
+
+
+def _bound_to():
+    if not os.path.exists(BOUND_TO):
+        return None
+    with open(BOUND_TO) as f:
+        return f.read()
 
 
 def _run(cmd, verbose):

@@ -65,3 +65,19 @@ def test_the_entry_point_builds_without_a_torch_that_has_hip(without, tmp_path):
     (tmp_path / "torch" / "__init__.py").write_text("raise ImportError('a torch without HIP')")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     assert r.returncode == 0, r.stdout
+
+
+def test_another_torch_gets_another_binding(monkeypatch, tmp_path):
+    if not _build.bindable():
+        pytest.skip("no torch with HIP")
+    log = made(monkeypatch)
+    monkeypatch.setattr(_build, "_stale", lambda target, deps: False)
+    monkeypatch.setattr(_build, "BOUND_TO", str(tmp_path / "torch.txt"), raising=False)
+    _build.build_ops()
+    assert log == [_build.OPS_LIB, _build.OPS_BINDING]
+    _build.build_ops()
+    assert log[2:] == [_build.OPS_LIB]                               # (the same torch: up to date)
+    version = _build.importlib.metadata.version
+    monkeypatch.setattr(_build.importlib.metadata, "version", lambda name: version(name) + ".1")
+    _build.build_ops()
+    assert log[3:] == [_build.OPS_LIB, _build.OPS_BINDING]
