@@ -81,3 +81,16 @@ def test_another_torch_gets_another_binding(monkeypatch, tmp_path):
     monkeypatch.setattr(_build.importlib.metadata, "version", lambda name: version(name) + ".1")
     _build.build_ops()
     assert log[3:] == [_build.OPS_LIB, _build.OPS_BINDING]
+
+
+@pytest.mark.parametrize("script,own", [("build_prof.sh", "kernels_home"), ("build_prof_gram.sh", "kernels_gram"), ("build_prof_seq.sh", "kernels_seq"),
+                                        ("build_variant.sh", "kernels_home"), ("build_tsan.sh", None)])
+def test_variants_of_the_samplers_library_hold_its_own_objects(script, own, tmp_path):
+    """The objects a script of tools/ links besides what it compiles itself."""
+    os.makedirs(str(tmp_path / "_obj"))
+    for src in _build.SOURCES + _build.OPS_SOURCES:
+        (tmp_path / "_obj" / (src + ".o")).write_text("")
+    line, = [a for a in open(os.path.join(ROOT, "tools", script)).read().splitlines() if a.startswith("OBJS=")]
+    out = subprocess.run(["bash", "-c", "FILE=kernels_home.hip; %s; echo $OBJS" % line], cwd=str(tmp_path), stdout=subprocess.PIPE, text=True, check=True).stdout
+    want = set(s for s in _build.SOURCES if s != "%s.hip" % own and (own or s.startswith("kernels_")))
+    assert set(os.path.basename(o)[:-2] for o in out.split()) == want

@@ -5,6 +5,6 @@ cd "$(dirname "$0")/../pybgmm_amd/csrc"
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p _obj
 hipcc $FLAGS -DBGMM_HOME_PROF -c kernels_home.hip -o _obj/kernels_home_prof.o
-OBJS=$(ls _obj/*.hip.o | grep -v kernels_home.hip.o)
+OBJS=$(ls _obj/api_*.hip.o _obj/kernels_*.hip.o | grep -v kernels_home.hip.o)
 hipcc --offload-arch=gfx950 -shared -fPIC -o ../libbgmm_hip_prof.so $OBJS _obj/kernels_home_prof.o
 echo built ../libbgmm_hip_prof.so

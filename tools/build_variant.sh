@@ -10,6 +10,6 @@ cd "$(dirname "$0")/../pybgmm_amd/csrc"
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fvisibility=hidden -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p _obj
 hipcc $FLAGS "$@" -c $FILE -o _obj/${BASE}_$NAME.o
-OBJS=$(ls _obj/*.hip.o | grep -v $FILE.o)
+OBJS=$(ls _obj/api_*.hip.o _obj/kernels_*.hip.o | grep -v $FILE.o)
 hipcc --offload-arch=gfx950 -shared -fPIC -o ../libbgmm_hip_$NAME.so $OBJS _obj/${BASE}_$NAME.o
 echo built ../libbgmm_hip_$NAME.so
