@@ -102,7 +102,11 @@ def _build_binding(force, verbose):
 
 def _torch_here():
     """Which torch a binding built now is for: its C++ interface differs between versions."""
-    return "%s %s" % (importlib.metadata.version("torch"), importlib.util.find_spec("torch").origin)
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:         # (a source tree on the path)
+        version = "unknown"
+    return "%s %s" % (version, importlib.util.find_spec("torch").origin)
 
 
 def _bound_to():

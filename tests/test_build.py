@@ -57,8 +57,10 @@ def test_the_entry_point_builds_without_a_torch_that_has_hip(without, tmp_path):
             sys.path.insert(0, %r)
         import __graft_entry__ as entry
         from pybgmm_amd import _build
-        _build.build = lambda *a, **k: _build.LIB
+        forced = []
+        _build.build = lambda force=False, **k: forced.append(force) or _build.LIB
         entry.build()
+        assert forced == [True]
         assert "pybgmm_amd.ops" not in sys.modules
     """ % (without, str(tmp_path))
     os.makedirs(str(tmp_path / "torch" / "lib"))
@@ -94,3 +96,13 @@ def test_variants_of_the_samplers_library_hold_its_own_objects(script, own, tmp_
     out = subprocess.run(["bash", "-c", "FILE=kernels_home.hip; %s; echo $OBJS" % line], cwd=str(tmp_path), stdout=subprocess.PIPE, text=True, check=True).stdout
     want = set(s for s in _build.SOURCES if s != "%s.hip" % own and (own or s.startswith("kernels_")))
     assert set(os.path.basename(o)[:-2] for o in out.split()) == want
+
+
+def test_a_torch_without_package_metadata_has_a_name(monkeypatch):
+    if not _build.bindable():
+        pytest.skip("no torch with HIP")
+
+    def version(name):
+        raise _build.importlib.metadata.PackageNotFoundError(name)
+    monkeypatch.setattr(_build.importlib.metadata, "version", version)
+    assert _build._torch_here().endswith("__init__.py")
