@@ -385,12 +385,11 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
 }
 
 // A number as two of bfloat16, which has its range: the upper half of its bits, and the rest rounded to 8 bits (2^-15 of the number
-// at most is lost) with 2^-20 of the number on top, so that it is of the number's sign and zero only with it: an infinite operand
-// stays infinite against either.  Infinities and NaN are themselves in both.
+// at most is lost).  Infinities and NaN are themselves in both.
 __device__ __forceinline__ void two_pieces(float v, bf16_t &high, bf16_t &low) {
     const float h = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
     high = (bf16_t)h;
-    low = (bf16_t)(__builtin_fabsf(v) < __builtin_inff() ? __builtin_fmaf(v, 0x1p-20f, v - h) : v);
+    low = (bf16_t)(__builtin_fabsf(v) < __builtin_inff() ? v - h : v);
 }
 
 // dW: the rows of a chunk are the contraction, both operands have it outermost (MTile).
@@ -601,6 +600,42 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kerne
         __syncthreads();
         if (s + 1 < n_steps) put(held, s + 1);
         __syncthreads();
+    }
+    if constexpr (PIECES) {
+        // An infinite number times a second piece that is zero is NaN where the whole numbers' product is infinite.  A wave that has a NaN
+        // adds up its results once more, whole numbers one by one.
+        bool undefined = false;
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+            for (int j = 0; j < FB; ++j)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) undefined = undefined || acc[i][j][x] != acc[i][j][x];
+        if (__any(undefined)) {
+#pragma unroll
+            for (int i = 0; i < FA; ++i)
+#pragma unroll
+                for (int j = 0; j < FB; ++j) acc[i][j] = (A4){0, 0, 0, 0};
+            for (int r = 0; r < n_rows; ++r) {
+                const int p = list[r];
+                const T *pi = (const T *)a.in + (i64)divide(p, a.in_div) * a.in_stride, *po = (const T *)a.d + (i64)divide(p, a.d_div) * a.d_stride;
+                A row[FB];
+#pragma unroll
+                for (int j = 0; j < FB; ++j) {
+                    const int m = i0 + (wi * FB + j) * 16 + (lane & 15);
+                    row[j] = (A)pi[m < a.idim ? m : i0];
+                }
+#pragma unroll
+                for (int i = 0; i < FA; ++i)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int n = o0 + (wo * FA + i) * 16 + result_col<T>(lane >> 4, x);
+                        const A v = (A)po[n < a.odim ? n : o0] * gates[p];
+#pragma unroll
+                        for (int j = 0; j < FB; ++j) acc[i][j][x] = __builtin_fmaf(v, row[j], acc[i][j][x]);
+                    }
+            }
+        }
     }
 
     // a component with one chunk is finished here; several leave partial sums, added in the chunks' order by weight_reduce

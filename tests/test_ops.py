@@ -1141,8 +1141,8 @@ def test_gates_of_any_size_in_the_weights_gradient(dt, n, k, K, din, dout, gate,
     """
     Gates times gradients that 16 bits cannot hold (nothing of 1e-4 x 1e-4 is left in half precision, 100 x 1000 is infinite there), next
     to ordinary ones.  The product takes g d as two bfloat16 numbers, which lose at most 2^-15 of it (the first has 8 bits, the rest is
-    rounded to 8: 2^-7 2^-8) and carry 2^-20 too much, in half precision x likewise (whose 11 bits are whole in two): 2^-14 of a term
-    covers both; 32-bit sums of a component's own rows (two to four products a term), and the result's own rounding.
+    rounded to 8: 2^-7 2^-8), in half precision x likewise (whose 11 bits are whole in two): 2^-14 of a term covers that with its
+    second pieces' own roundings; 32-bit sums of a component's own rows (two to four products a term), and the result's own rounding.
     """
     from pybgmm_amd import ops
     if gate == 1e30 and dt == torch.float16:
@@ -1339,3 +1339,51 @@ def test_a_grouping_recorded_on_another_stream_keeps_its_memory():
     assert torch.equal(y, want)
     with pytest.raises(RuntimeError):                                # (as Tensor.record_stream)
         ops.group_rows(z, 7).record_stream(3)
+
+
+# components' rows around a tile's, a step's and a chunk's borders; and enough rows for longer chunks
+BORDERS = [0, 1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 4095, 4097, 8193]
+MANY = [600001, 300000, 131072, 65537, 32769, 32767, 16385, 8191, 2049, 1023, 513, 255, 20, 0, 3]
+
+
+@gpu
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("din,dout,sizes", [(16, 16, BORDERS), (5, 100, BORDERS), (130, 7, BORDERS), (64, 64, BORDERS), (40, 128, BORDERS), (128, 33, BORDERS),
+                                            (131, 140, BORDERS), (3, 4, MANY), (16, 70, MANY), (70, 9, MANY), (129, 130, MANY[1:])])
+def test_sums_of_whole_numbers_are_exact(dt, gated, din, dout, sizes):
+    """
+    Small whole numbers and gates that are powers of two: every product and every partial sum is held exactly (in quarters below 2^24, which
+    the magnitudes' sum shows), so that a row, a step or a chunk that is lost, doubled or misplaced cannot hide behind a tolerance;
+    what is left is the result's one rounding.
+    """
+    from pybgmm_amd import ops
+    K, n = len(sizes), sum(sizes)
+    g = torch.Generator("cuda").manual_seed(din * dout)
+
+    def whole(*s):
+        return torch.randint(-2, 3, s, generator=g, device="cuda").to(dt)
+    z = torch.repeat_interleave(torch.arange(K, device="cuda"), torch.tensor(sizes, device="cuda"))[torch.randperm(n, device="cuda", generator=g)]
+    x, w, b, dy = whole(n, din), whole(K, din, dout), whole(K, dout), whole(n, dout)
+    gates = 2.0 ** torch.randint(-2, 2, (n,), generator=g, device="cuda").to(acc_of(dt)) if gated else None
+    leaves = [t.requires_grad_() for t in (x, w, b, gates) if t is not None]
+    y = ops.grouped_matmul(x, w, ops.group_rows(z, K), bias=b, gates=gates)
+    grads = torch.autograd.grad(y, leaves, dy)
+    got = dict(zip(("x", "w", "b", "g"), grads), y=y.detach())
+    want = {a: torch.zeros(t.shape, dtype=torch.float64, device="cuda") for a, t in got.items()}
+    largest = 0.0
+    with torch.no_grad():
+        for e in range(K):
+            i = torch.nonzero(z == e)[:, 0]
+            xe, de, we, be = x[i].double(), dy[i].double(), w[e].double(), b[e].double()
+            ge = gates[i].double()[:, None] if gated else 1.0
+            u, v = xe @ we + be, de @ we.t().contiguous()
+            want["y"][i], want["x"][i], want["w"][e], want["b"][e] = ge * u, ge * v, xe.t().contiguous() @ (ge * de), (ge * de).sum(0)
+            if gated:
+                want["g"][i] = (de * u).sum(1)
+            largest = max(largest, float((xe.abs().t().contiguous() @ (ge * de).abs()).max())) if i.numel() else largest
+    assert largest * 4 < 2 ** 24
+    for name, t in got.items():
+        exact = want[name].float().to(t.dtype) if t.dtype != torch.float64 else want[name]
+        off = t != exact
+        assert not bool(off.any()), (name, int(off.sum()), torch.nonzero(off)[:4].tolist(), t[off][:4].tolist(), want[name][off][:4].tolist())
