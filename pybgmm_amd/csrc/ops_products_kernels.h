@@ -2,8 +2,6 @@
 #pragma once
 #include "ops_products.h"
 
-template <class T> __device__ __forceinline__ float as_f32(T v) { return (float)v; }
-
 // Consecutive elements of an output row from accumulators, as one store where all of them exist (at any alignment).
 template <int N, class T, class V> __device__ __forceinline__ void store_run(T *p, const V &v, int from, int avail) {
     struct Run { T e[N]; } o;
