@@ -37,6 +37,7 @@ enum { BGMM_F64 = 0, BGMM_F32 = 1, BGMM_F16 = 2, BGMM_BF16 = 3 };
 enum {
     BGMM_OPS_MAX_COMPONENTS = 8000,  /* components of a grouping                               */
     BGMM_OPS_MAX_CHOSEN = 32,        /* components chosen per row by bgmm_route                */
+    BGMM_OPS_MAX_AXIS = (1 << 27) - 1,  /* d_in and d_out of a product                           */
     BGMM_OPS_LEVELS = 8              /* chunk sizes of a grouping: 256, 512, ..., 32768 rows   */
 };
 

@@ -60,6 +60,7 @@ int check(const char *what, int dtype, i64 P, int K, int a, int b) {
     if (P < 0 || P > 0x7fffffff - 65536 || K < 1 || a < 1 || b < 1)
         return ops_fail(BGMM_OPS_EINVAL, "%s: P = %lld, K = %d, dimensions %d and %d", what, (long long)P, K, a, b);
     if (K > BGMM_OPS_MAX_COMPONENTS) return ops_fail(BGMM_OPS_EUNSUPPORTED, "%s: K = %d components (at most %d)", what, K, BGMM_OPS_MAX_COMPONENTS);
+    if (a > BGMM_OPS_MAX_AXIS || b > BGMM_OPS_MAX_AXIS) return ops_fail(BGMM_OPS_EUNSUPPORTED, "%s: dimensions %d and %d (at most %d)", what, a, b, BGMM_OPS_MAX_AXIS);
     return BGMM_OPS_OK;
 }
 
@@ -149,7 +150,6 @@ extern "C" int bgmm_weight_product(int32_t dtype, const void *in, int64_t in_str
     if (in_div < 1 || d_div < 1 || in_stride < 0 || d_stride < 0) return ops_fail(BGMM_OPS_EINVAL, "weight_product: divisors %d %d, strides %lld %lld", in_div, d_div, (long long)in_stride, (long long)d_stride);
     if (ws_bytes < bgmm_weight_product_ws(dtype, P, K, idim, odim) || (ws_bytes > 0 && (!ws || ((uintptr_t)ws & 15))))
         return ops_fail(BGMM_OPS_EINVAL, "weight_product: workspace of %lld bytes", (long long)ws_bytes);
-    if (K > 65535) return ops_fail(BGMM_OPS_EUNSUPPORTED, "weight_product: K = %d", K);
     const WeightTiles w = weight_tiles(P, idim, odim);
     WeightArgs a;
     a.level = w.level;

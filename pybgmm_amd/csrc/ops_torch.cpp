@@ -353,7 +353,7 @@ Tensor grouped_matmul(const Tensor &x, const Tensor &weight, const Groups &g, co
     const Tensor b = given(bias), gt = given(gates);
     if (weight.scalar_type() != x.scalar_type() || (b.defined() && b.scalar_type() != x.scalar_type()))
         refuse(BGMM_OPS_EINVAL, "%s: x, weight and bias have to be of one type", what);
-    if (weight.dim() != 3 || weight.size(0) != g->K || weight.size(1) < 1 || weight.size(2) < 1 || weight.size(1) > 0x7ffffff || weight.size(2) > 0x7ffffff)
+    if (weight.dim() != 3 || weight.size(0) != g->K || weight.size(1) < 1 || weight.size(2) < 1 || weight.size(1) > BGMM_OPS_MAX_AXIS || weight.size(2) > BGMM_OPS_MAX_AXIS)
         refuse(BGMM_OPS_EINVAL, "%s: weight is %s, not (%lld, d_in, d_out)", what, shape_of(weight).c_str(), (long long)g->K);
     const int64_t d_in = weight.size(1), d_out = weight.size(2);
     const bool per_label = x.dim() == 3 && g->shape.size() == 2;

@@ -1387,3 +1387,16 @@ def test_sums_of_whole_numbers_are_exact(dt, gated, din, dout, sizes):
         exact = want[name].float().to(t.dtype) if t.dtype != torch.float64 else want[name]
         off = t != exact
         assert not bool(off.any()), (name, int(off.sum()), torch.nonzero(off)[:4].tolist(), t[off][:4].tolist(), want[name][off][:4].tolist())
+
+
+def test_c_entry_points_refuse_axes_whose_bytes_32_bits_do_not_count():
+    from pybgmm_amd.ops import _native as nat
+    L = nat.load()
+    buf = ctypes.create_string_buffer(64)
+    p, big = ctypes.addressof(buf), 1 << 27
+    assert L.bgmm_rows_product_splits(0, 8, 2, 1 << 28, 4) == 1             # (2^31 bytes of doubles)
+    assert L.bgmm_weight_product_ws(0, 1000, 2, big, 4) == 0
+    for kdim, ndim in ((big, 4), (4, big)):
+        assert L.bgmm_rows_product(0, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 1, None, 0, 1, None, 8, 2, kdim, ndim, p, p, None) == -5
+        assert L.bgmm_weight_product(0, p, 4, 1, p, 4, 1, None, p, None, None, 0, 8, 2, kdim, ndim, p, p, p, None) == -5
+    assert L.bgmm_combine(0, p, 1, 4, 1, 2, p, None, p, 4, big, None, None, 0, None, 0, None, 0, 1, 1, None) == -5
