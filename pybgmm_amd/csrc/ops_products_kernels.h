@@ -383,11 +383,11 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(
 }
 
 // A number as two of bfloat16, which has its range: the upper half of its bits, and the rest rounded to 8 bits (2^-15 of the number
-// at most is lost).  Infinities and NaN are themselves in both.
+// at most is lost).  The second is NaN beside infinity.
 __device__ __forceinline__ void two_pieces(float v, bf16_t &high, bf16_t &low) {
     const float h = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
     high = (bf16_t)h;
-    low = (bf16_t)(__builtin_fabsf(v) < __builtin_inff() ? v - h : v);
+    low = (bf16_t)(v - h);
 }
 
 // dW: the rows of a chunk are the contraction, both operands have it outermost (MTile).
@@ -395,7 +395,7 @@ __device__ __forceinline__ void two_pieces(float v, bf16_t &high, bf16_t &low) {
 // the range (a gate of 1e-4 times a gradient of 1e-4 is zero there).  It goes into the product as two of bfloat16, the rows in half
 // precision too (11 bits are whole in two): two or four products of pieces in one accumulator, 2^-15 of a term lost.  Forward and this,
 // 16384 rows of 64 experts, 1024 x 2048: bfloat16 330 us with g d rounded, 380 in pieces (25 the second product, 25 to make them),
-// half precision 334 and 530.
+// half precision 334 and 490.
 // 64 experts of 1024 x 2048 from 16384 rows, bfloat16: 190 us, 360 TFLOP/s, without pieces.  A component's 256 rows are four steps, so the time is
 // what four steps do not hide: finding the chunk, its rows and the first loads (a quarter, alone), and the results' stores (4 MB
 // for 1.5 MB of operands; a third).
@@ -600,8 +600,8 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kerne
         __syncthreads();
     }
     if constexpr (PIECES) {
-        // An infinite number times a second piece that is zero is NaN where the whole numbers' product is infinite.  A wave that has a NaN
-        // adds up its results once more, whole numbers one by one.
+        // An infinite number makes NaN in pieces, by its own second one or another's that is zero.  A wave that has a NaN adds up its
+        // results once more, whole numbers one by one.
         bool undefined = false;
 #pragma unroll
         for (int i = 0; i < FA; ++i)
