@@ -74,7 +74,8 @@ template <int N> __device__ __forceinline__ void exps(const double *x, double *y
     for (int q = 0; q < N; ++q) y[q] = __builtin_ldexp(y[q], (int)k[q]);
 }
 // Single: 2^(x log2 e) on the hardware's exponential, the rounding of the product made good to first order (its error alone is |x|
-// half steps); below e^-87 the result is zero.
+// half steps).  The hardware's results end at the smallest normal number, 2^-126; below, -inf among them, they are zero.  (Subnormal ones
+// by taking the exponent's whole part apart: 500000 x 200, k = 4, 128 -> 140 us.)
 template <int N> __device__ __forceinline__ void exps(const float *x, float *y) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
@@ -82,7 +83,7 @@ template <int N> __device__ __forceinline__ void exps(const float *x, float *y) 
         const float t = v * 1.44269504f;
         const float low = __builtin_fmaf(v, 1.44269504f, -t) + v * 1.92596303e-8f;
         const float e = __builtin_amdgcn_exp2f(t);
-        y[q] = x[q] > -87.0f ? __builtin_fmaf(e, low * 0.693147181f, e) : 0.0f;
+        y[q] = __builtin_fmaf(e, low * 0.693147181f, e);
     }
 }
 

@@ -13,6 +13,7 @@ def route(log_weights, k, renormalise=True):
     the chosen components (``renormalise=True``) or over all of them (``False``: the posterior's own shares), float64 for float64
     input and float32 otherwise.  Components at -inf (no members, masked) or NaN are never chosen and have no weight; a row with
     fewer than ``k`` others fills up with label -1, weight 0 -- what ``group_rows`` takes for "no component".
+    Weights held in 32 bits that are below their smallest normal number, 2^-126 of the largest, are zero.
     ``weights`` is differentiable with respect to ``log_weights``.  float64 / 32 / 16, bfloat16; k at most 32.
     """
     return _b.route(log_weights, k, renormalise)

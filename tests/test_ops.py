@@ -1400,3 +1400,23 @@ def test_c_entry_points_refuse_axes_whose_bytes_32_bits_do_not_count():
         assert L.bgmm_rows_product(0, p, 4, 1, p, 4, 4, 0, None, 0, None, p, 4, None, 1, None, 0, 1, None, 8, 2, kdim, ndim, p, p, None) == -5
         assert L.bgmm_weight_product(0, p, 4, 1, p, 4, 1, None, p, None, None, 0, 8, 2, kdim, ndim, p, p, p, None) == -5
     assert L.bgmm_combine(0, p, 1, 4, 1, 2, p, None, p, 4, big, None, None, 0, None, 0, None, 0, 1, 1, None) == -5
+
+
+@gpu
+@pytest.mark.parametrize("K", [5, 300, 3000, 20001])
+def test_route_weights_down_to_the_smallest_normal_number(K):
+    """
+    Single precision.  The difference x from the maximum is rounded, |x| 2^-24, which is that much of the result; exp is off by at most
+    2^-21 (the hardware's one step, the argument's correction, three roundings and the quotient's); below 2^-126 it is zero.
+    """
+    from pybgmm_amd import ops
+    down = torch.arange(1, 401, dtype=torch.float64) * -0.2625                # to -105; e^-87.34 is 2^-126
+    lw = torch.full((400, K), -math.inf)
+    lw[:, 1], lw[:, 3] = 2.0, (2.0 + down).float()
+    labels, w = ops.route(lw.cuda(), 3, False)
+    x = lw[:, 3].double() - 2.0
+    want = torch.exp(x) / (1 + torch.exp(x))
+    assert bool((labels.cpu() == torch.tensor([1, 3, -1])).all())
+    off = (w[:, 1].cpu().double() - want).abs()
+    assert bool((off <= (2.0 ** -21 + 2.0 ** -24 * x.abs()) * want)[x > -87.3].all())
+    assert bool((off <= want)[x <= -87.3].all()) and bool((w[-5:, 1].cpu() == 0).all()) and not w[:, 2].any()
