@@ -343,7 +343,10 @@ template <class T> __global__ __launch_bounds__(256) void route_backward_kernel(
     }
 }
 
-// The form for this K and k: 8 lanes up to 16 elements each, then 16, 32, 64 -- at least k --, then workgroups.
+// The form for this K and k: 8 lanes up to 16 elements each, then 16, 32, 64 -- at least k --, then workgroups.  A lane has 16 elements or
+// the least of 4, 8 and 14 that hold the row: every element costs six instructions a round (k = 4, shares of all, 14 and 16: 1e6 x 200
+// double 478 and 520 us, 1e6 x 400 952 and 1046, 1e6 x 201 single 305 and 316, 1e6 x 101 bfloat16 122 and 130; 12 in 14's place serve
+// 1e6 x 180 double, 420 and 457, but not 193 to 224).
 template <class T, int G, int E> void route_by_size(const RouteArgs &a, hipStream_t st) {
     const int need = (a.K + G * E - 1) / (G * E);
     constexpr int kMost = 16 / E;

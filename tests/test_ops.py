@@ -1420,3 +1420,43 @@ def test_route_weights_down_to_the_smallest_normal_number(K):
     off = (w[:, 1].cpu().double() - want).abs()
     assert bool((off <= (2.0 ** -21 + 2.0 ** -24 * x.abs()) * want)[x > -87.3].all())
     assert bool((off <= want)[x <= -87.3].all()) and bool((w[-5:, 1].cpu() == 0).all()) and not w[:, 2].any()
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=str)
+def test_a_large_grouping_and_gated_gradients_captured_and_replayed(dt):
+    """A grouping in several launches, whose workspace is gone when it returns, and the product of 16-bit pieces."""
+    from pybgmm_amd import ops
+    n, K = 140000, 2500
+    g = torch.Generator("cuda").manual_seed(8)
+
+    def inputs():
+        z = (torch.rand(n, device="cuda", generator=g) ** 2 * (K + 1)).long() - 1
+        return [z] + [torch.randn(*s, device="cuda", generator=g).to(dt) for s in ((n, 20), (K, 20, 24), (n, 24))] + [torch.rand(n, device="cuda", generator=g)]
+
+    def step(z, x, w, dy, gates):
+        groups = ops.group_rows(z, K)
+        y = ops.grouped_matmul(x, w, groups, gates=gates)
+        return (groups.order, y.detach()) + torch.autograd.grad(y, (x, w, gates), dy)
+    static = inputs()
+    for i in (1, 2, 4):
+        static[i].requires_grad_()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(*static)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*static)
+    for r in range(4):
+        new = inputs()
+        with torch.no_grad():
+            for dst, src in zip(static, new):
+                dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        for i in (1, 2, 4):
+            new[i].requires_grad_()
+        for a, b in zip(got, step(*new)):
+            assert torch.equal(a, b), r
