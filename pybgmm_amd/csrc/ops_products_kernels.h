@@ -117,10 +117,10 @@ __device__ __forceinline__ void store_tile(char *lds, int wn, int wm, int n_rows
     }
 }
 
-// What bounds it.  1e6 rows of 64 doubles: memory, 240 us for 1.04 GB.  2e6 of 128 doubles: 1.32 ms, 49 TFLOP/s, the matrix pipe 61 %
+// What bounds it.  1e6 rows of 64 doubles: memory, 240 us for 1.04 GB.  2e6 of 128 doubles: 1.32 ms, 49 TFLOP/s, the matrix pipe 64 %
 // busy; the rest is the beginnings and ends of tiles of eight steps (without the results' stores 1.19 of 1.44 ms when that was
-// measured, without loads 1.37).  16384 rows, 64 experts of 1024 x 2048, bfloat16: 140 - 150 us, 470 TFLOP/s; every byte of a tile
-// comes from L2 (1.2 GB for both operands, 8 TB/s), ragged ends are a fifth of the tiles.  A tile of 256 columns halves
+// measured, without loads 1.37).  16384 rows, 64 experts of 1024 x 2048, bfloat16: 130 - 150 us, 500 TFLOP/s; every byte of a tile
+// comes from L2 (1.3 GB for both operands, 9 TB/s), ragged ends are a fifth of the tiles.  A tile of 256 columns halves
 // the rows' share of that and takes two workgroups a compute unit instead of three: 182 against 146 us.
 template <class T, bool KCONTIG, int BM, int BN, int WN, int WM>
 __global__ __launch_bounds__(256, (kWavesPerSimd<T, BM * BN>)) void rows_kernel(RowsArgs a) {
@@ -394,7 +394,7 @@ __device__ __forceinline__ void two_pieces(float v, bf16_t &high, bf16_t &low) {
 // PIECES, the gates of 16-bit types: g d in 16 bits would be a rounding more than the operands have, and in half precision it leaves
 // the range (a gate of 1e-4 times a gradient of 1e-4 is zero there).  It goes into the product as two of bfloat16, the rows in half
 // precision too (11 bits are whole in two): two or four products of pieces in one accumulator, 2^-15 of a term lost.  Forward and this,
-// 16384 rows of 64 experts, 1024 x 2048: bfloat16 330 us with g d rounded, 380 in pieces (25 the second product, 25 to make them),
+// 16384 rows of 64 experts, 1024 x 2048: bfloat16 330 us with g d rounded, 375 in pieces (25 the second product, 25 to make them),
 // half precision 334 and 490.
 // 64 experts of 1024 x 2048 from 16384 rows, bfloat16: 190 us, 360 TFLOP/s, without pieces.  A component's 256 rows are four steps, so the time is
 // what four steps do not hide: finding the chunk, its rows and the first loads (a quarter, alone), and the results' stores (4 MB
