@@ -601,7 +601,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, BI * BO>)) void weight_kerne
     }
     if constexpr (PIECES) {
         // An infinite number makes NaN in pieces, by its own second one or another's that is zero.  A wave that has a NaN adds up its
-        // results once more, whole numbers one by one.
+        // results once more, whole numbers one by one (forward and this where every result is NaN: 0.41 -> 1.9 ms, 16384 rows as above).
         bool undefined = false;
 #pragma unroll
         for (int i = 0; i < FA; ++i)
